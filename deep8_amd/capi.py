@@ -18,6 +18,7 @@ STATIC_SCRATCH_BYTES = 32 << 20  # D8_STATIC_SCRATCH_BYTES of include/deep8_hip.
 c_int, c_long, c_size_t, c_float, c_void_p = (ctypes.c_int, ctypes.c_long, ctypes.c_size_t, ctypes.c_float,
                                               ctypes.c_void_p)
 _I, _L, _Z, _F, _P = c_int, c_long, c_size_t, c_float, c_void_p
+_D = ctypes.c_double
 _PP = ctypes.POINTER(c_void_p)
 
 # name -> (restype, argtypes); mirrors include/deep8_hip.h declaration by declaration
@@ -119,6 +120,16 @@ SIGNATURES = {
     "d8_avgpool2d_grad": (_I, [_I, _P, _P] + [_I] * 9 + [_P]),
     "d8_avgpool2d_grad_overwrite": (_I, [_I, _P, _P] + [_I] * 9 + [_P]),
     "d8_adam_update": (_I, [_I, _P, _P, _P, _P, _F, _F, _F, _F, _F, ctypes.c_long, ctypes.c_long, _P]),
+    "d8_rotary_table": (_I, [_P, _I, _I, _D, _D, _D, _D, _P]),
+    "d8_head_norm_rotary": (_I, [_I] + [_P, _L, _I, _P, _P, _L] * 2 + [_I, _I, _I, _F, _P, _P, _I, _I, _I, _P]),
+    "d8_head_norm_rotary_grad_scratch_bytes": (_Z, [_I] * 5),
+    "d8_head_norm_rotary_grad": (_I, [_I] + [_P, _L, _I, _P, _P, _L, _P, _L, _P] * 2 + [_I, _I, _I, _F, _P, _P, _I, _I, _I, _I, _P, _Z, _P]),
+    "d8_attention_scratch_bytes": (_Z, [_I] * 9),
+    "d8_attention": (_I, [_I] + [_P, _L] * 4 + [_P, _P, _P] + [_I] * 6 + [_F, _I, _P, _Z, _P]),
+    "d8_attention_grad": (_I, [_I] + [_P, _L] * 4 + [_P] + [_P, _L] * 4 + [_P, _P] + [_I] * 6 + [_F, _I, _I, _P, _Z, _P]),
+    "d8_matmul_gated_scratch_bytes": (_Z, [_I] * 5),
+    "d8_matmul_gated": (_I, [_I, _P, _I, _I, _P, _I, _I, _P, _P, _P, _Z, _P]),
+    "d8_matmul_gated_grad": (_I, [_I, _P, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _P, _Z, _P]),
     "d8_gemm_phase_record": (_I, [_P, _Z]),
     "d8_mfma_stream_out_bytes": (_Z, []),
     "d8_mfma_stream": (_I, [_I, _P, _Z, _P, _I, ctypes.POINTER(ctypes.c_double), _P]),

@@ -626,3 +626,141 @@ def avgpool2d_grad(xshape, dy, FH, FW, covered=False, sy=1, sx=1, dx=None, overw
     fn = lib.d8_avgpool2d_grad_overwrite if overwrite else lib.d8_avgpool2d_grad
     check(fn(dt, b.ptr, c.ptr, B, IH, IW, C, FH, FW, int(covered), sy, sx, None))
     return b.numpy()
+
+
+# ---- a transformer layer: head norm with rotation, attention, gated product ------------------------------------------
+class _Rows:
+    """(tokens, heads, dim) on the device with `pad` elements between two rows, which hold NaN; read back checks them"""
+
+    def __init__(self, a, pad=0):
+        a = np.ascontiguousarray(a)
+        self.shape, width = a.shape, int(np.prod(a.shape[1:]))
+        self.ld, self.width = width + pad, width
+        rows = np.full((max(a.shape[0], 1), self.ld), np.nan, a.dtype)
+        rows[: a.shape[0], :width] = a.reshape(a.shape[0], width)
+        self.d = DeviceArray.from_numpy(rows)
+
+    @property
+    def args(self):
+        return self.d.ptr, self.ld
+
+    def numpy(self):
+        rows = self.d.numpy()
+        if not np.isnan(rows[:, self.width:]).all():
+            raise AssertionError("written between two rows")
+        return rows[: self.shape[0], : self.width].reshape(self.shape).copy()
+
+
+def _ints(a):
+    return None if a is None else DeviceArray.from_numpy(np.ascontiguousarray(a, np.int32))
+
+
+def rotary_table(positions, rotary, base=10000.0, factor=1.0, keep_below=0.0, slow_above=0.0):
+    """(positions, rotary / 2, 2) cosines and sines"""
+    lib = capi.init()
+    t = DeviceArray((positions, rotary // 2, 2), np.float32)
+    check(lib.d8_rotary_table(t.ptr, positions, rotary, base, factor, keep_below, slow_above, None))
+    return t.numpy()
+
+
+def _side(x, weight, *more):
+    return [None if a is None else DeviceArray.from_numpy(np.ascontiguousarray(a, x.dtype)) for a in (weight,) + more]
+
+
+def head_norm_rotary(q, k, q_weight=None, k_weight=None, table=None, positions=None, rotary=0, interleaved=False, norm=True, epsilon=1e-6,
+                     pad=0, in_place=False, stream=None):
+    """normed and turned (q, k), both (tokens, heads, dim)"""
+    lib = capi.init()
+    dt = _same_dtype(q, k)
+    T, H, D = q.shape
+    t, p = None if table is None else DeviceArray.from_numpy(np.ascontiguousarray(table, np.float32)), _ints(positions)
+    qi, ki, (wq,), (wk,) = _Rows(q, pad), _Rows(k, pad), _side(q, q_weight), _side(q, k_weight)
+    qo, ko = (qi, ki) if in_place else (_Rows(np.zeros_like(q), pad), _Rows(np.zeros_like(k), pad))
+    check(lib.d8_head_norm_rotary(dt, *qi.args, H, wq and wq.ptr, *qo.args, *ki.args, k.shape[1], wk and wk.ptr, *ko.args, T, D, int(norm), epsilon,
+                                  p and p.ptr, t and t.ptr, 0 if table is None else table.shape[0], rotary, int(interleaved), stream))
+    capi.sync(stream)
+    return qo.numpy(), ko.numpy()
+
+
+def head_norm_rotary_grad(q, k, dq_out, dk_out, q_weight=None, k_weight=None, table=None, positions=None, rotary=0, interleaved=False, norm=True,
+                          epsilon=1e-6, pad=0, into=None):
+    """(dq, dk, dq_weight, dk_weight), added to `into` (the four) if given; a weight's gradient is wanted where the weight is given"""
+    lib = capi.init()
+    dt = _same_dtype(q, k, dq_out, dk_out)
+    T, H, D = q.shape
+    t, p = None if table is None else DeviceArray.from_numpy(np.ascontiguousarray(table, np.float32)), _ints(positions)
+    old = into or (np.full_like(q, np.nan), np.full_like(k, np.nan), np.full(D, np.nan), np.full(D, np.nan))
+    (wq, dwq), (wk, dwk) = _side(q, q_weight, None if q_weight is None else old[2]), _side(q, k_weight, None if k_weight is None else old[3])
+    qi, ki, gq, gk, dq, dk = (_Rows(a, pad) for a in (q, k, dq_out, dk_out, old[0], old[1]))
+    nb = lib.d8_head_norm_rotary_grad_scratch_bytes(dt, T, H, k.shape[1], D)
+    ws = _scratch(nb)
+    check(lib.d8_head_norm_rotary_grad(dt, *qi.args, H, wq and wq.ptr, *gq.args, *dq.args, dwq and dwq.ptr, *ki.args, k.shape[1], wk and wk.ptr, *gk.args,
+                                       *dk.args, dwk and dwk.ptr, T, D, int(norm), epsilon, p and p.ptr, t and t.ptr,
+                                       0 if table is None else table.shape[0], rotary, int(interleaved), 0 if into else 3, ws.ptr, nb, None))
+    return dq.numpy(), dk.numpy(), dwq and dwq.numpy(), dwk and dwk.numpy()
+
+
+def _attention_sizes(q, k, q_starts):
+    return len(q_starts) - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]
+
+
+def attention(q, k, v, q_starts, k_starts, scale, causal=True, pad=0, o=None, stream=None):
+    """(o, lse) of packed sequences: q (queries, heads, dim), k and v (keys, kv_heads, dim); o: what the output holds before"""
+    lib = capi.init()
+    dt = _same_dtype(q, k, v)
+    n = _attention_sizes(q, k, q_starts)
+    qi, ki, vi, oo = (_Rows(a, pad) for a in (q, k, v, np.zeros_like(q) if o is None else o))
+    lse = DeviceArray.from_numpy(np.full((q.shape[1], q.shape[0]), np.nan, np.float32))
+    qs, ks = _ints(q_starts), _ints(k_starts)
+    nb = lib.d8_attention_scratch_bytes(dt, 0, *n, int(causal))
+    ws = _scratch(nb)
+    check(lib.d8_attention(dt, *qi.args, *ki.args, *vi.args, *oo.args, lse.ptr, qs.ptr, ks.ptr, *n, scale, int(causal), ws.ptr, nb, stream))
+    capi.sync(stream)
+    return oo.numpy(), lse.numpy()
+
+
+def attention_grad(q, k, v, o, lse, do, q_starts, k_starts, scale, causal=True, pad=0, into=None):
+    """(dq, dk, dv), added to `into` (the three) if given"""
+    lib = capi.init()
+    dt = _same_dtype(q, k, v, o, do)
+    n = _attention_sizes(q, k, q_starts)
+    rows = [_Rows(a, pad) for a in (q, k, v, o, do)]
+    out = [_Rows(a, pad) for a in (into or (np.full_like(q, np.nan), np.full_like(k, np.nan), np.full_like(v, np.nan)))]
+    ls, qs, ks = DeviceArray.from_numpy(np.ascontiguousarray(lse, np.float32)), _ints(q_starts), _ints(k_starts)
+    nb = lib.d8_attention_scratch_bytes(dt, 1, *n, int(causal))
+    ws = _scratch(nb)
+    check(lib.d8_attention_grad(dt, *rows[0].args, *rows[1].args, *rows[2].args, *rows[3].args, ls.ptr, *rows[4].args, *out[0].args, *out[1].args, *out[2].args,
+                                qs.ptr, ks.ptr, *n, scale, int(causal), 0 if into else 7, ws.ptr, nb, None))
+    return tuple(a.numpy() for a in out)
+
+
+GATES = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+
+def matmul_gated(x, w, act="silu", keep=True, stream=None):
+    """(h, pre) of x (rows, inner) and w (inner, 2 cols); pre is None unless kept"""
+    lib = capi.init()
+    x, w = np.ascontiguousarray(x), np.ascontiguousarray(w)
+    dt = _same_dtype(x, w)
+    (rows, inner), cols = x.shape, w.shape[1] // 2
+    dx_, dw_, h = DeviceArray.from_numpy(x), DeviceArray.from_numpy(w), DeviceArray.from_numpy(np.full((rows, cols), np.nan, x.dtype))
+    pre = DeviceArray.from_numpy(np.full((rows, 2 * cols), np.nan, x.dtype)) if keep else None
+    nb = lib.d8_matmul_gated_scratch_bytes(dt, 0, rows, inner, cols)
+    ws = _scratch(nb)
+    check(lib.d8_matmul_gated(dt, dx_.ptr, rows, inner, dw_.ptr, cols, GATES[act], pre and pre.ptr, h.ptr, ws.ptr, nb, stream))
+    capi.sync(stream)
+    return h.numpy(), pre and pre.numpy()
+
+
+def matmul_gated_grad(x, w, pre, dh, act="silu", into=None):
+    """(dx, dw), added to `into` (the two) if given"""
+    lib = capi.init()
+    x, w, pre, dh = (np.ascontiguousarray(a) for a in (x, w, pre, dh))
+    dt = _same_dtype(x, w, pre, dh)
+    (rows, inner), cols = x.shape, w.shape[1] // 2
+    xi, wi, pi, gi = (DeviceArray.from_numpy(a) for a in (x, w, pre, dh))
+    dx_, dw_ = (DeviceArray.from_numpy(np.ascontiguousarray(a)) for a in (into or (np.full_like(x, np.nan), np.full_like(w, np.nan))))
+    nb = lib.d8_matmul_gated_scratch_bytes(dt, 1, rows, inner, cols)
+    ws = _scratch(nb)
+    check(lib.d8_matmul_gated_grad(dt, xi.ptr, dx_.ptr, rows, inner, wi.ptr, dw_.ptr, cols, GATES[act], pi.ptr, gi.ptr, 0 if into else 3, ws.ptr, nb, None))
+    return dx_.numpy(), dw_.numpy()

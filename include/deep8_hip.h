@@ -441,6 +441,69 @@ int d8_maxpool2d_grad_overwrite(int dtype, const void *x, void *dx, const void *
 int d8_avgpool2d_grad_overwrite(int dtype, void *dx, const void *dy, int B, int IH, int IW, int C,
                                 int FH, int FW, int covered, int sy, int sx, void *stream);
 
+/* ---- a transformer layer --------------------------------------------------------------------------
+ * What such a layer needs besides MatrixMultiply and Add; no counterpart in the reference.  Float16 and Float32.  Rows
+ * (tokens) of several heads lie `ld` elements apart, the heads of a row next to each other, so that queries, keys and values
+ * may be parts of one product's rows.  Gradients are added to what their destination holds unless their bit of `overwrite` is set.
+ * Sums, statistics of norms and softmax are fp32; results are rounded once.
+ *
+ * d8_rotary_table        table[p][i] = (cos, sin)(p f_i) in fp32, i < rotary / 2, positions p < positions, f_i = base^(-2 i / rotary);
+ *                        angles in fp64.  For contexts longer than a model was trained on, factor > 1 slows the rotation down:
+ *                        every f_i is divided by it when slow_above is 0; else those with a wave length (2 pi / f_i positions)
+ *                        of at least slow_above, those of at most keep_below stay, and between the two the share that stays
+ *                        goes linearly with 1 / wave length.
+ * d8_head_norm_rotary    each head x of `dim` elements of queries and keys becomes n = x / sqrt(mean(x^2) + epsilon) * weight (norm != 0;
+ *                        weight: dim elements or NULL for ones), and the first `rotary` elements of n are turned by the angles of
+ *                        the token's position: the pairs (i, i + rotary / 2), or with interleaved != 0 the pairs (2 i, 2 i + 1).
+ *                        positions[tokens] (NULL: a token's row); a position outside the table counts as its nearest.
+ *                        Outputs may be the inputs.  q_heads or k_heads may be 0.  dim <= 2048.
+ * d8_head_norm_rotary_grad  from q, k and the gradients of the outputs (dq_out, dk_out) those of q, k (bit 0 of overwrite) and of
+ *                        the weights (bit 1; NULL: not wanted).  dq may be dq_out, dk may be dk_out.
+ * d8_attention           sequence s has queries q_starts[s] .. q_starts[s + 1] - 1 and keys k_starts[s] .. k_starts[s + 1] - 1 (rows of
+ *                        q and k; arrays of sequences + 1 on the device; what reaches beyond the tensors is cut).  A query sees its
+ *                        sequence's keys, causal != 0: query t of nq sees the keys up to t + nk - nq, so the last query sees them
+ *                        all.  o = softmax(scale q k^T) v, head i with the keys and values of head i / (heads / kv_heads).
+ *                        lse[heads][q_tokens] (may be NULL): the logarithm of the sum of exp(score).  A query that sees nothing
+ *                        gets o = 0 and lse = -infinity.  Rows of no sequence are left alone.  dim <= 256.  The same
+ *                        call serves training (q_starts = k_starts), a prompt's next part and a step of decoding (one query a sequence).
+ * d8_attention_grad      the gradients of q (bit 0 of overwrite), k (bit 1) and v (bit 2) from those of o (dout), with o and lse as the
+ *                        forward call left them.  The same bits every time.
+ *     scratch: d8_attention_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.
+ * d8_matmul_gated        h = act(g) * u with (g | u) = x w: w is [inner][2 * cols], its first `cols` columns the gate's.  act: D8_GATE_*.
+ *                        pre (may be NULL): [rows][2 * cols], receives g and u for the gradients.
+ * d8_matmul_gated_grad   dx (bit 0 of overwrite) and dw (bit 1) from dh, with pre as the forward call left it.
+ *     scratch: d8_matmul_gated_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.                                */
+#define D8_GATE_SILU    0 /* a sigmoid(a)                 */
+#define D8_GATE_GELU    1 /* a (1 + erf(a / sqrt 2)) / 2  */
+#define D8_GATE_RELU    2
+#define D8_GATE_SIGMOID 3
+int d8_rotary_table(float *table, int positions, int rotary, double base, double factor, double keep_below, double slow_above,
+                    void *stream);
+int d8_head_norm_rotary(int dtype, const void *q, long ldq, int q_heads, const void *q_weight, void *q_out, long ldq_out,
+                        const void *k, long ldk, int k_heads, const void *k_weight, void *k_out, long ldk_out,
+                        int tokens, int dim, int norm, float epsilon, const int *positions, const float *table,
+                        int table_positions, int rotary, int interleaved, void *stream);
+size_t d8_head_norm_rotary_grad_scratch_bytes(int dtype, int tokens, int q_heads, int k_heads, int dim);
+int d8_head_norm_rotary_grad(int dtype, const void *q, long ldq, int q_heads, const void *q_weight, const void *dq_out, long lddq_out,
+                             void *dq, long lddq, void *dq_weight, const void *k, long ldk, int k_heads, const void *k_weight,
+                             const void *dk_out, long lddk_out, void *dk, long lddk, void *dk_weight, int tokens, int dim, int norm,
+                             float epsilon, const int *positions, const float *table, int table_positions, int rotary,
+                             int interleaved, int overwrite, void *scratch, size_t scratch_bytes, void *stream);
+size_t d8_attention_scratch_bytes(int dtype, int which, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim,
+                                  int causal);
+int d8_attention(int dtype, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, void *o, long ldo, float *lse,
+                 const int *q_starts, const int *k_starts, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim,
+                 float scale, int causal, void *scratch, size_t scratch_bytes, void *stream);
+int d8_attention_grad(int dtype, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, const void *o, long ldo,
+                      const float *lse, const void *dout, long lddo, void *dq, long lddq, void *dk, long lddk, void *dv, long lddv,
+                      const int *q_starts, const int *k_starts, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads,
+                      int dim, float scale, int causal, int overwrite, void *scratch, size_t scratch_bytes, void *stream);
+size_t d8_matmul_gated_scratch_bytes(int dtype, int which, int rows, int inner, int cols);
+int d8_matmul_gated(int dtype, const void *x, int rows, int inner, const void *w, int cols, int act, void *pre, void *h,
+                    void *scratch, size_t scratch_bytes, void *stream);
+int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner, const void *w, void *dw, int cols, int act,
+                         const void *pre, const void *dh, int overwrite, void *scratch, size_t scratch_bytes, void *stream);
+
 /* ---- measurement aid (no counterpart in the reference) ---------------------------------------
  * d8_mfma_stream issues the GEMM kernels' MFMA instruction for `dtype` (D8_FLOAT16, D8_FLOAT32 or
  * D8_FLOAT64) back to back on operands taken from `operands` (any device buffer; 16-byte aligned)
