@@ -82,6 +82,8 @@ __device__ __forceinline__ bool locate(const Args &a, int id, Span &span, int &s
             s = __builtin_amdgcn_readfirstlane(s);
             item = __builtin_amdgcn_readfirstlane(item);
             span = span_of(a, s);
+            span.q0 = __builtin_amdgcn_readfirstlane(span.q0), span.nq = __builtin_amdgcn_readfirstlane(span.nq);
+            span.k0 = __builtin_amdgcn_readfirstlane(span.k0), span.nk = __builtin_amdgcn_readfirstlane(span.nk);
             return true;
         }
         before += __shfl(upto, 63);
@@ -181,6 +183,135 @@ template <class T>
 __device__ __forceinline__ typename Type<T>::frag read_rows(const char *tile, int pitch, int u, int lane) {
     return *(const typename Type<T>::frag *)(tile + (lane & 31) * pitch + u * 32 + (lane >> 5) * 16);
 }
+
+// ---- tiles that go from memory straight into LDS ----------------------------------------------------------------------
+// A row takes PB bytes (a power of two) in LDS, its 16-byte piece c at position c ^ swizzle(row): the lanes of a load land 16 bytes
+// apart, so rows cannot be padded, and the exclusive-or keeps what a read's lanes want in different banks, both along rows (eight
+// lanes a cycle, one piece of eight rows) and along columns (four rows of two pieces each, or a row's neighbours).
+template <int PB>
+__device__ __forceinline__ int swizzle(int row) {
+    constexpr int PER_SPAN = PB >= 256 ? 1 : 256 / PB, PIECES = PB / 16 < 16 ? PB / 16 : 16;
+    return ((row / PER_SPAN) & (PIECES / 2 - 1)) << 1;
+}
+
+template <class T, int DP>
+constexpr int row_bytes() {  // the power of two that holds DP elements
+    int b = 64;
+    while (b < DP * (int)sizeof(T)) b *= 2;
+    return b;
+}
+
+// read_rows and read_cols of such a tile, whose address is a multiple of PB; r0 a multiple of 16, c0 of 32
+template <class T, int PB>
+__device__ __forceinline__ typename Type<T>::frag rows_frag(const char *tile, int r0, int u, int lane) {
+    const int row = r0 + (lane & 31);
+    return *(const typename Type<T>::frag *)(tile + row * PB + (((2 * u + (lane >> 5)) ^ swizzle<PB>(row)) << 4));
+}
+template <class T, int PB>
+__device__ __forceinline__ typename Type<T>::frag cols_frag(const char *tile, int r0, int c0, int lane) {
+    typename Type<T>::frag r;
+    if constexpr (sizeof(T) == 2) {
+        const int i = lane & 15, j = lane >> 4, row = r0 + 4 * (j >> 1) + (i >> 2), at = c0 * 2 + 32 * (j & 1) + 8 * (i & 3);
+        const char *p = tile + row * PB + ((((at >> 4) ^ swizzle<PB>(row)) << 4) | (at & 15));
+        const tr_f16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16(ATTN_LDS(tr_f16x4, p));
+        const tr_f16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16(ATTN_LDS(tr_f16x4, p + 8 * PB));  // (row + 8 has row's swizzle)
+        r = __builtin_bit_cast(typename Type<T>::frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+        const int at = (c0 + (lane & 31)) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = r0 + 4 * (lane >> 5) + e;
+            r[e] = *(const float *)(tile + row * PB + ((((at >> 4) ^ swizzle<PB>(row)) << 4) | (at & 15)));
+        }
+    }
+    return r;
+}
+
+typedef unsigned desc_t __attribute__((ext_vector_type(4)));
+
+// s_waitcnt: at most n vector-memory instructions outstanding; all LDS reads have arrived
+#define ATTN_VMCNT(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (((n) >> 4) << 14) | 0x0f70)
+__device__ __forceinline__ void lds_reads_done() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    asm volatile("" ::: "memory");
+}
+
+// One 16-byte piece a lane from memory into LDS at `target` + 16 * lane.  asm, so that the compiler does not hold every later LDS read
+// until it has landed; the kernels wait by count.  Beyond the descriptor's bytes zeros are written.  (s_nop 4: the
+// hardware does not interlock scalars that a vector instruction has just written, nor m0.)
+__device__ __forceinline__ void load_to_lds(const desc_t &desc, unsigned voffset, unsigned target) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(target), "v"(voffset), "s"(desc) : "memory");
+}
+
+// Rows of one tensor on their way into tiles: `first` is the first row's head, rows are `ld` elements apart.
+template <class T, int PB>
+struct TileLoader {
+    unsigned voff;  // the lane's row and piece within 1 KB of LDS, as an offset from the tile's first row, before the swizzle
+    unsigned row_stride;
+    int lane_row, lane_pos, pieces;
+    static constexpr int ROWS = PB >= 1024 ? 1 : 1024 / PB;  // rows of one load
+
+    __device__ __forceinline__ void init(long ld, int dim, int lane) {
+        static_assert(PB <= 1024, "a row is one load at most");
+        lane_row = lane / (PB / 16), lane_pos = lane % (PB / 16);
+        row_stride = (unsigned)(ld * sizeof(T));
+        voff = lane_row * row_stride;
+        pieces = dim / Type<T>::V;
+    }
+    // descriptor over the head's part of `rows` rows from `first` on
+    static __device__ __forceinline__ desc_t desc(const T *first, int rows, long ld, int dim) {
+        const unsigned long p = (unsigned long)first;
+        const unsigned bytes = rows > 0 ? (unsigned)((rows - 1) * (unsigned)(ld * sizeof(T)) + dim * (int)sizeof(T)) : 0u;
+        return desc_t{(unsigned)__builtin_amdgcn_readfirstlane((int)p), (unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32)) & 0xffffu,
+                      (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+    }
+    // load t of a tile: rows t * ROWS .. of it, to LDS byte address `tile`
+    __device__ __forceinline__ void load(const desc_t &d, int t, unsigned tile) const {
+        const int piece = lane_pos ^ swizzle<PB>(t * ROWS + lane_row);
+        const unsigned at = piece < pieces ? voff + t * ROWS * row_stride + piece * 16 : 0x80000000u;
+        load_to_lds(d, at, __builtin_amdgcn_readfirstlane(tile + t * 1024));
+    }
+};
+
+__device__ __forceinline__ unsigned lds_address(const void *p) { return (unsigned)(size_t)ATTN_LDS(const char, p); }
+
+// ---- the running softmax of a lane's row ---------------------------------------------------------------------------------
+// Scores times c (log2 e times the scale, positive) enter as powers of two relative to `base`, which follows their maximum only when that has
+// grown by more than 8: sums and outputs are then up to 2^8 larger than they would be, which fp32 (and a half up to 256) does
+// not notice, and most tiles need no pass over the accumulators.
+struct Softmax {
+    float base, sum;
+    __device__ __forceinline__ void init() { base = -INFINITY, sum = 0.f; }
+    // scores -> powers; returns what the accumulators have to be multiplied by, 1 for every lane if nothing changes
+    template <int N>
+    __device__ __forceinline__ bool step(f32x16 (&s)[N], float c, float &keep) {
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[b][e]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * c;
+        const bool moved = __ballot(top > base + 8.f) != 0;
+        keep = 1.f;
+        if (moved) {
+            const float next = fmaxf(base, top);
+            keep = next == base ? 1.f : __builtin_amdgcn_exp2f(base - next);
+            sum *= keep;
+            base = next;
+        }
+        const float at = base == -INFINITY ? 0.f : base;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], c, -at));
+                part[e & 3] += s[b][e];
+            }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        return moved;
+    }
+};
 
 int check(const Args &a, int dtype, const char *name);
 bool in_pieces(int dtype, int dim, std::initializer_list<const void *> p, std::initializer_list<long> ld);

@@ -17,7 +17,7 @@ namespace {
 enum { ROWS = 128, KEYS = 32 };
 
 template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_kernel(Args a) {
+__global__ __launch_bounds__(256) void attention_any_kernel(Args a) {
     typedef Type<T> M;
     typedef typename M::frag frag;
     constexpr int PITCH = pitch_of<DP, T>(), UNITS = DP / M::STEP, PIECES = DP / M::V;
@@ -103,16 +103,345 @@ __global__ __launch_bounds__(256) void attention_kernel(Args a) {
     if (a.lse && h == 0) a.lse[(long)head * a.q_tokens + sp.q0 + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
+// The lane's row of q as fragments, negated where the scale is negative (the softmax below takes |scale|).
+template <class T, int DP>
+__device__ __forceinline__ void load_query(const Args &a, const T *q, bool there, int h, typename Type<T>::frag (&qf)[DP / Type<T>::STEP]) {
+#pragma unroll
+    for (int u = 0; u < DP / Type<T>::STEP; ++u) {
+        qf[u] = load_piece<T>(q, u * Type<T>::STEP + h * Type<T>::V, a.dim, there, 1);
+        if (a.scale < 0.f) qf[u] = -qf[u];
+    }
+}
+// (a scale of zero as one so small that no score is seen: infinite hidden scores times zero would be no number)
+__device__ __forceinline__ float exponent_scale(const Args &a) { return fmaxf(fabsf(a.scale) * LOG2E, 1e-30f); }
+
+// Large outputs.  128 rows a workgroup, keys in tiles of 64 (32 where a row takes more than 256 bytes) that go from memory straight into one of
+// two stages of LDS, the next tile's while this one is worked on; one barrier a tile.  Two workgroups a compute unit, so that
+// one's products run under the other's exponentials.
+template <class T, int DP>
+__global__ __launch_bounds__(256, (DP * (int)sizeof(T) <= 256 ? 2 : 1)) void attention_rows_kernel(Args a) {
+    typedef Type<T> M;
+    typedef typename M::frag frag;
+    constexpr int PB = row_bytes<T, DP>(), KB = PB <= 256 ? 64 : 32, NB = KB / 32, TILE = KB * PB, LOADS = TILE / 1024 / 4;
+    static_assert(LOADS >= 1, "every wave has a share of a tile");
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int hk = blockIdx.x % a.kv_heads;
+    Span sp;
+    int seq, tile;
+    auto tiles_of = [&](const Span &s) { return (int)(((long)s.nq * a.group + ROWS - 1) / ROWS); };
+    if (!locate(a, blockIdx.x / a.kv_heads, sp, seq, tile, tiles_of)) return;
+    const int group = a.group, rows = sp.nq * group;
+    tile = tiles_of(sp) - 1 - tile;  // the rows that see most keys first
+    const int r = tile * ROWS + wave * 32 + (lane & 31);
+    const bool there = r < rows;
+    const int t = (there ? r : rows - 1) / group, head = hk * group + (there ? r - t * group : 0);
+    frag qf[DP / M::STEP];
+    load_query<T, DP>(a, (const T *)a.q + (long)(sp.q0 + t) * a.ldq + (long)head * a.dim, there, h, qf);
+    const int back = sp.nk - sp.nq;
+    const int last = a.causal ? min(sp.nk - 1, t + back) : sp.nk - 1;  // last key that the lane's row sees
+    const int end = a.causal ? min(sp.nk, (min(rows, (tile + 1) * ROWS) - 1) / group + back + 1) : sp.nk;
+    // what all rows of the wave see, and the end of what one of them sees
+    const int wave_all = __builtin_amdgcn_readfirstlane(__shfl(last, 0)), wave_end = __builtin_amdgcn_readfirstlane(__shfl(last, 31)) + 1;
+    const float c = exponent_scale(a);
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][e] = 0.f;
+    Softmax soft;
+    soft.init();
+    const T *k = (const T *)a.k + (long)sp.k0 * a.ldk + (long)hk * a.dim, *v = (const T *)a.v + (long)sp.k0 * a.ldv + (long)hk * a.dim;
+    TileLoader<T, PB> lk, lv;
+    lk.init(a.ldk, a.dim, lane), lv.init(a.ldv, a.dim, lane);
+    const unsigned lds0 = lds_address(lds);
+    auto fetch = [&](int j0, int stage) {
+        const desc_t dk = lk.desc(k + (long)j0 * a.ldk, min(KB, sp.nk - j0), a.ldk, a.dim), dv = lv.desc(v + (long)j0 * a.ldv, min(KB, sp.nk - j0), a.ldv, a.dim);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) lk.load(dk, wave * LOADS + i, lds0 + stage * 2 * TILE);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) lv.load(dv, wave * LOADS + i, lds0 + stage * 2 * TILE + TILE);
+    };
+    if (end > 0) fetch(0, 0);
+    for (int j0 = 0, stage = 0; j0 < end; j0 += KB, stage ^= 1) {
+        // this tile has landed, and every wave is through with the other stage
+        ATTN_VMCNT(0);
+        lds_reads_done();
+        __syncthreads();
+        if (j0 + KB < end) fetch(j0 + KB, stage ^ 1);
+        if (j0 >= wave_end) continue;
+        const char *tk = lds + stage * 2 * TILE, *tv = tk + TILE;
+        f32x16 s[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
+#pragma unroll
+        for (int u = 0; u < DP / M::STEP; ++u)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) M::mma(s[b], rows_frag<T, PB>(tk, b * 32, u, lane), qf[u]);
+        if (j0 + KB - 1 > wave_all) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[b][e] = j0 + b * 32 + 8 * (e >> 2) + 4 * h + (e & 3) <= last ? s[b][e] : -INFINITY;
+        }
+        float keep;
+        if (soft.step<NB>(s, c, keep)) {
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[b][e] *= keep;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int u = 0; u < 32 / M::STEP; ++u) {
+                const frag p = M::pack(s[b], u);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) M::mma(acc[d], cols_frag<T, PB>(tv, b * 32 + u * M::STEP, d * 32, lane), p);
+            }
+    }
+    const float sum = soft.sum + __shfl_xor(soft.sum, 32);
+    if (!there) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T *o = (T *)a.o + (long)(sp.q0 + t) * a.ldo + (long)head * a.dim;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = d * 32 + 2 * e + 4 * h;
+            T out[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] = (T)(acc[d][e + i] * inv);
+            if (at < a.dim) __builtin_memcpy(__builtin_assume_aligned(o + at, 4 * sizeof(T)), out, 4 * sizeof(T));
+        }
+    if (a.lse && h == 0) a.lse[(long)head * a.q_tokens + sp.q0 + t] = sum == 0.f ? -INFINITY : (soft.base + log2f(sum)) * LN2;
+}
+
+// Few rows: 32 a workgroup, whose waves have the same rows and take every WAVES-th tile of 32 keys, each with its own LDS and no
+// barrier: the keys and values of a tile are asked for again as soon as the last read of their place has been answered.  The keys of
+// a sequence are cut into chunks of one length for the whole call, found from the lengths on the device, so that the
+// pieces of work are alike whatever the lengths; a row's chunks are joined by a second launch (their unnormalised outputs with
+// their maxima and sums).
+struct Cut {
+    int chunk;  // keys
+    __device__ __forceinline__ int tiles(const Args &a, const Span &s) const { return (int)(((long)s.nq * a.group + 31) / 32); }
+    __device__ __forceinline__ int chunks(const Span &s) const { return max(1, (int)(((long)s.nk + chunk - 1) / chunk)); }
+    __device__ __forceinline__ void init(const Args &a, int grain) {
+        chunk = 1 << 30;
+        if (!a.pieces) return;
+        const Cut &self = *this;
+        const long work = total_of(a, [&](const Span &s) { return (long)self.tiles(a, s) * s.nk; });
+        const long want = (work + a.pieces - 1) / a.pieces;
+        chunk = __builtin_amdgcn_readfirstlane((int)min((long)(1 << 30), (max(want, 1L) + grain - 1) / grain * grain));
+    }
+    // keys that some row of the tile sees
+    __device__ __forceinline__ int end(const Args &a, const Span &s, int tile) const {
+        const int rows = s.nq * a.group;
+        return a.causal ? max(0, min(s.nk, (min(rows, (tile + 1) * 32) - 1) / a.group + s.nk - s.nq + 1)) : s.nk;
+    }
+};
+enum { CHUNK_GRAIN = 256 };
+
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_keys_kernel(Args a) {
+    typedef Type<T> M;
+    typedef typename M::frag frag;
+    constexpr int PB = row_bytes<T, DP>(), TILE = 32 * PB, LOADS = TILE / 1024, OUT = DP + 4;
+    constexpr int STAGES = WAVES * 2 * TILE, JOIN = WAVES * 32 * OUT * 4;
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES > JOIN ? STAGES : JOIN];
+    __shared__ float wave_base[WAVES][32], wave_sum[WAVES][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    Cut cut;
+    cut.init(a, CHUNK_GRAIN);
+    Span sp;
+    int seq, item;
+    if (!locate(a, unit, sp, seq, item, [&](const Span &s) { return cut.tiles(a, s) * cut.chunks(s); })) return;
+    const int chunks = cut.chunks(sp), tile = item / chunks, begin = (item - tile * chunks) * cut.chunk;
+    const int group = a.group, rows = sp.nq * group, all = cut.end(a, sp, tile), end = min(all, begin + cut.chunk);
+    if (begin > 0 && begin >= all) return;  // (the first chunk is there even if its rows see nothing)
+    const bool whole = all <= cut.chunk;
+    const int r = tile * 32 + (lane & 31);
+    const bool there = r < rows;
+    const int t = (there ? r : rows - 1) / group, head = hk * group + (there ? r - t * group : 0);
+    frag qf[DP / M::STEP];
+    load_query<T, DP>(a, (const T *)a.q + (long)(sp.q0 + t) * a.ldq + (long)head * a.dim, there, h, qf);
+    const int last = a.causal ? min(sp.nk - 1, t + sp.nk - sp.nq) : sp.nk - 1;
+    const int wave_all = __builtin_amdgcn_readfirstlane(__shfl(last, 0));
+    const float c = exponent_scale(a);
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][e] = 0.f;
+    Softmax soft;
+    soft.init();
+    const T *k = (const T *)a.k + (long)sp.k0 * a.ldk + (long)hk * a.dim, *v = (const T *)a.v + (long)sp.k0 * a.ldv + (long)hk * a.dim;
+    TileLoader<T, PB> lk, lv;
+    lk.init(a.ldk, a.dim, lane), lv.init(a.ldv, a.dim, lane);
+    const char *tk = lds + wave * 2 * TILE, *tv = tk + TILE;
+    const unsigned at_k = lds_address(lds) + wave * 2 * TILE, at_v = at_k + TILE;
+    auto fetch = [&](const TileLoader<T, PB> &l, const T *x, long ld, int j, unsigned at) {
+        const desc_t d = l.desc(x + (long)j * ld, min(32, sp.nk - j), ld, a.dim);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) l.load(d, i, at);
+    };
+    int j = begin + wave * 32;
+    if (j < end) fetch(lk, k, a.ldk, j, at_k), fetch(lv, v, a.ldv, j, at_v);
+    for (; j < end; j += WAVES * 32) {
+        const bool more = j + WAVES * 32 < end;
+        ATTN_VMCNT(LOADS);  // the keys have landed, the values may be on their way
+        asm volatile("" ::: "memory");
+        f32x16 s[1];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[0][e] = 0.f;
+#pragma unroll
+        for (int u = 0; u < DP / M::STEP; ++u) M::mma(s[0], rows_frag<T, PB>(tk, 0, u, lane), qf[u]);
+        lds_reads_done();
+        if (more) fetch(lk, k, a.ldk, j + WAVES * 32, at_k);
+        if (j + 31 > wave_all) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[0][e] = j + 8 * (e >> 2) + 4 * h + (e & 3) <= last ? s[0][e] : -INFINITY;
+        }
+        float keep;
+        if (soft.step<1>(s, c, keep)) {
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[b][e] *= keep;
+        }
+        if (more) ATTN_VMCNT(LOADS);
+        else ATTN_VMCNT(0);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < 32 / M::STEP; ++u) {
+            const frag p = M::pack(s[0], u);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) M::mma(acc[d], cols_frag<T, PB>(tv, u * M::STEP, d * 32, lane), p);
+        }
+        lds_reads_done();
+        if (more) fetch(lv, v, a.ldv, j + WAVES * 32, at_v);
+    }
+    // the waves' results joined through LDS, a row's elements next to each other
+    __syncthreads();
+    float *mine = (float *)lds + (wave * 32 + (lane & 31)) * OUT;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *(f32x4 *)(mine + d * 32 + 2 * e + 4 * h) = f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+    const float sum = soft.sum + __shfl_xor(soft.sum, 32);
+    if (h == 0) wave_base[wave][lane] = soft.base, wave_sum[wave][lane] = sum;
+    __syncthreads();
+    const int n = min(32, rows - tile * 32);
+    for (int row = wave; row < n; row += WAVES) {
+        float base = wave_base[0][row], total = 0.f, by[WAVES];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) base = fmaxf(base, wave_base[w][row]);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            by[w] = wave_base[w][row] == base ? (base == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(wave_base[w][row] - base);
+            total += wave_sum[w][row] * by[w];
+        }
+        const int rt = (tile * 32 + row) / group, rh = hk * group + tile * 32 + row - rt * group;
+        const float inv = !whole ? 1.f : total == 0.f ? 0.f : 1.f / total;
+        const long slot = ((long)unit * a.kv_heads + hk) * 32 + row;
+        for (int d = lane; d < a.dim; d += 64) {
+            float x = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) x += ((const float *)lds)[(w * 32 + row) * OUT + d] * by[w];
+            if (whole) ((T *)a.o)[(long)(sp.q0 + rt) * a.ldo + (long)rh * a.dim + d] = (T)(x * inv);
+            else a.part[slot * a.dim + d] = x;
+        }
+        if (lane == 0) {
+            if (!whole) a.part_ml[slot * 2] = base, a.part_ml[slot * 2 + 1] = total;
+            else if (a.lse) a.lse[(long)rh * a.q_tokens + sp.q0 + rt] = total == 0.f ? -INFINITY : (base + log2f(total)) * LN2;
+        }
+    }
+}
+
+// the chunks of a tile's rows joined: a wave has a row at a time
 template <class T>
-int launch(const Args &a, hipStream_t stream) {
-    const dim3 grid((unsigned)a.tiles * a.kv_heads);
-    if (a.dim <= 32) hipLaunchKernelGGL((attention_kernel<T, 32>), grid, dim3(256), 0, stream, a);
-    else if (a.dim <= 64) hipLaunchKernelGGL((attention_kernel<T, 64>), grid, dim3(256), 0, stream, a);
-    else if (a.dim <= 128) hipLaunchKernelGGL((attention_kernel<T, 128>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attention_kernel<T, 256>), grid, dim3(256), 0, stream, a);
+__global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    Cut cut;
+    cut.init(a, CHUNK_GRAIN);
+    Span sp;
+    int seq, item;
+    if (!locate(a, unit, sp, seq, item, [&](const Span &s) { return cut.tiles(a, s) * cut.chunks(s); })) return;
+    const int chunks = cut.chunks(sp), tile = item / chunks, all = cut.end(a, sp, tile);
+    if (item != tile * chunks || all <= cut.chunk) return;
+    const int parts = (all + cut.chunk - 1) / cut.chunk, rows = sp.nq * a.group, n = min(32, rows - tile * 32);
+    const long first = ((long)unit * a.kv_heads + hk) * 32, step = (long)a.kv_heads * 32;
+    for (int row = wave; row < n; row += 4) {
+        const long slot = first + row;
+        float base = -INFINITY, total = 0.f;
+        for (int i = 0; i < parts; ++i) base = fmaxf(base, a.part_ml[(slot + i * step) * 2]);
+        const float at = base == -INFINITY ? 0.f : base;
+        for (int i = 0; i < parts; ++i) total += a.part_ml[(slot + i * step) * 2 + 1] * __builtin_amdgcn_exp2f(a.part_ml[(slot + i * step) * 2] - at);
+        const int rt = (tile * 32 + row) / a.group, rh = hk * a.group + tile * 32 + row - rt * a.group;
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        for (int d = lane; d < a.dim; d += 64) {
+            float x = 0.f;
+            for (int i = 0; i < parts; ++i) x += a.part[(slot + i * step) * a.dim + d] * __builtin_amdgcn_exp2f(a.part_ml[(slot + i * step) * 2] - at);
+            ((T *)a.o)[(long)(sp.q0 + rt) * a.ldo + (long)rh * a.dim + d] = (T)(x * inv);
+        }
+        if (lane == 0 && a.lse) a.lse[(long)rh * a.q_tokens + sp.q0 + rt] = total == 0.f ? -INFINITY : (base + log2f(total)) * LN2;
+    }
+}
+
+// How a forward call runs.
+enum Way { ANY, BY_ROWS, BY_KEYS };
+struct Plan {
+    Way way;
+    int tiles, pieces, units;
+};
+
+// Tensors that cannot be moved in 16-byte pieces: ANY.  128 rows a workgroup where that gives the chip two rounds of workgroups and
+// sequences are not shorter than half of it; else 32, and their keys in pieces while there are fewer workgroups than compute units need.
+Plan plan_of(bool vec, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads) {
+    Plan p;
+    const long rows = (long)q_tokens * (heads / kv_heads), cus = cu_count();
+    const long some = sequences < q_tokens ? sequences : q_tokens;
+    const long big = (rows + ROWS - 1) / ROWS, small = (rows + 31) / 32;
+    p.pieces = p.units = 0;
+    p.way = !vec ? ANY : big * kv_heads >= 2 * cus && rows >= some * (ROWS / 2) ? BY_ROWS : BY_KEYS;
+    p.tiles = (int)((p.way == BY_KEYS ? small : big) + sequences);
+    if (p.way == BY_KEYS) {
+        const long groups = (small > some ? small : some) * kv_heads;
+        if (groups < 2 * cus && k_tokens > CHUNK_GRAIN) p.pieces = (int)((4 * cus + kv_heads - 1) / kv_heads);
+        p.units = p.tiles + p.pieces;
+    }
+    return p;
+}
+
+template <class T, int DP>
+int launch_dim(const Args &a, const Plan &p, hipStream_t stream) {
+    constexpr int WAVES = row_bytes<T, DP>() > 512 ? 2 : 4;
+    if (p.way == ANY) hipLaunchKernelGGL((attention_any_kernel<T, DP>), dim3((unsigned)p.tiles * a.kv_heads), dim3(256), 0, stream, a);
+    else if (p.way == BY_ROWS) hipLaunchKernelGGL((attention_rows_kernel<T, DP>), dim3((unsigned)p.tiles * a.kv_heads), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attention_keys_kernel<T, DP, WAVES>), dim3((unsigned)p.units * a.kv_heads), dim3(WAVES * 64), 0, stream, a);
     D8_LAUNCH_CHECK();
     return 0;
 }
+
+template <class T>
+int launch(const Args &a, const Plan &p, hipStream_t stream) {
+    int rc;
+    if (a.dim <= 32) rc = launch_dim<T, 32>(a, p, stream);
+    else if (a.dim <= 64) rc = launch_dim<T, 64>(a, p, stream);
+    else if (a.dim <= 96) rc = launch_dim<T, 96>(a, p, stream);
+    else if (a.dim <= 128) rc = launch_dim<T, 128>(a, p, stream);
+    else rc = launch_dim<T, 256>(a, p, stream);
+    if (rc || !p.pieces) return rc;
+    hipLaunchKernelGGL(attention_join_kernel<T>, dim3((unsigned)p.units * a.kv_heads), dim3(256), 0, stream, a);
+    D8_LAUNCH_CHECK();
+    return 0;
+}
+
+size_t part_rows(const Plan &p, int kv_heads) { return p.pieces ? (size_t)p.units * kv_heads * 32 : 0; }
 
 }  // namespace
 
@@ -145,9 +474,11 @@ bool in_pieces(int dtype, int dim, std::initializer_list<const void *> p, std::i
 using namespace d8;
 
 extern "C" size_t d8_attention_scratch_bytes(int dtype, int which, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim, int causal) {
-    (void)causal, (void)sequences, (void)k_tokens, (void)kv_heads, (void)dim;
-    if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || q_tokens < 0 || heads < 1) return 0;
-    return which == 1 ? attention::grad_scratch_bytes(q_tokens, heads) : 0;
+    (void)causal;
+    if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || sequences < 0 || q_tokens < 0 || k_tokens < 0 || kv_heads < 1 || heads < kv_heads || dim < 1) return 0;
+    if (which == 1) return attention::grad_scratch_bytes(q_tokens, heads);
+    const attention::Plan p = attention::plan_of(true, sequences, q_tokens, k_tokens, heads, kv_heads);
+    return attention::part_rows(p, kv_heads) * (size_t)(dim + 2) * sizeof(float);
 }
 
 extern "C" int d8_attention(int dtype, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, void *o, long ldo, float *lse,
@@ -161,11 +492,15 @@ extern "C" int d8_attention(int dtype, const void *q, long ldq, const void *k, l
     if (int rc = attention::check(a, dtype, "attention")) return rc;
     if (!sequences || !q_tokens) return 0;
     D8_REQUIRE(q && o && q_starts && k_starts && (!k_tokens || (k && v)), "attention: null tensor");
-    (void)scratch, (void)scratch_bytes;
     a.group = heads / kv_heads;
     a.vec = attention::in_pieces(dtype, dim, {q, k, v}, {ldq, ldk, ldv});
-    const long tiles = ((long)q_tokens * a.group + attention::ROWS - 1) / attention::ROWS + sequences;
-    D8_REQUIRE(tiles * kv_heads < (1L << 31), "attention: too many sequences");
-    a.tiles = (int)tiles;
-    return dtype == D8_FLOAT16 ? attention::launch<f16>(a, as_stream(stream)) : attention::launch<float>(a, as_stream(stream));
+    // (a tile's rows are addressed by 32 bits)
+    const bool fast = a.vec && attention::in_pieces(dtype, dim, {o}, {ldo}) && ldk < (1 << 23) && ldv < (1 << 23);
+    const attention::Plan p = attention::plan_of(fast, sequences, q_tokens, k_tokens, heads, kv_heads);
+    const size_t part = attention::part_rows(p, kv_heads), need = part * (size_t)(dim + 2) * sizeof(float);
+    D8_REQUIRE(!need || (scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0), "attention: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
+    D8_REQUIRE((long)(p.tiles + p.pieces) * kv_heads < (1L << 31), "attention: too many sequences");
+    a.tiles = p.tiles, a.units = p.units, a.pieces = p.pieces;
+    a.part = (float *)scratch, a.part_ml = a.part + part * dim;
+    return dtype == D8_FLOAT16 ? attention::launch<f16>(a, p, as_stream(stream)) : attention::launch<float>(a, p, as_stream(stream));
 }

@@ -2,6 +2,7 @@
 import math
 
 import numpy as np
+from threadpoolctl import threadpool_limits
 
 EPS = 1e-6
 
@@ -74,6 +75,7 @@ def _weights(q, k, seen, scale):
     return e / np.where(total > 0, total, 1), lse[:, 0]
 
 
+@threadpool_limits.wrap(limits=1)  # many small products
 def attention(q, k, v, q_starts, k_starts, scale, causal, do=None):
     """(o, lse), or with do (dq, dk, dv); NaN in rows of no sequence"""
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))

@@ -86,6 +86,27 @@ def test_forward_and_gradient(cfg, dtype):
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("dim,H,G,causal", [(32, 16, 16, True), (64, 16, 16, True), (80, 24, 12, True), (128, 16, 16, True), (128, 15, 15, False), (256, 16, 16, True), (200, 16, 8, False)])
+def test_many_rows(dtype, dim, H, G, causal):
+    """enough rows for workgroups of 128 of them; lengths that end inside tiles of rows and of keys, queries fewer and more than keys"""
+    from deep8_amd import ops
+    r = rng(dim + H)
+    nq = list(r.integers(150, 390, 15)) + [1, 300]
+    nk = [int(max(0, n + r.integers(-70, 130))) for n in nq]
+    q, k, v, do = _inputs(nq, nk, H, G, dim, dtype, dim)
+    qs, ks, scale = _starts(nq), _starts(nk), -(dim ** -0.5)
+    want, lse = lo.attention(q, k, v, qs, ks, scale, causal)
+    got, got_lse = ops.attention(q, k, v, qs, ks, scale, causal, pad=8)
+    _near(got, want, TOL[dtype])
+    empty = np.isneginf(lse)
+    assert np.array_equal(np.isneginf(got_lse), empty) and np.abs(got_lse - lse)[~empty].max() <= 1e-5 * np.abs(lse[~empty]).max()
+    grads = lo.attention(q, k, v, qs, ks, scale, causal, do)
+    back = ops.attention_grad(q, k, v, got, got_lse, do, qs, ks, scale, causal, pad=8)
+    for g, w in zip(back, grads):
+        _near(g, w, TOL[dtype])
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
 def test_long_cache(dtype):
     """one query against tens of thousands of keys, the largest score far from the first"""
     from deep8_amd import ops
