@@ -2,8 +2,8 @@
 //
 //   dv = p^T do,  dp = do v^T,  ds = p (dp - delta) with delta = rowsum(do o) = rowsum(p dp),  dq = scale ds k,  dk = scale ds^T q
 //
-// Three launches: delta of every row; dk and dv, a workgroup for 128 keys that walks the rows that see them (those of all heads that
-// share the keys, so that the sums over shared heads stay in its registers); dq, a workgroup for 128 rows that walks the keys.  The
+// Three launches: delta of every row; dq, a workgroup for some rows that walks the keys; dk and dv, a workgroup for some keys that walks
+// the rows that see them (those of all heads that share the keys, so that the sums over shared heads stay in its registers).  The
 // scores are computed twice, seven products for the five that the formulas have, and in return no two workgroups add to one
 // place: no atomics, the same bits every time.
 //
@@ -16,53 +16,57 @@ namespace d8 {
 namespace attention {
 namespace {
 
-enum { KEYS = 128, ROWS = 128, TILE = 32 };
+enum { TILE = 32 };
 enum { NORM_GROUPS = 512 };  // workgroups of the first launch: entries of each list of norms
 constexpr float P_SHIFT = 15.f;
 
 template <class T>
 constexpr bool scaled() { return sizeof(T) == 2; }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
-}
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
     return v;
 }
 
-// delta[head][token] = sum of do o; a wave has a row.  In half also the largest squared norms of the rows of do and of v.
+// delta[head][token] = sum of do o; a group of lanes has a row, 16 bytes a lane.  In half also the largest squared norms of the rows
+// of do and of v.
 template <class T>
-__global__ __launch_bounds__(256) void attention_delta_kernel(Args a) {
+__global__ __launch_bounds__(256) void attention_delta_kernel(Args a, int lanes) {
+    typedef typename Type<T>::frag frag;
+    constexpr int V = Type<T>::V;
     __shared__ float most[2][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = threadIdx.x & (lanes - 1);
+    const long step = (long)gridDim.x * 256 / lanes, mine = ((long)blockIdx.x * 256 + threadIdx.x) / lanes;
     float top_do = 0.f, top_v = 0.f;
     const long rows = (long)a.q_tokens * a.heads;
-    for (long r = (long)blockIdx.x * 4 + wave; r < rows; r += (long)gridDim.x * 4) {
+    for (long r = mine; r < rows; r += step) {
         const long t = r / a.heads;
         const int head = (int)(r - t * a.heads);
-        const T *g = (const T *)a.dout + t * a.lddo + (long)head * a.dim, *o = (const T *)a.o + t * a.ldo + (long)head * a.dim;
+        const frag g = load_piece<T>((const T *)a.dout + t * a.lddo + (long)head * a.dim, l * V, a.dim, true, a.vec);
+        const frag o = load_piece<T>((const T *)a.o + t * a.ldo + (long)head * a.dim, l * V, a.dim, true, a.vec);
         float dot = 0.f, sq = 0.f;
-        for (int d = lane; d < a.dim; d += 64) {
-            const float x = (float)g[d];
-            dot += x * (float)o[d], sq += x * x;
+#pragma unroll
+        for (int e = 0; e < V; ++e) dot += (float)g[e] * (float)o[e], sq += (float)g[e] * (float)g[e];
+        for (int d = 1; d < lanes; d <<= 1) {
+            dot += __shfl_xor(dot, d);
+            if (scaled<T>()) sq += __shfl_xor(sq, d);
         }
-        dot = wave_sum(dot);
-        if (lane == 0) a.delta[(long)head * a.q_tokens + t] = dot;
-        if (scaled<T>()) top_do = fmaxf(top_do, wave_sum(sq));
+        if (l == 0) a.delta[(long)head * a.q_tokens + t] = dot;
+        top_do = fmaxf(top_do, sq);
     }
     if (!scaled<T>()) return;
     const long krows = (long)a.k_tokens * a.kv_heads;
-    for (long r = (long)blockIdx.x * 4 + wave; r < krows; r += (long)gridDim.x * 4) {
+    for (long r = mine; r < krows; r += step) {
         const long t = r / a.kv_heads;
-        const T *v = (const T *)a.v + t * a.ldv + (r - t * a.kv_heads) * a.dim;
+        const frag v = load_piece<T>((const T *)a.v + t * a.ldv + (r - t * a.kv_heads) * a.dim, l * V, a.dim, true, a.vec);
         float sq = 0.f;
-        for (int d = lane; d < a.dim; d += 64) sq += (float)v[d] * (float)v[d];
-        top_v = fmaxf(top_v, wave_sum(sq));
+#pragma unroll
+        for (int e = 0; e < V; ++e) sq += (float)v[e] * (float)v[e];
+        for (int d = 1; d < lanes; d <<= 1) sq += __shfl_xor(sq, d);
+        top_v = fmaxf(top_v, sq);
     }
+    top_do = wave_max(top_do), top_v = wave_max(top_v);
     if (lane == 0) most[0][wave] = top_do, most[1][wave] = top_v;
     __syncthreads();
     if (threadIdx.x < 2) {
@@ -83,9 +87,11 @@ __device__ __forceinline__ float ds_scale(const Args &a) {
     return exp2f(-(float)(ilogbf(bound) + 1));
 }
 
+enum { KEYS = 128, ROWS = 128 };  // of a workgroup of the two kernels for tensors that cannot be moved in 16-byte pieces
+
 // dk and dv
 template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_grad_kv_kernel(Args a) {
+__global__ __launch_bounds__(256) void attention_grad_kv_any_kernel(Args a) {
     typedef Type<T> M;
     typedef typename M::frag frag;
     constexpr int PITCH = pitch_of<DP, T>(), UNITS = DP / M::STEP, PIECES = DP / M::V;
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(256) void attention_grad_kv_kernel(Args a) {
 
 // dq
 template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_grad_q_kernel(Args a) {
+__global__ __launch_bounds__(256) void attention_grad_q_any_kernel(Args a) {
     typedef Type<T> M;
     typedef typename M::frag frag;
     constexpr int PITCH = pitch_of<DP, T>(), UNITS = DP / M::STEP, PIECES = DP / M::V;
@@ -254,27 +260,348 @@ __global__ __launch_bounds__(256) void attention_grad_q_kernel(Args a) {
         }
 }
 
+// a lane's column of sums (32 b + 8 (e / 4) + 4 h + e % 4) times `by`, over or onto four elements at a time
 template <class T, int DP>
-int launch_dim(const Args &a, int key_blocks, hipStream_t stream) {
-    if (key_blocks) {
-        hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP>), dim3((unsigned)key_blocks * a.kv_heads), dim3(256), 0, stream, a);
-        D8_LAUNCH_CHECK();
+__device__ __forceinline__ void store_sums(T *to, const f32x16 (&x)[DP / 32], float by, int dim, int h, bool overwrite) {
+    typedef T four __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = n * 32 + 2 * e + 4 * h;
+            if (d >= dim) continue;
+            four out;
+            if (overwrite) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[i] = (T)(x[n][e + i] * by);
+            } else {
+                const four old = *(const four *)(to + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[i] = (T)(x[n][e + i] * by + (float)old[i]);
+            }
+            *(four *)(to + d) = out;
+        }
+}
+
+// The same two for tensors whose rows can be moved in 16-byte pieces: tiles straight into one of two stages of LDS, the next while this one is
+// worked on.  A wave has 32 keys (rows) of its own, whose fragments and sums stay in registers.  SPLIT = 1: four waves, 128 keys
+// (rows) a workgroup, each walks every tile; SPLIT = 2, where that would leave compute units idle: 64, two waves have the same
+// 32 and take every other tile, and their sums are joined through LDS at the end.
+template <class T, int DP, int SPLIT>
+struct Shape {
+    static constexpr int PB = row_bytes<T, DP>(), OWN = 128 / SPLIT, BLOCKS = PB <= 256 || SPLIT == 2 ? 2 : 1;
+    static constexpr int KB = 32 * BLOCKS, TILE_BYTES = KB * PB, LOADS = TILE_BYTES / 1024 / 4;
+    static constexpr int OCCUPANCY = DP * (int)sizeof(T) <= 256 ? 2 : 1;
+    static_assert(LOADS >= 1 && 4 * TILE_BYTES <= 160 * 1024, "a tile is at least a load of every wave, and two stages fit");
+};
+
+// rows of q or do (of all heads of a group) on their way into a tile
+template <class T, int PB>
+struct RowLoader {
+    int lane_row, lane_pos, pieces;
+    __device__ __forceinline__ void init(int dim, int lane) { lane_row = lane / (PB / 16), lane_pos = lane % (PB / 16), pieces = dim / Type<T>::V; }
+    // `first`: query t0's first head; row r0 + i of the sequence goes to row i of the tile
+    __device__ __forceinline__ void load(const T *first, long ld, int dim, int group, int r0, int t0, int rows, int i0, unsigned tile) const {
+        constexpr int PER = TileLoader<T, PB>::ROWS;
+        const unsigned long p = (unsigned long)first;
+        const desc_t d = desc_t{(unsigned)__builtin_amdgcn_readfirstlane((int)p), (unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
+        const int i = i0 * PER + lane_row, r = r0 + i, t = r / group, piece = lane_pos ^ swizzle<PB>(i);
+        const unsigned at = (unsigned)(t - t0) * (unsigned)(ld * sizeof(T)) + (unsigned)((r - t * group) * dim * (int)sizeof(T) + piece * 16);
+        load_to_lds(d, r < rows && piece < pieces ? at : 0x80000000u, __builtin_amdgcn_readfirstlane(tile + i0 * 1024));
     }
-    if (a.tiles) {
-        hipLaunchKernelGGL((attention_grad_q_kernel<T, DP>), dim3((unsigned)a.tiles * a.kv_heads), dim3(256), 0, stream, a);
-        D8_LAUNCH_CHECK();
+};
+
+template <class T, int DP, int SPLIT>
+__global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attention_grad_kv_kernel(Args a) {
+    typedef Type<T> M;
+    typedef typename M::frag frag;
+    typedef Shape<T, DP, SPLIT> S;
+    constexpr int PB = S::PB, UNITS = DP / M::STEP, N = DP / 32;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * S::TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) float row_lse[2][S::KB], row_delta[2][S::KB];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int hk = blockIdx.x % a.kv_heads;
+    Span sp;
+    int seq, block;
+    if (!locate(a, blockIdx.x / a.kv_heads, sp, seq, block, [](const Span &s) { return (s.nk + S::OWN - 1) / S::OWN; })) return;
+    const int group = a.group, rows = sp.nq * group, back = sp.nk - sp.nq;
+    const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
+    const int j0 = block * S::OWN + wave % (4 / SPLIT) * 32, j = j0 + (lane & 31);  // the wave's first key, the lane's
+    const bool there = j < sp.nk;
+    const long key = sp.k0 + (there ? j : 0);
+    frag kf[UNITS], vf[UNITS];
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        kf[u] = load_piece<T>((const T *)a.k + key * a.ldk + (long)hk * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
+        vf[u] = load_piece<T>((const T *)a.v + key * a.ldv + (long)hk * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
     }
+    f32x16 dk[N], dv[N];
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[b][e] = dv[b][e] = 0.f;
+    RowLoader<T, PB> loader;
+    loader.init(a.dim, lane);
+    const unsigned lds0 = lds_address(lds);
+    const T *q = (const T *)a.q + (long)sp.q0 * a.ldq + (long)hk * group * a.dim, *g = (const T *)a.dout + (long)sp.q0 * a.lddo + (long)hk * group * a.dim;
+    float next_lse = 0.f, next_delta = 0.f;  // of row tid of the next tile
+    auto fetch = [&](int r0, int stage) {
+        const int t0 = r0 / group;
+#pragma unroll
+        for (int i = 0; i < S::LOADS; ++i) loader.load(q + (long)t0 * a.ldq, a.ldq, a.dim, group, r0, t0, rows, wave * S::LOADS + i, lds0 + stage * 2 * S::TILE_BYTES);
+#pragma unroll
+        for (int i = 0; i < S::LOADS; ++i)
+            loader.load(g + (long)t0 * a.lddo, a.lddo, a.dim, group, r0, t0, rows, wave * S::LOADS + i, lds0 + stage * 2 * S::TILE_BYTES + S::TILE_BYTES);
+        if (tid < S::KB) {
+            const int r = r0 + tid;
+            const bool in = r < rows;
+            const int t = in ? r / group : 0;
+            const long at = (long)(hk * group + (in ? r - t * group : 0)) * a.q_tokens + sp.q0 + t;
+            next_lse = in ? a.lse[at] * LOG2E - shift : INFINITY;  // (rows that are not there: probability zero)
+            next_delta = in ? a.delta[at] * mult : 0.f;
+        }
+    };
+    // the first row that sees a key of the block (its query is the block's first key less nk - nq)
+    const long first = a.causal ? (long)max(0, block * S::OWN - back) * group : 0;
+    const int r_begin = (int)min(first / 32 * 32, (long)rows);
+    if (r_begin < rows) fetch(r_begin, 0);
+    for (int r0 = r_begin, stage = 0; r0 < rows; r0 += S::KB, stage ^= 1) {
+        if (tid < S::KB) row_lse[stage][tid] = next_lse, row_delta[stage][tid] = next_delta;
+        ATTN_VMCNT(0);
+        lds_reads_done();
+        __syncthreads();
+        if (r0 + S::KB < rows) fetch(r0 + S::KB, stage ^ 1);
+        const char *tq = lds + stage * 2 * S::TILE_BYTES, *tg = tq + S::TILE_BYTES;
+#pragma unroll 1
+        for (int i = 0; i < S::BLOCKS / SPLIT; ++i) {
+            const int b = SPLIT == 1 ? i : wave / (4 / SPLIT), rb = r0 + b * 32;
+            // queries of the block's first and last row: what the first sees, all see; what the last does not see, none sees
+            if (rb >= rows || (a.causal && j0 > (min(rb + 31, rows - 1)) / group + back)) continue;
+            f32x16 s, w;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = w[e] = 0.f;
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) M::mma(s, rows_frag<T, PB>(tq, b * 32, u, lane), kf[u]);
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) M::mma(w, rows_frag<T, PB>(tg, b * 32, u, lane), vf[u]);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const f32x4 l4 = *(const f32x4 *)&row_lse[stage][b * 32 + 2 * e + 4 * h], d4 = *(const f32x4 *)&row_delta[stage][b * 32 + 2 * e + 4 * h];
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) {
+                    s[e + i4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + i4], c, -l4[i4]));
+                    w[e + i4] = __builtin_fmaf(w[e + i4], mult, -d4[i4]);
+                }
+            }
+            if (a.causal && j0 + 31 > rb / group + back) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool seen = j <= (rb + 8 * (e >> 2) + 4 * h + (e & 3)) / group + back;
+                    s[e] = seen ? s[e] : 0.f, w[e] = seen ? w[e] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] *= s[e];
+#pragma unroll
+            for (int u = 0; u < 32 / M::STEP; ++u) {
+                const frag p = M::pack(s, u), d = M::pack(w, u);
+#pragma unroll
+                for (int n = 0; n < N; ++n) M::mma(dv[n], cols_frag<T, PB>(tg, b * 32 + u * M::STEP, n * 32, lane), p);
+#pragma unroll
+                for (int n = 0; n < N; ++n) M::mma(dk[n], cols_frag<T, PB>(tq, b * 32 + u * M::STEP, n * 32, lane), d);
+            }
+        }
+    }
+    if constexpr (SPLIT == 2) {
+        __syncthreads();
+        float *to = (float *)lds + (wave & 1) * 2 * N * 16 * 64 + lane;
+        if (wave >= 2) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) to[(n * 16 + e) * 64] = dk[n][e], to[((N + n) * 16 + e) * 64] = dv[n][e];
+        }
+        __syncthreads();
+        if (wave >= 2) return;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dk[n][e] += to[(n * 16 + e) * 64], dv[n][e] += to[((N + n) * 16 + e) * 64];
+    }
+    if (!there) return;
+    const float unshift = exp2f(-shift), by = a.scale * unshift / mult;
+    T *pk = (T *)a.dk + key * a.lddk + (long)hk * a.dim, *pv = (T *)a.dv + key * a.lddv + (long)hk * a.dim;
+    store_sums<T, DP>(pk, dk, by, a.dim, h, a.overwrite & 2);
+    store_sums<T, DP>(pv, dv, unshift, a.dim, h, a.overwrite & 4);
+}
+
+template <class T, int DP, int SPLIT>
+__global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attention_grad_q_kernel(Args a) {
+    typedef Type<T> M;
+    typedef typename M::frag frag;
+    typedef Shape<T, DP, SPLIT> S;
+    constexpr int PB = S::PB, UNITS = DP / M::STEP, N = DP / 32;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * S::TILE_BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int hk = blockIdx.x % a.kv_heads;
+    Span sp;
+    int seq, tile;
+    auto tiles_of = [&](const Span &s) { return (int)(((long)s.nq * a.group + S::OWN - 1) / S::OWN); };
+    if (!locate(a, blockIdx.x / a.kv_heads, sp, seq, tile, tiles_of)) return;
+    const int group = a.group, rows = sp.nq * group, back = sp.nk - sp.nq;
+    tile = tiles_of(sp) - 1 - tile;  // the rows that see most keys first
+    const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
+    const int r = tile * S::OWN + wave % (4 / SPLIT) * 32 + (lane & 31);
+    const bool there = r < rows;
+    const int t = (there ? r : rows - 1) / group, head = hk * group + (there ? r - t * group : 0);
+    frag qf[UNITS], gf[UNITS];
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        qf[u] = load_piece<T>((const T *)a.q + (long)(sp.q0 + t) * a.ldq + (long)head * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
+        gf[u] = load_piece<T>((const T *)a.dout + (long)(sp.q0 + t) * a.lddo + (long)head * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
+    }
+    const long at = (long)head * a.q_tokens + sp.q0 + t;
+    const float lse = there ? a.lse[at] * LOG2E - shift : INFINITY;
+    float delta = there ? a.delta[at] * mult : 0.f;
+    const int last = a.causal ? min(sp.nk - 1, t + back) : sp.nk - 1;
+    const int end = a.causal ? min(sp.nk, (min(rows, (tile + 1) * S::OWN) - 1) / group + back + 1) : sp.nk;
+    const int wave_all = __builtin_amdgcn_readfirstlane(__shfl(last, 0)), wave_end = __builtin_amdgcn_readfirstlane(__shfl(last, 31)) + 1;
+    f32x16 dq[N];
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dq[b][e] = 0.f;
+    const T *k = (const T *)a.k + (long)sp.k0 * a.ldk + (long)hk * a.dim, *v = (const T *)a.v + (long)sp.k0 * a.ldv + (long)hk * a.dim;
+    TileLoader<T, PB> lk, lv;
+    lk.init(a.ldk, a.dim, lane), lv.init(a.ldv, a.dim, lane);
+    const unsigned lds0 = lds_address(lds);
+    auto fetch = [&](int j0, int stage) {
+        const desc_t dk = lk.desc(k + (long)j0 * a.ldk, min(S::KB, sp.nk - j0), a.ldk, a.dim), dv = lv.desc(v + (long)j0 * a.ldv, min(S::KB, sp.nk - j0), a.ldv, a.dim);
+#pragma unroll
+        for (int i = 0; i < S::LOADS; ++i) lk.load(dk, wave * S::LOADS + i, lds0 + stage * 2 * S::TILE_BYTES);
+#pragma unroll
+        for (int i = 0; i < S::LOADS; ++i) lv.load(dv, wave * S::LOADS + i, lds0 + stage * 2 * S::TILE_BYTES + S::TILE_BYTES);
+    };
+    if (end > 0) fetch(0, 0);
+    for (int j0 = 0, stage = 0; j0 < end; j0 += S::KB, stage ^= 1) {
+        ATTN_VMCNT(0);
+        lds_reads_done();
+        __syncthreads();
+        if (j0 + S::KB < end) fetch(j0 + S::KB, stage ^ 1);
+        const char *tk = lds + stage * 2 * S::TILE_BYTES, *tv = tk + S::TILE_BYTES;
+#pragma unroll 1
+        for (int i = 0; i < S::BLOCKS / SPLIT; ++i) {
+            const int b = SPLIT == 1 ? i : wave / (4 / SPLIT), jb = j0 + b * 32;
+            if (jb >= wave_end) continue;
+            f32x16 s, w;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = w[e] = 0.f;
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) M::mma(s, rows_frag<T, PB>(tk, b * 32, u, lane), qf[u]);
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) M::mma(w, rows_frag<T, PB>(tv, b * 32, u, lane), gf[u]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lse));
+            if (jb + 31 > wave_all) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool seen = jb + 8 * (e >> 2) + 4 * h + (e & 3) <= last;
+                    s[e] = seen ? s[e] : 0.f, w[e] = seen ? w[e] : 0.f;
+                }
+            }
+            if (end <= 32) {
+                // rows of few keys: delta from the probabilities themselves; do o has the rounding of o in it, which there weighs as much as
+                // the rounding of ds
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum += s[e] * w[e];
+                sum += __shfl_xor(sum, 32);
+                sum *= exp2f(-shift);
+                if (there && h == 0) a.delta[at] = sum;
+                delta = sum * mult;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = s[e] * __builtin_fmaf(w[e], mult, -delta);
+#pragma unroll
+            for (int u = 0; u < 32 / M::STEP; ++u) {
+                const frag d = M::pack(w, u);
+#pragma unroll
+                for (int n = 0; n < N; ++n) M::mma(dq[n], cols_frag<T, PB>(tk, b * 32 + u * M::STEP, n * 32, lane), d);
+            }
+        }
+    }
+    if constexpr (SPLIT == 2) {
+        __syncthreads();
+        float *to = (float *)lds + (wave & 1) * N * 16 * 64 + lane;
+        if (wave >= 2) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) to[(n * 16 + e) * 64] = dq[n][e];
+        }
+        __syncthreads();
+        if (wave >= 2) return;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dq[n][e] += to[(n * 16 + e) * 64];
+    }
+    if (!there) return;
+    store_sums<T, DP>((T *)a.dq + (long)(sp.q0 + t) * a.lddq + (long)head * a.dim, dq, a.scale * exp2f(-shift) / mult, a.dim, h, a.overwrite & 1);
+}
+
+// SPLIT for so many keys (rows), of which a workgroup has 128 or 64
+int split_for(long own, int kv_heads) { return (own + 127) / 128 * kv_heads < 2 * cu_count() ? 2 : 1; }
+
+template <class T, int DP, int SPLIT>
+int launch_kv(const Args &a, hipStream_t stream) {
+    const long blocks = ((long)a.k_tokens + 128 / SPLIT - 1) / (128 / SPLIT) + a.sequences;
+    hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP, SPLIT>), dim3((unsigned)blocks * a.kv_heads), dim3(256), 0, stream, a);
+    D8_LAUNCH_CHECK();
+    return 0;
+}
+template <class T, int DP, int SPLIT>
+int launch_q(const Args &a, hipStream_t stream) {
+    const long tiles = ((long)a.q_tokens * a.group + 128 / SPLIT - 1) / (128 / SPLIT) + a.sequences;
+    hipLaunchKernelGGL((attention_grad_q_kernel<T, DP, SPLIT>), dim3((unsigned)tiles * a.kv_heads), dim3(256), 0, stream, a);
+    D8_LAUNCH_CHECK();
     return 0;
 }
 
+template <class T, int DP>
+int launch_dim(const Args &a, bool fast, hipStream_t stream) {
+    constexpr bool CAN_SPLIT = row_bytes<T, DP>() <= 512;
+    if (a.q_tokens) {  // dq first: it may set delta anew
+        const int split = split_for((long)a.q_tokens * a.group, a.kv_heads);
+        if (!fast) {
+            const long tiles = ((long)a.q_tokens * a.group + ROWS - 1) / ROWS + a.sequences;
+            hipLaunchKernelGGL((attention_grad_q_any_kernel<T, DP>), dim3((unsigned)tiles * a.kv_heads), dim3(256), 0, stream, a);
+            D8_LAUNCH_CHECK();
+        } else if (int rc = CAN_SPLIT && split == 2 ? launch_q<T, DP, CAN_SPLIT ? 2 : 1>(a, stream) : launch_q<T, DP, 1>(a, stream)) {
+            return rc;
+        }
+    }
+    if (!a.k_tokens) return 0;
+    if (!fast) {
+        const long blocks = ((long)a.k_tokens + KEYS - 1) / KEYS + a.sequences;
+        hipLaunchKernelGGL((attention_grad_kv_any_kernel<T, DP>), dim3((unsigned)blocks * a.kv_heads), dim3(256), 0, stream, a);
+        D8_LAUNCH_CHECK();
+        return 0;
+    }
+    return CAN_SPLIT && split_for(a.k_tokens, a.kv_heads) == 2 ? launch_kv<T, DP, CAN_SPLIT ? 2 : 1>(a, stream) : launch_kv<T, DP, 1>(a, stream);
+}
+
 template <class T>
-int launch(const Args &a, int key_blocks, hipStream_t stream) {
-    hipLaunchKernelGGL(attention_delta_kernel<T>, dim3(NORM_GROUPS), dim3(256), 0, stream, a);
+int launch(const Args &a, bool fast, hipStream_t stream) {
+    int lanes = 1;
+    while (lanes * Type<T>::V < a.dim) lanes *= 2;
+    hipLaunchKernelGGL(attention_delta_kernel<T>, dim3(NORM_GROUPS), dim3(256), 0, stream, a, lanes);
     D8_LAUNCH_CHECK();
-    if (a.dim <= 32) return launch_dim<T, 32>(a, key_blocks, stream);
-    if (a.dim <= 64) return launch_dim<T, 64>(a, key_blocks, stream);
-    if (a.dim <= 128) return launch_dim<T, 128>(a, key_blocks, stream);
-    return launch_dim<T, 256>(a, key_blocks, stream);
+    if (a.dim <= 32) return launch_dim<T, 32>(a, fast, stream);
+    if (a.dim <= 64) return launch_dim<T, 64>(a, fast, stream);
+    if (a.dim <= 96) return launch_dim<T, 96>(a, fast, stream);
+    if (a.dim <= 128) return launch_dim<T, 128>(a, fast, stream);
+    return launch_dim<T, 256>(a, fast, stream);
 }
 
 }  // namespace
@@ -307,10 +634,10 @@ extern "C" int d8_attention_grad(int dtype, const void *q, long ldq, const void 
     D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_grad: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
     a.norms = (float *)scratch, a.delta = a.norms + 2 * attention::NORM_GROUPS;
     a.group = heads / kv_heads;
-    a.vec = attention::in_pieces(dtype, dim, {q, k, v, dout}, {ldq, ldk, ldv, lddo});
-    const long tiles = q_tokens ? ((long)q_tokens * a.group + attention::ROWS - 1) / attention::ROWS + sequences : 0;
-    const long blocks = k_tokens ? ((long)k_tokens + attention::KEYS - 1) / attention::KEYS + sequences : 0;
-    D8_REQUIRE((tiles + blocks) * kv_heads < (1L << 31), "attention_grad: too many sequences");
-    a.tiles = (int)tiles;
-    return dtype == D8_FLOAT16 ? attention::launch<f16>(a, (int)blocks, as_stream(stream)) : attention::launch<float>(a, (int)blocks, as_stream(stream));
+    a.vec = attention::in_pieces(dtype, dim, {q, k, v, o, dout}, {ldq, ldk, ldv, ldo, lddo});
+    // (a tile's rows are addressed by 31 bits)
+    const long most = 1 << 21;
+    const bool fast = a.vec && attention::in_pieces(dtype, dim, {dq, dk, dv}, {lddq, lddk, lddv}) && ldq < most && ldk < most && ldv < most && lddo < most;
+    D8_REQUIRE((((long)q_tokens * a.group + k_tokens) / 64 + 2 * (long)sequences + 2) * kv_heads < (1L << 31), "attention_grad: too many sequences");
+    return dtype == D8_FLOAT16 ? attention::launch<f16>(a, fast, as_stream(stream)) : attention::launch<float>(a, fast, as_stream(stream));
 }
