@@ -34,6 +34,7 @@ struct Args {
     long ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
     const int *q_starts, *k_starts;
     int sequences, q_tokens, k_tokens, heads, kv_heads, group, dim, causal;
+    unsigned group_rcp;  // floor((2^32 - 1) / group)
     float scale;
     int vec;        // rows of every tensor can be moved in 16-byte pieces
     int tiles;      // row tiles (key blocks) of all sequences at most
@@ -57,6 +58,12 @@ __device__ __forceinline__ Span span_of(const Args &a, int s) {
     r.k0 = min(max(a.k_starts[s], 0), a.k_tokens);
     r.nk = max(min(a.k_starts[s + 1], a.k_tokens) - r.k0, 0);
     return r;
+}
+
+// Row r's query, r < 2^31: r times the reciprocal over 2^32 is the quotient or one less.
+__device__ __forceinline__ int query_of(const Args &a, int r) {
+    const int t = (int)__umulhi((unsigned)r, a.group_rcp);
+    return t + (r - t * a.group >= a.group ? 1 : 0);
 }
 
 // Which sequence holds item `id` of a list in which sequence s has count(span) items: sets s, the item's number in it and the span; false
@@ -314,6 +321,7 @@ struct Softmax {
 };
 
 int check(const Args &a, int dtype, const char *name);
+inline void set_group(Args &a) { a.group = a.heads / a.kv_heads, a.group_rcp = 0xffffffffu / (unsigned)a.group; }
 bool in_pieces(int dtype, int dim, std::initializer_list<const void *> p, std::initializer_list<long> ld);
 size_t grad_scratch_bytes(int q_tokens, int heads);
 

@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void attention_any_kernel(Args a) {
     const int group = a.group, rows = sp.nq * group;
     tile = tiles_of(sp) - 1 - tile;  // the rows that see most keys first
     const int r = tile * ROWS + wave * 32 + (lane & 31);
-    const int t = r / group, head = hk * group + r - t * group;
+    const int t = query_of(a, r), head = hk * group + r - t * group;
     const bool there = r < rows;
     const T *q = (const T *)a.q + (long)(sp.q0 + (there ? t : 0)) * a.ldq + (long)head * a.dim;
     frag qf[UNITS];
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void attention_any_kernel(Args a) {
     for (int u = 0; u < UNITS; ++u) qf[u] = load_piece<T>(q, u * M::STEP + h * M::V, a.dim, there, a.vec);
     const int back = sp.nk - sp.nq;
     const int last = a.causal ? min(sp.nk - 1, t + back) : sp.nk - 1;  // last key that the lane's row sees
-    const int t_end = (min(rows, (tile + 1) * ROWS) - 1) / group;
+    const int t_end = query_of(a, min(rows, (tile + 1) * ROWS) - 1);
     const int end = a.causal ? min(sp.nk, t_end + back + 1) : sp.nk;
     const float c = a.scale * LOG2E;
     f32x16 acc[DP / 32];
@@ -135,12 +135,12 @@ __global__ __launch_bounds__(256, (DP * (int)sizeof(T) <= 256 ? 2 : 1)) void att
     tile = tiles_of(sp) - 1 - tile;  // the rows that see most keys first
     const int r = tile * ROWS + wave * 32 + (lane & 31);
     const bool there = r < rows;
-    const int t = (there ? r : rows - 1) / group, head = hk * group + (there ? r - t * group : 0);
+    const int t = query_of(a, there ? r : rows - 1), head = hk * group + (there ? r - t * group : 0);
     frag qf[DP / M::STEP];
     load_query<T, DP>(a, (const T *)a.q + (long)(sp.q0 + t) * a.ldq + (long)head * a.dim, there, h, qf);
     const int back = sp.nk - sp.nq;
     const int last = a.causal ? min(sp.nk - 1, t + back) : sp.nk - 1;  // last key that the lane's row sees
-    const int end = a.causal ? min(sp.nk, (min(rows, (tile + 1) * ROWS) - 1) / group + back + 1) : sp.nk;
+    const int end = a.causal ? min(sp.nk, query_of(a, min(rows, (tile + 1) * ROWS) - 1) + back + 1) : sp.nk;
     // what all rows of the wave see, and the end of what one of them sees
     const int wave_all = __builtin_amdgcn_readfirstlane(__shfl(last, 0)), wave_end = __builtin_amdgcn_readfirstlane(__shfl(last, 31)) + 1;
     const float c = exponent_scale(a);
@@ -239,7 +239,7 @@ struct Cut {
     // keys that some row of the tile sees
     __device__ __forceinline__ int end(const Args &a, const Span &s, int tile) const {
         const int rows = s.nq * a.group;
-        return a.causal ? max(0, min(s.nk, (min(rows, (tile + 1) * 32) - 1) / a.group + s.nk - s.nq + 1)) : s.nk;
+        return a.causal ? max(0, min(s.nk, query_of(a, min(rows, (tile + 1) * 32) - 1) + s.nk - s.nq + 1)) : s.nk;
     }
 };
 enum { CHUNK_GRAIN = 256 };
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_keys_kernel(Args a) {
     const bool whole = all <= cut.chunk;
     const int r = tile * 32 + (lane & 31);
     const bool there = r < rows;
-    const int t = (there ? r : rows - 1) / group, head = hk * group + (there ? r - t * group : 0);
+    const int t = query_of(a, there ? r : rows - 1), head = hk * group + (there ? r - t * group : 0);
     frag qf[DP / M::STEP];
     load_query<T, DP>(a, (const T *)a.q + (long)(sp.q0 + t) * a.ldq + (long)head * a.dim, there, h, qf);
     const int last = a.causal ? min(sp.nk - 1, t + sp.nk - sp.nq) : sp.nk - 1;
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_keys_kernel(Args a) {
             by[w] = wave_base[w][row] == base ? (base == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(wave_base[w][row] - base);
             total += wave_sum[w][row] * by[w];
         }
-        const int rt = (tile * 32 + row) / group, rh = hk * group + tile * 32 + row - rt * group;
+        const int rt = query_of(a, tile * 32 + row), rh = hk * group + tile * 32 + row - rt * group;
         const float inv = !whole ? 1.f : total == 0.f ? 0.f : 1.f / total;
         const long slot = ((long)unit * a.kv_heads + hk) * 32 + row;
         for (int d = lane; d < a.dim; d += 64) {
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
         for (int i = 0; i < parts; ++i) base = fmaxf(base, a.part_ml[(slot + i * step) * 2]);
         const float at = base == -INFINITY ? 0.f : base;
         for (int i = 0; i < parts; ++i) total += a.part_ml[(slot + i * step) * 2 + 1] * __builtin_amdgcn_exp2f(a.part_ml[(slot + i * step) * 2] - at);
-        const int rt = (tile * 32 + row) / a.group, rh = hk * a.group + tile * 32 + row - rt * a.group;
+        const int rt = query_of(a, tile * 32 + row), rh = hk * a.group + tile * 32 + row - rt * a.group;
         const float inv = total == 0.f ? 0.f : 1.f / total;
         for (int d = lane; d < a.dim; d += 64) {
             float x = 0.f;
@@ -492,7 +492,7 @@ extern "C" int d8_attention(int dtype, const void *q, long ldq, const void *k, l
     if (int rc = attention::check(a, dtype, "attention")) return rc;
     if (!sequences || !q_tokens) return 0;
     D8_REQUIRE(q && o && q_starts && k_starts && (!k_tokens || (k && v)), "attention: null tensor");
-    a.group = heads / kv_heads;
+    attention::set_group(a);
     a.vec = attention::in_pieces(dtype, dim, {q, k, v}, {ldq, ldk, ldv});
     // (a tile's rows are addressed by 32 bits)
     const bool fast = a.vec && attention::in_pieces(dtype, dim, {o}, {ldo}) && ldk < (1 << 23) && ldv < (1 << 23);

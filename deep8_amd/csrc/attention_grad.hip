@@ -127,14 +127,14 @@ __global__ __launch_bounds__(256) void attention_grad_kv_any_kernel(Args a) {
             const int row = p / PIECES, d = (p - row * PIECES) * M::V;
             const int r = (int)r0 + row;
             const bool in = r < rows;
-            const int t = in ? r / group : 0, head = hk * group + (in ? r - t * group : 0);
+            const int t = in ? query_of(a, r) : 0, head = hk * group + (in ? r - t * group : 0);
             *(frag *)(tile_q + row * PITCH + d * (int)sizeof(T)) = load_piece<T>((const T *)a.q + (long)(sp.q0 + t) * a.ldq + (long)head * a.dim, d, a.dim, in, a.vec);
             *(frag *)(tile_g + row * PITCH + d * (int)sizeof(T)) = load_piece<T>((const T *)a.dout + (long)(sp.q0 + t) * a.lddo + (long)head * a.dim, d, a.dim, in, a.vec);
         }
         if (tid < TILE) {
             const int r = (int)r0 + tid;
             const bool in = r < rows;
-            const int t = in ? r / group : 0, head = hk * group + (in ? r - t * group : 0);
+            const int t = in ? query_of(a, r) : 0, head = hk * group + (in ? r - t * group : 0);
             const long at = (long)head * a.q_tokens + sp.q0 + t;
             row_lse[tid] = in ? a.lse[at] * LOG2E - shift : INFINITY;
             row_delta[tid] = in ? a.delta[at] : 0.f;
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256) void attention_grad_q_any_kernel(Args a) {
     const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
     const int r = tile * ROWS + wave * 32 + (lane & 31);
     const bool there = r < rows;
-    const int t = there ? r / group : 0, head = hk * group + (there ? r - t * group : 0);
+    const int t = there ? query_of(a, r) : 0, head = hk * group + (there ? r - t * group : 0);
     frag qf[UNITS], gf[UNITS];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256) void attention_grad_q_any_kernel(Args a) {
     const long at = (long)head * a.q_tokens + sp.q0 + t;
     const float lse = there ? a.lse[at] * LOG2E - shift : INFINITY, delta = there ? a.delta[at] : 0.f;
     const int last = !there ? -1 : a.causal ? min(sp.nk - 1, t + back) : sp.nk - 1;
-    const int t_end = (min(rows, (tile + 1) * ROWS) - 1) / group;
+    const int t_end = query_of(a, min(rows, (tile + 1) * ROWS) - 1);
     const int end = a.causal ? min(sp.nk, t_end + back + 1) : sp.nk;
     f32x16 dq[DP / 32];
 #pragma unroll
@@ -291,82 +291,112 @@ template <class T, int DP, int SPLIT>
 struct Shape {
     static constexpr int PB = row_bytes<T, DP>(), OWN = 128 / SPLIT, BLOCKS = PB <= 256 || SPLIT == 2 ? 2 : 1;
     static constexpr int KB = 32 * BLOCKS, TILE_BYTES = KB * PB, LOADS = TILE_BYTES / 1024 / 4;
-    static constexpr int OCCUPANCY = DP * (int)sizeof(T) <= 256 ? 2 : 1;
+    static constexpr int OCCUPANCY = DP * (int)sizeof(T) <= 256 ? 2 : 1;     // waves of a SIMD, dq
+    static constexpr int OCCUPANCY_KV = DP * (int)sizeof(T) <= 256 ? 2 : 1;  // ... dk and dv, whose sums and operands alone are 192 registers at 128 halves
+    // dk and dv at 128 halves, two waves of a SIMD: the registers are a few fragments short, and the compiler's own way out would be scratch memory,
+    // whose answers wait behind the tiles on their way (waits are in order); so some fragments of the values stay in LDS
+    static constexpr int SPARE = DP == 128 && sizeof(T) == 2 ? 3 : 0;
     static_assert(LOADS >= 1 && 4 * TILE_BYTES <= 160 * 1024, "a tile is at least a load of every wave, and two stages fit");
 };
 
-// rows of q or do (of all heads of a group) on their way into a tile
+// The rows that dk and dv walk are ordered so that those of one load are neighbours in memory: CT tokens (the rows of a load) of one head, then
+// the same tokens of the group's next head.  Row r is token Q CT + r % CT of head g with r / CT = Q group + g.  A load then has one
+// descriptor and an offset that a lane keeps, instead of a division and two products for each row.
 template <class T, int PB>
-struct RowLoader {
-    int lane_row, lane_pos, pieces;
-    __device__ __forceinline__ void init(int dim, int lane) { lane_row = lane / (PB / 16), lane_pos = lane % (PB / 16), pieces = dim / Type<T>::V; }
-    // `first`: query t0's first head; row r0 + i of the sequence goes to row i of the tile
-    __device__ __forceinline__ void load(const T *first, long ld, int dim, int group, int r0, int t0, int rows, int i0, unsigned tile) const {
-        constexpr int PER = TileLoader<T, PB>::ROWS;
-        const unsigned long p = (unsigned long)first;
-        const desc_t d = desc_t{(unsigned)__builtin_amdgcn_readfirstlane((int)p), (unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
-        const int i = i0 * PER + lane_row, r = r0 + i, t = r / group, piece = lane_pos ^ swizzle<PB>(i);
-        const unsigned at = (unsigned)(t - t0) * (unsigned)(ld * sizeof(T)) + (unsigned)((r - t * group) * dim * (int)sizeof(T) + piece * 16);
-        load_to_lds(d, r < rows && piece < pieces ? at : 0x80000000u, __builtin_amdgcn_readfirstlane(tile + i0 * 1024));
+struct ChunkLoader {
+    static constexpr int CT = TileLoader<T, PB>::ROWS;
+    // LOADS loads from load `first` of the tile that starts at row r0 on; `x` is the group's first head of the sequence's first query.  What
+    // lies beyond the last query is beyond the descriptor.
+    template <int LOADS, int KB>
+    static __device__ __forceinline__ void load(const Args &a, const TileLoader<T, PB> &l, const T *x, long ld, int nq, int r0, int first, unsigned tile) {
+        const int t0 = query_of(a, r0 / CT) * CT, chunk = r0 / CT + first;
+        int Q = query_of(a, chunk), g = chunk - Q * a.group;
+        const unsigned long p = (unsigned long)(x + (long)t0 * ld);
+        const unsigned row = (unsigned)(ld * sizeof(T)), head = (unsigned)a.dim * (unsigned)sizeof(T);
+        const int left = min(nq - t0, KB + CT);
+        const desc_t d = {(unsigned)__builtin_amdgcn_readfirstlane((int)p), (unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32)) & 0xffffu,
+                          (unsigned)__builtin_amdgcn_readfirstlane(left > 0 ? (int)((left - 1) * row + a.group * head) : 0), 0x00020000u};
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int piece = l.lane_pos ^ swizzle<PB>((first + i) * CT + l.lane_row);
+            const unsigned at = (unsigned)(Q * CT - t0) * row + (unsigned)g * head;
+            load_to_lds(d, piece < l.pieces ? l.voff + piece * 16 + at : 0x80000000u, __builtin_amdgcn_readfirstlane(tile + (first + i) * 1024));
+            const bool wrap = g + 1 == a.group;
+            g = wrap ? 0 : g + 1, Q += wrap ? 1 : 0;
+        }
     }
+    static __device__ __forceinline__ int token(const Args &a, int r, int &g) {
+        const int chunk = r / CT, Q = query_of(a, chunk);
+        g = chunk - Q * a.group;
+        return Q * CT + r % CT;
+    }
+    static __device__ __forceinline__ int rows(const Args &a, int nq) { return (nq + CT - 1) / CT * CT * a.group; }
 };
 
 template <class T, int DP, int SPLIT>
-__global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attention_grad_kv_kernel(Args a) {
+__global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void attention_grad_kv_kernel(Args a) {
     typedef Type<T> M;
     typedef typename M::frag frag;
     typedef Shape<T, DP, SPLIT> S;
     constexpr int PB = S::PB, UNITS = DP / M::STEP, N = DP / 32;
     __shared__ __attribute__((aligned(1024))) char lds[4 * S::TILE_BYTES];
     __shared__ __attribute__((aligned(16))) float row_lse[2][S::KB], row_delta[2][S::KB];
+    __shared__ __attribute__((aligned(16))) frag spare[S::SPARE ? S::SPARE : 1][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int hk = blockIdx.x % a.kv_heads;
     Span sp;
     int seq, block;
     if (!locate(a, blockIdx.x / a.kv_heads, sp, seq, block, [](const Span &s) { return (s.nk + S::OWN - 1) / S::OWN; })) return;
-    const int group = a.group, rows = sp.nq * group, back = sp.nk - sp.nq;
+    typedef ChunkLoader<T, PB> Rows;
+    const int group = a.group, rows = Rows::rows(a, sp.nq), back = sp.nk - sp.nq;
     const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
-    const int j0 = block * S::OWN + wave % (4 / SPLIT) * 32, j = j0 + (lane & 31);  // the wave's first key, the lane's
-    const bool there = j < sp.nk;
-    const long key = sp.k0 + (there ? j : 0);
-    frag kf[UNITS], vf[UNITS];
+    const int j0 = block * S::OWN + wave % (4 / SPLIT) * 32;  // the wave's first key
+    frag kf[UNITS], vf[UNITS - S::SPARE];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
+        const int j = j0 + (lane & 31);
+        const bool there = j < sp.nk;
+        const long key = sp.k0 + (there ? j : 0);
         kf[u] = load_piece<T>((const T *)a.k + key * a.ldk + (long)hk * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
-        vf[u] = load_piece<T>((const T *)a.v + key * a.ldv + (long)hk * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
+        const frag v = load_piece<T>((const T *)a.v + key * a.ldv + (long)hk * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
+        if (u < UNITS - S::SPARE) vf[u] = v;
+        else spare[u - (UNITS - S::SPARE)][tid] = v;
     }
     f32x16 dk[N], dv[N];
 #pragma unroll
     for (int b = 0; b < N; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[b][e] = dv[b][e] = 0.f;
-    RowLoader<T, PB> loader;
-    loader.init(a.dim, lane);
     const unsigned lds0 = lds_address(lds);
     const T *q = (const T *)a.q + (long)sp.q0 * a.ldq + (long)hk * group * a.dim, *g = (const T *)a.dout + (long)sp.q0 * a.lddo + (long)hk * group * a.dim;
     float next_lse = 0.f, next_delta = 0.f;  // of row tid of the next tile
     auto fetch = [&](int r0, int stage) {
-        const int t0 = r0 / group;
-#pragma unroll
-        for (int i = 0; i < S::LOADS; ++i) loader.load(q + (long)t0 * a.ldq, a.ldq, a.dim, group, r0, t0, rows, wave * S::LOADS + i, lds0 + stage * 2 * S::TILE_BYTES);
-#pragma unroll
-        for (int i = 0; i < S::LOADS; ++i)
-            loader.load(g + (long)t0 * a.lddo, a.lddo, a.dim, group, r0, t0, rows, wave * S::LOADS + i, lds0 + stage * 2 * S::TILE_BYTES + S::TILE_BYTES);
+        int fl = lane;
+        asm volatile("" : "+v"(fl));  // (what follows from the lane is formed anew each time: registers are what this kernel is short of)
+        TileLoader<T, PB> lq, lg;
+        lq.init(a.ldq, a.dim, fl), lg.init(a.lddo, a.dim, fl);
+        const int tid = wave * 64 + fl;
+        Rows::template load<S::LOADS, S::KB>(a, lq, q, a.ldq, sp.nq, r0, wave * S::LOADS, lds0 + stage * 2 * S::TILE_BYTES);
+        Rows::template load<S::LOADS, S::KB>(a, lg, g, a.lddo, sp.nq, r0, wave * S::LOADS, lds0 + stage * 2 * S::TILE_BYTES + S::TILE_BYTES);
         if (tid < S::KB) {
-            const int r = r0 + tid;
-            const bool in = r < rows;
-            const int t = in ? r / group : 0;
-            const long at = (long)(hk * group + (in ? r - t * group : 0)) * a.q_tokens + sp.q0 + t;
+            int head;
+            const int t = Rows::token(a, r0 + tid, head);
+            const bool in = t < sp.nq;
+            const long at = (long)(hk * group + head) * a.q_tokens + sp.q0 + (in ? t : 0);
             next_lse = in ? a.lse[at] * LOG2E - shift : INFINITY;  // (rows that are not there: probability zero)
             next_delta = in ? a.delta[at] * mult : 0.f;
         }
     };
     // the first row that sees a key of the block (its query is the block's first key less nk - nq)
-    const long first = a.causal ? (long)max(0, block * S::OWN - back) * group : 0;
+    const long first = a.causal ? (long)(max(0, block * S::OWN - back) / Rows::CT * Rows::CT) * group : 0;
     const int r_begin = (int)min(first / 32 * 32, (long)rows);
     if (r_begin < rows) fetch(r_begin, 0);
     for (int r0 = r_begin, stage = 0; r0 < rows; r0 += S::KB, stage ^= 1) {
-        if (tid < S::KB) row_lse[stage][tid] = next_lse, row_delta[stage][tid] = next_delta;
+        if (wave * 64 < S::KB) {
+            int wl = lane;
+            asm volatile("" : "+v"(wl));
+            if (wave * 64 + wl < S::KB) row_lse[stage][wave * 64 + wl] = next_lse, row_delta[stage][wave * 64 + wl] = next_delta;
+        }
         ATTN_VMCNT(0);
         lds_reads_done();
         __syncthreads();
@@ -375,28 +405,32 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
 #pragma unroll 1
         for (int i = 0; i < S::BLOCKS / SPLIT; ++i) {
             const int b = SPLIT == 1 ? i : wave / (4 / SPLIT), rb = r0 + b * 32;
-            // queries of the block's first and last row: what the first sees, all see; what the last does not see, none sees
-            if (rb >= rows || (a.causal && j0 > (min(rb + 31, rows - 1)) / group + back)) continue;
+            // (a block of rows that see none of the wave's keys is masked, not left out: a way round the products makes the compiler move the sums
+            // to and fro, and few are such)
+            int l = lane;
+            asm volatile("" : "+v"(l));  // fragments' addresses are formed here, not kept in registers across the loop
             f32x16 s, w;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = w[e] = 0.f;
 #pragma unroll
-            for (int u = 0; u < UNITS; ++u) M::mma(s, rows_frag<T, PB>(tq, b * 32, u, lane), kf[u]);
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u) M::mma(w, rows_frag<T, PB>(tg, b * 32, u, lane), vf[u]);
+            for (int u = 0; u < UNITS; ++u) {
+                M::mma(s, rows_frag<T, PB>(tq, b * 32, u, l), kf[u]);
+                M::mma(w, rows_frag<T, PB>(tg, b * 32, u, l), u < UNITS - S::SPARE ? vf[u] : spare[u - (UNITS - S::SPARE)][wave * 64 + l]);
+            }
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-                const f32x4 l4 = *(const f32x4 *)&row_lse[stage][b * 32 + 2 * e + 4 * h], d4 = *(const f32x4 *)&row_delta[stage][b * 32 + 2 * e + 4 * h];
+                const f32x4 l4 = *(const f32x4 *)&row_lse[stage][b * 32 + 2 * e + 4 * (l >> 5)], d4 = *(const f32x4 *)&row_delta[stage][b * 32 + 2 * e + 4 * (l >> 5)];
 #pragma unroll
                 for (int i4 = 0; i4 < 4; ++i4) {
                     s[e + i4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + i4], c, -l4[i4]));
                     w[e + i4] = __builtin_fmaf(w[e + i4], mult, -d4[i4]);
                 }
             }
-            if (a.causal && j0 + 31 > rb / group + back) {
+            if (a.causal && j0 + 31 > query_of(a, rb / Rows::CT) * Rows::CT + back) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const bool seen = j <= (rb + 8 * (e >> 2) + 4 * h + (e & 3)) / group + back;
+                    int head;
+                    const bool seen = j0 + (l & 31) <= Rows::token(a, rb + 8 * (e >> 2) + 4 * (l >> 5) + (e & 3), head) + back;
                     s[e] = seen ? s[e] : 0.f, w[e] = seen ? w[e] : 0.f;
                 }
             }
@@ -406,15 +440,18 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
             for (int u = 0; u < 32 / M::STEP; ++u) {
                 const frag p = M::pack(s, u), d = M::pack(w, u);
 #pragma unroll
-                for (int n = 0; n < N; ++n) M::mma(dv[n], cols_frag<T, PB>(tg, b * 32 + u * M::STEP, n * 32, lane), p);
-#pragma unroll
-                for (int n = 0; n < N; ++n) M::mma(dk[n], cols_frag<T, PB>(tq, b * 32 + u * M::STEP, n * 32, lane), d);
+                for (int n = 0; n < N; ++n) {
+                    M::mma(dv[n], cols_frag<T, PB>(tg, b * 32 + u * M::STEP, n * 32, l), p);
+                    M::mma(dk[n], cols_frag<T, PB>(tq, b * 32 + u * M::STEP, n * 32, l), d);
+                }
             }
         }
     }
+    int el = lane;
+    asm volatile("" : "+v"(el));
     if constexpr (SPLIT == 2) {
         __syncthreads();
-        float *to = (float *)lds + (wave & 1) * 2 * N * 16 * 64 + lane;
+        float *to = (float *)lds + (wave & 1) * 2 * N * 16 * 64 + el;
         if (wave >= 2) {
 #pragma unroll
             for (int n = 0; n < N; ++n)
@@ -428,11 +465,13 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
 #pragma unroll
             for (int e = 0; e < 16; ++e) dk[n][e] += to[(n * 16 + e) * 64], dv[n][e] += to[((N + n) * 16 + e) * 64];
     }
-    if (!there) return;
+    const int j = j0 + (el & 31);
+    if (j >= sp.nk) return;
+    const long key = sp.k0 + j;
     const float unshift = exp2f(-shift), by = a.scale * unshift / mult;
     T *pk = (T *)a.dk + key * a.lddk + (long)hk * a.dim, *pv = (T *)a.dv + key * a.lddv + (long)hk * a.dim;
-    store_sums<T, DP>(pk, dk, by, a.dim, h, a.overwrite & 2);
-    store_sums<T, DP>(pv, dv, unshift, a.dim, h, a.overwrite & 4);
+    store_sums<T, DP>(pk, dk, by, a.dim, el >> 5, a.overwrite & 2);
+    store_sums<T, DP>(pv, dv, unshift, a.dim, el >> 5, a.overwrite & 4);
 }
 
 template <class T, int DP, int SPLIT>
@@ -453,7 +492,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
     const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
     const int r = tile * S::OWN + wave % (4 / SPLIT) * 32 + (lane & 31);
     const bool there = r < rows;
-    const int t = (there ? r : rows - 1) / group, head = hk * group + (there ? r - t * group : 0);
+    const int t = query_of(a, there ? r : rows - 1), head = hk * group + (there ? r - t * group : 0);
     frag qf[UNITS], gf[UNITS];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -464,7 +503,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
     const float lse = there ? a.lse[at] * LOG2E - shift : INFINITY;
     float delta = there ? a.delta[at] * mult : 0.f;
     const int last = a.causal ? min(sp.nk - 1, t + back) : sp.nk - 1;
-    const int end = a.causal ? min(sp.nk, (min(rows, (tile + 1) * S::OWN) - 1) / group + back + 1) : sp.nk;
+    const int end = a.causal ? min(sp.nk, query_of(a, min(rows, (tile + 1) * S::OWN) - 1) + back + 1) : sp.nk;
     const int wave_all = __builtin_amdgcn_readfirstlane(__shfl(last, 0)), wave_end = __builtin_amdgcn_readfirstlane(__shfl(last, 31)) + 1;
     f32x16 dq[N];
 #pragma unroll
@@ -633,7 +672,7 @@ extern "C" int d8_attention_grad(int dtype, const void *q, long ldq, const void 
     const size_t need = attention::grad_scratch_bytes(q_tokens, heads);
     D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_grad: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
     a.norms = (float *)scratch, a.delta = a.norms + 2 * attention::NORM_GROUPS;
-    a.group = heads / kv_heads;
+    attention::set_group(a);
     a.vec = attention::in_pieces(dtype, dim, {q, k, v, o, dout}, {ldq, ldk, ldv, ldo, lddo});
     // (a tile's rows are addressed by 31 bits)
     const long most = 1 << 21;
