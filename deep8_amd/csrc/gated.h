@@ -1,0 +1,54 @@
+// Arguments of the gated product's kernels and what they share (gated.hip, gated_wide.hip).
+#ifndef DEEP8_AMD_GATED_H
+#define DEEP8_AMD_GATED_H
+
+#include "attention.h"
+
+namespace d8 {
+namespace gated {
+
+struct Args {
+    const void *x, *w;
+    void *pre, *h;
+    const void *dh;
+    void *dpre;
+    int rows, inner, cols, act;
+    // x and w as they lie: row strides, where the factor's columns begin, elements of a row (a half row of w) with the zeros behind it
+    long ldx, ldw;
+    int up, inner_there, cols_there;
+    int chunk, parts;  // few rows: K of a workgroup, and how many it is cut into
+    float *part;       // ... their sums [parts][rows][2 cols]
+    int vec;           // the way back: rows of pre, dh and dpre can be moved in 16-byte pieces
+};
+
+// Half: the hardware's reciprocal and power of two, good to 1 ulp of fp32.
+template <class T>
+__device__ __forceinline__ float sigmoid(float a) {
+    if (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * a));
+    return 1.f / (1.f + expf(-a));
+}
+
+template <class T>
+__device__ __forceinline__ float activation(float a, int act) {
+    switch (act) {
+        case D8_GATE_SILU: return a * sigmoid<T>(a);
+        case D8_GATE_GELU: return 0.5f * a * (1.f + erff(a * 0.70710678f));
+        case D8_GATE_RELU: return a > 0.f ? a : 0.f;
+        default: return sigmoid<T>(a);
+    }
+}
+
+// element (m, n) of both projections into h and, if it is kept, pre
+template <class T>
+__device__ __forceinline__ void store(const Args &a, int m, int n, float g, float u) {
+    ((T *)a.h)[(long)m * a.cols + n] = (T)(activation<T>(g, a.act) * u);
+    if (a.pre) {
+        T *p = (T *)a.pre + (long)m * 2 * a.cols + n;
+        p[0] = (T)g, p[a.cols] = (T)u;
+    }
+}
+
+}  // namespace gated
+}  // namespace d8
+
+#endif

@@ -4,29 +4,19 @@
 // Both projections, the activation and the product are one kernel: a workgroup has the same columns of both halves, a lane's
 // accumulators hold the gate and the factor of the same elements, and h is formed from the fp32 sums.  pre is written
 // (rounded once) only where the way back will need it.
-#include "attention.h"
+//
+// Three kernels: many rows and columns in half on 256 x 256 tiles (gated_wide.hip); few rows, where reading w is the work (below:
+// gated_rows_kernel); everything else on 128 x 64 tiles.  All move operands in 16-byte pieces; operands whose rows do not start at
+// multiples of 16 bytes are copied to rows that do, into scratch, first.
+#include "gated.h"
 
 namespace d8 {
 namespace gated {
 namespace {
 
-struct Args {
-    const void *x, *w;
-    void *pre, *h;
-    const void *dh;
-    void *dpre;
-    int rows, inner, cols, act;
-    int vec_x, vec_w;
-};
-
-__device__ __forceinline__ float activation(float a, int act) {
-    switch (act) {
-        case D8_GATE_SILU: return a / (1.f + expf(-a));
-        case D8_GATE_GELU: return 0.5f * a * (1.f + erff(a * 0.70710678f));
-        case D8_GATE_RELU: return a > 0.f ? a : 0.f;
-        default: return 1.f / (1.f + expf(-a));
-    }
-}
+using attention::desc_t;
+using attention::load_to_lds;
+using attention::swizzle;
 
 // activation and its slope
 __device__ __forceinline__ void activation_slope(float a, int act, float &f, float &df) {
@@ -51,44 +41,94 @@ __device__ __forceinline__ void activation_slope(float a, int act, float &f, flo
     }
 }
 
+// The columns of one workgroup on their way into a tile of `rows of w` x PB bytes: the gate's in the first half of a row, the factor's in the second.
+template <class T, int PB>
+struct WeightLoader {
+    static constexpr int V = attention::Type<T>::V, ROWS = 1024 / PB, HALF = PB / 32;  // rows of a load, pieces of half a row
+    int lane_row, lane_pos, left;  // left: pieces of the columns that are there
+    unsigned stride, up;
+    __device__ __forceinline__ void init(const Args &a, int n0, int lane) {
+        lane_row = lane / (PB / 16), lane_pos = lane % (PB / 16), left = (a.cols_there - n0) / V;
+        stride = (unsigned)a.ldw * (unsigned)sizeof(T), up = (unsigned)a.up * (unsigned)sizeof(T);
+    }
+    // row k0's column n0 of w on, `rows` rows
+    __device__ __forceinline__ desc_t desc(const Args &a, int k0, int n0, int rows) const {
+        const unsigned long p = (unsigned long)((const T *)a.w + (long)k0 * a.ldw + n0);
+        const unsigned bytes = rows > 0 ? (unsigned)(rows - 1) * stride + up + (unsigned)(a.cols_there - n0) * (unsigned)sizeof(T) : 0u;
+        return desc_t{(unsigned)__builtin_amdgcn_readfirstlane((int)p), (unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32)) & 0xffffu,
+                      (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+    }
+    __device__ __forceinline__ void load(const desc_t &d, int t, unsigned tile) const {
+        const int row = t * ROWS + lane_row, c = lane_pos ^ swizzle<PB>(row), second = c >= HALF, piece = c - (second ? HALF : 0);
+        load_to_lds(d, piece < left ? row * stride + (second ? up : 0u) + piece * 16 : 0x80000000u, __builtin_amdgcn_readfirstlane(tile + t * 1024));
+    }
+};
+
+// columns c0 .. c0 + 31 of a tile of w as an operand fragment whose k is in the order of read_rows
+template <class T, int PB>
+__device__ __forceinline__ typename attention::Type<T>::frag weight_frag(const char *tile, int r0, int c0, int lane) {
+    if constexpr (sizeof(T) == 2) {
+        typedef attention::tr_f16x4 tr;
+        const int i = lane & 15, j = lane >> 4, row = r0 + 8 * (j >> 1) + (i >> 2), at = c0 * 2 + 32 * (j & 1) + 8 * (i & 3);
+        const char *lo = tile + row * PB + ((((at >> 4) ^ swizzle<PB>(row)) << 4) | (at & 15));
+        const char *hi = tile + (row + 4) * PB + ((((at >> 4) ^ swizzle<PB>(row + 4)) << 4) | (at & 15));
+        const tr x = __builtin_amdgcn_ds_read_tr16_b64_v4f16(ATTN_LDS(tr, lo)), y = __builtin_amdgcn_ds_read_tr16_b64_v4f16(ATTN_LDS(tr, hi));
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+        return attention::cols_frag<T, PB>(tile, r0, c0, lane);
+    }
+}
+
+// 128 rows x 64 columns of both halves a workgroup, a wave 64 x 32 of each.  K in steps of 128 bytes of x, both tiles straight into one of two
+// stages of LDS, the next step's while this one is worked on.
 enum { BM = 128, BN = 64 };
 
-// 128 rows x 64 columns of both halves a workgroup, a wave 64 x 32 of each
 template <class T>
-__global__ __launch_bounds__(256) void gated_tile_kernel(Args a) {
+__global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
     typedef attention::Type<T> M;
     typedef typename M::frag frag;
-    constexpr int BK = 2 * M::STEP, PX = BK * (int)sizeof(T) + 16, PW = 2 * BN * (int)sizeof(T) + 16;
-    __shared__ __attribute__((aligned(16))) char tile_x[BM * PX], tile_w[BK * PW];
+    constexpr int PX = 128, BK = PX / (int)sizeof(T), PW = 2 * BN * (int)sizeof(T), TX = BM * PX, TW = BK * PW;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * (TX + TW)];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN, wm = (wave >> 1) * 64, wn = (wave & 1) * 32;
-    const T *x = (const T *)a.x, *w = (const T *)a.w;
+    // (the workgroups of an XCD, ids congruent mod 8, have a run of row tiles by columns: what they share stays in its L2)
+    const int tiles_m = (a.rows + BM - 1) / BM, total = gridDim.x;
+    int id = blockIdx.x;
+    if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
+    const int m0 = id % tiles_m * BM, n0 = id / tiles_m * BN, wm = (wave >> 1) * 64, wn = (wave & 1) * 32;
+    attention::TileLoader<T, PX> lx;
+    lx.init(a.ldx, a.inner, lane);
+    WeightLoader<T, PW> lw;
+    lw.init(a, n0, lane);
+    const unsigned lds0 = attention::lds_address(lds);
+    auto fetch = [&](int k0, int stage) {
+        const unsigned to = lds0 + stage * (TX + TW);
+        lx.pieces = (a.inner_there - k0) / M::V;
+        const desc_t dx = lx.desc((const T *)a.x + (long)m0 * a.ldx + k0, min(BM, a.rows - m0), a.ldx, a.inner_there - k0);
+        const desc_t dw = lw.desc(a, k0, n0, min(BK, a.inner - k0));
+#pragma unroll
+        for (int i = 0; i < TX / 4096; ++i) lx.load(dx, wave * (TX / 4096) + i, to);
+#pragma unroll
+        for (int i = 0; i < TW / 4096; ++i) lw.load(dw, wave * (TW / 4096) + i, to + TX);
+    };
     f32x16 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i >> 1][i & 1][e] = 0.f;
-    for (int k0 = 0; k0 < a.inner; k0 += BK) {
+    fetch(0, 0);
+    for (int k0 = 0, stage = 0; k0 < a.inner; k0 += BK, stage ^= 1) {
+        ATTN_VMCNT(0);
+        attention::lds_reads_done();
         __syncthreads();
-        for (int p = tid; p < BM * BK / M::V; p += 256) {
-            const int r = p / (BK / M::V), c = p % (BK / M::V) * M::V;
-            const bool in = m0 + r < a.rows;
-            *(frag *)(tile_x + r * PX + c * (int)sizeof(T)) = attention::load_piece<T>(x + (long)(in ? m0 + r : 0) * a.inner, k0 + c, a.inner, in, a.vec_x);
-        }
-        for (int p = tid; p < BK * 2 * BN / M::V; p += 256) {
-            const int r = p / (2 * BN / M::V), c = p % (2 * BN / M::V) * M::V, up = c >= BN;
-            const bool in = k0 + r < a.inner;
-            *(frag *)(tile_w + r * PW + c * (int)sizeof(T)) =
-                attention::load_piece<T>(w + (long)(in ? k0 + r : 0) * 2 * a.cols + (up ? a.cols : 0), n0 + c - (up ? BN : 0), a.cols, in, a.vec_w);
-        }
-        __syncthreads();
+        if (k0 + BK < a.inner) fetch(k0 + BK, stage ^ 1);
+        const char *tx = lds + stage * (TX + TW), *tw = tx + TX;
 #pragma unroll
         for (int u = 0; u < BK / M::STEP; ++u) {
             frag xf[2], wf[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                xf[i] = attention::read_rows<T>(tile_x + (wm + i * 32) * PX, PX, u, lane);
-                wf[i] = M::template read_cols<true>(tile_w, PW, u * M::STEP, i * BN + wn, lane);
+                xf[i] = attention::rows_frag<T, PX>(tx, wm + i * 32, u, lane);
+                wf[i] = weight_frag<T, PW>(tw, u * M::STEP, i * BN + wn, lane);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -103,14 +143,122 @@ __global__ __launch_bounds__(256) void gated_tile_kernel(Args a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (m >= a.rows) continue;
-            const float g = acc[i][0][e], u = acc[i][1][e];
-            ((T *)a.h)[(long)m * a.cols + n] = (T)(activation(g, a.act) * u);
-            if (a.pre) {
-                T *p = (T *)a.pre + (long)m * 2 * a.cols + n;
-                p[0] = (T)g, p[a.cols] = (T)u;
+            if (m < a.rows) store<T>(a, m, n, acc[i][0][e], acc[i][1][e]);
+        }
+}
+
+// Few rows.  A workgroup has 128 bytes of columns of both halves and a chunk of K, of which its four waves take every fourth tile of 32 rows of w,
+// each with two stages of LDS of its own and no barrier; all rows of x (32 RB at most) are the other operand.  The waves' sums are joined through LDS; those of several chunks go through scratch (gated_join_kernel).
+template <class T, int RB>
+__global__ __launch_bounds__(256, (RB == 1 && sizeof(T) == 2 ? 2 : 1)) void gated_rows_kernel(Args a) {
+    typedef attention::Type<T> M;
+    typedef typename M::frag frag;
+    constexpr int PB = 256, BK = 32, TILE = BK * PB, LOADS = TILE / 1024, COLS = 128 / (int)sizeof(T), N = 2 * COLS / 32, UNITS = BK / M::STEP;
+    constexpr int PX = BK * (int)sizeof(T), TX = RB * 32 * PX, LOADS_X = TX / 1024, STAGE = TILE + TX;
+    constexpr int JOIN = 4 * N * RB * 16 * 64 * 4, STAGES = 4 * 2 * STAGE;
+    __shared__ __attribute__((aligned(1024))) char lds[JOIN > STAGES ? JOIN : STAGES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int blocks = (a.cols + COLS - 1) / COLS, n0 = blockIdx.x % blocks * COLS, part = blockIdx.x / blocks;
+    const int begin = part * a.chunk, end = min(a.inner, begin + a.chunk);
+    WeightLoader<T, PB> lw;
+    lw.init(a, n0, lane);
+    attention::TileLoader<T, PX> lx;
+    lx.init(a.ldx, a.inner, lane);
+    const unsigned to = attention::lds_address(lds) + wave * 2 * STAGE;
+    const int there = min((end + M::V - 1) / M::V * M::V, a.inner_there);  // of a row of x (chunks are whole pieces; zeros behind the last)
+    auto fetch = [&](int k0, int stage) {
+        const desc_t d = lw.desc(a, k0, n0, min(BK, end - k0)), dx = lx.desc((const T *)a.x + k0, a.rows, a.ldx, there - k0);
+        lx.pieces = (there - k0) / M::V;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) lw.load(d, i, to + stage * STAGE);
+#pragma unroll
+        for (int i = 0; i < LOADS_X; ++i) lx.load(dx, i, to + stage * STAGE + TILE);
+    };
+    f32x16 acc[N][RB];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[n][r][e] = 0.f;
+    int k0 = begin + wave * BK;
+    if (k0 < end) fetch(k0, 0);
+    for (int stage = 0; k0 < end; k0 += 4 * BK, stage ^= 1) {
+        if (k0 + 4 * BK < end) {
+            fetch(k0 + 4 * BK, stage ^ 1);
+            ATTN_VMCNT(LOADS + LOADS_X);  // everything but the next tile has landed
+        } else {
+            ATTN_VMCNT(0);
+        }
+        asm volatile("" ::: "memory");
+        const char *tw = lds + wave * 2 * STAGE + stage * STAGE, *tx = tw + TILE;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            frag xf[RB];
+#pragma unroll
+            for (int r = 0; r < RB; ++r) xf[r] = attention::rows_frag<T, PX>(tx, r * 32, u, lane);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const frag wf = weight_frag<T, PB>(tw, u * M::STEP, n * 32, lane);
+#pragma unroll
+                for (int r = 0; r < RB; ++r) M::mma(acc[n][r], wf, xf[r]);
             }
         }
+        attention::lds_reads_done();
+    }
+    // element (column i, row j) of block (n, r) lies in lane j + 32 h, register e, i = 8 (e / 4) + 4 h + e % 4
+    __syncthreads();
+    float *all = (float *)lds;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) all[((wave * N + n) * RB + r) * 1024 + e * 64 + lane] = acc[n][r][e];
+    __syncthreads();
+    // a thread has a column of the block for every so many rows
+    for (int i = tid; i < COLS * a.rows; i += 256) {
+        const int c = i % COLS, row = i / COLS, n = n0 + c;
+        if (n >= a.cols) continue;
+        const int at = ((c >> 5) * RB + (row >> 5)) * 1024 + (((c & 31) >> 3) * 4 + (c & 3)) * 64 + (row & 31) + 32 * ((c >> 2) & 1);
+        float g = 0.f, u = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) g += all[w * N * RB * 1024 + at], u += all[(w * N + N / 2) * RB * 1024 + at];
+        if (a.parts == 1) {
+            store<T>(a, row, n, g, u);
+        } else {
+            float *p = a.part + ((long)part * a.rows + row) * 2 * a.cols + n;
+            p[0] = g, p[a.cols] = u;
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void gated_join_kernel(Args a) {
+    const long n = (long)a.rows * a.cols, i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int row = (int)(i / a.cols), c = (int)(i - (long)row * a.cols);
+    float g = 0.f, u = 0.f;
+    for (int p = 0; p < a.parts; ++p) {
+        const float *from = a.part + ((long)p * a.rows + row) * 2 * a.cols + c;
+        g += from[0], u += from[a.cols];
+    }
+    store<T>(a, row, c, g, u);
+}
+
+// rows of `from` (width elements, `gap` elements after every `width`, as two halves where there are two) to rows that start at multiples of 16
+// bytes, zeros behind them
+template <class T>
+__global__ __launch_bounds__(256) void gated_copy_kernel(const T *from, T *to, long rows, int width, int padded) {
+    typedef typename attention::Type<T>::frag frag;
+    constexpr int V = attention::Type<T>::V;
+    const int per_row = padded / V;
+    const long n = rows * per_row;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+        const long row = i / per_row;
+        const int c = (int)(i - row * per_row) * V;
+        *(frag *)(to + row * padded + c) = attention::load_piece<T>(from + row * width, c, width, true, 0);
+    }
 }
 
 // dpre = (dh pre_u act'(pre_g), dh act(pre_g)); a thread has 16 bytes of each half
@@ -124,8 +272,8 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(Args a) {
         const long row = i / per_row;
         const int c = (int)(i - row * per_row) * V;
         const T *pre = (const T *)a.pre + row * 2 * a.cols;
-        const frag g = attention::load_piece<T>(pre, c, a.cols, true, a.vec_w), u = attention::load_piece<T>(pre + a.cols, c, a.cols, true, a.vec_w);
-        const frag d = attention::load_piece<T>((const T *)a.dh + row * a.cols, c, a.cols, true, a.vec_w);
+        const frag g = attention::load_piece<T>(pre, c, a.cols, true, a.vec), u = attention::load_piece<T>(pre + a.cols, c, a.cols, true, a.vec);
+        const frag d = attention::load_piece<T>((const T *)a.dh + row * a.cols, c, a.cols, true, a.vec);
         frag dg, du;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -134,7 +282,7 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(Args a) {
             dg[e] = (T)((float)d[e] * (float)u[e] * df), du[e] = (T)((float)d[e] * f);
         }
         T *to = (T *)a.dpre + row * 2 * a.cols;
-        if (a.vec_w) {
+        if (a.vec) {
             *(frag *)(to + c) = dg, *(frag *)(to + a.cols + c) = du;
         } else {
 #pragma unroll
@@ -148,9 +296,43 @@ size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 int check(int dtype, int rows, int inner, int cols, int act, const char *name) {
     if (dtype != D8_FLOAT16 && dtype != D8_FLOAT32) return fail(D8_ERR_DTYPE, "%s: type %d is not support", name, dtype);
-    D8_REQUIRE(rows >= 1 && inner >= 1 && cols >= 1 && cols < (1 << 30), "%s: %d x %d times %d x 2 * %d", name, rows, inner, inner, cols);
+    D8_REQUIRE(rows >= 1 && inner >= 1 && cols >= 1 && cols < (1 << 28) && inner < (1 << 28), "%s: %d x %d times %d x 2 * %d", name, rows, inner, inner, cols);
     D8_REQUIRE(act >= D8_GATE_SILU && act <= D8_GATE_SIGMOID, "%s: activation %d is not support", name, act);
     return 0;
+}
+
+enum { FEW_ROWS = 64 };
+
+// How a forward call runs and what it takes of the scratch: copies of x and w (bytes, 0: read as they lie), partial sums.
+struct Plan {
+    enum { ROWS, WIDE, TILES } way;
+    int parts, chunk;
+    size_t x_copy, w_copy, part;
+    size_t bytes() const { return x_copy + w_copy + part; }
+};
+
+Plan plan_of(int dtype, int rows, int inner, int cols, bool x_aligned, bool w_aligned) {
+    Plan p;
+    memset(&p, 0, sizeof(p));
+    const size_t es = dtype_bytes(dtype);
+    const int v = 16 / (int)es;
+    const long inner_p = (inner + v - 1L) / v * v, cols_p = (cols + v - 1L) / v * v;
+    if (!x_aligned || inner % v) p.x_copy = round256(es * rows * inner_p);
+    if (!w_aligned || cols % v) p.w_copy = round256(es * inner * 2 * cols_p);
+    if (rows <= FEW_ROWS) {
+        // two workgroups a compute unit, chunks of K of at least four tiles a wave's
+        p.way = Plan::ROWS;
+        const long blocks = (cols * (long)es + 127) / 128, most = (inner + 511) / 512;
+        long parts = blocks >= 2 * cu_count() ? 1 : (2 * cu_count() + blocks - 1) / blocks;
+        parts = parts > most ? most : parts;
+        p.chunk = (int)(((inner + parts - 1) / parts + 127) / 128 * 128);
+        p.parts = (int)((inner + p.chunk - 1L) / p.chunk);
+        if (p.parts > 1) p.part = round256(sizeof(float) * p.parts * (size_t)rows * 2 * cols);
+        return p;
+    }
+    p.way = Plan::TILES;
+    p.parts = 1, p.chunk = inner;
+    return p;
 }
 
 }  // namespace
@@ -160,27 +342,70 @@ int check(int dtype, int rows, int inner, int cols, int act, const char *name) {
 using namespace d8;
 
 extern "C" size_t d8_matmul_gated_scratch_bytes(int dtype, int which, int rows, int inner, int cols) {
-    if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || rows < 1 || inner < 1 || cols < 1 || cols >= (1 << 30)) return 0;
-    if (which != 1) return 0;
+    if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || rows < 1 || inner < 1 || cols < 1 || cols >= (1 << 28) || inner >= (1 << 28)) return 0;
+    if (which != 1) return gated::plan_of(dtype, rows, inner, cols, true, true).bytes();
     return gated::round256(dtype_bytes(dtype) * 2 * (size_t)rows * cols) + d8_matmul_scratch_bytes(dtype, 3, 1, rows, inner, 1, inner, 2 * cols);
 }
+
+namespace d8 {
+namespace gated {
+namespace {
+
+template <class T>
+int copy_rows(const void *from, void *to, long rows, int width, int padded, hipStream_t stream) {
+    const long groups = (rows * (padded / attention::Type<T>::V) + 255) / 256;
+    hipLaunchKernelGGL(gated_copy_kernel<T>, dim3((unsigned)(groups < 8192 ? groups : 8192)), dim3(256), 0, stream, (const T *)from, (T *)to, rows, width, padded);
+    D8_LAUNCH_CHECK();
+    return 0;
+}
+
+template <class T>
+int forward(Args a, const Plan &p, char *scratch, hipStream_t stream) {
+    constexpr int V = attention::Type<T>::V;
+    a.ldx = a.inner_there = a.inner, a.ldw = 2L * a.cols, a.up = a.cols_there = a.cols;
+    if (p.x_copy) {
+        a.ldx = a.inner_there = (a.inner + V - 1) / V * V;
+        if (int rc = copy_rows<T>(a.x, scratch, a.rows, a.inner, a.inner_there, stream)) return rc;
+        a.x = scratch, scratch += p.x_copy;
+    }
+    if (p.w_copy) {  // (a row of w is two rows of `cols`)
+        a.up = a.cols_there = (a.cols + V - 1) / V * V, a.ldw = 2L * a.up;
+        if (int rc = copy_rows<T>(a.w, scratch, 2L * a.inner, a.cols, a.cols_there, stream)) return rc;
+        a.w = scratch, scratch += p.w_copy;
+    }
+    a.part = (float *)scratch, a.parts = p.parts, a.chunk = p.chunk;
+    if (p.way == Plan::ROWS) {
+        const dim3 grid((unsigned)ceil_div((long)a.cols * sizeof(T), 128) * p.parts);
+        if (a.rows <= 32) hipLaunchKernelGGL((gated_rows_kernel<T, 1>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((gated_rows_kernel<T, 2>), grid, dim3(256), 0, stream, a);
+        D8_LAUNCH_CHECK();
+        if (p.parts == 1) return 0;
+        hipLaunchKernelGGL(gated_join_kernel<T>, dim3(ceil_div((long)a.rows * a.cols, 256)), dim3(256), 0, stream, a);
+        D8_LAUNCH_CHECK();
+        return 0;
+    }
+    const long tiles = (long)ceil_div(a.rows, BM) * ceil_div(a.cols, BN);
+    D8_REQUIRE(tiles < (1L << 31), "matmul_gated: too many rows");
+    hipLaunchKernelGGL(gated_tile_kernel<T>, dim3((unsigned)tiles), dim3(256), 0, stream, a);
+    D8_LAUNCH_CHECK();
+    return 0;
+}
+
+}  // namespace
+}  // namespace gated
+}  // namespace d8
 
 extern "C" int d8_matmul_gated(int dtype, const void *x, int rows, int inner, const void *w, int cols, int act, void *pre, void *h, void *scratch,
                                size_t scratch_bytes, void *stream) {
     if (int rc = gated::check(dtype, rows, inner, cols, act, "matmul_gated")) return rc;
     D8_REQUIRE(x && w && h, "matmul_gated: null tensor");
-    (void)scratch, (void)scratch_bytes;
     gated::Args a;
     memset(&a, 0, sizeof(a));
     a.x = x, a.w = w, a.pre = pre, a.h = h, a.rows = rows, a.inner = inner, a.cols = cols, a.act = act;
-    const int v = 16 / (int)dtype_bytes(dtype);
-    a.vec_x = inner % v == 0 && ((size_t)x & 15) == 0, a.vec_w = cols % v == 0 && ((size_t)w & 15) == 0;
-    const dim3 grid(ceil_div(cols, gated::BN), ceil_div(rows, gated::BM));
-    D8_REQUIRE(grid.y < 65536u, "matmul_gated: too many rows");
-    if (dtype == D8_FLOAT16) hipLaunchKernelGGL(gated::gated_tile_kernel<f16>, grid, dim3(256), 0, as_stream(stream), a);
-    else hipLaunchKernelGGL(gated::gated_tile_kernel<float>, grid, dim3(256), 0, as_stream(stream), a);
-    D8_LAUNCH_CHECK();
-    return 0;
+    const gated::Plan p = gated::plan_of(dtype, rows, inner, cols, ((size_t)x & 15) == 0, ((size_t)w & 15) == 0);
+    const size_t need = p.bytes();
+    D8_REQUIRE(!need || (scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0), "matmul_gated: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
+    return dtype == D8_FLOAT16 ? gated::forward<f16>(a, p, (char *)scratch, as_stream(stream)) : gated::forward<float>(a, p, (char *)scratch, as_stream(stream));
 }
 
 extern "C" int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner, const void *w, void *dw, int cols, int act, const void *pre,
@@ -193,7 +418,7 @@ extern "C" int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows
     memset(&a, 0, sizeof(a));
     a.pre = (void *)pre, a.dh = dh, a.dpre = scratch, a.rows = rows, a.inner = inner, a.cols = cols, a.act = act;
     const int v = 16 / (int)dtype_bytes(dtype);
-    a.vec_w = cols % v == 0 && (((size_t)pre | (size_t)dh) & 15) == 0;
+    a.vec = cols % v == 0 && (((size_t)pre | (size_t)dh) & 15) == 0;
     const long threads = (long)rows * ceil_div(cols, v);
     const dim3 grid((unsigned)((threads + 255) / 256 < 16384 ? (threads + 255) / 256 : 16384));
     if (dtype == D8_FLOAT16) hipLaunchKernelGGL(gated::gated_slope_kernel<f16>, grid, dim3(256), 0, as_stream(stream), a);
