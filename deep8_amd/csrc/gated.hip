@@ -305,7 +305,7 @@ enum { FEW_ROWS = 64 };
 
 // How a forward call runs and what it takes of the scratch: copies of x and w (bytes, 0: read as they lie), partial sums.
 struct Plan {
-    enum { ROWS, WIDE, TILES } way;
+    enum { ROWS, TILES } way;
     int parts, chunk;
     size_t x_copy, w_copy, part;
     size_t bytes() const { return x_copy + w_copy + part; }
@@ -402,6 +402,7 @@ extern "C" int d8_matmul_gated(int dtype, const void *x, int rows, int inner, co
     gated::Args a;
     memset(&a, 0, sizeof(a));
     a.x = x, a.w = w, a.pre = pre, a.h = h, a.rows = rows, a.inner = inner, a.cols = cols, a.act = act;
+    if (dtype == D8_FLOAT16 && gated::wide_eligible(a)) return gated::wide_launch(a, as_stream(stream));
     const gated::Plan p = gated::plan_of(dtype, rows, inner, cols, ((size_t)x & 15) == 0, ((size_t)w & 15) == 0);
     const size_t need = p.bytes();
     D8_REQUIRE(!need || (scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0), "matmul_gated: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);

@@ -14,7 +14,8 @@ SIZES = [
     # rows, inner, cols
     (1, 1, 1), (1, 64, 8), (1, 1000, 999), (2, 512, 1024), (3, 200, 72), (8, 2048, 96), (16, 136, 640), (17, 64, 264), (31, 300, 130), (64, 256, 256),
     (100, 100, 100), (128, 64, 64), (129, 33, 65), (256, 512, 128), (300, 130, 520), (257, 72, 200), (512, 256, 1024), (777, 100, 135), (1024, 192, 640),
-    (1, 4096, 64), (5, 5000, 40), (4, 8, 4096),
+    (1, 4096, 64), (5, 5000, 40), (4, 8, 4096), (33, 96, 72), (64, 1031, 520), (60, 2000, 24),
+    (4096, 64, 1536), (4100, 128, 1544), (8200, 192, 1288), (256, 64, 24576),  # large tiles, more of them than compute units, moved back inside
 ]
 
 
