@@ -43,6 +43,7 @@ struct Args {
     int overwrite;
     float *part;    // split forward: partial outputs [units * kv_heads][rows][dim] and [..][rows][2] maximum and sum
     float *part_ml;
+    int4 *joins;    // ... what the second launch joins, by piece: chunks, first query, row tile, rows of the sequence
     float *delta;   // gradient: rowsum(do o) [heads][q_tokens]
     float *norms;   // gradient, half: largest squared norms of rows of do and of v, by workgroup of the first pass
 };
@@ -96,17 +97,6 @@ __device__ __forceinline__ bool locate(const Args &a, int id, Span &span, int &s
         before += __shfl(upto, 63);
     }
     return false;
-}
-
-// sum of count(span) over the sequences
-template <class Count>
-__device__ __forceinline__ long total_of(const Args &a, Count &&count) {
-    const int lane = threadIdx.x & 63;
-    long n = 0;
-    for (int s = lane; s < a.sequences; s += 64) n += count(span_of(a, s));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
-    return n;
 }
 
 template <class T>

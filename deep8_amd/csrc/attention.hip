@@ -226,15 +226,22 @@ __global__ __launch_bounds__(256, (DP * (int)sizeof(T) <= 256 ? 2 : 1)) void att
 // their maxima and sums).
 struct Cut {
     int chunk;  // keys
-    __device__ __forceinline__ int tiles(const Args &a, const Span &s) const { return (int)(((long)s.nq * a.group + 31) / 32); }
-    __device__ __forceinline__ int chunks(const Span &s) const { return max(1, (int)(((long)s.nk + chunk - 1) / chunk)); }
+    __device__ __forceinline__ int tiles(const Args &a, const Span &s) const { return (s.nq * a.group + 31) / 32; }
+    __device__ __forceinline__ int chunks(const Span &s) const { return max(1, (s.nk + chunk - 1) / chunk); }
+    // tiles times keys over the pieces wanted, rounded up to whole grains.  In fp32, a little too long rather than too short: there are then never
+    // more chunks than pieces and tiles.  Every wave of the call computes the same bits.
     __device__ __forceinline__ void init(const Args &a, int grain) {
         chunk = 1 << 30;
         if (!a.pieces) return;
-        const Cut &self = *this;
-        const long work = total_of(a, [&](const Span &s) { return (long)self.tiles(a, s) * s.nk; });
-        const long want = (work + a.pieces - 1) / a.pieces;
-        chunk = __builtin_amdgcn_readfirstlane((int)min((long)(1 << 30), (max(want, 1L) + grain - 1) / grain * grain));
+        float work = 0.f;
+        for (int s = threadIdx.x & 63; s < a.sequences; s += 64) {
+            const Span sp = span_of(a, s);
+            work += (float)tiles(a, sp) * (float)sp.nk;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) work += __shfl_xor(work, d);
+        const float grains = ceilf(work * 1.0001f / (float)a.pieces / (float)grain);
+        chunk = __builtin_amdgcn_readfirstlane(max(1, (int)fminf(grains, (float)((1 << 29) / grain))) * grain);
     }
     // keys that some row of the tile sees
     __device__ __forceinline__ int end(const Args &a, const Span &s, int tile) const {
@@ -256,13 +263,15 @@ __global__ __launch_bounds__(WAVES * 64) void attention_keys_kernel(Args a) {
     const int hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
     Cut cut;
     cut.init(a, CHUNK_GRAIN);
-    Span sp;
-    int seq, item;
-    if (!locate(a, unit, sp, seq, item, [&](const Span &s) { return cut.tiles(a, s) * cut.chunks(s); })) return;
-    const int chunks = cut.chunks(sp), tile = item / chunks, begin = (item - tile * chunks) * cut.chunk;
-    const int group = a.group, rows = sp.nq * group, all = cut.end(a, sp, tile), end = min(all, begin + cut.chunk);
-    if (begin > 0 && begin >= all) return;  // (the first chunk is there even if its rows see nothing)
+    Span sp = {0, 0, 0, 0};
+    int seq = 0, item = 0;
+    const bool there_is = locate(a, unit, sp, seq, item, [&](const Span &s) { return cut.tiles(a, s) * cut.chunks(s); });
+    const int chunks = there_is ? cut.chunks(sp) : 1, tile = item / chunks, begin = (item - tile * chunks) * cut.chunk;
+    const int group = a.group, rows = sp.nq * group, all = there_is ? cut.end(a, sp, tile) : 0, end = min(all, begin + cut.chunk);
     const bool whole = all <= cut.chunk;
+    // for the second launch: how many chunks the tile that begins here has, and which rows
+    if (a.pieces && hk == 0 && tid == 0) a.joins[unit] = make_int4(there_is && !whole && begin == 0 ? (all + cut.chunk - 1) / cut.chunk : 0, sp.q0, tile, rows);
+    if (!there_is || (begin > 0 && begin >= all)) return;  // (the first chunk is there even if its rows see nothing)
     const int r = tile * 32 + (lane & 31);
     const bool there = r < rows;
     const int t = query_of(a, there ? r : rows - 1), head = hk * group + (there ? r - t * group : 0);
@@ -361,34 +370,35 @@ __global__ __launch_bounds__(WAVES * 64) void attention_keys_kernel(Args a) {
     }
 }
 
-// the chunks of a tile's rows joined: a wave has a row at a time
+// the chunks of a tile's rows joined: a wave for each row
 template <class T>
 __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
-    Cut cut;
-    cut.init(a, CHUNK_GRAIN);
-    Span sp;
-    int seq, item;
-    if (!locate(a, unit, sp, seq, item, [&](const Span &s) { return cut.tiles(a, s) * cut.chunks(s); })) return;
-    const int chunks = cut.chunks(sp), tile = item / chunks, all = cut.end(a, sp, tile);
-    if (item != tile * chunks || all <= cut.chunk) return;
-    const int parts = (all + cut.chunk - 1) / cut.chunk, rows = sp.nq * a.group, n = min(32, rows - tile * 32);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    const int4 join = a.joins[unit];
+    const int parts = join.x, q0 = join.y, tile = join.z, n = min(32, join.w - tile * 32);
+    if (!parts) return;
     const long first = ((long)unit * a.kv_heads + hk) * 32, step = (long)a.kv_heads * 32;
-    for (int row = wave; row < n; row += 4) {
+    for (int row = blockIdx.y * 4 + wave; row < n; row += gridDim.y * 4) {
         const long slot = first + row;
-        float base = -INFINITY, total = 0.f;
-        for (int i = 0; i < parts; ++i) base = fmaxf(base, a.part_ml[(slot + i * step) * 2]);
+        // lane i has the maximum and the sum of chunk i, of every 64th one
+        float base = -INFINITY;
+        for (int i = lane; i < parts; i += 64) base = fmaxf(base, a.part_ml[(slot + i * step) * 2]);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) base = fmaxf(base, __shfl_xor(base, d));
         const float at = base == -INFINITY ? 0.f : base;
-        for (int i = 0; i < parts; ++i) total += a.part_ml[(slot + i * step) * 2 + 1] * __builtin_amdgcn_exp2f(a.part_ml[(slot + i * step) * 2] - at);
+        float total = 0.f;
+        for (int i = lane; i < parts; i += 64) total += a.part_ml[(slot + i * step) * 2 + 1] * __builtin_amdgcn_exp2f(a.part_ml[(slot + i * step) * 2] - at);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
         const int rt = query_of(a, tile * 32 + row), rh = hk * a.group + tile * 32 + row - rt * a.group;
         const float inv = total == 0.f ? 0.f : 1.f / total;
         for (int d = lane; d < a.dim; d += 64) {
             float x = 0.f;
+#pragma unroll 4
             for (int i = 0; i < parts; ++i) x += a.part[(slot + i * step) * a.dim + d] * __builtin_amdgcn_exp2f(a.part_ml[(slot + i * step) * 2] - at);
-            ((T *)a.o)[(long)(sp.q0 + rt) * a.ldo + (long)rh * a.dim + d] = (T)(x * inv);
+            ((T *)a.o)[(long)(q0 + rt) * a.ldo + (long)rh * a.dim + d] = (T)(x * inv);
         }
-        if (lane == 0 && a.lse) a.lse[(long)rh * a.q_tokens + sp.q0 + rt] = total == 0.f ? -INFINITY : (base + log2f(total)) * LN2;
+        if (lane == 0 && a.lse) a.lse[(long)rh * a.q_tokens + q0 + rt] = total == 0.f ? -INFINITY : (base + log2f(total)) * LN2;
     }
 }
 
@@ -436,12 +446,17 @@ int launch(const Args &a, const Plan &p, hipStream_t stream) {
     else if (a.dim <= 128) rc = launch_dim<T, 128>(a, p, stream);
     else rc = launch_dim<T, 256>(a, p, stream);
     if (rc || !p.pieces) return rc;
-    hipLaunchKernelGGL(attention_join_kernel<T>, dim3((unsigned)p.units * a.kv_heads), dim3(256), 0, stream, a);
+    // (a tile has up to 32 rows; where no sequence has more than one query, the heads of a group)
+    const int most = a.sequences >= a.q_tokens && a.group < 32 ? a.group : 32;
+    hipLaunchKernelGGL(attention_join_kernel<T>, dim3((unsigned)p.units * a.kv_heads, (most + 3) / 4), dim3(256), 0, stream, a);
     D8_LAUNCH_CHECK();
     return 0;
 }
 
 size_t part_rows(const Plan &p, int kv_heads) { return p.pieces ? (size_t)p.units * kv_heads * 32 : 0; }
+size_t part_bytes(const Plan &p, int kv_heads, int dim) {
+    return part_rows(p, kv_heads) * (size_t)(dim + 2) * sizeof(float) + (p.pieces ? (size_t)p.units * sizeof(int4) : 0);
+}
 
 }  // namespace
 
@@ -478,7 +493,7 @@ extern "C" size_t d8_attention_scratch_bytes(int dtype, int which, int sequences
     if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || sequences < 0 || q_tokens < 0 || k_tokens < 0 || kv_heads < 1 || heads < kv_heads || dim < 1) return 0;
     if (which == 1) return attention::grad_scratch_bytes(q_tokens, heads);
     const attention::Plan p = attention::plan_of(true, sequences, q_tokens, k_tokens, heads, kv_heads);
-    return attention::part_rows(p, kv_heads) * (size_t)(dim + 2) * sizeof(float);
+    return attention::part_bytes(p, kv_heads, dim);
 }
 
 extern "C" int d8_attention(int dtype, const void *q, long ldq, const void *k, long ldk, const void *v, long ldv, void *o, long ldo, float *lse,
@@ -497,10 +512,10 @@ extern "C" int d8_attention(int dtype, const void *q, long ldq, const void *k, l
     // (a tile's rows are addressed by 32 bits)
     const bool fast = a.vec && attention::in_pieces(dtype, dim, {o}, {ldo}) && ldk < (1 << 23) && ldv < (1 << 23);
     const attention::Plan p = attention::plan_of(fast, sequences, q_tokens, k_tokens, heads, kv_heads);
-    const size_t part = attention::part_rows(p, kv_heads), need = part * (size_t)(dim + 2) * sizeof(float);
+    const size_t part = attention::part_rows(p, kv_heads), need = attention::part_bytes(p, kv_heads, dim);
     D8_REQUIRE(!need || (scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0), "attention: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
     D8_REQUIRE((long)(p.tiles + p.pieces) * kv_heads < (1L << 31), "attention: too many sequences");
     a.tiles = p.tiles, a.units = p.units, a.pieces = p.pieces;
-    a.part = (float *)scratch, a.part_ml = a.part + part * dim;
+    a.joins = (int4 *)scratch, a.part = (float *)(a.joins + (p.pieces ? p.units : 0)), a.part_ml = a.part + part * dim;
     return dtype == D8_FLOAT16 ? attention::launch<f16>(a, p, as_stream(stream)) : attention::launch<float>(a, p, as_stream(stream));
 }

@@ -6,8 +6,9 @@
 // (rounded once) only where the way back will need it.
 //
 // Three kernels: many rows and columns in half on 256 x 256 tiles (gated_wide.hip); few rows, where reading w is the work (below:
-// gated_rows_kernel); everything else on 128 x 64 tiles.  All move operands in 16-byte pieces; operands whose rows do not start at
-// multiples of 16 bytes are copied to rows that do, into scratch, first.
+// gated_rows_kernel); everything else on tiles of 64 or 128 rows.  All move operands in 16-byte pieces; operands whose rows do not start at
+// multiples of 16 bytes are copied to rows that do, into scratch, first (single precision moved by elements, without copies, was no faster: 777 x
+// 1000 times 1000 x 2 * 1351 69.4 us against 67.6).
 #include "gated.h"
 
 namespace d8 {
@@ -79,14 +80,18 @@ __device__ __forceinline__ typename attention::Type<T>::frag weight_frag(const c
     }
 }
 
-// 128 rows x 64 columns of both halves a workgroup, a wave 64 x 32 of each.  K in steps of 128 bytes of x, both tiles straight into one of two
-// stages of LDS, the next step's while this one is worked on.
-enum { BM = 128, BN = 64 };
+// K in steps of 128 bytes of x, both tiles straight into one of two stages of LDS, the next step's while this one is worked on.  A workgroup's
+// tile by SHAPE: TALL 128 rows x 64 columns of both halves, a wave 64 x 32 of each; SQUARE 64 x 64, a wave 32 x 32 of each; SMALL 64 x 32, a wave
+// 32 x 32 of one half, and gate and factor meet through LDS at the end.
+enum Shape { TALL, SQUARE, SMALL };
+constexpr int tile_rows(int shape) { return shape == TALL ? 128 : 64; }
+constexpr int tile_cols(int shape) { return shape == SMALL ? 32 : 64; }
 
-template <class T>
+template <class T, int SHAPE>
 __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
     typedef attention::Type<T> M;
     typedef typename M::frag frag;
+    constexpr int BM = tile_rows(SHAPE), BN = tile_cols(SHAPE), R = SHAPE == TALL ? 2 : 1, H = SHAPE == SMALL ? 1 : 2;  // row blocks, halves of a wave
     constexpr int PX = 128, BK = PX / (int)sizeof(T), PW = 2 * BN * (int)sizeof(T), TX = BM * PX, TW = BK * PW;
     __shared__ __attribute__((aligned(1024))) char lds[2 * (TX + TW)];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -94,7 +99,8 @@ __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
     const int tiles_m = (a.rows + BM - 1) / BM, total = gridDim.x;
     int id = blockIdx.x;
     if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
-    const int m0 = id % tiles_m * BM, n0 = id / tiles_m * BN, wm = (wave >> 1) * 64, wn = (wave & 1) * 32;
+    const int m0 = id % tiles_m * BM, n0 = id / tiles_m * BN;
+    const int wm = (wave >> 1) * 32 * R, wn = SHAPE == SMALL ? 0 : (wave & 1) * 32, half = SHAPE == SMALL ? wave & 1 : 0;
     attention::TileLoader<T, PX> lx;
     lx.init(a.ldx, a.inner, lane);
     WeightLoader<T, PW> lw;
@@ -110,11 +116,11 @@ __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < TW / 4096; ++i) lw.load(dw, wave * (TW / 4096) + i, to + TX);
     };
-    f32x16 acc[2][2];
+    f32x16 acc[R][H];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < R * H; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i >> 1][i & 1][e] = 0.f;
+        for (int e = 0; e < 16; ++e) acc[i / H][i % H][e] = 0.f;
     fetch(0, 0);
     for (int k0 = 0, stage = 0; k0 < a.inner; k0 += BK, stage ^= 1) {
         ATTN_VMCNT(0);
@@ -124,27 +130,42 @@ __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
         const char *tx = lds + stage * (TX + TW), *tw = tx + TX;
 #pragma unroll
         for (int u = 0; u < BK / M::STEP; ++u) {
-            frag xf[2], wf[2];
+            frag xf[R], wf[H];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                xf[i] = attention::rows_frag<T, PX>(tx, wm + i * 32, u, lane);
-                wf[i] = weight_frag<T, PW>(tw, u * M::STEP, i * BN + wn, lane);
-            }
+            for (int i = 0; i < R; ++i) xf[i] = attention::rows_frag<T, PX>(tx, wm + i * 32, u, lane);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < H; ++j) wf[j] = weight_frag<T, PW>(tw, u * M::STEP, (half + j) * BN + wn, lane);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) M::mma(acc[i][j], xf[i], wf[j]);
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int j = 0; j < H; ++j) M::mma(acc[i][j], xf[i], wf[j]);
         }
     }
     const int n = n0 + wn + (lane & 31);
-    if (n >= a.cols) return;
+    if constexpr (SHAPE == SMALL) {
+        __syncthreads();
+        float *to = (float *)lds + (wave >> 1) * 1024 + lane;
+        if (half) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+            for (int e = 0; e < 16; ++e) to[e * 64] = acc[0][0][e];
+        }
+        __syncthreads();
+        if (half || n >= a.cols) return;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (m < a.rows) store<T>(a, m, n, acc[i][0][e], acc[i][1][e]);
+            const int m = m0 + wm + 8 * (e >> 2) + 4 * h + (e & 3);
+            if (m < a.rows) store<T>(a, m, n, acc[0][0][e], to[e * 64]);
         }
+    } else {
+        if (n >= a.cols) return;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+                if (m < a.rows) store<T>(a, m, n, acc[i][0][e], acc[i][H - 1][e]);
+            }
+    }
 }
 
 // Few rows.  A workgroup has 128 bytes of columns of both halves and a chunk of K, of which its four waves take every fourth tile of 32 rows of w,
@@ -306,7 +327,7 @@ enum { FEW_ROWS = 64 };
 // How a forward call runs and what it takes of the scratch: copies of x and w (bytes, 0: read as they lie), partial sums.
 struct Plan {
     enum { ROWS, TILES } way;
-    int parts, chunk;
+    int shape, parts, chunk;
     size_t x_copy, w_copy, part;
     size_t bytes() const { return x_copy + w_copy + part; }
 };
@@ -332,6 +353,14 @@ Plan plan_of(int dtype, int rows, int inner, int cols, bool x_aligned, bool w_al
     }
     p.way = Plan::TILES;
     p.parts = 1, p.chunk = inner;
+    // the shape whose busiest compute unit has least to do: blocks of 32 x 32 products, weighed with what a block costs in it
+    static const float cost[2][3] = {{1.f, 1.25f, 1.6f}, {1.f, 1.05f, 1.1f}};  // half, single
+    float best = 0.f;
+    for (int s = TALL; s <= SMALL; ++s) {
+        const long tiles = (long)ceil_div(rows, tile_rows(s)) * ceil_div(cols, tile_cols(s));
+        const float t = (float)((tiles + cu_count() - 1) / cu_count()) * (tile_rows(s) / 32) * (tile_cols(s) / 32) * cost[dtype == D8_FLOAT32][s];
+        if (s == TALL || t < best) best = t, p.shape = s;
+    }
     return p;
 }
 
@@ -355,6 +384,15 @@ template <class T>
 int copy_rows(const void *from, void *to, long rows, int width, int padded, hipStream_t stream) {
     const long groups = (rows * (padded / attention::Type<T>::V) + 255) / 256;
     hipLaunchKernelGGL(gated_copy_kernel<T>, dim3((unsigned)(groups < 8192 ? groups : 8192)), dim3(256), 0, stream, (const T *)from, (T *)to, rows, width, padded);
+    D8_LAUNCH_CHECK();
+    return 0;
+}
+
+template <class T, int SHAPE>
+int launch_tiles(const Args &a, hipStream_t stream) {
+    const long tiles = (long)ceil_div(a.rows, tile_rows(SHAPE)) * ceil_div(a.cols, tile_cols(SHAPE));
+    D8_REQUIRE(tiles < (1L << 31), "matmul_gated: too many rows");
+    hipLaunchKernelGGL((gated_tile_kernel<T, SHAPE>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
     D8_LAUNCH_CHECK();
     return 0;
 }
@@ -384,11 +422,11 @@ int forward(Args a, const Plan &p, char *scratch, hipStream_t stream) {
         D8_LAUNCH_CHECK();
         return 0;
     }
-    const long tiles = (long)ceil_div(a.rows, BM) * ceil_div(a.cols, BN);
-    D8_REQUIRE(tiles < (1L << 31), "matmul_gated: too many rows");
-    hipLaunchKernelGGL(gated_tile_kernel<T>, dim3((unsigned)tiles), dim3(256), 0, stream, a);
-    D8_LAUNCH_CHECK();
-    return 0;
+    switch (p.shape) {
+        case TALL: return launch_tiles<T, TALL>(a, stream);
+        case SQUARE: return launch_tiles<T, SQUARE>(a, stream);
+        default: return launch_tiles<T, SMALL>(a, stream);
+    }
 }
 
 }  // namespace
