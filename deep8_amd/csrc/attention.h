@@ -38,10 +38,11 @@ struct Args {
     float scale;
     int vec;        // rows of every tensor can be moved in 16-byte pieces
     int tiles;      // row tiles (key blocks) of all sequences at most
-    int units;      // split forward: pieces of work that the launch has room for, of each kv head
-    int pieces;     // ... that the keys are cut into, about
+    int units;      // pieces of work that the launch has room for, of each kv head
+    int pieces;     // ... that the keys (dk and dv: the rows) are cut into, about; 0: not at all
+    int split_kv;   // gradient: keys of a workgroup are 128 over this
     int overwrite;
-    float *part;    // split forward: partial outputs [units * kv_heads][rows][dim] and [..][rows][2] maximum and sum
+    float *part;    // partial sums of the pieces; forward: partial outputs [units * kv_heads][rows][dim] and [..][rows][2] maximum and sum
     float *part_ml;
     int4 *joins;    // ... what the second launch joins, by piece: chunks, first query, row tile, rows of the sequence
     float *delta;   // gradient: rowsum(do o) [heads][q_tokens]
@@ -313,7 +314,7 @@ struct Softmax {
 int check(const Args &a, int dtype, const char *name);
 inline void set_group(Args &a) { a.group = a.heads / a.kv_heads, a.group_rcp = 0xffffffffu / (unsigned)a.group; }
 bool in_pieces(int dtype, int dim, std::initializer_list<const void *> p, std::initializer_list<long> ld);
-size_t grad_scratch_bytes(int q_tokens, int heads);
+size_t grad_scratch_bytes(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim);
 
 template <int DP, class T>
 constexpr int pitch_of() { return DP * (int)sizeof(T) + 16; }  // the 16 bytes keep a column's rows in different banks

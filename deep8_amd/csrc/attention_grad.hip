@@ -17,6 +17,7 @@ namespace attention {
 namespace {
 
 enum { TILE = 32 };
+enum { ROW_GRAIN = 512 };    // rows of a chunk are a multiple of this
 enum { NORM_GROUPS = 512 };  // workgroups of the first launch: entries of each list of norms
 constexpr float P_SHIFT = 15.f;
 
@@ -333,6 +334,32 @@ struct ChunkLoader {
     static __device__ __forceinline__ int rows(const Args &a, int nq) { return (nq + CT - 1) / CT * CT * a.group; }
 };
 
+// The rows that a workgroup for some keys walks, cut into chunks of one length for the whole call so that no workgroup has much more to do than
+// another (causal, the first keys of a long sequence are seen by all its rows, the last ones by few).  Found on the device from the
+// lengths: blocks of keys times rows, over the pieces wanted.  The sums of a block's chunks meet through scratch in a second launch,
+// in the order of the chunks.
+template <class T, int DP, int SPLIT>
+struct RowCut {
+    typedef Shape<T, DP, SPLIT> S;
+    typedef ChunkLoader<T, S::PB> Rows;
+    int chunk;  // rows
+    static __device__ __forceinline__ int blocks(const Span &s) { return (s.nk + S::OWN - 1) / S::OWN; }
+    __device__ __forceinline__ int chunks(const Args &a, const Span &s) const { return max(1, (Rows::rows(a, s.nq) + chunk - 1) / chunk); }
+    __device__ __forceinline__ void init(const Args &a) {
+        chunk = 1 << 30;
+        if (!a.pieces) return;
+        float work = 0.f;
+        for (int s = threadIdx.x & 63; s < a.sequences; s += 64) {
+            const Span sp = span_of(a, s);
+            work += (float)blocks(sp) * (float)Rows::rows(a, sp.nq);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) work += __shfl_xor(work, d);
+        const float grains = ceilf(work * 1.0001f / (float)a.pieces / (float)ROW_GRAIN);  // (rather too long: never more chunks than room)
+        chunk = __builtin_amdgcn_readfirstlane(max(1, (int)fminf(grains, (float)((1 << 29) / ROW_GRAIN))) * ROW_GRAIN);
+    }
+};
+
 template <class T, int DP, int SPLIT>
 __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void attention_grad_kv_kernel(Args a) {
     typedef Type<T> M;
@@ -343,12 +370,23 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
     __shared__ __attribute__((aligned(16))) float row_lse[2][S::KB], row_delta[2][S::KB];
     __shared__ __attribute__((aligned(16))) frag spare[S::SPARE ? S::SPARE : 1][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int hk = blockIdx.x % a.kv_heads;
-    Span sp;
-    int seq, block;
-    if (!locate(a, blockIdx.x / a.kv_heads, sp, seq, block, [](const Span &s) { return (s.nk + S::OWN - 1) / S::OWN; })) return;
+    const int hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
     typedef ChunkLoader<T, PB> Rows;
+    RowCut<T, DP, SPLIT> cut;
+    cut.init(a);
+    Span sp = {0, 0, 0, 0};
+    int seq = 0, item = 0;
+    const bool there_is = locate(a, unit, sp, seq, item, [&](const Span &s) { return cut.blocks(s) * cut.chunks(a, s); });
+    const int chunks = there_is ? cut.chunks(a, sp) : 1, block = item / chunks, part = item - block * chunks;
     const int group = a.group, rows = Rows::rows(a, sp.nq), back = sp.nk - sp.nq;
+    // the first row that sees a key of the block (its query is the block's first key less nk - nq), and the chunk that it is in
+    const int begin = a.causal ? (int)min((long)(max(0, block * S::OWN - back) / Rows::CT * Rows::CT) * group / S::KB * S::KB, (long)rows) : 0;
+    const int first_part = min(begin / cut.chunk, chunks - 1), parts = chunks - first_part;
+    // for the second launch: how many chunks the block that begins here has, and which keys
+    if (a.pieces && hk == 0 && tid == 0)
+        a.joins[unit] = make_int4(there_is && part == first_part && parts > 1 ? parts : 0, sp.k0 + block * S::OWN, min(S::OWN, sp.nk - block * S::OWN), 0);
+    if (!there_is || part < first_part) return;
+    const int r_begin = max(begin, part * cut.chunk), r_end = min((long)rows, (part + 1L) * cut.chunk);
     const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
     const int j0 = block * S::OWN + wave % (4 / SPLIT) * 32;  // the wave's first key
     frag kf[UNITS], vf[UNITS - S::SPARE];
@@ -387,11 +425,8 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
             next_delta = in ? a.delta[at] * mult : 0.f;
         }
     };
-    // the first row that sees a key of the block (its query is the block's first key less nk - nq)
-    const long first = a.causal ? (long)(max(0, block * S::OWN - back) / Rows::CT * Rows::CT) * group : 0;
-    const int r_begin = (int)min(first / 32 * 32, (long)rows);
-    if (r_begin < rows) fetch(r_begin, 0);
-    for (int r0 = r_begin, stage = 0; r0 < rows; r0 += S::KB, stage ^= 1) {
+    if (r_begin < r_end) fetch(r_begin, 0);
+    for (int r0 = r_begin, stage = 0; r0 < r_end; r0 += S::KB, stage ^= 1) {
         if (wave * 64 < S::KB) {
             int wl = lane;
             asm volatile("" : "+v"(wl));
@@ -400,7 +435,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
         ATTN_VMCNT(0);
         lds_reads_done();
         __syncthreads();
-        if (r0 + S::KB < rows) fetch(r0 + S::KB, stage ^ 1);
+        if (r0 + S::KB < r_end) fetch(r0 + S::KB, stage ^ 1);
         const char *tq = lds + stage * 2 * S::TILE_BYTES, *tg = tq + S::TILE_BYTES;
 #pragma unroll 1
         for (int i = 0; i < S::BLOCKS / SPLIT; ++i) {
@@ -464,6 +499,14 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) dk[n][e] += to[(n * 16 + e) * 64], dv[n][e] += to[((N + n) * 16 + e) * 64];
+    }
+    if (parts > 1) {  // as the registers hold them: the second launch's lanes hold the same elements
+        float *to = a.part + (((long)unit * a.kv_heads + hk) * (S::OWN / 32) + wave % (4 / SPLIT)) * 2 * N * 16 * 64 + el;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) to[(n * 16 + e) * 64] = dk[n][e], to[((N + n) * 16 + e) * 64] = dv[n][e];
+        return;
     }
     const int j = j0 + (el & 31);
     if (j >= sp.nk) return;
@@ -589,13 +632,46 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
     store_sums<T, DP>((T *)a.dq + (long)(sp.q0 + t) * a.lddq + (long)head * a.dim, dq, a.scale * exp2f(-shift) / mult, a.dim, h, a.overwrite & 1);
 }
 
+// the chunks of a block of keys joined; a wave has dk or dv of 32 keys
+template <class T, int DP, int SPLIT>
+__global__ __launch_bounds__(256) void attention_grad_join_kernel(Args a) {
+    typedef Shape<T, DP, SPLIT> S;
+    constexpr int N = DP / 32;
+    const int lane = threadIdx.x & 63, hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    const int4 join = a.joins[unit];
+    if (!join.x) return;
+    const float mult = ds_scale<T>(a), unshift = exp2f(scaled<T>() ? -P_SHIFT : 0.f);
+    for (int i = threadIdx.x >> 6; i < S::OWN / 32 * 2; i += 4) {
+        const int keys = i >> 1, which = i & 1;
+        const float *from = a.part + (((long)unit * a.kv_heads + hk) * (S::OWN / 32) + keys) * 2 * N * 16 * 64 + which * N * 16 * 64 + lane;
+        const long step = (long)a.kv_heads * (S::OWN / 32) * 2 * N * 16 * 64;
+        f32x16 x[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[n][e] = from[(n * 16 + e) * 64];
+        for (int p = 1; p < join.x; ++p)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[n][e] += from[p * step + (n * 16 + e) * 64];
+        const int j = keys * 32 + (lane & 31);
+        if (j >= join.z) continue;
+        const long key = join.y + j;
+        if (which == 0) store_sums<T, DP>((T *)a.dk + key * a.lddk + (long)hk * a.dim, x, a.scale * unshift / mult, a.dim, lane >> 5, a.overwrite & 2);
+        else store_sums<T, DP>((T *)a.dv + key * a.lddv + (long)hk * a.dim, x, unshift, a.dim, lane >> 5, a.overwrite & 4);
+    }
+}
+
 // SPLIT for so many keys (rows), of which a workgroup has 128 or 64
 int split_for(long own, int kv_heads) { return (own + 127) / 128 * kv_heads < 2 * cu_count() ? 2 : 1; }
 
 template <class T, int DP, int SPLIT>
 int launch_kv(const Args &a, hipStream_t stream) {
-    const long blocks = ((long)a.k_tokens + 128 / SPLIT - 1) / (128 / SPLIT) + a.sequences;
-    hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP, SPLIT>), dim3((unsigned)blocks * a.kv_heads), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_grad_kv_kernel<T, DP, SPLIT>), dim3((unsigned)a.units * a.kv_heads), dim3(256), 0, stream, a);
+    D8_LAUNCH_CHECK();
+    if (!a.pieces) return 0;
+    hipLaunchKernelGGL((attention_grad_join_kernel<T, DP, SPLIT>), dim3((unsigned)a.units * a.kv_heads), dim3(256), 0, stream, a);
     D8_LAUNCH_CHECK();
     return 0;
 }
@@ -627,7 +703,7 @@ int launch_dim(const Args &a, bool fast, hipStream_t stream) {
         D8_LAUNCH_CHECK();
         return 0;
     }
-    return CAN_SPLIT && split_for(a.k_tokens, a.kv_heads) == 2 ? launch_kv<T, DP, CAN_SPLIT ? 2 : 1>(a, stream) : launch_kv<T, DP, 1>(a, stream);
+    return CAN_SPLIT && a.split_kv == 2 ? launch_kv<T, DP, CAN_SPLIT ? 2 : 1>(a, stream) : launch_kv<T, DP, 1>(a, stream);
 }
 
 template <class T>
@@ -645,8 +721,32 @@ int launch(const Args &a, bool fast, hipStream_t stream) {
 
 }  // namespace
 
-size_t grad_scratch_bytes(int q_tokens, int heads) {
-    return sizeof(float) * (2 * NORM_GROUPS + (size_t)q_tokens * heads);
+// How dk and dv are cut: keys of a workgroup, pieces that the rows are cut into (0: not at all), pieces of work there is room for.  Four
+// workgroups a compute unit, two rounds of what runs at once, are wanted.
+struct GradPlan {
+    int split, pieces, units;
+    size_t lists, parts;  // bytes
+};
+static GradPlan grad_plan(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim) {
+    GradPlan p;
+    const int padded = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;
+    p.split = dtype == D8_FLOAT32 && padded == 256 ? 1 : split_for(k_tokens, kv_heads);
+    const int own = 128 / p.split;
+    const long blocks = ((long)k_tokens + own - 1) / own + sequences, rows = (long)q_tokens * (heads / kv_heads);
+    const long want = (4L * cu_count() + kv_heads - 1) / kv_heads, most = (blocks * rows + ROW_GRAIN - 1) / ROW_GRAIN;
+    p.pieces = (int)(blocks >= 2 * want ? 0 : want < most ? want : most);
+    if (rows <= ROW_GRAIN) p.pieces = 0;
+    p.units = (int)(blocks + p.pieces);
+    p.lists = p.pieces ? ((size_t)p.units * sizeof(int4) + 255) & ~(size_t)255 : 0;
+    p.parts = p.pieces ? (size_t)p.units * kv_heads * own * 2 * padded * sizeof(float) : 0;
+    return p;
+}
+
+static size_t row_bytes_of(int q_tokens, int heads) { return (sizeof(float) * (2 * NORM_GROUPS + (size_t)q_tokens * heads) + 255) & ~(size_t)255; }
+
+size_t grad_scratch_bytes(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim) {
+    const GradPlan p = grad_plan(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim);
+    return row_bytes_of(q_tokens, heads) + p.lists + p.parts;
 }
 
 }  // namespace attention
@@ -669,14 +769,17 @@ extern "C" int d8_attention_grad(int dtype, const void *q, long ldq, const void 
     D8_REQUIRE(lddo >= qrow && lddq >= qrow && lddk >= krow && lddv >= krow, "attention_grad: rows of %ld and %ld elements do not fit their leading dimensions", qrow, krow);
     if (!sequences || (!q_tokens && !k_tokens)) return 0;
     D8_REQUIRE(q_starts && k_starts && (!q_tokens || (q && o && lse && dout && dq)) && (!k_tokens || (k && v && dk && dv)), "attention_grad: null tensor");
-    const size_t need = attention::grad_scratch_bytes(q_tokens, heads);
+    const attention::GradPlan plan = attention::grad_plan(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim);
+    const size_t need = attention::grad_scratch_bytes(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim);
     D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_grad: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
     a.norms = (float *)scratch, a.delta = a.norms + 2 * attention::NORM_GROUPS;
+    a.joins = (int4 *)((char *)scratch + attention::row_bytes_of(q_tokens, heads)), a.part = (float *)((char *)a.joins + plan.lists);
+    a.pieces = plan.pieces, a.units = plan.units, a.split_kv = plan.split;
     attention::set_group(a);
     a.vec = attention::in_pieces(dtype, dim, {q, k, v, o, dout}, {ldq, ldk, ldv, ldo, lddo});
     // (a tile's rows are addressed by 31 bits)
     const long most = 1 << 21;
     const bool fast = a.vec && attention::in_pieces(dtype, dim, {dq, dk, dv}, {lddq, lddk, lddv}) && ldq < most && ldk < most && ldv < most && lddo < most;
-    D8_REQUIRE((((long)q_tokens * a.group + k_tokens) / 64 + 2 * (long)sequences + 2) * kv_heads < (1L << 31), "attention_grad: too many sequences");
+    D8_REQUIRE((((long)q_tokens * a.group + k_tokens) / 64 + 2 * (long)sequences + plan.pieces + 2) * kv_heads < (1L << 31), "attention_grad: too many sequences");
     return dtype == D8_FLOAT16 ? attention::launch<f16>(a, fast, as_stream(stream)) : attention::launch<float>(a, fast, as_stream(stream));
 }
