@@ -184,12 +184,14 @@ __device__ __forceinline__ typename Type<T>::frag read_rows(const char *tile, in
 
 // ---- tiles that go from memory straight into LDS ----------------------------------------------------------------------
 // A row takes PB bytes (a power of two) in LDS, its 16-byte piece c at position c ^ swizzle(row): the lanes of a load land 16 bytes
-// apart, so rows cannot be padded, and the exclusive-or keeps what a read's lanes want in different banks, both along rows (eight
-// lanes a cycle, one piece of eight rows) and along columns (four rows of two pieces each, or a row's neighbours).
+// apart, so rows cannot be padded, and the exclusive-or keeps what a read's lanes want in different banks, both along rows (one piece of
+// sixteen rows, in whatever order the lanes are served) and along columns (four rows of four pieces each, or a row's neighbours).
 template <int PB>
 __device__ __forceinline__ int swizzle(int row) {
-    constexpr int PER_SPAN = PB >= 256 ? 1 : 256 / PB, PIECES = PB / 16 < 16 ? PB / 16 : 16;
-    return ((row / PER_SPAN) & (PIECES / 2 - 1)) << 1;
+    // of the 256 bytes that the banks span, a row takes PB: the rows of a column read, four in a row, go to different quarters, sixteen rows to
+    // different sixteenths
+    constexpr int PER_SPAN = PB >= 256 ? 1 : 256 / PB;
+    return (((row & 3) / PER_SPAN) << 2) | ((row >> 2) & 3);
 }
 
 template <class T, int DP>
@@ -211,8 +213,9 @@ __device__ __forceinline__ typename Type<T>::frag cols_frag(const char *tile, in
     if constexpr (sizeof(T) == 2) {
         const int i = lane & 15, j = lane >> 4, row = r0 + 4 * (j >> 1) + (i >> 2), at = c0 * 2 + 32 * (j & 1) + 8 * (i & 3);
         const char *p = tile + row * PB + ((((at >> 4) ^ swizzle<PB>(row)) << 4) | (at & 15));
+        const char *q = tile + (row + 8) * PB + ((((at >> 4) ^ swizzle<PB>(row + 8)) << 4) | (at & 15));
         const tr_f16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16(ATTN_LDS(tr_f16x4, p));
-        const tr_f16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16(ATTN_LDS(tr_f16x4, p + 8 * PB));  // (row + 8 has row's swizzle)
+        const tr_f16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16(ATTN_LDS(tr_f16x4, q));
         r = __builtin_bit_cast(typename Type<T>::frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
         const int at = (c0 + (lane & 31)) * 4;
