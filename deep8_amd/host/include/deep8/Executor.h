@@ -92,6 +92,12 @@ Variable &add(Variable &x, Variable &y);
 Variable &relu(Variable &x);
 Variable &matrixMultiplyBiasReLu(Variable &x, Variable &y, Variable &bias);  // relu(x * y + bias) as one node
 Variable &conv2dBiasReLu(Variable &x, Variable &filter, Variable &bias, bool covered = true, int strideY = 1, int strideX = 1, int dilationY = 1, int dilationX = 1);
+// a transformer layer (the nodes HeadNormRotary, Attention and MatrixMultiplyGated)
+Variable &rotaryTable(Executor *executor, size_t positions, size_t rotary, double base = 10000, double factor = 1, double keepBelow = 0, double slowAbove = 0);
+Variable &headNormRotary(Variable &x, Variable &weight, Variable &positions, Variable &table, int heads, float epsilon = 1e-6f, bool interleaved = false);
+Variable &headRotary(Variable &x, Variable &positions, Variable &table, int heads, bool interleaved = false);
+Variable &attention(Variable &q, Variable &k, Variable &v, Variable &qStarts, Variable &kStarts, int heads, int kvHeads, float scale = 0, bool causal = true);
+Variable &matrixMultiplyGated(Variable &x, Variable &w, Math::GateType act = Math::GateType::SiLU);
 Variable &operator-(Variable &x, Variable &y);  // Minus, with broadcasting
 Variable &minus(Variable &x, Variable &y);
 Variable &l1Norm(Variable &x);

@@ -129,6 +129,33 @@ void Conv2dBiasReLu(const Tensor &x, const Tensor &y, const Tensor &bias, Tensor
 // over every axis but the last.  Replaces ReLuGradGPU (ReLu.cu:61-116) followed by AddGradYGPU (Add.cu:99-133).
 void BiasReLuGrad(const Tensor &z, const Tensor &dz, Tensor &dpre, Tensor &dbias);
 
+// A transformer layer's operators (d8_rotary_table, d8_head_norm_rotary, d8_attention, d8_matmul_gated; no counterpart in the
+// reference).  Tokens are rows: queries [tokens, heads * dim], keys and values [tokens, kvHeads * dim], the batch axis counting as
+// more rows.  Positions and starts are Int32 tensors.  Pointers may be null where a tensor is optional.
+/** table [positions, rotary], Float32: the cosines and sines of positions 0 .. positions - 1 */
+void RotaryTable(Tensor &table, double base = 10000, double factor = 1, double keepBelow = 0, double slowAbove = 0);
+/** y = each head of x divided by its root mean square, times weight [dim] (weight null: left as it is), its first `rotary` elements
+ *  turned by the position of its row (positions null: the row's number; table null: not turned) */
+void HeadNormRotary(const Tensor &x, const Tensor *weight, const Tensor *positions, const Tensor *table, Tensor &y, int heads,
+                    float epsilon = 1e-6f, bool interleaved = false);
+/** dx, dweight (null: not wanted) += */
+void HeadNormRotaryGrad(const Tensor &x, Tensor &dx, const Tensor *weight, Tensor *dweight, const Tensor *positions, const Tensor *table,
+                        const Tensor &y, const Tensor &dy, int heads, float epsilon = 1e-6f, bool interleaved = false);
+/** o = softmax(scale q k^T) v, sequence s having queries qStarts[s] .. qStarts[s + 1] - 1 and keys kStarts[s] .. kStarts[s + 1] - 1; causal:
+ *  a sequence's last query sees all its keys, the one before all but the last, ...  lse (null: not wanted): Float32, heads * tokens */
+void Attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &qStarts, const Tensor &kStarts, Tensor &o, Tensor *lse,
+               int heads, int kvHeads, float scale, bool causal = true);
+/** dq, dk, dv += from one call; lse as the forward call left it.  Three different tensors. */
+void AttentionGrad(const Tensor &q, Tensor &dq, const Tensor &k, Tensor &dk, const Tensor &v, Tensor &dv, const Tensor &qStarts,
+                   const Tensor &kStarts, const Tensor &o, const Tensor &lse, const Tensor &dout, int heads, int kvHeads, float scale,
+                   bool causal = true);
+/** h = act(g) * u, (g | u) = x w: x [rows, inner], w [inner, 2 cols]; pre (null: not wanted) [rows, 2 cols] receives g and u */
+enum class GateType { SiLU = 0, GeLU, ReLu, Sigmoid };
+void MatrixMultiplyGated(const Tensor &x, const Tensor &w, Tensor *pre, Tensor &h, GateType act = GateType::SiLU);
+/** dx, dw += from one call; pre as the forward call left it */
+void MatrixMultiplyGatedGrad(const Tensor &x, Tensor &dx, const Tensor &w, Tensor &dw, const Tensor &pre, const Tensor &h, const Tensor &dh,
+                             GateType act = GateType::SiLU);
+
 }  // namespace Math
 }  // namespace Deep8
 

@@ -11,6 +11,7 @@
 
 #include <unordered_map>
 
+#include "deep8/Math.h"
 #include "deep8/Model.h"
 
 namespace Deep8 {
@@ -98,6 +99,12 @@ public:
     // element of the result's last dimension
     Variable &matrixMultiplyBiasReLu(Variable &y, Variable &bias);
     Variable &conv2dBiasReLu(Variable &filter, Variable &bias, bool covered = true, int strideY = 1, int strideX = 1, int dilationY = 1, int dilationX = 1);
+    // a transformer layer: each head's norm and rotation (headRotary: rotation alone), attention of this variable's queries, and
+    // act(g) * u with (g | u) = this * w; see the nodes HeadNormRotary, Attention and MatrixMultiplyGated
+    Variable &headNormRotary(Variable &weight, Variable &positions, Variable &table, int heads, float epsilon = 1e-6f, bool interleaved = false);
+    Variable &headRotary(Variable &positions, Variable &table, int heads, bool interleaved = false);
+    Variable &attention(Variable &k, Variable &v, Variable &qStarts, Variable &kStarts, int heads, int kvHeads, float scale = 0, bool causal = true);
+    Variable &matrixMultiplyGated(Variable &w, Math::GateType act = Math::GateType::SiLU);
     // what a loss needs (deep8/src/nodes/Variable.cpp:342-346,461-465,521-535)
     Variable &minus(Variable &y);
     Variable &l1Norm();
@@ -114,7 +121,7 @@ public:
 };
 
 enum class FunctionType { Unkown = 0, Conv2d, DeConv2d, MatrixMultiply, Add, ReLu, Minus, L1Norm, L2Norm, ReduceMean, MaxPooling2d, AvgPooling2d,
-                          MatrixMultiplyBiasReLu, Conv2dBiasReLu };
+                          MatrixMultiplyBiasReLu, Conv2dBiasReLu, HeadNormRotary, Attention, MatrixMultiplyGated };
 
 class Function : public Node {
 protected:
@@ -225,6 +232,71 @@ public:
                   size_t index, Tensor *iGradient) override;
     using Function::forward;
     void backward() override;
+};
+
+// Norm of each head and its rotation by the position of its row.  Inputs: x [tokens, heads * dim], weight [dim] (only with a norm),
+// positions (Int32, one per row), table (Float32 [positions, rotary], Math::RotaryTable).  No counterpart in the reference, like the two
+// nodes below: see include/deep8_hip.h for what they compute.
+class HeadNormRotary : public Function {
+public:
+    int heads;
+    bool norm;
+    float epsilon;
+    bool interleaved;
+
+    explicit HeadNormRotary(std::vector<Node *> &inputs, int heads, bool norm = true, float epsilon = 1e-6f, bool interleaved = false);
+    Shape checkShape(std::vector<Shape> &inputShapes) override;
+    ElementType checkElementType(std::vector<ElementType> &inputTypes) override;
+    void forward(const std::vector<const Tensor *> &inputs, Tensor *output) override;
+    void backward(const std::vector<const Tensor *> &inputs, const Tensor *output, const Tensor *outputGradient,
+                  size_t index, Tensor *iGradient) override;
+    using Function::forward;
+    void backward() override;  // both gradients through one Math call
+};
+
+// Attention of sequences of any lengths.  Inputs: q [tokens, heads * dim], k, v [keys, kvHeads * dim], qStarts, kStarts (Int32, sequences + 1
+// each, first rows of the sequences' queries and keys).  scale 0: 1 / sqrt(dim).  Rows of no sequence are 0.
+// Keeps the softmax statistics of its last forward call for the backward call.
+class Attention : public Function {
+public:
+    int heads, kvHeads;
+    float scale;
+    bool causal;
+
+    explicit Attention(std::vector<Node *> &inputs, int heads, int kvHeads, float scale = 0, bool causal = true);
+    Shape checkShape(std::vector<Shape> &inputShapes) override;
+    ElementType checkElementType(std::vector<ElementType> &inputTypes) override;
+    void forward(const std::vector<const Tensor *> &inputs, Tensor *output) override;
+    // one input at a time (computes all three on every call)
+    void backward(const std::vector<const Tensor *> &inputs, const Tensor *output, const Tensor *outputGradient,
+                  size_t index, Tensor *iGradient) override;
+    using Function::forward;
+    void backward() override;  // all three gradients through one Math call
+
+protected:
+    Tensor lse;
+    float scaleOf(const Tensor &q) const;
+};
+
+// act(g) * u with (g | u) = x * w.  Inputs: x [rows, inner], w [inner, 2 * cols], the gate's columns first.
+// Keeps g and u of its last forward call for the backward call when its inputs take a gradient.
+class MatrixMultiplyGated : public Function {
+public:
+    Math::GateType act;
+
+    explicit MatrixMultiplyGated(std::vector<Node *> &inputs, Math::GateType act = Math::GateType::SiLU);
+    Shape checkShape(std::vector<Shape> &inputShapes) override;
+    ElementType checkElementType(std::vector<ElementType> &inputTypes) override;
+    void forward(const std::vector<const Tensor *> &inputs, Tensor *output) override;
+    // one input at a time (computes both on every call)
+    void backward(const std::vector<const Tensor *> &inputs, const Tensor *output, const Tensor *outputGradient,
+                  size_t index, Tensor *iGradient) override;
+    void forward() override;
+    void backward() override;  // both gradients through one Math call
+
+protected:
+    Tensor pre;
+    void run(const std::vector<const Tensor *> &inputs, Tensor *output, bool keep);
 };
 
 // z = x - y under the same broadcasting rule (deep8/include/nodes/Minus.h, deep8/src/nodes/Minus.cpp:6-39)

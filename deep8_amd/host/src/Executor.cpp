@@ -256,4 +256,20 @@ Variable &conv2dBiasReLu(Variable &x, Variable &filter, Variable &bias, bool cov
     return x.conv2dBiasReLu(filter, bias, covered, strideY, strideX, dilationY, dilationX);
 }
 
+Variable &rotaryTable(Executor *executor, size_t positions, size_t rotary, double base, double factor, double keepBelow, double slowAbove) {
+    Variable *table = executor->addVariable(std::vector<size_t>{positions, rotary}, DType::Float32, false);
+    Math::RotaryTable(table->value, base, factor, keepBelow, slowAbove);
+    return *table;
+}
+Variable &headNormRotary(Variable &x, Variable &weight, Variable &positions, Variable &table, int heads, float epsilon, bool interleaved) {
+    return x.headNormRotary(weight, positions, table, heads, epsilon, interleaved);
+}
+Variable &headRotary(Variable &x, Variable &positions, Variable &table, int heads, bool interleaved) {
+    return x.headRotary(positions, table, heads, interleaved);
+}
+Variable &attention(Variable &q, Variable &k, Variable &v, Variable &qStarts, Variable &kStarts, int heads, int kvHeads, float scale, bool causal) {
+    return q.attention(k, v, qStarts, kStarts, heads, kvHeads, scale, causal);
+}
+Variable &matrixMultiplyGated(Variable &x, Variable &w, Math::GateType act) { return x.matrixMultiplyGated(w, act); }
+
 }  // namespace Deep8

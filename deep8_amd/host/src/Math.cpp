@@ -814,5 +814,168 @@ void BiasReLuGrad(const Tensor &z, const Tensor &dz, Tensor &dpre, Tensor &dbias
     D8_CHECK(d8_bias_relu_grad(dt, z.raw(), dz.raw(), dpre.raw(), dbias.raw(), rows, cols, fresh ? 0 : 1, ws.ptr, ws.bytes, nullptr));
 }
 
+// ---- a transformer layer -----------------------------------------------------------------------------------------------
+namespace {
+int rowsOf(const Tensor &t) { return (int)(t.shape.batch * t.shape.row()); }
+
+void checkRows(const Tensor &t, size_t cols, const char *what) {
+    DEEP8_ARGUMENT_CHECK(2 == t.shape.nDims && t.shape.col() == cols, "the " << what << " must have rows of " << cols << " elements");
+}
+
+void checkSame(const Tensor &a, const Tensor &b) {
+    DEEP8_ARGUMENT_CHECK(a.deviceType() == b.deviceType(), "the device type must be same");
+    DEEP8_ARGUMENT_CHECK(a.elementType == b.elementType, "the data type must be same");
+}
+
+const int *indices(const Tensor *t, size_t atLeast, const char *what) {
+    if (nullptr == t) return nullptr;
+    requireGPU(*t);
+    DEEP8_ARGUMENT_CHECK(DType::Int32 == t->elementType.id, "the " << what << " must be Int32");
+    DEEP8_ARGUMENT_CHECK(t->size() >= atLeast, "the " << what << " need " << atLeast << " elements");
+    return (const int *)t->raw();
+}
+
+struct Heads {
+    int rows, dim, positions, rotary;
+    const float *table;
+    const int *at;
+};
+
+Heads checkHeads(const Tensor &x, const Tensor *weight, const Tensor *positions, const Tensor *table, const Tensor &y, int heads) {
+    checkSame(x, y);
+    DEEP8_ARGUMENT_CHECK(heads >= 1 && 2 == x.nDims() && 0 == x.col() % heads, "a row must hold whole heads");
+    DEEP8_ARGUMENT_CHECK(x.shape == y.shape, "the shape must be same");
+    requireGPU(x);
+    Heads h{rowsOf(x), (int)x.col() / heads, 0, 0, nullptr, indices(positions, (size_t)rowsOf(x), "positions")};
+    if (weight) {
+        checkSame(x, *weight);
+        DEEP8_ARGUMENT_CHECK((int)weight->size() == h.dim, "the weight must have one value per element of a head");
+    }
+    if (table) {
+        requireGPU(*table);
+        DEEP8_ARGUMENT_CHECK(DType::Float32 == table->elementType.id && 1 == table->batch() && 2 == table->nDims(), "the table must be Float32 [positions, rotary]");
+        h.positions = (int)table->row(), h.rotary = (int)table->col();
+        DEEP8_ARGUMENT_CHECK(0 == h.rotary % 2 && h.rotary <= h.dim, "the table turns an even number of elements, at most a head's");
+        h.table = (const float *)table->raw();
+    }
+    return h;
+}
+
+struct Seen {
+    int sequences, queries, keys, dim;
+    const int *qStarts, *kStarts;
+};
+
+Seen checkAttention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &qStarts, const Tensor &kStarts, const Tensor &o,
+                    const Tensor *lse, int heads, int kvHeads) {
+    checkSame(q, k), checkSame(q, v), checkSame(q, o);
+    DEEP8_ARGUMENT_CHECK(heads >= 1 && kvHeads >= 1 && 0 == heads % kvHeads, "the heads must be a multiple of the heads of keys");
+    DEEP8_ARGUMENT_CHECK(2 == q.nDims() && 0 == q.col() % heads, "a row must hold whole heads");
+    const size_t dim = q.col() / heads;
+    checkRows(k, dim * kvHeads, "keys"), checkRows(v, dim * kvHeads, "values");
+    DEEP8_ARGUMENT_CHECK(rowsOf(k) == rowsOf(v), "each key needs its value");
+    DEEP8_ARGUMENT_CHECK(q.shape == o.shape, "the shape must be same");
+    requireGPU(q);
+    if (lse) {
+        requireGPU(*lse);
+        DEEP8_ARGUMENT_CHECK(DType::Float32 == lse->elementType.id && lse->size() == (size_t)heads * rowsOf(q), "the lse must be Float32, one value per query and head");
+    }
+    DEEP8_ARGUMENT_CHECK(qStarts.size() >= 1 && qStarts.size() == kStarts.size(), "queries and keys need the same number of starts");
+    const size_t n = qStarts.size();
+    return Seen{(int)n - 1, rowsOf(q), rowsOf(k), (int)dim, indices(&qStarts, n, "starts"), indices(&kStarts, n, "starts")};
+}
+
+void checkGated(const Tensor &x, const Tensor &w, const Tensor *pre, const Tensor &h) {
+    checkSame(x, w), checkSame(x, h);
+    DEEP8_ARGUMENT_CHECK(2 == x.nDims() && 2 == w.nDims() && 1 == w.batch() && x.col() == w.row(), "the shape is error");
+    DEEP8_ARGUMENT_CHECK(0 == w.col() % 2, "the weight needs a gate's column for every column");
+    checkRows(h, w.col() / 2, "output");
+    DEEP8_ARGUMENT_CHECK(rowsOf(x) == rowsOf(h), "the shape is error");
+    if (pre) {
+        checkSame(x, *pre), checkRows(*pre, w.col(), "products");
+        DEEP8_ARGUMENT_CHECK(rowsOf(x) == rowsOf(*pre), "the shape is error");
+    }
+    requireGPU(x);
+}
+}  // namespace
+
+void RotaryTable(Tensor &table, double base, double factor, double keepBelow, double slowAbove) {
+    requireGPU(table);
+    DEEP8_ARGUMENT_CHECK(DType::Float32 == table.elementType.id && 1 == table.batch() && 2 == table.nDims(), "the table must be Float32 [positions, rotary]");
+    table.takeZero();  // every element is written
+    D8_CHECK(d8_rotary_table((float *)table.raw(), (int)table.row(), (int)table.col(), base, factor, keepBelow, slowAbove, nullptr));
+}
+
+void HeadNormRotary(const Tensor &x, const Tensor *weight, const Tensor *positions, const Tensor *table, Tensor &y, int heads, float epsilon,
+                    bool interleaved) {
+    const Heads h = checkHeads(x, weight, positions, table, y, heads);
+    const long ld = (long)x.col();
+    y.takeZero();
+    D8_CHECK(d8_head_norm_rotary(dtypeOf(x), x.raw(), ld, heads, weight ? weight->raw() : nullptr, y.raw(), ld, nullptr, 0, 0, nullptr, nullptr, 0,
+                                 h.rows, h.dim, weight ? 1 : 0, epsilon, h.at, h.table, h.positions, h.rotary, interleaved ? 1 : 0, nullptr));
+}
+
+void HeadNormRotaryGrad(const Tensor &x, Tensor &dx, const Tensor *weight, Tensor *dweight, const Tensor *positions, const Tensor *table,
+                        const Tensor &y, const Tensor &dy, int heads, float epsilon, bool interleaved) {
+    const Heads h = checkHeads(x, weight, positions, table, y, heads);
+    checkSame(x, dx), checkSame(x, dy);
+    DEEP8_ARGUMENT_CHECK(x.shape == dx.shape && x.shape == dy.shape, "the shape must be same");
+    DEEP8_ARGUMENT_CHECK(nullptr == dweight || (weight && weight->shape == dweight->shape && weight->elementType == dweight->elementType),
+                         "the weight and its gradient must be alike");
+    const long ld = (long)x.col();
+    const int dt = dtypeOf(x), overwrite = (dx.takeZero() ? 1 : 0) | (dweight && dweight->takeZero() ? 2 : 0);
+    PoolScratch ws(x.device(), d8_head_norm_rotary_grad_scratch_bytes(dt, h.rows, heads, 0, h.dim));
+    D8_CHECK(d8_head_norm_rotary_grad(dt, x.raw(), ld, heads, weight ? weight->raw() : nullptr, dy.raw(), ld, dx.raw(), ld,
+                                      dweight ? dweight->raw() : nullptr, nullptr, 0, 0, nullptr, nullptr, 0, nullptr, 0, nullptr, h.rows, h.dim,
+                                      weight ? 1 : 0, epsilon, h.at, h.table, h.positions, h.rotary, interleaved ? 1 : 0, overwrite, ws.ptr,
+                                      ws.bytes, nullptr));
+}
+
+void Attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &qStarts, const Tensor &kStarts, Tensor &o, Tensor *lse, int heads,
+               int kvHeads, float scale, bool causal) {
+    const Seen s = checkAttention(q, k, v, qStarts, kStarts, o, lse, heads, kvHeads);
+    const int dt = dtypeOf(q);
+    PoolScratch ws(q.device(), d8_attention_scratch_bytes(dt, 0, s.sequences, s.queries, s.keys, heads, kvHeads, s.dim, causal ? 1 : 0));
+    // (rows of no sequence keep what the output holds: a deferred zero fill is performed)
+    D8_CHECK(d8_attention(dt, q.raw(), (long)q.col(), k.raw(), (long)k.col(), v.raw(), (long)v.col(), o.raw(), (long)o.col(),
+                          lse ? (float *)lse->raw() : nullptr, s.qStarts, s.kStarts, s.sequences, s.queries, s.keys, heads, kvHeads, s.dim, scale,
+                          causal ? 1 : 0, ws.ptr, ws.bytes, nullptr));
+}
+
+void AttentionGrad(const Tensor &q, Tensor &dq, const Tensor &k, Tensor &dk, const Tensor &v, Tensor &dv, const Tensor &qStarts,
+                   const Tensor &kStarts, const Tensor &o, const Tensor &lse, const Tensor &dout, int heads, int kvHeads, float scale, bool causal) {
+    const Seen s = checkAttention(q, k, v, qStarts, kStarts, o, &lse, heads, kvHeads);
+    checkSame(q, dq), checkSame(q, dk), checkSame(q, dv), checkSame(q, dout);
+    DEEP8_ARGUMENT_CHECK(q.shape == dq.shape && k.shape == dk.shape && v.shape == dv.shape && q.shape == dout.shape, "the shape must be same");
+    DEEP8_ARGUMENT_CHECK(dq.raw() != dk.raw() && dq.raw() != dv.raw() && dk.raw() != dv.raw(), "the gradients must be different tensors");
+    const int dt = dtypeOf(q);
+    PoolScratch ws(q.device(), d8_attention_scratch_bytes(dt, 1, s.sequences, s.queries, s.keys, heads, kvHeads, s.dim, causal ? 1 : 0));
+    D8_CHECK(d8_attention_grad(dt, q.raw(), (long)q.col(), k.raw(), (long)k.col(), v.raw(), (long)v.col(), o.raw(), (long)o.col(),
+                               (const float *)lse.raw(), dout.raw(), (long)dout.col(), dq.raw(), (long)dq.col(), dk.raw(), (long)dk.col(), dv.raw(),
+                               (long)dv.col(), s.qStarts, s.kStarts, s.sequences, s.queries, s.keys, heads, kvHeads, s.dim, scale, causal ? 1 : 0, 0,
+                               ws.ptr, ws.bytes, nullptr));
+}
+
+void MatrixMultiplyGated(const Tensor &x, const Tensor &w, Tensor *pre, Tensor &h, GateType act) {
+    checkGated(x, w, pre, h);
+    const int dt = dtypeOf(x), rows = rowsOf(x), inner = (int)x.col(), cols = (int)h.col();
+    PoolScratch ws(x.device(), d8_matmul_gated_scratch_bytes(dt, 0, rows, inner, cols));
+    h.takeZero();
+    if (pre) pre->takeZero();
+    D8_CHECK(d8_matmul_gated(dt, x.raw(), rows, inner, w.raw(), cols, (int)act, pre ? pre->raw() : nullptr, h.raw(), ws.ptr, ws.bytes, nullptr));
+}
+
+void MatrixMultiplyGatedGrad(const Tensor &x, Tensor &dx, const Tensor &w, Tensor &dw, const Tensor &pre, const Tensor &h, const Tensor &dh,
+                             GateType act) {
+    checkGated(x, w, &pre, h);
+    checkSame(x, dx), checkSame(x, dw), checkSame(x, dh);
+    DEEP8_ARGUMENT_CHECK(x.shape == dx.shape && w.shape == dw.shape && h.shape == dh.shape, "the shape must be same");
+    const int dt = dtypeOf(x), rows = rowsOf(x), inner = (int)x.col(), cols = (int)h.col();
+    PoolScratch ws(x.device(), d8_matmul_gated_scratch_bytes(dt, 1, rows, inner, cols));
+    const int overwrite = (dx.takeZero() ? 1 : 0) | (dw.takeZero() ? 2 : 0);
+    D8_CHECK(d8_matmul_gated_grad(dt, x.raw(), dx.raw(), rows, inner, w.raw(), dw.raw(), cols, (int)act, pre.raw(), dh.raw(), overwrite, ws.ptr,
+                                  ws.bytes, nullptr));
+}
+
 }  // namespace Math
 }  // namespace Deep8

@@ -2,6 +2,7 @@
 #include "deep8/Nodes.h"
 
 #include <algorithm>
+#include <cmath>
 #include <random>
 
 #include "deep8/Executor.h"
@@ -182,6 +183,30 @@ Variable &Variable::conv2dBiasReLu(Variable &filter, Variable &bias, bool covere
     DEEP8_ARGUMENT_CHECK(nullptr != executor, "the Variable does not belong to an Executor");
     std::vector<Node *> in = {this, &filter, &bias};
     return *executor->addFunction(new Conv2dBiasReLu(in, covered, strideY, strideX, dilationY, dilationX));
+}
+
+Variable &Variable::headNormRotary(Variable &weight, Variable &positions, Variable &table, int heads, float epsilon, bool interleaved) {
+    DEEP8_ARGUMENT_CHECK(nullptr != executor, "the Variable does not belong to an Executor");
+    std::vector<Node *> in = {this, &weight, &positions, &table};
+    return *executor->addFunction(new HeadNormRotary(in, heads, true, epsilon, interleaved));
+}
+
+Variable &Variable::headRotary(Variable &positions, Variable &table, int heads, bool interleaved) {
+    DEEP8_ARGUMENT_CHECK(nullptr != executor, "the Variable does not belong to an Executor");
+    std::vector<Node *> in = {this, &positions, &table};
+    return *executor->addFunction(new HeadNormRotary(in, heads, false, 0, interleaved));
+}
+
+Variable &Variable::attention(Variable &k, Variable &v, Variable &qStarts, Variable &kStarts, int heads, int kvHeads, float scale, bool causal) {
+    DEEP8_ARGUMENT_CHECK(nullptr != executor, "the Variable does not belong to an Executor");
+    std::vector<Node *> in = {this, &k, &v, &qStarts, &kStarts};
+    return *executor->addFunction(new Attention(in, heads, kvHeads, scale, causal));
+}
+
+Variable &Variable::matrixMultiplyGated(Variable &w, Math::GateType act) {
+    DEEP8_ARGUMENT_CHECK(nullptr != executor, "the Variable does not belong to an Executor");
+    std::vector<Node *> in = {this, &w};
+    return *executor->addFunction(new MatrixMultiplyGated(in, act));
 }
 
 Variable &Variable::minus(Variable &y) {
@@ -599,6 +624,165 @@ void Conv2dBiasReLu::backward() {
     }, [this](const std::vector<const Tensor *> &v, const Tensor &z, const Tensor &dz, Tensor &gx, Tensor &gw) {
         Math::Conv2dGradXY(*v[0], gx, *v[1], gw, z, dz, covered, strideY, strideX, dilationY, dilationX);
     });
+}
+
+// ---- a transformer layer ------------------------------------------------------------------------------------------------
+namespace {
+// a tensor of the device pool (released with its last copy)
+Tensor tensorOn(Device *dev, Shape shape, ElementType type) {
+    const size_t bytes = type.byteWidth * shape.size();
+    void *ptr = dev->malloc(bytes);
+    size_t *ref = (size_t *)dev->mallocCPU(sizeof(size_t));
+    TensorStorage storage(ptr, ref, bytes, dev);
+    return Tensor(storage, 0, shape, type);
+}
+
+// where a gradient goes: the variable's own, or a tensor that nobody reads
+Tensor gradientOr(Variable *v, const Tensor &value) { return v->updateGradient ? v->gradient : tensorLike(value); }
+
+ElementType checkTypes(std::vector<ElementType> &types, size_t values, size_t indices) {
+    for (size_t i = 1; i < values; ++i) DEEP8_ARGUMENT_CHECK(types[0] == types[i], "the input's ElementType must be same");
+    for (size_t i = values; i < values + indices; ++i) DEEP8_ARGUMENT_CHECK(DType::Int32 == types[i].id, "positions and starts must be Int32");
+    return types[0];
+}
+}  // namespace
+
+HeadNormRotary::HeadNormRotary(std::vector<Node *> &in, int h, bool n, float e, bool i)
+    : Function(in), heads(h), norm(n), epsilon(e), interleaved(i) {
+    DEEP8_ARGUMENT_CHECK((norm ? 4u : 3u) == inputs.size(), "the HeadNormRotary Function needs x, a weight (with a norm), positions and a table");
+    DEEP8_ARGUMENT_CHECK(heads >= 1, "the heads must >= 1");
+}
+
+Shape HeadNormRotary::checkShape(std::vector<Shape> &shapes) {
+    DEEP8_ARGUMENT_CHECK((norm ? 4u : 3u) == shapes.size(), "the input count is error");
+    const Shape &x = shapes[0], &positions = shapes[norm ? 2 : 1], &table = shapes[norm ? 3 : 2];
+    DEEP8_ARGUMENT_CHECK(2 == x.nDims && 0 == x.col() % heads, "a row must hold whole heads");
+    const size_t dim = x.col() / heads;
+    DEEP8_ARGUMENT_CHECK(!norm || shapes[1].size() == dim, "the weight must have one value per element of a head");
+    DEEP8_ARGUMENT_CHECK(positions.size() >= x.batch * x.row(), "every row needs its position");
+    DEEP8_ARGUMENT_CHECK(1 == table.batch && 2 == table.nDims && 0 == table.col() % 2 && table.col() <= dim, "the table must be [positions, rotary]");
+    return x;
+}
+
+ElementType HeadNormRotary::checkElementType(std::vector<ElementType> &types) {
+    DEEP8_ARGUMENT_CHECK((norm ? 4u : 3u) == types.size(), "the input count is error");
+    DEEP8_ARGUMENT_CHECK(DType::Float32 == types.back().id, "the table must be Float32");
+    return checkTypes(types, norm ? 2 : 1, 1);
+}
+
+void HeadNormRotary::forward(const std::vector<const Tensor *> &in, Tensor *output) {
+    Math::HeadNormRotary(*in[0], norm ? in[1] : nullptr, in[norm ? 2 : 1], in[norm ? 3 : 2], *output, heads, epsilon, interleaved);
+}
+
+void HeadNormRotary::backward(const std::vector<const Tensor *> &in, const Tensor *output, const Tensor *outputGradient, size_t index,
+                              Tensor *iGradient) {
+    DEEP8_ARGUMENT_CHECK(0 == index || (norm && 1 == index), "positions and tables have no gradient");
+    Tensor unused;
+    if (1 == index) unused = tensorLike(*in[0]);
+    Math::HeadNormRotaryGrad(*in[0], 0 == index ? *iGradient : unused, norm ? in[1] : nullptr, 1 == index ? iGradient : nullptr, in[norm ? 2 : 1],
+                             in[norm ? 3 : 2], *output, *outputGradient, heads, epsilon, interleaved);
+}
+
+void HeadNormRotary::backward() {
+    Variable *x = (Variable *)inputs[0], *weight = norm ? (Variable *)inputs[1] : nullptr;
+    if (!weight || !x->updateGradient || !weight->updateGradient || x == weight) return Function::backward();
+    Variable *out = nullptr;
+    std::vector<const Tensor *> in = gatherInputs(this, out);
+    Math::HeadNormRotaryGrad(*in[0], x->gradient, in[1], &weight->gradient, in[2], in[3], out->value, out->gradient, heads, epsilon, interleaved);
+}
+
+Attention::Attention(std::vector<Node *> &in, int h, int kv, float s, bool c) : Function(in), heads(h), kvHeads(kv), scale(s), causal(c) {
+    DEEP8_ARGUMENT_CHECK(5 == inputs.size(), "the Attention Function needs queries, keys, values and the starts of both");
+    DEEP8_ARGUMENT_CHECK(heads >= 1 && kvHeads >= 1 && 0 == heads % kvHeads, "the heads must be a multiple of the heads of keys");
+}
+
+Shape Attention::checkShape(std::vector<Shape> &shapes) {
+    DEEP8_ARGUMENT_CHECK(5 == shapes.size(), "the input count must be 5");
+    const Shape &q = shapes[0], &k = shapes[1], &v = shapes[2];
+    DEEP8_ARGUMENT_CHECK(2 == q.nDims && 2 == k.nDims && 2 == v.nDims && 0 == q.col() % heads, "a row must hold whole heads");
+    DEEP8_ARGUMENT_CHECK(k.col() == q.col() / heads * kvHeads && v.col() == k.col(), "a row of keys or values must hold whole heads of the queries' size");
+    DEEP8_ARGUMENT_CHECK(k.batch * k.row() == v.batch * v.row(), "each key needs its value");
+    DEEP8_ARGUMENT_CHECK(shapes[3].size() == shapes[4].size(), "queries and keys need the same number of starts");
+    return q;
+}
+
+ElementType Attention::checkElementType(std::vector<ElementType> &types) {
+    DEEP8_ARGUMENT_CHECK(5 == types.size(), "the input count must be 5");
+    return checkTypes(types, 3, 2);
+}
+
+float Attention::scaleOf(const Tensor &q) const { return 0 != scale ? scale : 1.0f / std::sqrt((float)(q.col() / heads)); }
+
+void Attention::forward(const std::vector<const Tensor *> &in, Tensor *output) {
+    const Shape &q = in[0]->shape;
+    lse = tensorOn(output->device(), Shape(std::vector<size_t>{(size_t)heads * q.batch * q.row()}), ElementType::from<float>());
+    output->zero();
+    Math::Attention(*in[0], *in[1], *in[2], *in[3], *in[4], *output, &lse, heads, kvHeads, scaleOf(*in[0]), causal);
+}
+
+void Attention::backward(const std::vector<const Tensor *> &in, const Tensor *output, const Tensor *outputGradient, size_t index,
+                         Tensor *iGradient) {
+    DEEP8_ARGUMENT_CHECK(index < 3, "starts have no gradient");
+    Tensor d[3];
+    for (size_t i = 0; i < 3; ++i) d[i] = i == index ? *iGradient : tensorLike(*in[i]);
+    Math::AttentionGrad(*in[0], d[0], *in[1], d[1], *in[2], d[2], *in[3], *in[4], *output, lse, *outputGradient, heads, kvHeads, scaleOf(*in[0]),
+                        causal);
+}
+
+void Attention::backward() {
+    Variable *q = (Variable *)inputs[0], *k = (Variable *)inputs[1], *v = (Variable *)inputs[2];
+    if (q == k || q == v || k == v) return Function::backward();  // (their gradients add up one after the other)
+    if (!q->updateGradient && !k->updateGradient && !v->updateGradient) return;
+    Variable *out = nullptr;
+    std::vector<const Tensor *> in = gatherInputs(this, out);
+    Tensor dq = gradientOr(q, *in[0]), dk = gradientOr(k, *in[1]), dv = gradientOr(v, *in[2]);
+    Math::AttentionGrad(*in[0], dq, *in[1], dk, *in[2], dv, *in[3], *in[4], out->value, lse, out->gradient, heads, kvHeads, scaleOf(*in[0]), causal);
+}
+
+MatrixMultiplyGated::MatrixMultiplyGated(std::vector<Node *> &in, Math::GateType a) : Function(in), act(a) {
+    DEEP8_ARGUMENT_CHECK(2 == inputs.size(), "the MatrixMultiplyGated Function needs 2 input");
+}
+
+Shape MatrixMultiplyGated::checkShape(std::vector<Shape> &shapes) {
+    DEEP8_ARGUMENT_CHECK(2 == shapes.size(), "the input count must be 2");
+    const Shape &x = shapes[0], &w = shapes[1];
+    DEEP8_ARGUMENT_CHECK(2 == x.nDims && 2 == w.nDims && 1 == w.batch, "the inputs dimensions is error");
+    DEEP8_ARGUMENT_CHECK(x.col() == w.row(), "the col of input1 must same to the row of input2");
+    DEEP8_ARGUMENT_CHECK(0 == w.col() % 2, "the weight needs a gate's column for every column");
+    return Shape(x.batch, {x.row(), w.col() / 2});
+}
+
+ElementType MatrixMultiplyGated::checkElementType(std::vector<ElementType> &types) {
+    DEEP8_ARGUMENT_CHECK(2 == types.size(), "the input count must be 2");
+    return Function::checkElementType(types);
+}
+
+void MatrixMultiplyGated::run(const std::vector<const Tensor *> &in, Tensor *output, bool keep) {
+    pre = keep ? tensorOn(output->device(), Shape(in[0]->shape.batch, {in[0]->row(), in[1]->col()}), in[0]->elementType) : Tensor();
+    Math::MatrixMultiplyGated(*in[0], *in[1], keep ? &pre : nullptr, *output, act);
+}
+
+void MatrixMultiplyGated::forward(const std::vector<const Tensor *> &in, Tensor *output) { run(in, output, true); }
+
+void MatrixMultiplyGated::forward() {
+    Variable *out = nullptr;
+    std::vector<const Tensor *> in = gatherInputs(this, out);
+    run(in, &out->value, out->updateGradient);
+}
+
+void MatrixMultiplyGated::backward(const std::vector<const Tensor *> &in, const Tensor *output, const Tensor *outputGradient, size_t index,
+                                   Tensor *iGradient) {
+    DEEP8_ARGUMENT_CHECK(index < 2, "the index is error");
+    Tensor unused = tensorLike(*in[1 - index]);
+    Math::MatrixMultiplyGatedGrad(*in[0], 0 == index ? *iGradient : unused, *in[1], 1 == index ? *iGradient : unused, pre, *output, *outputGradient, act);
+}
+
+void MatrixMultiplyGated::backward() {
+    Variable *x = (Variable *)inputs[0], *w = (Variable *)inputs[1];
+    if (!x->updateGradient || !w->updateGradient || x == w) return Function::backward();
+    Variable *out = nullptr;
+    std::vector<const Tensor *> in = gatherInputs(this, out);
+    Math::MatrixMultiplyGatedGrad(*in[0], x->gradient, *in[1], w->gradient, pre, out->value, out->gradient, act);
 }
 
 // ---- Add / ReLu -------------------------------------------------------------------------------------------------

@@ -1008,6 +1008,290 @@ TEST_GPU(fused_bias_relu_nodes_match_the_chain_of_nodes) {
     EXPECT(throws<std::invalid_argument>([&] { conv2dBiasReLu(x, w, bad); }));
 }
 
+// ---- a transformer layer: HeadNormRotary, Attention, MatrixMultiplyGated --------------------------------------------------
+// Each node against its formula in double, its gradients against central differences of that formula.
+typedef std::vector<double> Doubles;
+
+Doubles differences(const std::function<Doubles(const std::vector<Doubles> &)> &f, std::vector<Doubles> in, size_t which, const Doubles &g) {
+    const double step = 1e-5;
+    auto along = [&] {
+        const Doubles y = f(in);
+        double s = 0;
+        for (size_t i = 0; i < y.size(); ++i) s += y[i] * g[i];
+        return s;
+    };
+    Doubles d(in[which].size());
+    for (size_t i = 0; i < d.size(); ++i) {
+        const double at = in[which][i];
+        in[which][i] = at + step;
+        const double up = along();
+        in[which][i] = at - step;
+        const double down = along();
+        in[which][i] = at;
+        d[i] = (up - down) / (2 * step);
+    }
+    return d;
+}
+
+void expectClose(HostTensor &got, const Doubles &want, double tolerance) {
+    download(got);
+    EXPECT(got.host.size() == want.size());
+    double num = 0, den = 0;
+    for (size_t i = 0; i < want.size(); ++i) num += (got.host[i] - want[i]) * (got.host[i] - want[i]), den += want[i] * want[i];
+    EXPECT(den > 0 && std::sqrt(num / den) <= tolerance);
+}
+
+HostTensor normalTensor(ElementType type, size_t batch, std::vector<size_t> dims) {
+    HostTensor h;
+    h.t = makeTensor(gpu(), type, batch, dims);
+    h.host.resize(h.t.size());
+    std::normal_distribution<float> nd;
+    for (float &v : h.host) v = DType::Float16 == type.id ? (float)half(nd(rng)) : nd(rng);
+    upload(h);
+    return h;
+}
+
+HostTensor intTensor(const std::vector<int> &v) {
+    HostTensor h;
+    h.t = makeTensor(gpu(), ElementType::from(DType::Int32), 1, {v.size()});
+    h.t.device()->copyFromCPUToGPU(v.data(), h.t.raw(), h.t.byteCount());
+    return h;
+}
+
+Doubles doubles(const HostTensor &h) { return Doubles(h.host.begin(), h.host.end()); }
+
+// forward, then each input's gradient on top of ones (a gradient call adds), against f and its differences
+template <typename NodeT>
+void layerCase(NodeT &node, std::vector<HostTensor *> in, size_t values, const std::function<Doubles(const std::vector<Doubles> &)> &f) {
+    std::vector<const Tensor *> tin;
+    std::vector<Shape> shapes;
+    std::vector<ElementType> types;
+    for (HostTensor *h : in) tin.push_back(&h->t), shapes.push_back(h->t.shape), types.push_back(h->t.elementType);
+    const Shape s = node.checkShape(shapes);
+    const ElementType type = node.checkElementType(types);
+    HostTensor out = normalTensor(type, s.batch, std::vector<size_t>(s.dims, s.dims + s.nDims));
+    HostTensor dout = normalTensor(type, s.batch, std::vector<size_t>(s.dims, s.dims + s.nDims));
+    node.forward(tin, &out.t);
+    std::vector<Doubles> host;
+    for (size_t i = 0; i < values; ++i) host.push_back(doubles(*in[i]));
+    // Float32: sums of some ten products, roundings of 6e-8 each, the attention's exponent of scores around 3: 1e-5 is ten times what they
+    // add up to.  Float16: the result's rounding is 2.8e-4 in the mean, and as much again for the attention's powers and the kept products.
+    const double tolerance = DType::Float16 == type.id ? 2e-3 : 1e-5;
+    expectClose(out, f(host), tolerance);
+    for (size_t i = 0; i < values; ++i) {
+        HostTensor d;
+        d.t = makeTensor(gpu(), type, in[i]->t.shape.batch, std::vector<size_t>(shapes[i].dims, shapes[i].dims + shapes[i].nDims));
+        d.host.assign(d.t.size(), 1.f);
+        upload(d);
+        node.backward(tin, &out.t, &dout.t, i, &d.t);
+        Doubles want = differences(f, host, i, doubles(dout));
+        for (double &v : want) v += 1;
+        expectClose(d, want, DType::Float16 == type.id ? 4e-3 : 2e-5);
+    }
+}
+
+TEST_GPU(head_norm_rotary_node) {
+    const int tokens = 7, heads = 3, dim = 8, rotary = 6;
+    const std::vector<int> at = {0, 1, 2, 3, 0, 1, 4};
+    for (DType id : {DType::Float32, DType::Float16})
+        for (int mode = 0; mode < 4; ++mode) {
+            const bool norm = mode & 1, interleaved = mode & 2;
+            const ElementType type = ElementType::from(id);
+            HostTensor x = normalTensor(type, 1, {tokens, heads * dim}), w = normalTensor(type, 1, {dim}), positions = intTensor(at);
+            HostTensor table;
+            table.t = makeTensor(gpu(), ElementType::from<float>(), 1, {5, rotary});
+            Math::RotaryTable(table.t);
+            Variable v0 = placeholder(type), v1 = placeholder(type), v2 = placeholder(type), v3 = placeholder(type);
+            std::vector<Node *> nodes = norm ? std::vector<Node *>{&v0, &v1, &v2, &v3} : std::vector<Node *>{&v0, &v2, &v3};
+            HeadNormRotary node(nodes, heads, norm, 1e-6f, interleaved);
+            auto f = [&](const std::vector<Doubles> &in) {
+                Doubles y = in[0];
+                for (int t = 0; t < tokens; ++t)
+                    for (int h = 0; h < heads; ++h) {
+                        double *n = &y[(t * heads + h) * dim], sum = 0;
+                        for (int e = 0; e < dim; ++e) sum += n[e] * n[e];
+                        for (int e = 0; norm && e < dim; ++e) n[e] *= in[1][e] / std::sqrt(sum / dim + 1e-6);
+                        for (int i = 0; i < rotary / 2; ++i) {
+                            const double angle = at[t] * std::pow(10000.0, -2.0 * i / rotary), c = std::cos(angle), s = std::sin(angle);
+                            double &a = n[interleaved ? 2 * i : i], &b = n[interleaved ? 2 * i + 1 : i + rotary / 2];
+                            const double p = a * c - b * s;
+                            b = a * s + b * c, a = p;
+                        }
+                    }
+                return y;
+            };
+            std::vector<HostTensor *> in = norm ? std::vector<HostTensor *>{&x, &w, &positions, &table} : std::vector<HostTensor *>{&x, &positions, &table};
+            layerCase(node, in, norm ? 2 : 1, f);
+        }
+}
+
+TEST_GPU(attention_node) {
+    // sequences of 3, 0, 1 and 5 queries with 4, 2, 0 and 5 keys (the second has keys alone, the third's query sees nothing)
+    const std::vector<int> qs = {0, 3, 3, 4, 9}, ks = {0, 4, 6, 6, 11};
+    const int heads = 4, kvHeads = 2, dim = 8, queries = 9, keys = 11;
+    for (DType id : {DType::Float32, DType::Float16})
+        for (bool causal : {true, false}) {
+            const ElementType type = ElementType::from(id);
+            HostTensor q = normalTensor(type, 1, {queries, heads * dim}), k = normalTensor(type, 1, {keys, kvHeads * dim}), v = normalTensor(type, 1, {keys, kvHeads * dim});
+            HostTensor qStarts = intTensor(qs), kStarts = intTensor(ks);
+            Variable v0 = placeholder(type), v1 = placeholder(type), v2 = placeholder(type), v3 = placeholder(type), v4 = placeholder(type);
+            std::vector<Node *> nodes = {&v0, &v1, &v2, &v3, &v4};
+            Attention node(nodes, heads, kvHeads, 0, causal);
+            auto f = [&](const std::vector<Doubles> &in) {
+                Doubles o(in[0].size(), 0.0);
+                for (size_t s = 0; s + 1 < qs.size(); ++s)
+                    for (int t = qs[s]; t < qs[s + 1]; ++t)
+                        for (int h = 0; h < heads; ++h) {
+                            const int nk = ks[s + 1] - ks[s], sees = causal ? std::min(nk, nk - (qs[s + 1] - qs[s]) + (t - qs[s]) + 1) : nk;
+                            double sum = 0;
+                            double *to = &o[(t * heads + h) * dim];
+                            for (int j = 0; j < sees; ++j) {
+                                const size_t at = (size_t)((ks[s] + j) * kvHeads + h / (heads / kvHeads)) * dim;
+                                double score = 0;
+                                for (int e = 0; e < dim; ++e) score += in[0][(t * heads + h) * dim + e] * in[1][at + e];
+                                const double p = std::exp(score / std::sqrt((double)dim));
+                                sum += p;
+                                for (int e = 0; e < dim; ++e) to[e] += p * in[2][at + e];
+                            }
+                            for (int e = 0; sum > 0 && e < dim; ++e) to[e] /= sum;
+                        }
+                return o;
+            };
+            layerCase(node, {&q, &k, &v, &qStarts, &kStarts}, 3, f);
+        }
+}
+
+TEST_GPU(matrix_multiply_gated_node) {
+    const int rows = 5, inner = 12, cols = 6;
+    const Math::GateType acts[] = {Math::GateType::SiLU, Math::GateType::GeLU, Math::GateType::ReLu, Math::GateType::Sigmoid};
+    for (DType id : {DType::Float32, DType::Float16})
+        for (Math::GateType act : acts) {
+            const ElementType type = ElementType::from(id);
+            HostTensor x = normalTensor(type, 1, {rows, inner}), w = normalTensor(type, 1, {inner, 2 * cols});
+            Variable v0 = placeholder(type), v1 = placeholder(type);
+            std::vector<Node *> nodes = {&v0, &v1};
+            MatrixMultiplyGated node(nodes, act);
+            auto f = [&](const std::vector<Doubles> &in) {
+                Doubles h(rows * cols);
+                for (int r = 0; r < rows; ++r)
+                    for (int c = 0; c < cols; ++c) {
+                        double g = 0, u = 0;
+                        for (int k = 0; k < inner; ++k) g += in[0][r * inner + k] * in[1][k * 2 * cols + c], u += in[0][r * inner + k] * in[1][k * 2 * cols + cols + c];
+                        const double sigmoid = 1 / (1 + std::exp(-g));
+                        const double a = act == Math::GateType::SiLU ? g * sigmoid : act == Math::GateType::GeLU ? g * 0.5 * (1 + std::erf(g / std::sqrt(2.0)))
+                                       : act == Math::GateType::ReLu ? std::max(g, 0.0) : sigmoid;
+                        h[r * cols + c] = a * u;
+                    }
+                return h;
+            };
+            layerCase(node, {&x, &w}, 2, f);
+        }
+}
+
+TEST_GPU(transformer_layer_backward_at_once_and_input_by_input) {
+    // the executor's pass (all gradients of a node from one call) against the nodes' own, input by input; and one variable as queries, keys
+    // and values, whose three gradients add up
+    EagerExecutor executor;
+    std::vector<int> first = {0, 4, 9}, at = {0, 1, 2, 3, 0, 1, 2, 3, 4};
+    auto fill = [&](Variable &v) {
+        std::vector<float> h(v.shape().size());
+        std::normal_distribution<float> nd;
+        for (float &f : h) f = nd(rng);
+        v.feed(h.data());
+    };
+    auto gradient = [&](Variable &v) {
+        std::vector<float> h(v.shape().size());
+        v.gradient.device()->copyFromGPUToCPU(v.gradient.raw(), h.data(), h.size() * 4);
+        return h;
+    };
+    Variable &x = parameter(&executor, {9, 16}), &w = parameter(&executor, {8}), &gate = parameter(&executor, {16, 24}), &same = parameter(&executor, {9, 16});
+    Variable &starts = *executor.addVariable(std::vector<size_t>{3}, DType::Int32, false), &positions = *executor.addVariable(std::vector<size_t>{9}, DType::Int32, false);
+    Variable &table = rotaryTable(&executor, 5, 8);
+    fill(x), fill(w), fill(gate), fill(same);
+    starts.feed(first.data()), positions.feed(at.data());
+    Variable &turned = headNormRotary(x, w, positions, table, 2), &h = matrixMultiplyGated(x, gate), &o = attention(same, same, same, starts, starts, 2, 2);
+    EXPECT(turned.shape() == x.shape() && h.shape() == Shape(1, {9, 12}) && o.shape() == x.shape());
+    HeadNormRotary *turn = (HeadNormRotary *)turned.inputs[0];
+    MatrixMultiplyGated *gated = (MatrixMultiplyGated *)h.inputs[0];
+    Attention *see = (Attention *)o.inputs[0];
+    backward(turned.l2NormLoss() + h.l2NormLoss() + o.l2NormLoss(), false);
+    const std::vector<float> gx = gradient(x), gw = gradient(w), gg = gradient(gate), gs = gradient(same);
+    x.zeroGradient(), w.zeroGradient(), gate.zeroGradient(), same.zeroGradient();
+    std::vector<const Tensor *> ti = {&x.value, &w.value, &positions.value, &table.value}, gi = {&x.value, &gate.value};
+    std::vector<const Tensor *> ai = {&same.value, &same.value, &same.value, &starts.value, &starts.value};
+    turn->backward(ti, &turned.value, &turned.gradient, 0, &x.gradient), turn->backward(ti, &turned.value, &turned.gradient, 1, &w.gradient);
+    gated->backward(gi, &h.value, &h.gradient, 0, &x.gradient), gated->backward(gi, &h.value, &h.gradient, 1, &gate.gradient);
+    for (size_t i = 0; i < 3; ++i) see->backward(ai, &o.value, &o.gradient, i, &same.gradient);
+    auto close = [&](const std::vector<float> &a, const std::vector<float> &b) {
+        double num = 0, den = 0;
+        for (size_t i = 0; i < a.size(); ++i) num += (double)(a[i] - b[i]) * (a[i] - b[i]), den += (double)a[i] * a[i];
+        return den > 0 && std::sqrt(num / den) <= 1e-6;  // (the same sums, added to the gradient in another order)
+    };
+    EXPECT(close(gx, gradient(x)) && close(gw, gradient(w)) && close(gg, gradient(gate)) && close(gs, gradient(same)));
+    EXPECT(throws<std::invalid_argument>([&] { turn->backward(ti, &turned.value, &turned.gradient, 2, &x.gradient); }));
+    EXPECT(throws<std::invalid_argument>([&] { see->backward(ai, &o.value, &o.gradient, 3, &x.gradient); }));
+    // what the Math functions refuse
+    EXPECT(throws<std::invalid_argument>([&] { Math::HeadNormRotary(x.value, &w.value, &starts.value, &table.value, turned.value, 2); }));    // three positions
+    EXPECT(throws<std::invalid_argument>([&] { Math::HeadNormRotary(x.value, &w.value, &positions.value, &gate.value, turned.value, 2); }));  // a table of 24 for heads of 8
+    EXPECT(throws<std::invalid_argument>([&] { Math::Attention(x.value, x.value, x.value, starts.value, table.value, o.value, nullptr, 2, 2, 1.f); }));
+    EXPECT(throws<std::invalid_argument>([&] {
+        Math::AttentionGrad(x.value, x.gradient, x.value, x.gradient, x.value, x.gradient, starts.value, starts.value, o.value, o.value, o.gradient, 2, 2, 1.f);
+    }));
+    executor.clearInterimNodes();
+}
+
+TEST_CPU(transformer_layer_shape_inference) {
+    const ElementType f32 = ElementType::from<float>(), h16 = ElementType::from<half>(), i32 = ElementType::from(DType::Int32);
+    struct Probe : Variable {
+        Probe() : Variable(0, "", nullptr) {}
+    } a, b, c, d, e;
+    std::vector<Node *> two = {&a, &b}, three = {&a, &b, &c}, four = {&a, &b, &c, &d}, five = {&a, &b, &c, &d, &e};
+    EXPECT(throws<std::invalid_argument>([&] { HeadNormRotary n(three, 4); }));
+    EXPECT(throws<std::invalid_argument>([&] { HeadNormRotary n(four, 0); }));
+    EXPECT(throws<std::invalid_argument>([&] { Attention n(four, 4, 2); }));
+    EXPECT(throws<std::invalid_argument>([&] { Attention n(five, 4, 3); }));
+    EXPECT(throws<std::invalid_argument>([&] { MatrixMultiplyGated n(three); }));
+
+    HeadNormRotary turn(four, 4);
+    std::vector<Shape> s = {Shape(2, {5, 32}), Shape(1, {8}), Shape(1, {10}), Shape(1, {64, 6})};
+    EXPECT(turn.checkShape(s) == Shape(2, {5, 32}));
+    auto refusesTurn = [&](size_t i, Shape shape) {
+        std::vector<Shape> t = s;
+        t[i] = shape;
+        return throws<std::invalid_argument>([&] { turn.checkShape(t); });
+    };
+    EXPECT(refusesTurn(0, Shape(2, {5, 30})) && refusesTurn(1, Shape(1, {7})) && refusesTurn(2, Shape(1, {9})) && refusesTurn(3, Shape(1, {64, 10})) &&
+           refusesTurn(3, Shape(1, {64, 5})));
+    std::vector<ElementType> t = {h16, h16, i32, f32};
+    EXPECT(turn.checkElementType(t) == h16);
+    t = {h16, f32, i32, f32};
+    EXPECT(throws<std::invalid_argument>([&] { turn.checkElementType(t); }));
+    t = {h16, h16, f32, f32};
+    EXPECT(throws<std::invalid_argument>([&] { turn.checkElementType(t); }));
+
+    Attention see(five, 4, 2);
+    std::vector<Shape> q = {Shape(1, {5, 32}), Shape(1, {9, 16}), Shape(1, {9, 16}), Shape(1, {3}), Shape(1, {3})};
+    EXPECT(see.checkShape(q) == Shape(1, {5, 32}));
+    auto refusesSee = [&](size_t i, Shape shape) {
+        std::vector<Shape> p = q;
+        p[i] = shape;
+        return throws<std::invalid_argument>([&] { see.checkShape(p); });
+    };
+    EXPECT(refusesSee(0, Shape(1, {5, 30})) && refusesSee(1, Shape(1, {9, 32})) && refusesSee(2, Shape(1, {8, 16})) && refusesSee(4, Shape(1, {4})));
+    t = {f32, f32, f32, i32, i32};
+    EXPECT(see.checkElementType(t) == f32);
+    t = {f32, f32, f32, i32, f32};
+    EXPECT(throws<std::invalid_argument>([&] { see.checkElementType(t); }));
+
+    MatrixMultiplyGated gated(two);
+    std::vector<Shape> g = {Shape(3, {5, 8}), Shape(1, {8, 24})};
+    EXPECT(gated.checkShape(g) == Shape(3, {5, 12}));
+    g[1] = Shape(1, {8, 23});
+    EXPECT(throws<std::invalid_argument>([&] { gated.checkShape(g); }));
+    g[1] = Shape(1, {7, 24});
+    EXPECT(throws<std::invalid_argument>([&] { gated.checkShape(g); }));
+}
+
 }  // namespace
 
 // Node-level step times at the three large configurations: forward + both gradients through Function::forward /

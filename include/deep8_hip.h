@@ -466,13 +466,18 @@ int d8_avgpool2d_grad_overwrite(int dtype, void *dx, const void *dy, int B, int 
  *                        lse[heads][q_tokens] (may be NULL): the logarithm of the sum of exp(score).  A query that sees nothing
  *                        gets o = 0 and lse = -infinity.  Rows of no sequence are left alone.  dim <= 256.  The same
  *                        call serves training (q_starts = k_starts), a prompt's next part and a step of decoding (one query a sequence).
+ *                        A cache with free places after each sequence's keys: count every gap as a sequence of keys without a query
+ *                        (q_starts 0, 1, 1, 2; k_starts 0, length 0, capacity, capacity + length 1).  NaN and infinities outside a
+ *                        query's sequence never reach it.  Inside it a hidden key's weight is 0, as if written out: NaN or infinity
+ *                        in that key's row of v (gradients: of k, v, and of the query's q, dout) can still make 0 times it, NaN.
  * d8_attention_grad      the gradients of q (bit 0 of overwrite), k (bit 1) and v (bit 2) from those of o (dout), with o and lse as the
  *                        forward call left them.  The same bits every time.
  *     scratch: d8_attention_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.
  * d8_matmul_gated        h = act(g) * u with (g | u) = x w: w is [inner][2 * cols], its first `cols` columns the gate's.  act: D8_GATE_*.
  *                        pre (may be NULL): [rows][2 * cols], receives g and u for the gradients.
  * d8_matmul_gated_grad   dx (bit 0 of overwrite) and dw (bit 1) from dh, with pre as the forward call left it.
- *     scratch: d8_matmul_gated_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.                                */
+ *     scratch: d8_matmul_gated_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.  It counts on x and w at
+ *     multiples of 16 bytes; elsewhere the forward call asks for a copy of each, rows padded to 16 bytes (its error says how much). */
 #define D8_GATE_SILU    0 /* a sigmoid(a)                 */
 #define D8_GATE_GELU    1 /* a (1 + erf(a / sqrt 2)) / 2  */
 #define D8_GATE_RELU    2
