@@ -409,9 +409,23 @@ struct Plan {
     int tiles, pieces, units;
 };
 
+constexpr int keys_waves(int row_bytes) { return row_bytes > 512 ? 2 : 4; }
+
+// Workgroups of attention_keys_kernel that a compute unit holds at once: what its LDS has room for, four at most.  As many pieces as that are
+// wanted: twice as many cost a round of first loads and joins more (half, 16 sequences of 8192 keys, one query each, 32 + 8 heads of 128: 118
+// us with four pieces a compute unit where two fit, 112 with two; single, heads of 80 over 5 prompts of 500: 76 with four where one fits, 60
+// with one), half as many leave none to compute while another one loads (145 us in the first).
+int at_once(int dtype, int dim) {
+    const int padded = dim <= 96 ? (dim + 31) / 32 * 32 : dim <= 128 ? 128 : 256;
+    int bytes = 64;
+    while (bytes < padded * (int)dtype_bytes(dtype)) bytes *= 2;
+    const int n = 160 * 1024 / (keys_waves(bytes) * 2 * 32 * bytes);
+    return n > 4 ? 4 : n;
+}
+
 // Tensors that cannot be moved in 16-byte pieces: ANY.  128 rows a workgroup where that gives the chip two rounds of workgroups and
 // sequences are not shorter than half of it; else 32, and their keys in pieces while there are fewer workgroups than compute units need.
-Plan plan_of(bool vec, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads) {
+Plan plan_of(int dtype, int dim, bool vec, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads) {
     Plan p;
     const long rows = (long)q_tokens * (heads / kv_heads), cus = cu_count();
     const long some = sequences < q_tokens ? sequences : q_tokens;
@@ -421,7 +435,7 @@ Plan plan_of(bool vec, int sequences, int q_tokens, int k_tokens, int heads, int
     p.tiles = (int)((p.way == BY_KEYS ? small : big) + sequences);
     if (p.way == BY_KEYS) {
         const long groups = (small > some ? small : some) * kv_heads;
-        if (groups < 2 * cus && k_tokens > CHUNK_GRAIN) p.pieces = (int)((4 * cus + kv_heads - 1) / kv_heads);
+        if (groups < 2 * cus && k_tokens > CHUNK_GRAIN) p.pieces = (int)((at_once(dtype, dim) * cus + kv_heads - 1) / kv_heads);
         p.units = p.tiles + p.pieces;
     }
     return p;
@@ -429,7 +443,7 @@ Plan plan_of(bool vec, int sequences, int q_tokens, int k_tokens, int heads, int
 
 template <class T, int DP>
 int launch_dim(const Args &a, const Plan &p, hipStream_t stream) {
-    constexpr int WAVES = row_bytes<T, DP>() > 512 ? 2 : 4;
+    constexpr int WAVES = keys_waves(row_bytes<T, DP>());
     if (p.way == ANY) hipLaunchKernelGGL((attention_any_kernel<T, DP>), dim3((unsigned)p.tiles * a.kv_heads), dim3(256), 0, stream, a);
     else if (p.way == BY_ROWS) hipLaunchKernelGGL((attention_rows_kernel<T, DP>), dim3((unsigned)p.tiles * a.kv_heads), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((attention_keys_kernel<T, DP, WAVES>), dim3((unsigned)p.units * a.kv_heads), dim3(WAVES * 64), 0, stream, a);
@@ -492,7 +506,7 @@ extern "C" size_t d8_attention_scratch_bytes(int dtype, int which, int sequences
     (void)causal;
     if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || sequences < 0 || q_tokens < 0 || k_tokens < 0 || kv_heads < 1 || heads < kv_heads || dim < 1) return 0;
     if (which == 1) return attention::grad_scratch_bytes(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim);
-    const attention::Plan p = attention::plan_of(true, sequences, q_tokens, k_tokens, heads, kv_heads);
+    const attention::Plan p = attention::plan_of(dtype, dim, true, sequences, q_tokens, k_tokens, heads, kv_heads);
     return attention::part_bytes(p, kv_heads, dim);
 }
 
@@ -511,7 +525,7 @@ extern "C" int d8_attention(int dtype, const void *q, long ldq, const void *k, l
     a.vec = attention::in_pieces(dtype, dim, {q, k, v}, {ldq, ldk, ldv});
     // (a tile's rows are addressed by 32 bits)
     const bool fast = a.vec && attention::in_pieces(dtype, dim, {o}, {ldo}) && ldk < (1 << 23) && ldv < (1 << 23);
-    const attention::Plan p = attention::plan_of(fast, sequences, q_tokens, k_tokens, heads, kv_heads);
+    const attention::Plan p = attention::plan_of(dtype, dim, fast, sequences, q_tokens, k_tokens, heads, kv_heads);
     const size_t part = attention::part_rows(p, kv_heads), need = attention::part_bytes(p, kv_heads, dim);
     D8_REQUIRE(!need || (scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0), "attention: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
     D8_REQUIRE((long)(p.tiles + p.pieces) * kv_heads < (1L << 31), "attention: too many sequences");
