@@ -16,8 +16,9 @@ struct Args {
     // x and w as they lie: row strides, where the factor's columns begin, elements of a row (a half row of w) with the zeros behind it
     long ldx, ldw;
     int up, inner_there, cols_there;
-    int chunk, parts;  // few rows: K of a workgroup, and how many it is cut into
-    float *part;       // ... their sums [parts][rows][2 cols]
+    int chunk, parts;  // K of a workgroup, and how many it is cut into: few rows, or the tiles from number `whole` on
+    int whole;
+    float *part;       // ... their sums: few rows [parts][rows][2 cols], else [tile][part][gate, factor][rows of a tile][its columns]
     int vec;           // the way back: rows of pre, dh and dpre can be moved in 16-byte pieces
 };
 

@@ -80,7 +80,7 @@ __device__ __forceinline__ typename attention::Type<T>::frag weight_frag(const c
     }
 }
 
-// K in steps of 128 bytes of x, both tiles straight into one of two stages of LDS, the next step's while this one is worked on.  A workgroup's
+// K in steps of 128 bytes of x, both tiles straight into a stage of LDS, the next steps' while this one is worked on.  A workgroup's
 // tile by SHAPE: TALL 128 rows x 64 columns of both halves, a wave 64 x 32 of each; SQUARE 64 x 64, a wave 32 x 32 of each; SMALL 64 x 32, a wave
 // 32 x 32 of one half, and gate and factor meet through LDS at the end.
 enum Shape { TALL, SQUARE, SMALL };
@@ -93,13 +93,18 @@ __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
     typedef typename M::frag frag;
     constexpr int BM = tile_rows(SHAPE), BN = tile_cols(SHAPE), R = SHAPE == TALL ? 2 : 1, H = SHAPE == SMALL ? 1 : 2;  // row blocks, halves of a wave
     constexpr int PX = 128, BK = PX / (int)sizeof(T), PW = 2 * BN * (int)sizeof(T), TX = BM * PX, TW = BK * PW;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * (TX + TW)];
+    // (half, small tiles: a third stage, since two hold too little work to wait for loads behind, 300 x 2048 x 2 * 2816 29 -> 24 us.  Larger tiles
+    // would then share a compute unit with one less: 64 x 64 39 -> 48 us at 2000 x 2048 x 2 * 1408.  Single: no gain.)
+    constexpr int STAGES = SHAPE == SMALL && sizeof(T) == 2 ? 3 : 2, LOADS = (TX + TW) / 4096;
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * (TX + TW)];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     // (the workgroups of an XCD, ids congruent mod 8, have a run of row tiles by columns: what they share stays in its L2)
-    const int tiles_m = (a.rows + BM - 1) / BM, total = gridDim.x;
+    const int tiles_m = (a.rows + BM - 1) / BM, unit = (int)blockIdx.x - a.whole;  // (unit: of the tiles in parts)
     int id = blockIdx.x;
-    if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
+    if (unit >= 0) id = a.whole + unit / a.parts;
+    else if (a.whole % 8 == 0) id = id % 8 * (a.whole / 8) + id / 8;
     const int m0 = id % tiles_m * BM, n0 = id / tiles_m * BN;
+    const int begin = unit >= 0 ? unit % a.parts * a.chunk : 0, end = unit >= 0 ? min(a.inner, begin + a.chunk) : a.inner;
     const int wm = (wave >> 1) * 32 * R, wn = SHAPE == SMALL ? 0 : (wave & 1) * 32, half = SHAPE == SMALL ? wave & 1 : 0;
     attention::TileLoader<T, PX> lx;
     lx.init(a.ldx, a.inner, lane);
@@ -110,7 +115,7 @@ __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
         const unsigned to = lds0 + stage * (TX + TW);
         lx.pieces = (a.inner_there - k0) / M::V;
         const desc_t dx = lx.desc((const T *)a.x + (long)m0 * a.ldx + k0, min(BM, a.rows - m0), a.ldx, a.inner_there - k0);
-        const desc_t dw = lw.desc(a, k0, n0, min(BK, a.inner - k0));
+        const desc_t dw = lw.desc(a, k0, n0, min(BK, end - k0));
 #pragma unroll
         for (int i = 0; i < TX / 4096; ++i) lx.load(dx, wave * (TX / 4096) + i, to);
 #pragma unroll
@@ -121,12 +126,17 @@ __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
     for (int i = 0; i < R * H; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i / H][i % H][e] = 0.f;
-    fetch(0, 0);
-    for (int k0 = 0, stage = 0; k0 < a.inner; k0 += BK, stage ^= 1) {
-        ATTN_VMCNT(0);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+        if (begin + i * BK < end) fetch(begin + i * BK, i);
+    for (int k0 = begin, stage = 0; k0 < end; k0 += BK, stage = STAGES == 2 ? stage ^ 1 : stage == STAGES - 1 ? 0 : stage + 1) {
+        // this step's tiles have landed; those of the steps after it may be on their way
+        if (STAGES > 2 && k0 + (STAGES - 2) * BK < end) ATTN_VMCNT((STAGES - 2) * LOADS);
+        else ATTN_VMCNT(0);
         attention::lds_reads_done();
         __syncthreads();
-        if (k0 + BK < a.inner) fetch(k0 + BK, stage ^ 1);
+        const int ahead = k0 + (STAGES - 1) * BK;
+        if (ahead < end) fetch(ahead, STAGES == 2 ? stage ^ 1 : stage == 0 ? STAGES - 1 : stage - 1);
         const char *tx = lds + stage * (TX + TW), *tw = tx + TX;
 #pragma unroll
         for (int u = 0; u < BK / M::STEP; ++u) {
@@ -142,6 +152,16 @@ __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
         }
     }
     const int n = n0 + wn + (lane & 31);
+    if (unit >= 0) {
+        float *to = a.part + ((long)unit * 2 + half) * BM * BN + wn + (lane & 31);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) to[(j * BM + wm + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * BN] = acc[i][j][e];
+        return;
+    }
     if constexpr (SHAPE == SMALL) {
         __syncthreads();
         float *to = (float *)lds + (wave >> 1) * 1024 + lane;
@@ -166,6 +186,19 @@ __global__ __launch_bounds__(256, 2) void gated_tile_kernel(Args a) {
                 if (m < a.rows) store<T>(a, m, n, acc[i][0][e], acc[i][H - 1][e]);
             }
     }
+}
+
+// the tiles in parts: a part's sums added up in order
+template <class T, int SHAPE>
+__global__ __launch_bounds__(256) void gated_parts_kernel(Args a) {
+    constexpr int BM = tile_rows(SHAPE), BN = tile_cols(SHAPE), N = BM * BN;
+    const int tiles_m = (a.rows + BM - 1) / BM, tile = blockIdx.x / (N / 256), at = blockIdx.x % (N / 256) * 256 + threadIdx.x, id = a.whole + tile;
+    const int m = id % tiles_m * BM + at / BN, n = id / tiles_m * BN + at % BN;
+    if (m >= a.rows || n >= a.cols) return;
+    float g = 0.f, u = 0.f;
+    const float *from = a.part + (long)tile * a.parts * 2 * N + at;
+    for (int p = 0; p < a.parts; ++p, from += 2 * N) g += from[0], u += from[N];
+    store<T>(a, m, n, g, u);
 }
 
 // Few rows.  A workgroup has 128 bytes of columns of both halves and a chunk of K, of which its four waves take every fourth tile of 32 rows of w,
@@ -323,11 +356,14 @@ int check(int dtype, int rows, int inner, int cols, int act, const char *name) {
 }
 
 enum { FEW_ROWS = 64 };
+// What a 32 x 32 block of both products takes a compute unit per element of K (microseconds): alone on it, where a workgroup waits for its
+// loads and barriers, and beside others; and what a second launch takes.
+constexpr float ALONE[2] = {0.0029f, 0.0135f}, TOGETHER[2] = {0.00135f, 0.0095f}, JOIN_US = 4.f;  // half, single
 
 // How a forward call runs and what it takes of the scratch: copies of x and w (bytes, 0: read as they lie), partial sums.
 struct Plan {
     enum { ROWS, TILES } way;
-    int shape, parts, chunk;
+    int shape, parts, chunk, whole;
     size_t x_copy, w_copy, part;
     size_t bytes() const { return x_copy + w_copy + part; }
 };
@@ -352,14 +388,30 @@ Plan plan_of(int dtype, int rows, int inner, int cols, bool x_aligned, bool w_al
         return p;
     }
     p.way = Plan::TILES;
-    p.parts = 1, p.chunk = inner;
-    // the shape whose busiest compute unit has least to do: blocks of 32 x 32 products, weighed with what a block costs in it
+    // The shape whose busiest compute unit is through first: blocks of 32 x 32 products, weighed with what a block costs in it.  The tiles that
+    // are left when every compute unit has had as many as all others may be cut along K into parts, so that they too go over the whole chip,
+    // where that saves more than the second launch and the partial sums' way through memory cost.  Single, 777 x 1000 x 2 * 1351 (559 tiles of
+    // 64 x 32, 47 of them in five parts): 76 -> 68 us; half, 128 x 4096 x 2 * 2048 (all 64 tiles of 64 x 64 in four): 37 -> 19 us.
     static const float cost[2][3] = {{1.f, 1.25f, 1.6f}, {1.f, 1.05f, 1.1f}};  // half, single
+    const int single = dtype == D8_FLOAT32, bk = 128 / (int)es;
+    const long cus = cu_count();
     float best = 0.f;
     for (int s = TALL; s <= SMALL; ++s) {
-        const long tiles = (long)ceil_div(rows, tile_rows(s)) * ceil_div(cols, tile_cols(s));
-        const float t = (float)((tiles + cu_count() - 1) / cu_count()) * (tile_rows(s) / 32) * (tile_cols(s) / 32) * cost[dtype == D8_FLOAT32][s];
-        if (s == TALL || t < best) best = t, p.shape = s;
+        const long tiles = (long)ceil_div(rows, tile_rows(s)) * ceil_div(cols, tile_cols(s)), rest = tiles % cus;
+        const float tile = (float)inner * (tile_rows(s) / 32) * (tile_cols(s) / 32) * cost[single][s];
+        for (int want = 1; want <= (rest ? 16 : 1); ++want) {
+            const int chunk = (int)(((inner + want - 1L) / want + bk - 1) / bk * bk), parts = (inner + chunk - 1) / chunk;
+            if (want > 1 && (parts < want || chunk < 4 * bk)) continue;
+            const float share = parts == 1 ? 1.f : (float)chunk / inner;  // of a tile, what a part is
+            const float longest = tiles >= cus ? 1.f : share, load = (float)(tiles / cus) + (float)((rest * parts + cus - 1) / cus) * share;
+            const float join = parts == 1 ? 0.f : JOIN_US + (float)rest * (parts + 1) * tile_rows(s) * tile_cols(s) * 16.f / 4e6f;
+            const float t = tile * fmaxf(ALONE[single] * longest, TOGETHER[single] * load) + join;
+            if ((s == TALL && want == 1) || t < (p.parts == 1 ? 0.95f : 1.f) * best) best = t, p.shape = s, p.parts = parts, p.chunk = parts == 1 ? inner : chunk, p.whole = (int)(parts == 1 ? tiles : tiles - rest);
+        }
+    }
+    if (p.parts > 1) {
+        const long rest = (long)ceil_div(rows, tile_rows(p.shape)) * ceil_div(cols, tile_cols(p.shape)) - p.whole;
+        p.part = round256(sizeof(float) * 2 * (size_t)rest * p.parts * tile_rows(p.shape) * tile_cols(p.shape));
     }
     return p;
 }
@@ -391,8 +443,12 @@ int copy_rows(const void *from, void *to, long rows, int width, int padded, hipS
 template <class T, int SHAPE>
 int launch_tiles(const Args &a, hipStream_t stream) {
     const long tiles = (long)ceil_div(a.rows, tile_rows(SHAPE)) * ceil_div(a.cols, tile_cols(SHAPE));
-    D8_REQUIRE(tiles < (1L << 31), "matmul_gated: too many rows");
-    hipLaunchKernelGGL((gated_tile_kernel<T, SHAPE>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
+    D8_REQUIRE(tiles < (1L << 30), "matmul_gated: too many rows");
+    const long rest = tiles - a.whole;
+    hipLaunchKernelGGL((gated_tile_kernel<T, SHAPE>), dim3((unsigned)(a.whole + rest * a.parts)), dim3(256), 0, stream, a);
+    D8_LAUNCH_CHECK();
+    if (!rest) return 0;
+    hipLaunchKernelGGL((gated_parts_kernel<T, SHAPE>), dim3((unsigned)(rest * (tile_rows(SHAPE) * tile_cols(SHAPE) / 256))), dim3(256), 0, stream, a);
     D8_LAUNCH_CHECK();
     return 0;
 }
@@ -411,7 +467,7 @@ int forward(Args a, const Plan &p, char *scratch, hipStream_t stream) {
         if (int rc = copy_rows<T>(a.w, scratch, 2L * a.inner, a.cols, a.cols_there, stream)) return rc;
         a.w = scratch, scratch += p.w_copy;
     }
-    a.part = (float *)scratch, a.parts = p.parts, a.chunk = p.chunk;
+    a.part = (float *)scratch, a.parts = p.parts, a.chunk = p.chunk, a.whole = p.whole;
     if (p.way == Plan::ROWS) {
         const dim3 grid((unsigned)ceil_div((long)a.cols * sizeof(T), 128) * p.parts);
         if (a.rows <= 32) hipLaunchKernelGGL((gated_rows_kernel<T, 1>), grid, dim3(256), 0, stream, a);

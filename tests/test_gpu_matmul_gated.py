@@ -118,3 +118,17 @@ def test_refusals():
     assert call(rows=0) == call(inner=0) == call(cols=-1) == call(act=4) == call(act=-1) == call(x=None) == 10001
     assert lib.d8_matmul_gated_grad(capi.FLOAT32, d.ptr, d.ptr, 2, 8, d.ptr, d.ptr, 4, 0, d.ptr, d.ptr, 3, None, 0, None) == 10001
     assert b"scratch" in lib.d8_last_error()
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("size", [(65, 1030, 37), (130, 2056, 200), (777, 600, 1351)])
+def test_tiles_in_parts(size, dtype):
+    """few tiles, or a few left over, over a long inner axis: parts of the sums meet in a second launch"""
+    from deep8_amd import ops
+    x, w, _ = _inputs(*size, dtype)
+    want, pre = lo.gated(x, w, "silu")
+    got, got_pre = ops.matmul_gated(x, w, "silu")
+    _near(got_pre, pre, TOL[dtype])
+    _near(got, want, TOL[dtype])
+    again, _ = ops.matmul_gated(x, w, "silu")
+    assert np.array_equal(got, again)
