@@ -266,7 +266,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_keys_kernel(Args a) {
     Span sp = {0, 0, 0, 0};
     int seq = 0, item = 0;
     const bool there_is = locate(a, unit, sp, seq, item, [&](const Span &s) { return cut.tiles(a, s) * cut.chunks(s); });
-    const int chunks = there_is ? cut.chunks(sp) : 1, tile = item / chunks, begin = (item - tile * chunks) * cut.chunk;
+    // (the rows that see most keys first, so that the last to start have little to do: single, 5 prompts of 500, heads of 80, 60 -> 55 us)
+    const int chunks = there_is ? cut.chunks(sp) : 1, nth = item / chunks, tile = cut.tiles(a, sp) - 1 - nth, begin = (item - nth * chunks) * cut.chunk;
     const int group = a.group, rows = sp.nq * group, all = there_is ? cut.end(a, sp, tile) : 0, end = min(all, begin + cut.chunk);
     const bool whole = all <= cut.chunk;
     // for the second launch: how many chunks the tile that begins here has, and which rows
