@@ -317,7 +317,7 @@ struct Softmax {
 int check(const Args &a, int dtype, const char *name);
 inline void set_group(Args &a) { a.group = a.heads / a.kv_heads, a.group_rcp = 0xffffffffu / (unsigned)a.group; }
 bool in_pieces(int dtype, int dim, std::initializer_list<const void *> p, std::initializer_list<long> ld);
-size_t grad_scratch_bytes(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim);
+size_t grad_scratch_bytes(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim, bool causal);
 
 template <int DP, class T>
 constexpr int pitch_of() { return DP * (int)sizeof(T) + 16; }  // the 16 bytes keep a column's rows in different banks

@@ -506,7 +506,7 @@ using namespace d8;
 extern "C" size_t d8_attention_scratch_bytes(int dtype, int which, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim, int causal) {
     (void)causal;
     if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || sequences < 0 || q_tokens < 0 || k_tokens < 0 || kv_heads < 1 || heads < kv_heads || dim < 1) return 0;
-    if (which == 1) return attention::grad_scratch_bytes(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim);
+    if (which == 1) return attention::grad_scratch_bytes(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim, causal != 0);
     const attention::Plan p = attention::plan_of(dtype, dim, true, sequences, q_tokens, k_tokens, heads, kv_heads);
     return attention::part_bytes(p, kv_heads, dim);
 }

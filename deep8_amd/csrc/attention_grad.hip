@@ -336,7 +336,7 @@ struct ChunkLoader {
 
 // The rows that a workgroup for some keys walks, cut into chunks of one length for the whole call so that no workgroup has much more to do than
 // another (causal, the first keys of a long sequence are seen by all its rows, the last ones by few).  Found on the device from the
-// lengths: blocks of keys times rows, over the pieces wanted.  The sums of a block's chunks meet through scratch in a second launch,
+// lengths: blocks of keys times the rows that see them, over the pieces wanted.  The sums of a block's chunks meet through scratch in a second launch,
 // in the order of the chunks.
 template <class T, int DP, int SPLIT>
 struct RowCut {
@@ -348,14 +348,18 @@ struct RowCut {
     __device__ __forceinline__ void init(const Args &a) {
         chunk = 1 << 30;
         if (!a.pieces) return;
-        float work = 0.f;
+        float all = 0.f, seen = 0.f, own = 0.f;
         for (int s = threadIdx.x & 63; s < a.sequences; s += 64) {
             const Span sp = span_of(a, s);
-            work += (float)blocks(sp) * (float)Rows::rows(a, sp.nq);
+            const float n = (float)min(sp.nq, sp.nk), pairs = 0.5f * n * n + (float)max(0, sp.nk - sp.nq) * (float)sp.nq;
+            own += (float)blocks(sp), all += (float)blocks(sp) * (float)Rows::rows(a, sp.nq), seen += pairs * (float)a.group / S::OWN;
         }
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) work += __shfl_xor(work, d);
-        const float grains = ceilf(work * 1.0001f / (float)a.pieces / (float)ROW_GRAIN);  // (rather too long: never more chunks than room)
+        for (int d = 1; d < 64; d <<= 1) own += __shfl_xor(own, d), all += __shfl_xor(all, d), seen += __shfl_xor(seen, d);
+        // What is seen in a causal call, counted as half of all at least; half a chunk a block is lost to rounding.  Rather too long: there are
+        // never more chunks than room, which is for twice as many as are wanted in a causal call.
+        const float work = a.causal ? fmaxf(seen, 0.5f * all) : all, wanted = fmaxf((float)a.pieces - 0.5f * own, 0.5f * (float)a.pieces);
+        const float grains = ceilf(work * 1.0001f / wanted / (float)ROW_GRAIN);
         chunk = __builtin_amdgcn_readfirstlane(max(1, (int)fminf(grains, (float)((1 << 29) / ROW_GRAIN))) * ROW_GRAIN);
     }
 };
@@ -370,14 +374,20 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
     __shared__ __attribute__((aligned(16))) float row_lse[2][S::KB], row_delta[2][S::KB];
     __shared__ __attribute__((aligned(16))) frag spare[S::SPARE ? S::SPARE : 1][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    const int hk = blockIdx.x % a.kv_heads;
+    int unit = blockIdx.x / a.kv_heads;
     typedef ChunkLoader<T, PB> Rows;
     RowCut<T, DP, SPLIT> cut;
     cut.init(a);
     Span sp = {0, 0, 0, 0};
     int seq = 0, item = 0;
     const bool there_is = locate(a, unit, sp, seq, item, [&](const Span &s) { return cut.blocks(s) * cut.chunks(a, s); });
-    const int chunks = there_is ? cut.chunks(a, sp) : 1, block = item / chunks, part = item - block * chunks;
+    const int chunks = there_is ? cut.chunks(a, sp) : 1, block = item / chunks, nth = item - block * chunks;
+    // (each block begins with another chunk: workgroups go round the XCDs, and with a multiple of 8 chunks one XCD would have all the last ones, to
+    // which a causal call gives most work: half, one sequence of 8192, 8 + 1 heads of 128, the whole gradient 925 -> 871 us; 725 with RowCut's count
+    // of what is seen)
+    const int turn = nth + block % chunks, part = turn < chunks ? turn : turn - chunks;
+    unit += part - nth;
     const int group = a.group, rows = Rows::rows(a, sp.nq), back = sp.nk - sp.nq;
     // the first row that sees a key of the block (its query is the block's first key less nk - nq), and the chunk that it is in
     const int begin = a.causal ? (int)min((long)(max(0, block * S::OWN - back) / Rows::CT * Rows::CT) * group / S::KB * S::KB, (long)rows) : 0;
@@ -727,7 +737,7 @@ struct GradPlan {
     int split, pieces, units;
     size_t lists, parts;  // bytes
 };
-static GradPlan grad_plan(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim) {
+static GradPlan grad_plan(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim, bool causal) {
     GradPlan p;
     const int padded = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;
     p.split = dtype == D8_FLOAT32 && padded == 256 ? 1 : split_for(k_tokens, kv_heads);
@@ -736,7 +746,7 @@ static GradPlan grad_plan(int dtype, int sequences, int q_tokens, int k_tokens, 
     const long want = (4L * cu_count() + kv_heads - 1) / kv_heads, most = (blocks * rows + ROW_GRAIN - 1) / ROW_GRAIN;
     p.pieces = (int)(blocks >= 2 * want ? 0 : want < most ? want : most);
     if (rows <= ROW_GRAIN) p.pieces = 0;
-    p.units = (int)(blocks + p.pieces);
+    p.units = (int)(blocks + (causal ? 2 : 1) * p.pieces);
     p.lists = p.pieces ? ((size_t)p.units * sizeof(int4) + 255) & ~(size_t)255 : 0;
     p.parts = p.pieces ? (size_t)p.units * kv_heads * own * 2 * padded * sizeof(float) : 0;
     return p;
@@ -744,8 +754,8 @@ static GradPlan grad_plan(int dtype, int sequences, int q_tokens, int k_tokens, 
 
 static size_t row_bytes_of(int q_tokens, int heads) { return (sizeof(float) * (2 * NORM_GROUPS + (size_t)q_tokens * heads) + 255) & ~(size_t)255; }
 
-size_t grad_scratch_bytes(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim) {
-    const GradPlan p = grad_plan(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim);
+size_t grad_scratch_bytes(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim, bool causal) {
+    const GradPlan p = grad_plan(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim, causal != 0);
     return row_bytes_of(q_tokens, heads) + p.lists + p.parts;
 }
 
@@ -769,8 +779,8 @@ extern "C" int d8_attention_grad(int dtype, const void *q, long ldq, const void 
     D8_REQUIRE(lddo >= qrow && lddq >= qrow && lddk >= krow && lddv >= krow, "attention_grad: rows of %ld and %ld elements do not fit their leading dimensions", qrow, krow);
     if (!sequences || (!q_tokens && !k_tokens)) return 0;
     D8_REQUIRE(q_starts && k_starts && (!q_tokens || (q && o && lse && dout && dq)) && (!k_tokens || (k && v && dk && dv)), "attention_grad: null tensor");
-    const attention::GradPlan plan = attention::grad_plan(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim);
-    const size_t need = attention::grad_scratch_bytes(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim);
+    const attention::GradPlan plan = attention::grad_plan(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim, causal != 0);
+    const size_t need = attention::grad_scratch_bytes(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim, causal != 0);
     D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_grad: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
     a.norms = (float *)scratch, a.delta = a.norms + 2 * attention::NORM_GROUPS;
     a.joins = (int4 *)((char *)scratch + attention::row_bytes_of(q_tokens, heads)), a.part = (float *)((char *)a.joins + plan.lists);
@@ -780,6 +790,6 @@ extern "C" int d8_attention_grad(int dtype, const void *q, long ldq, const void 
     // (a tile's rows are addressed by 31 bits)
     const long most = 1 << 21;
     const bool fast = a.vec && attention::in_pieces(dtype, dim, {dq, dk, dv}, {lddq, lddk, lddv}) && ldq < most && ldk < most && ldv < most && lddo < most;
-    D8_REQUIRE((((long)q_tokens * a.group + k_tokens) / 64 + 2 * (long)sequences + plan.pieces + 2) * kv_heads < (1L << 31), "attention_grad: too many sequences");
+    D8_REQUIRE((((long)q_tokens * a.group + k_tokens) / 64 + 2 * (long)sequences + 2 * plan.pieces + 2) * kv_heads < (1L << 31), "attention_grad: too many sequences");
     return dtype == D8_FLOAT16 ? attention::launch<f16>(a, fast, as_stream(stream)) : attention::launch<float>(a, fast, as_stream(stream));
 }
