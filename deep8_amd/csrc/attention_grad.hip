@@ -31,7 +31,8 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 
 // delta[head][token] = sum of do o; a group of lanes has a row, 16 bytes a lane.  In half also the largest squared norms of the rows
-// of do and of v.
+// of do and of v.  Bound by bytes: 56 MB (6144 tokens, 16 + 4 heads of 128 halves) in 19 us; four rows' loads at once took 2 us off that
+// and added as much to small calls.
 template <class T>
 __global__ __launch_bounds__(256) void attention_delta_kernel(Args a, int lanes) {
     typedef typename Type<T>::frag frag;
@@ -287,7 +288,9 @@ __device__ __forceinline__ void store_sums(T *to, const f32x16 (&x)[DP / 32], fl
 // The same two for tensors whose rows can be moved in 16-byte pieces: tiles straight into one of two stages of LDS, the next while this one is
 // worked on.  A wave has 32 keys (rows) of its own, whose fragments and sums stay in registers.  SPLIT = 1: four waves, 128 keys
 // (rows) a workgroup, each walks every tile; SPLIT = 2, where that would leave compute units idle: 64, two waves have the same
-// 32 and take every other tile, and their sums are joined through LDS at the end.
+// 32 and take every other tile, and their sums are joined through LDS at the end.  Half, causal, sequences of 2010, 1461 and 2673, 16 + 4 heads of
+// 128: dk and dv 220 us + 20 for the join (four products, 490 TFLOP/s: two waves of a SIMD with every register taken wait for LDS and
+// barriers), dq 115 us (three, 710 TFLOP/s).  Single, 2048 tokens in four sequences, 8 heads of 64: 83 and 63 us (52 TFLOP/s).
 template <class T, int DP, int SPLIT>
 struct Shape {
     static constexpr int PB = row_bytes<T, DP>(), OWN = 128 / SPLIT, BLOCKS = PB <= 256 || SPLIT == 2 ? 2 : 1;
@@ -295,8 +298,9 @@ struct Shape {
     static constexpr int OCCUPANCY = DP * (int)sizeof(T) <= 256 ? 2 : 1;     // waves of a SIMD, dq
     static constexpr int OCCUPANCY_KV = DP * (int)sizeof(T) <= 256 ? 2 : 1;  // ... dk and dv, whose sums and operands alone are 192 registers at 128 halves
     // dk and dv at 128 halves, two waves of a SIMD: the registers are a few fragments short, and the compiler's own way out would be scratch memory,
-    // whose answers wait behind the tiles on their way (waits are in order); so some fragments of the values stay in LDS
-    static constexpr int SPARE = DP == 128 && sizeof(T) == 2 ? 3 : 0;
+    // whose answers wait behind the tiles on their way (waits are in order); so some fragments of the values stay in LDS, where
+    // the two waves of SPLIT = 2 share them (one more there than would fit twice: 388 -> 379 us for the whole gradient above)
+    static constexpr int SPARE = DP == 128 && sizeof(T) == 2 ? (SPLIT == 2 ? 4 : 3) : 0;
     static_assert(LOADS >= 1 && 4 * TILE_BYTES <= 160 * 1024, "a tile is at least a load of every wave, and two stages fit");
 };
 
@@ -372,7 +376,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
     constexpr int PB = S::PB, UNITS = DP / M::STEP, N = DP / 32;
     __shared__ __attribute__((aligned(1024))) char lds[4 * S::TILE_BYTES];
     __shared__ __attribute__((aligned(16))) float row_lse[2][S::KB], row_delta[2][S::KB];
-    __shared__ __attribute__((aligned(16))) frag spare[S::SPARE ? S::SPARE : 1][256];
+    __shared__ __attribute__((aligned(16))) frag spare[S::SPARE ? S::SPARE : 1][256 / SPLIT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int hk = blockIdx.x % a.kv_heads;
     int unit = blockIdx.x / a.kv_heads;
@@ -408,7 +412,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
         kf[u] = load_piece<T>((const T *)a.k + key * a.ldk + (long)hk * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
         const frag v = load_piece<T>((const T *)a.v + key * a.ldv + (long)hk * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
         if (u < UNITS - S::SPARE) vf[u] = v;
-        else spare[u - (UNITS - S::SPARE)][tid] = v;
+        else spare[u - (UNITS - S::SPARE)][tid % (256 / SPLIT)] = v;
     }
     f32x16 dk[N], dv[N];
 #pragma unroll
@@ -460,7 +464,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) {
                 M::mma(s, rows_frag<T, PB>(tq, b * 32, u, l), kf[u]);
-                M::mma(w, rows_frag<T, PB>(tg, b * 32, u, l), u < UNITS - S::SPARE ? vf[u] : spare[u - (UNITS - S::SPARE)][wave * 64 + l]);
+                M::mma(w, rows_frag<T, PB>(tg, b * 32, u, l), u < UNITS - S::SPARE ? vf[u] : spare[u - (UNITS - S::SPARE)][wave % (4 / SPLIT) * 64 + l]);
             }
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
@@ -642,7 +646,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
     store_sums<T, DP>((T *)a.dq + (long)(sp.q0 + t) * a.lddq + (long)head * a.dim, dq, a.scale * exp2f(-shift) / mult, a.dim, h, a.overwrite & 1);
 }
 
-// the chunks of a block of keys joined; a wave has dk or dv of 32 keys
+// the chunks of a block of keys joined; a wave has dk or dv of 32 keys.  Bound by the partial sums' bytes.
 template <class T, int DP, int SPLIT>
 __global__ __launch_bounds__(256) void attention_grad_join_kernel(Args a) {
     typedef Shape<T, DP, SPLIT> S;

@@ -10,6 +10,9 @@
 // heads of one token and keeps the token's cosines and sines, which would otherwise be read from L2 once a head, as many bytes
 // as the heads themselves.  Heads that cannot be moved in 16-byte pieces go through LDS, one wave each.
 //
+// Half, 8192 tokens of 32 + 8 heads of 128: 38 us, 172 MB at 4.5 TB/s (a large copy 5.1).  Back, single, 4099 tokens of 12 + 4 heads of 96: 17 us,
+// 77 MB at 4.5 TB/s, and 4 for the weights' sums.  8 tokens: 4 us, a launch.
+//
 // All sums are fp32.  The sums behind dw go over workgroups through scratch and are added in a fixed order.
 #include "common.h"
 
