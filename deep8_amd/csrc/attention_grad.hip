@@ -422,6 +422,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
     const unsigned lds0 = lds_address(lds);
     const T *q = (const T *)a.q + (long)sp.q0 * a.ldq + (long)hk * group * a.dim, *g = (const T *)a.dout + (long)sp.q0 * a.lddo + (long)hk * group * a.dim;
     float next_lse = 0.f, next_delta = 0.f;  // of row tid of the next tile
+    bool next_in = false;
     auto fetch = [&](int r0, int stage) {
         int fl = lane;
         asm volatile("" : "+v"(fl));  // (what follows from the lane is formed anew each time: registers are what this kernel is short of)
@@ -430,21 +431,22 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
         const int tid = wave * 64 + fl;
         Rows::template load<S::LOADS, S::KB>(a, lq, q, a.ldq, sp.nq, r0, wave * S::LOADS, lds0 + stage * 2 * S::TILE_BYTES);
         Rows::template load<S::LOADS, S::KB>(a, lg, g, a.lddo, sp.nq, r0, wave * S::LOADS, lds0 + stage * 2 * S::TILE_BYTES + S::TILE_BYTES);
-        if (tid < S::KB) {
-            int head;
-            const int t = Rows::token(a, r0 + tid, head);
-            const bool in = t < sp.nq;
-            const long at = (long)(hk * group + head) * a.q_tokens + sp.q0 + (in ? t : 0);
-            next_lse = in ? a.lse[at] * LOG2E - shift : INFINITY;  // (rows that are not there: probability zero)
-            next_delta = in ? a.delta[at] * mult : 0.f;
-        }
+        // (every lane asks, and nothing is done with the answers here: that would wait for them, and for the tiles asked for before them)
+        int head;
+        const int t = Rows::token(a, r0 + min(tid, S::KB - 1), head);
+        next_in = t < sp.nq;
+        const long at = (long)(hk * group + head) * a.q_tokens + sp.q0 + (next_in ? t : 0);
+        next_lse = a.lse[at], next_delta = a.delta[at];
     };
     if (r_begin < r_end) fetch(r_begin, 0);
     for (int r0 = r_begin, stage = 0; r0 < r_end; r0 += S::KB, stage ^= 1) {
         if (wave * 64 < S::KB) {
             int wl = lane;
             asm volatile("" : "+v"(wl));
-            if (wave * 64 + wl < S::KB) row_lse[stage][wave * 64 + wl] = next_lse, row_delta[stage][wave * 64 + wl] = next_delta;
+            if (wave * 64 + wl < S::KB) {  // (rows that are not there: probability zero)
+                row_lse[stage][wave * 64 + wl] = next_in ? next_lse * LOG2E - shift : INFINITY;
+                row_delta[stage][wave * 64 + wl] = next_in ? next_delta * mult : 0.f;
+            }
         }
         ATTN_VMCNT(0);
         lds_reads_done();
