@@ -289,7 +289,7 @@ __device__ __forceinline__ void store_sums(T *to, const f32x16 (&x)[DP / 32], fl
 // worked on.  A wave has 32 keys (rows) of its own, whose fragments and sums stay in registers.  SPLIT = 1: four waves, 128 keys
 // (rows) a workgroup, each walks every tile; SPLIT = 2, where that would leave compute units idle: 64, two waves have the same
 // 32 and take every other tile, and their sums are joined through LDS at the end.  Half, causal, sequences of 2010, 1461 and 2673, 16 + 4 heads of
-// 128: dk and dv 220 us + 20 for the join (four products, 490 TFLOP/s: two waves of a SIMD with every register taken wait for LDS and
+// 128: dk and dv 195 us + 20 for the join (four products, 560 TFLOP/s: two waves of a SIMD with every register taken wait for LDS and
 // barriers), dq 115 us (three, 710 TFLOP/s).  Single, 2048 tokens in four sequences, 8 heads of 64: 83 and 63 us (52 TFLOP/s).
 template <class T, int DP, int SPLIT>
 struct Shape {
@@ -609,7 +609,8 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
             }
             if (end <= 32) {
                 // rows of few keys: delta from the probabilities themselves; do o has the rounding of o in it, which there weighs as much as
-                // the rounding of ds
+                // the rounding of ds (up to 64 keys, by a pass before: 3.1 instead of 3.5 10^-4 of dq at 5 sequences of 26 in half, but then
+                // the loop's fragments no longer stay in registers, and the gradient of long sequences takes 640 us for 370)
                 float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sum += s[e] * w[e];
