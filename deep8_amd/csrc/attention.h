@@ -49,17 +49,29 @@ struct Args {
     float *norms;   // gradient, half: largest squared norms of rows of do and of v, by workgroup of the first pass
 };
 
-// One sequence as its tensors have it.  Starts that run backwards or leave the tensors are cut to what is there.
+// One sequence as its tensors have it.
 struct Span {
     int q0, nq, k0, nk;
 };
-__device__ __forceinline__ Span span_of(const Args &a, int s) {
-    Span r;
-    r.q0 = min(max(a.q_starts[s], 0), a.q_tokens);
-    r.nq = max(min(a.q_starts[s + 1], a.q_tokens) - r.q0, 0);
-    r.k0 = min(max(a.k_starts[s], 0), a.k_tokens);
-    r.nk = max(min(a.k_starts[s + 1], a.k_tokens) - r.k0, 0);
-    return r;
+// The lane's sequence of the 64 from `first` on, an empty one beyond the last; q_top, k_top: the largest starts before them, and then up to
+// their end.  Starts count as the tensors' ends where they leave the tensors, and as an earlier start where they lie before it: sequences never
+// overlap, so what is counted here in tiles, blocks and chunks stays within what launches and scratch were sized by from the numbers of tokens,
+// whatever the starts are.  All lanes of a wave take part.
+__device__ __forceinline__ Span spans_from(const Args &a, int first, int &q_top, int &k_top) {
+    const int lane = threadIdx.x & 63, at = min(first + lane, a.sequences), next = min(first + lane + 1, a.sequences);
+    int q0 = min(max(a.q_starts[at], 0), a.q_tokens), q1 = min(max(a.q_starts[next], 0), a.q_tokens);
+    int k0 = min(max(a.k_starts[at], 0), a.k_tokens), k1 = min(max(a.k_starts[next], 0), a.k_tokens);
+    if (__ballot(q0 < q_top || q1 < q0 || k0 < k_top || k1 < k0)) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int q = __shfl_up(q0, d), k = __shfl_up(k0, d);
+            q0 = lane >= d ? max(q0, q) : q0, k0 = lane >= d ? max(k0, k) : k0;
+        }
+        q0 = max(q0, q_top), k0 = max(k0, k_top);
+        q1 = max(q1, q0), k1 = max(k1, k0);
+    }
+    q_top = __builtin_amdgcn_readlane(q1, 63), k_top = __builtin_amdgcn_readlane(k1, 63);
+    return Span{q0, q1 - q0, k0, k1 - k0};
 }
 
 // Row r's query, r < 2^31: r times the reciprocal over 2^32 is the quotient or one less.
@@ -68,15 +80,15 @@ __device__ __forceinline__ int query_of(const Args &a, int r) {
     return t + (r - t * a.group >= a.group ? 1 : 0);
 }
 
-// Which sequence holds item `id` of a list in which sequence s has count(span) items: sets s, the item's number in it and the span; false
+// Which sequence holds item `id` of a list in which sequence s has count(span) items (none if it is empty): sets s, the item's number in it and the span; false
 // beyond the list.  All lanes of a wave take part, 64 sequences at a time.
 template <class Count>
 __device__ __forceinline__ bool locate(const Args &a, int id, Span &span, int &s, int &item, Count &&count) {
     const int lane = threadIdx.x & 63;
-    int before = 0;
+    int before = 0, q_top = 0, k_top = 0;
     for (int first = 0; first < a.sequences; first += 64) {
-        int n = 0;
-        if (first + lane < a.sequences) n = count(span_of(a, first + lane));
+        const Span own = spans_from(a, first, q_top, k_top);
+        const int n = count(own);
         int upto = n;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -90,9 +102,9 @@ __device__ __forceinline__ bool locate(const Args &a, int id, Span &span, int &s
             item = id - before - (__shfl(upto, l) - __shfl(n, l));
             s = __builtin_amdgcn_readfirstlane(s);
             item = __builtin_amdgcn_readfirstlane(item);
-            span = span_of(a, s);
-            span.q0 = __builtin_amdgcn_readfirstlane(span.q0), span.nq = __builtin_amdgcn_readfirstlane(span.nq);
-            span.k0 = __builtin_amdgcn_readfirstlane(span.k0), span.nk = __builtin_amdgcn_readfirstlane(span.nk);
+            const int from = __builtin_amdgcn_readfirstlane(l);
+            span.q0 = __builtin_amdgcn_readlane(own.q0, from), span.nq = __builtin_amdgcn_readlane(own.nq, from);
+            span.k0 = __builtin_amdgcn_readlane(own.k0, from), span.nk = __builtin_amdgcn_readlane(own.nk, from);
             return true;
         }
         before += __shfl(upto, 63);

@@ -237,8 +237,8 @@ struct Cut {
         chunk = 1 << 30;
         if (!a.pieces) return;
         float work = 0.f;
-        for (int s = threadIdx.x & 63; s < a.sequences; s += 64) {
-            const Span sp = span_of(a, s);
+        for (int first = 0, q_top = 0, k_top = 0; first < a.sequences; first += 64) {
+            const Span sp = spans_from(a, first, q_top, k_top);
             work += (float)tiles(a, sp) * (float)sp.nk;
         }
 #pragma unroll
@@ -485,7 +485,7 @@ int check(const Args &a, int dtype, const char *name) {
     D8_REQUIRE(a.dim >= 1 && a.dim <= MOST_DIM, "%s: a head has 1 to %d elements, not %d", name, (int)MOST_DIM, a.dim);
     const long qrow = (long)a.heads * a.dim, krow = (long)a.kv_heads * a.dim;
     D8_REQUIRE(a.ldq >= qrow && a.ldo >= qrow && a.ldk >= krow && a.ldv >= krow, "%s: rows of %ld and %ld elements do not fit their leading dimensions", name, qrow, krow);
-    D8_REQUIRE((long)a.q_tokens * a.heads < (1L << 30) && a.k_tokens < (1 << 30), "%s: too many queries or keys", name);
+    D8_REQUIRE((long)a.q_tokens * a.heads < (1L << 30) && a.k_tokens < (1 << 30) && a.sequences < (1 << 30), "%s: too many queries, keys or sequences", name);
     D8_REQUIRE(a.scale == a.scale, "%s: the scale is no number", name);
     return 0;
 }

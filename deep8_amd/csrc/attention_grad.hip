@@ -353,8 +353,8 @@ struct RowCut {
         chunk = 1 << 30;
         if (!a.pieces) return;
         float all = 0.f, seen = 0.f, own = 0.f;
-        for (int s = threadIdx.x & 63; s < a.sequences; s += 64) {
-            const Span sp = span_of(a, s);
+        for (int first = 0, q_top = 0, k_top = 0; first < a.sequences; first += 64) {
+            const Span sp = spans_from(a, first, q_top, k_top);
             const float n = (float)min(sp.nq, sp.nk), pairs = 0.5f * n * n + (float)max(0, sp.nk - sp.nq) * (float)sp.nq;
             own += (float)blocks(sp), all += (float)blocks(sp) * (float)Rows::rows(a, sp.nq), seen += pairs * (float)a.group / S::OWN;
         }

@@ -460,7 +460,8 @@ int d8_avgpool2d_grad_overwrite(int dtype, void *dx, const void *dy, int B, int 
  * d8_head_norm_rotary_grad  from q, k and the gradients of the outputs (dq_out, dk_out) those of q, k (bit 0 of overwrite) and of
  *                        the weights (bit 1; NULL: not wanted).  dq may be dq_out, dk may be dk_out.
  * d8_attention           sequence s has queries q_starts[s] .. q_starts[s + 1] - 1 and keys k_starts[s] .. k_starts[s + 1] - 1 (rows of
- *                        q and k; arrays of sequences + 1 on the device; what reaches beyond the tensors is cut).  A query sees its
+ *                        q and k; arrays of sequences + 1 on the device; what reaches beyond the tensors is cut, and a start that lies before
+ *                        an earlier one counts as that one, so sequences never overlap).  A query sees its
  *                        sequence's keys, causal != 0: query t of nq sees the keys up to t + nk - nq, so the last query sees them
  *                        all.  o = softmax(scale q k^T) v, head i with the keys and values of head i / (heads / kv_heads).
  *                        lse[heads][q_tokens] (may be NULL): the logarithm of the sum of exp(score).  A query that sees nothing
