@@ -46,7 +46,8 @@ struct Args {
     float *part_ml;
     int4 *joins;    // ... what the second launch joins, by piece: chunks, first query, row tile, rows of the sequence
     float *delta;   // gradient: rowsum(do o) [heads][q_tokens]
-    float *norms;   // gradient, half: largest squared norms of rows of do and of v, by workgroup of the first pass
+    float *norms;   // gradient, half: norms of the rows of do [heads][q_tokens] and of v [kv_heads][k_tokens], 0 for one that is not finite
+    float *v_norms;
 };
 
 // One sequence as its tensors have it.

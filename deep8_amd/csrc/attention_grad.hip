@@ -8,8 +8,11 @@
 // place: no atomics, the same bits every time.
 //
 // In half, p and ds are rounded to half for the products that follow.  p is scaled by 2^15 (it is at most 1) and ds by a power of two
-// that a bound on it allows, |dp - delta| <= 2 max |do_i| max |v_j| over all rows, so that small probabilities of long rows keep
-// their bits: a probability of 10^-5 would otherwise be a subnormal half.  The scales are taken out again in fp32.
+// that a bound on it allows, so that small probabilities of long rows keep their bits: a probability of 10^-5 would otherwise be a
+// subnormal half.  The bound is one of what meets in a sum: for dq |dp - delta| <= 2 |do_i| max |v_j| of the row's own and the keys that its
+// tile sees, for dk max |do_i| max |v_j| + max |delta_i| of a workgroup's rows and keys.  Rows elsewhere do not matter, and rows that are
+// no number leave the bound alone: their own results are no number, the others keep their bits.  The scales are taken out again in
+// fp32, before sums of several workgroups meet.
 #include "attention.h"
 
 namespace d8 {
@@ -18,7 +21,7 @@ namespace {
 
 enum { TILE = 32 };
 enum { ROW_GRAIN = 512 };    // rows of a chunk are a multiple of this
-enum { NORM_GROUPS = 512 };  // workgroups of the first launch: entries of each list of norms
+enum { DELTA_GROUPS = 512 }; // workgroups of the first launch
 constexpr float P_SHIFT = 15.f;
 
 template <class T>
@@ -30,17 +33,18 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-// delta[head][token] = sum of do o; a group of lanes has a row, 16 bytes a lane.  In half also the largest squared norms of the rows
-// of do and of v.  Bound by bytes: 56 MB (6144 tokens, 16 + 4 heads of 128 halves) in 19 us; four rows' loads at once took 2 us off that
+// 0 where it is not finite
+__device__ __forceinline__ float finite(float v) { return fabsf(v) <= 3.4e38f ? v : 0.f; }
+
+// delta = sum of do o of each row; a group of lanes has a row, 16 bytes a lane.  In half also the norms of the rows of do and of v.
+// Bound by bytes: 56 MB (6144 tokens, 16 + 4 heads of 128 halves) in 19 us; four rows' loads at once took 2 us off that
 // and added as much to small calls.
 template <class T>
 __global__ __launch_bounds__(256) void attention_delta_kernel(Args a, int lanes) {
     typedef typename Type<T>::frag frag;
     constexpr int V = Type<T>::V;
-    __shared__ float most[2][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = threadIdx.x & (lanes - 1);
+    const int l = threadIdx.x & (lanes - 1);
     const long step = (long)gridDim.x * 256 / lanes, mine = ((long)blockIdx.x * 256 + threadIdx.x) / lanes;
-    float top_do = 0.f, top_v = 0.f;
     const long rows = (long)a.q_tokens * a.heads;
     for (long r = mine; r < rows; r += step) {
         const long t = r / a.heads;
@@ -54,39 +58,75 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(Args a, int lanes)
             dot += __shfl_xor(dot, d);
             if (scaled<T>()) sq += __shfl_xor(sq, d);
         }
-        if (l == 0) a.delta[(long)head * a.q_tokens + t] = dot;
-        top_do = fmaxf(top_do, sq);
+        if (l == 0) {
+            a.delta[(long)head * a.q_tokens + t] = dot;
+            if (scaled<T>()) a.norms[(long)head * a.q_tokens + t] = finite(sqrtf(sq));
+        }
     }
     if (!scaled<T>()) return;
     const long krows = (long)a.k_tokens * a.kv_heads;
     for (long r = mine; r < krows; r += step) {
         const long t = r / a.kv_heads;
-        const frag v = load_piece<T>((const T *)a.v + t * a.ldv + (r - t * a.kv_heads) * a.dim, l * V, a.dim, true, a.vec);
+        const int head = (int)(r - t * a.kv_heads);
+        const frag v = load_piece<T>((const T *)a.v + t * a.ldv + (long)head * a.dim, l * V, a.dim, true, a.vec);
         float sq = 0.f;
 #pragma unroll
         for (int e = 0; e < V; ++e) sq += (float)v[e] * (float)v[e];
         for (int d = 1; d < lanes; d <<= 1) sq += __shfl_xor(sq, d);
-        top_v = fmaxf(top_v, sq);
-    }
-    top_do = wave_max(top_do), top_v = wave_max(top_v);
-    if (lane == 0) most[0][wave] = top_do, most[1][wave] = top_v;
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        const float *m = most[threadIdx.x];
-        a.norms[threadIdx.x * NORM_GROUPS + blockIdx.x] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        if (l == 0) a.v_norms[(long)head * a.k_tokens + t] = finite(sqrtf(sq));
     }
 }
 
-// 2^-e with |dp - delta| < 2^e for every row and key of the call (1 where there is no such bound); every wave computes it
+// 2^-e with bound < 2^e (1 where there is nothing to bound); half: p 2^15 of at most 1 times what is bounded stays below 2^15
+__device__ __forceinline__ float scale_for(float bound) { return bound > 0.f ? exp2f(-(float)(ilogbf(bound) + 1)) : 1.f; }
+
+// the largest of each wave's values, for all of the workgroup (through LDS; every thread takes part)
+template <int N>
+__device__ __forceinline__ void group_max(float (&v)[N]) {
+    __shared__ float most[N][4];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = wave_max(v[i]);
+        if ((threadIdx.x & 63) == 0) most[i][threadIdx.x >> 6] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = fmaxf(fmaxf(most[i][0], most[i][1]), fmaxf(most[i][2], most[i][3]));
+}
+
+// half: the largest norm of the rows of v of keys 0 .. n - 1 of a sequence
 template <class T>
-__device__ __forceinline__ float ds_scale(const Args &a) {
+__device__ __forceinline__ float largest_v(const Args &a, const Span &sp, int hk, int n) {
+    if (!scaled<T>()) return 0.f;
+    const float *from = a.v_norms + (long)hk * a.k_tokens + sp.k0;
+    float v[1] = {0.f};
+#pragma unroll 4
+    for (int j = threadIdx.x; j < n; j += 256) v[0] = fmaxf(v[0], from[j]);
+    group_max(v);
+    return v[0];
+}
+
+// What a row's ds is scaled by in the sums of dq.
+template <class T>
+__device__ __forceinline__ float row_scale(float norm, float v) { return scaled<T>() ? scale_for(2.f * norm * v) : 1.f; }
+
+// ... in the sums of dk of keys j0 .. j0 + n - 1 over all heads' rows of queries t0 .. t1 - 1 of a sequence
+template <class T>
+__device__ __forceinline__ float keys_scale(const Args &a, const Span &sp, int hk, int j0, int n, int t0, int t1) {
     if (!scaled<T>()) return 1.f;
-    const int lane = threadIdx.x & 63;
-    float d = 0.f, v = 0.f;
-    for (int i = lane; i < NORM_GROUPS; i += 64) d = fmaxf(d, a.norms[i]), v = fmaxf(v, a.norms[NORM_GROUPS + i]);
-    const float bound = 2.f * sqrtf(wave_max(d)) * sqrtf(wave_max(v));
-    if (!(bound > 0.f) || bound > 3e38f) return 1.f;
-    return exp2f(-(float)(ilogbf(bound) + 1));
+    float m[3] = {0.f, 0.f, 0.f};  // norms of do, delta, norms of v
+    const long first = (long)hk * a.group * a.q_tokens + sp.q0 + t0;
+    const int tokens = max(t1 - t0, 1), all = (t1 - t0) * a.group;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < all; i += 256) {
+        const int g = (unsigned)i / (unsigned)tokens;
+        const long at = first + (long)g * a.q_tokens + (i - g * tokens);
+        m[0] = fmaxf(m[0], a.norms[at]), m[1] = fmaxf(m[1], fabsf(finite(a.delta[at])));
+    }
+    const int j = j0 + (int)threadIdx.x;
+    if ((int)threadIdx.x < n && j < sp.nk) m[2] = a.v_norms[(long)hk * a.k_tokens + sp.k0 + j];
+    group_max(m);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, scale_for(m[0] * m[2] + m[1]))));
 }
 
 enum { KEYS = 128, ROWS = 128 };  // of a workgroup of the two kernels for tensors that cannot be moved in 16-byte pieces
@@ -106,7 +146,8 @@ __global__ __launch_bounds__(256) void attention_grad_kv_any_kernel(Args a) {
     int seq, block;
     if (!locate(a, blockIdx.x / a.kv_heads, sp, seq, block, [](const Span &s) { return (s.nk + KEYS - 1) / KEYS; })) return;
     const int group = a.group, rows = sp.nq * group, back = sp.nk - sp.nq;
-    const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
+    const int t_first = a.causal ? max(0, block * KEYS - back) : 0;  // the first query that sees a key of the block
+    const float mult = keys_scale<T>(a, sp, hk, block * KEYS, KEYS, min(t_first, sp.nq), sp.nq), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
     const int j = block * KEYS + wave * 32 + (lane & 31);  // the lane's key
     const bool there = j < sp.nk;
     const long key = sp.k0 + (there ? j : 0);
@@ -121,8 +162,7 @@ __global__ __launch_bounds__(256) void attention_grad_kv_any_kernel(Args a) {
     for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[b][e] = dv[b][e] = 0.f;
-    // the first row that sees a key of the block (its query is the block's first key less nk - nq)
-    const long first = a.causal ? (long)max(0, block * KEYS - back) * group : 0;
+    const long first = (long)t_first * group;
     for (long r0 = first / TILE * TILE; r0 < rows; r0 += TILE) {
         __syncthreads();
         for (int p = tid; p < TILE * PIECES; p += 256) {
@@ -198,7 +238,7 @@ __global__ __launch_bounds__(256) void attention_grad_q_any_kernel(Args a) {
     if (!locate(a, blockIdx.x / a.kv_heads, sp, seq, tile, tiles_of)) return;
     const int group = a.group, rows = sp.nq * group, back = sp.nk - sp.nq;
     tile = tiles_of(sp) - 1 - tile;
-    const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
+    const float c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
     const int r = tile * ROWS + wave * 32 + (lane & 31);
     const bool there = r < rows;
     const int t = there ? query_of(a, r) : 0, head = hk * group + (there ? r - t * group : 0);
@@ -209,10 +249,11 @@ __global__ __launch_bounds__(256) void attention_grad_q_any_kernel(Args a) {
         gf[u] = load_piece<T>((const T *)a.dout + (long)(sp.q0 + t) * a.lddo + (long)head * a.dim, u * M::STEP + h * M::V, a.dim, there, a.vec);
     }
     const long at = (long)head * a.q_tokens + sp.q0 + t;
-    const float lse = there ? a.lse[at] * LOG2E - shift : INFINITY, delta = there ? a.delta[at] : 0.f;
+    const float lse = there ? a.lse[at] * LOG2E - shift : INFINITY, delta = there ? a.delta[at] : 0.f, norm = scaled<T>() && there ? a.norms[at] : 0.f;
     const int last = !there ? -1 : a.causal ? min(sp.nk - 1, t + back) : sp.nk - 1;
     const int t_end = query_of(a, min(rows, (tile + 1) * ROWS) - 1);
     const int end = a.causal ? min(sp.nk, t_end + back + 1) : sp.nk;
+    const float mult = row_scale<T>(norm, largest_v<T>(a, sp, hk, end));
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b)
@@ -296,10 +337,14 @@ struct Shape {
     static constexpr int PB = row_bytes<T, DP>(), OWN = 128 / SPLIT, BLOCKS = PB <= 256 || SPLIT == 2 ? 2 : 1;
     static constexpr int KB = 32 * BLOCKS, TILE_BYTES = KB * PB, LOADS = TILE_BYTES / 1024 / 4;
     static constexpr int OCCUPANCY = DP * (int)sizeof(T) <= 256 ? 2 : 1;     // waves of a SIMD, dq
-    static constexpr int OCCUPANCY_KV = DP * (int)sizeof(T) <= 256 ? 2 : 1;  // ... dk and dv, whose sums and operands alone are 192 registers at 128 halves
+    // ... dk and dv, whose sums and operands alone are 192 registers at 128 halves (at 64, three registers more than
+    // let a third wave in: 475 -> 510 us for the same call)
+    static constexpr int OCCUPANCY_KV = DP * (int)sizeof(T) <= 128 ? 3 : DP * (int)sizeof(T) <= 256 ? 2 : 1;
     // dk and dv at 128 halves, two waves of a SIMD: the registers are a few fragments short, and the compiler's own way out would be scratch memory,
     // whose answers wait behind the tiles on their way (waits are in order); so some fragments of the values stay in LDS, where
-    // the two waves of SPLIT = 2 share them (one more there than would fit twice: 388 -> 379 us for the whole gradient above)
+    // the two waves of SPLIT = 2 share them (one more there than would fit twice: 388 -> 379 us for the whole gradient above).  SPLIT = 1, at 64
+    // halves too, is still three registers short: 12 bytes of scratch memory a thread (a fragment more in LDS, which 64 halves have room for, leaves
+    // that as it is: 741 -> 748 us for 2 x 4096 tokens of 32 + 8 heads).  Heads above 128 in single are 130 to 390 registers short in all kernels.
     static constexpr int SPARE = DP == 128 && sizeof(T) == 2 ? (SPLIT == 2 ? 4 : 3) : 0;
     static_assert(LOADS >= 1 && 4 * TILE_BYTES <= 160 * 1024, "a tile is at least a load of every wave, and two stages fit");
 };
@@ -401,7 +446,9 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
         a.joins[unit] = make_int4(there_is && part == first_part && parts > 1 ? parts : 0, sp.k0 + block * S::OWN, min(S::OWN, sp.nk - block * S::OWN), 0);
     if (!there_is || part < first_part) return;
     const int r_begin = max(begin, part * cut.chunk), r_end = min((long)rows, (part + 1L) * cut.chunk);
-    const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
+    // (of the rows from the first query of r_begin's load to the last one of the load before r_end)
+    const int t_begin = min(query_of(a, r_begin / Rows::CT) * Rows::CT, sp.nq), t_end = r_begin < r_end ? min(sp.nq, (query_of(a, (r_end - 1) / Rows::CT) + 1) * Rows::CT) : t_begin;
+    const float mult = keys_scale<T>(a, sp, hk, block * S::OWN, S::OWN, t_begin, t_end), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
     const int j0 = block * S::OWN + wave % (4 / SPLIT) * 32;  // the wave's first key
     frag kf[UNITS], vf[UNITS - S::SPARE];
 #pragma unroll
@@ -516,18 +563,18 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY_KV)) void atte
 #pragma unroll
             for (int e = 0; e < 16; ++e) dk[n][e] += to[(n * 16 + e) * 64], dv[n][e] += to[((N + n) * 16 + e) * 64];
     }
+    const float unshift = exp2f(-shift), by = a.scale * unshift / mult;
     if (parts > 1) {  // as the registers hold them: the second launch's lanes hold the same elements
         float *to = a.part + (((long)unit * a.kv_heads + hk) * (S::OWN / 32) + wave % (4 / SPLIT)) * 2 * N * 16 * 64 + el;
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) to[(n * 16 + e) * 64] = dk[n][e], to[((N + n) * 16 + e) * 64] = dv[n][e];
+            for (int e = 0; e < 16; ++e) to[(n * 16 + e) * 64] = dk[n][e] * by, to[((N + n) * 16 + e) * 64] = dv[n][e] * unshift;
         return;
     }
     const int j = j0 + (el & 31);
     if (j >= sp.nk) return;
     const long key = sp.k0 + j;
-    const float unshift = exp2f(-shift), by = a.scale * unshift / mult;
     T *pk = (T *)a.dk + key * a.lddk + (long)hk * a.dim, *pv = (T *)a.dv + key * a.lddv + (long)hk * a.dim;
     store_sums<T, DP>(pk, dk, by, a.dim, el >> 5, a.overwrite & 2);
     store_sums<T, DP>(pv, dv, unshift, a.dim, el >> 5, a.overwrite & 4);
@@ -548,7 +595,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
     if (!locate(a, blockIdx.x / a.kv_heads, sp, seq, tile, tiles_of)) return;
     const int group = a.group, rows = sp.nq * group, back = sp.nk - sp.nq;
     tile = tiles_of(sp) - 1 - tile;  // the rows that see most keys first
-    const float mult = ds_scale<T>(a), c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
+    const float c = a.scale * LOG2E, shift = scaled<T>() ? P_SHIFT : 0.f;
     const int r = tile * S::OWN + wave % (4 / SPLIT) * 32 + (lane & 31);
     const bool there = r < rows;
     const int t = query_of(a, there ? r : rows - 1), head = hk * group + (there ? r - t * group : 0);
@@ -559,11 +606,13 @@ __global__ __launch_bounds__(256, (Shape<T, DP, SPLIT>::OCCUPANCY)) void attenti
         gf[u] = load_piece<T>((const T *)a.dout + (long)(sp.q0 + t) * a.lddo + (long)head * a.dim, u * M::STEP + h * M::V, a.dim, there, 1);
     }
     const long at = (long)head * a.q_tokens + sp.q0 + t;
-    const float lse = there ? a.lse[at] * LOG2E - shift : INFINITY;
-    float delta = there ? a.delta[at] * mult : 0.f;
+    const float lse = there ? a.lse[at] * LOG2E - shift : INFINITY, norm = scaled<T>() && there ? a.norms[at] : 0.f;
+    float delta = there ? a.delta[at] : 0.f;
     const int last = a.causal ? min(sp.nk - 1, t + back) : sp.nk - 1;
     const int end = a.causal ? min(sp.nk, query_of(a, min(rows, (tile + 1) * S::OWN) - 1) + back + 1) : sp.nk;
     const int wave_all = __builtin_amdgcn_readfirstlane(__shfl(last, 0)), wave_end = __builtin_amdgcn_readfirstlane(__shfl(last, 31)) + 1;
+    const float mult = row_scale<T>(norm, largest_v<T>(a, sp, hk, end));
+    delta *= mult;
     f32x16 dq[N];
 #pragma unroll
     for (int b = 0; b < N; ++b)
@@ -657,7 +706,6 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(Args a) {
     const int lane = threadIdx.x & 63, hk = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
     const int4 join = a.joins[unit];
     if (!join.x) return;
-    const float mult = ds_scale<T>(a), unshift = exp2f(scaled<T>() ? -P_SHIFT : 0.f);
     for (int i = threadIdx.x >> 6; i < S::OWN / 32 * 2; i += 4) {
         const int keys = i >> 1, which = i & 1;
         const float *from = a.part + (((long)unit * a.kv_heads + hk) * (S::OWN / 32) + keys) * 2 * N * 16 * 64 + which * N * 16 * 64 + lane;
@@ -675,8 +723,8 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(Args a) {
         const int j = keys * 32 + (lane & 31);
         if (j >= join.z) continue;
         const long key = join.y + j;
-        if (which == 0) store_sums<T, DP>((T *)a.dk + key * a.lddk + (long)hk * a.dim, x, a.scale * unshift / mult, a.dim, lane >> 5, a.overwrite & 2);
-        else store_sums<T, DP>((T *)a.dv + key * a.lddv + (long)hk * a.dim, x, unshift, a.dim, lane >> 5, a.overwrite & 4);
+        if (which == 0) store_sums<T, DP>((T *)a.dk + key * a.lddk + (long)hk * a.dim, x, 1.f, a.dim, lane >> 5, a.overwrite & 2);
+        else store_sums<T, DP>((T *)a.dv + key * a.lddv + (long)hk * a.dim, x, 1.f, a.dim, lane >> 5, a.overwrite & 4);
     }
 }
 
@@ -727,7 +775,7 @@ template <class T>
 int launch(const Args &a, bool fast, hipStream_t stream) {
     int lanes = 1;
     while (lanes * Type<T>::V < a.dim) lanes *= 2;
-    hipLaunchKernelGGL(attention_delta_kernel<T>, dim3(NORM_GROUPS), dim3(256), 0, stream, a, lanes);
+    hipLaunchKernelGGL(attention_delta_kernel<T>, dim3(DELTA_GROUPS), dim3(256), 0, stream, a, lanes);
     D8_LAUNCH_CHECK();
     if (a.dim <= 32) return launch_dim<T, 32>(a, fast, stream);
     if (a.dim <= 64) return launch_dim<T, 64>(a, fast, stream);
@@ -759,11 +807,15 @@ static GradPlan grad_plan(int dtype, int sequences, int q_tokens, int k_tokens, 
     return p;
 }
 
-static size_t row_bytes_of(int q_tokens, int heads) { return (sizeof(float) * (2 * NORM_GROUPS + (size_t)q_tokens * heads) + 255) & ~(size_t)255; }
+// delta and norms
+static size_t row_bytes_of(int dtype, int q_tokens, int k_tokens, int heads, int kv_heads) {
+    const size_t rows = (size_t)q_tokens * heads, floats = dtype == D8_FLOAT16 ? 2 * rows + (size_t)k_tokens * kv_heads : rows;
+    return (sizeof(float) * floats + 255) & ~(size_t)255;
+}
 
 size_t grad_scratch_bytes(int dtype, int sequences, int q_tokens, int k_tokens, int heads, int kv_heads, int dim, bool causal) {
     const GradPlan p = grad_plan(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim, causal != 0);
-    return row_bytes_of(q_tokens, heads) + p.lists + p.parts;
+    return row_bytes_of(dtype, q_tokens, k_tokens, heads, kv_heads) + p.lists + p.parts;
 }
 
 }  // namespace attention
@@ -789,8 +841,8 @@ extern "C" int d8_attention_grad(int dtype, const void *q, long ldq, const void 
     const attention::GradPlan plan = attention::grad_plan(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim, causal != 0);
     const size_t need = attention::grad_scratch_bytes(dtype, sequences, q_tokens, k_tokens, heads, kv_heads, dim, causal != 0);
     D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_grad: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
-    a.norms = (float *)scratch, a.delta = a.norms + 2 * attention::NORM_GROUPS;
-    a.joins = (int4 *)((char *)scratch + attention::row_bytes_of(q_tokens, heads)), a.part = (float *)((char *)a.joins + plan.lists);
+    a.delta = (float *)scratch, a.norms = a.delta + (size_t)q_tokens * heads, a.v_norms = a.norms + (size_t)q_tokens * heads;
+    a.joins = (int4 *)((char *)scratch + attention::row_bytes_of(dtype, q_tokens, k_tokens, heads, kv_heads)), a.part = (float *)((char *)a.joins + plan.lists);
     a.pieces = plan.pieces, a.units = plan.units, a.split_kv = plan.split;
     attention::set_group(a);
     a.vec = attention::in_pieces(dtype, dim, {q, k, v, o, dout}, {ldq, ldk, ldv, ldo, lddo});

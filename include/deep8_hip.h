@@ -472,7 +472,10 @@ int d8_avgpool2d_grad_overwrite(int dtype, void *dx, const void *dy, int B, int 
  *                        query's sequence never reach it.  Inside it a hidden key's weight is 0, as if written out: NaN or infinity
  *                        in that key's row of v (gradients: of k, v, and of the query's q, dout) can still make 0 times it, NaN.
  * d8_attention_grad      the gradients of q (bit 0 of overwrite), k (bit 1) and v (bit 2) from those of o (dout), with o and lse as the
- *                        forward call left them.  The same bits every time.
+ *                        forward call left them.  The same bits every time.  Float16: probabilities and the scores' gradients are halves in the
+ *                        products, the latter relative to the largest that they can be: in a row of dq its own and its keys', in a key's dk that of
+ *                        the rows (same sequence, heads that share the key) and keys beside it.  A term keeps its bits down to 2^-28 of
+ *                        that and is lost below 2^-39.
  *     scratch: d8_attention_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.
  * d8_matmul_gated        h = act(g) * u with (g | u) = x w: w is [inner][2 * cols], its first `cols` columns the gate's.  act: D8_GATE_*.
  *                        pre (may be NULL): [rows][2 * cols], receives g and u for the gradients.
