@@ -360,6 +360,13 @@ int check(int dtype, int rows, int inner, int cols, int act, const char *name) {
 }
 
 enum { FEW_ROWS = 64 };
+// Offsets into a tile are 32 bits, and 2^31 stands for what is not there: the rows of x that a tile has, at most 128, and the 32 (half, more
+// than FEW_ROWS rows: 64) rows of w of a step must not be more bytes than that.  (gated_wide.hip asks for less than 2^31 of each whole operand.)
+bool fits(int dtype, long rows, long inner, long cols) {
+    const long es = (long)dtype_bytes(dtype), v = 16 / es, step = rows > FEW_ROWS && dtype == D8_FLOAT16 ? 64 : 32;
+    const long x_row = (inner + v - 1) / v * 16, w_row = 2 * ((cols + v - 1) / v * 16);
+    return (rows < 128 ? rows : 128) * x_row <= (1L << 31) && step * w_row <= (1L << 31);
+}
 // What a 32 x 32 block of both products takes a compute unit per element of K (microseconds): alone on it, where a workgroup waits for its
 // loads and barriers, and beside others; and what a second launch takes.
 constexpr float ALONE[2] = {0.0029f, 0.0135f}, TOGETHER[2] = {0.00135f, 0.0095f}, JOIN_US = 4.f;  // half, single
@@ -428,7 +435,7 @@ using namespace d8;
 
 extern "C" size_t d8_matmul_gated_scratch_bytes(int dtype, int which, int rows, int inner, int cols) {
     if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || rows < 1 || inner < 1 || cols < 1 || cols >= (1 << 28) || inner >= (1 << 28)) return 0;
-    if (which != 1) return gated::plan_of(dtype, rows, inner, cols, true, true).bytes();
+    if (which != 1) return !gated::fits(dtype, rows, inner, cols) ? 0 : gated::plan_of(dtype, rows, inner, cols, true, true).bytes();
     return gated::round256(dtype_bytes(dtype) * 2 * (size_t)rows * cols) + d8_matmul_scratch_bytes(dtype, 3, 1, rows, inner, 1, inner, 2 * cols);
 }
 
@@ -496,6 +503,7 @@ int forward(Args a, const Plan &p, char *scratch, hipStream_t stream) {
 extern "C" int d8_matmul_gated(int dtype, const void *x, int rows, int inner, const void *w, int cols, int act, void *pre, void *h, void *scratch,
                                size_t scratch_bytes, void *stream) {
     if (int rc = gated::check(dtype, rows, inner, cols, act, "matmul_gated")) return rc;
+    D8_REQUIRE(gated::fits(dtype, rows, inner, cols), "matmul_gated: rows of %d and 2 * %d elements are too long", inner, cols);
     D8_REQUIRE(x && w && h, "matmul_gated: null tensor");
     gated::Args a;
     memset(&a, 0, sizeof(a));

@@ -478,7 +478,8 @@ int d8_avgpool2d_grad_overwrite(int dtype, void *dx, const void *dy, int B, int 
  *                        that and is lost below 2^-39.
  *     scratch: d8_attention_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.
  * d8_matmul_gated        h = act(g) * u with (g | u) = x w: w is [inner][2 * cols], its first `cols` columns the gate's.  act: D8_GATE_*.
- *                        pre (may be NULL): [rows][2 * cols], receives g and u for the gradients.
+ *                        pre (may be NULL): [rows][2 * cols], receives g and u for the gradients.  Refused: 128 rows of x (all, if they
+ *                        are fewer) or 32 rows of w (Float16, more than 64 rows of x: 64) of more than 2 GiB.
  * d8_matmul_gated_grad   dx (bit 0 of overwrite) and dw (bit 1) from dh, with pre as the forward call left it.
  *     scratch: d8_matmul_gated_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.  It counts on x and w at
  *     multiples of 16 bytes; elsewhere the forward call asks for a copy of each, rows padded to 16 bytes (its error says how much). */
