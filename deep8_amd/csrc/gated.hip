@@ -20,6 +20,7 @@ using attention::load_to_lds;
 using attention::swizzle;
 
 // activation and its slope
+template <class T>
 __device__ __forceinline__ void activation_slope(float a, int act, float &f, float &df) {
     switch (act) {
         case D8_GATE_SILU: {
@@ -28,7 +29,7 @@ __device__ __forceinline__ void activation_slope(float a, int act, float &f, flo
             break;
         }
         case D8_GATE_GELU: {
-            const float p = 0.5f * (1.f + erff(a * 0.70710678f));
+            const float p = normal_integral<T>(a);
             f = a * p, df = p + a * 0.39894228f * expf(-0.5f * a * a);
             break;
         }
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(256) void gated_slope_kernel(Args a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             float f, df;
-            activation_slope((float)g[e], a.act, f, df);
+            activation_slope<T>((float)g[e], a.act, f, df);
             dg[e] = (T)((float)d[e] * (float)u[e] * df), du[e] = (T)((float)d[e] * f);
         }
         T *to = (T *)a.dpre + row * 2 * a.cols;
