@@ -436,7 +436,7 @@ using namespace d8;
 
 extern "C" size_t d8_matmul_gated_scratch_bytes(int dtype, int which, int rows, int inner, int cols) {
     if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || rows < 1 || inner < 1 || cols < 1 || cols >= (1 << 28) || inner >= (1 << 28)) return 0;
-    if (which != 1) return !gated::fits(dtype, rows, inner, cols) ? 0 : gated::plan_of(dtype, rows, inner, cols, true, true).bytes();
+    if (which != 1) return !gated::fits(dtype, rows, inner, cols) ? 0 : gated::plan_of(dtype, rows, inner, cols, which != 2, which != 2).bytes();
     return gated::round256(dtype_bytes(dtype) * 2 * (size_t)rows * cols) + d8_matmul_scratch_bytes(dtype, 3, 1, rows, inner, 1, inner, 2 * cols);
 }
 

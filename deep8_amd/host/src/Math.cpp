@@ -959,7 +959,8 @@ void AttentionGrad(const Tensor &q, Tensor &dq, const Tensor &k, Tensor &dk, con
 void MatrixMultiplyGated(const Tensor &x, const Tensor &w, Tensor *pre, Tensor &h, GateType act) {
     checkGated(x, w, pre, h);
     const int dt = dtypeOf(x), rows = rowsOf(x), inner = (int)x.col(), cols = (int)h.col();
-    PoolScratch ws(x.device(), d8_matmul_gated_scratch_bytes(dt, 0, rows, inner, cols));
+    const bool aligned = 0 == (((size_t)x.raw() | (size_t)w.raw()) & 15);  // (a view may start anywhere)
+    PoolScratch ws(x.device(), d8_matmul_gated_scratch_bytes(dt, aligned ? 0 : 2, rows, inner, cols));
     h.takeZero();
     if (pre) pre->takeZero();
     D8_CHECK(d8_matmul_gated(dt, x.raw(), rows, inner, w.raw(), cols, (int)act, pre ? pre->raw() : nullptr, h.raw(), ws.ptr, ws.bytes, nullptr));

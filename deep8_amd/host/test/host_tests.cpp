@@ -1188,6 +1188,29 @@ TEST_GPU(matrix_multiply_gated_node) {
         }
 }
 
+TEST_GPU(matrix_multiply_gated_of_views) {
+    // inputs that start one element into their storage: the same product as that of whole tensors
+    for (DType id : {DType::Float32, DType::Float16})
+        for (int rows : {5, 100}) {
+            const ElementType type = ElementType::from(id);
+            const size_t inner = 24, cols = 16, at = type.byteWidth;
+            HostTensor x = normalTensor(type, 1, {(size_t)rows, inner}), w = normalTensor(type, 1, {inner, 2 * cols}), h = normalTensor(type, 1, {(size_t)rows, cols}), hv = normalTensor(type, 1, {(size_t)rows, cols});
+            auto view = [&](HostTensor &whole) {
+                HostTensor room = normalTensor(type, 1, {whole.t.size() + 1});
+                std::vector<size_t> dims(whole.t.shape.dims, whole.t.shape.dims + 2);
+                Tensor v(room.t.storage, at, dims, type);
+                gpu().copyFromGPUToGPU(whole.t.raw(), v.raw(), whole.t.byteCount());
+                return v;
+            };
+            Math::MatrixMultiplyGated(x.t, w.t, nullptr, h.t);
+            download(h);
+            for (int which = 1; which < 4; ++which) {
+                Math::MatrixMultiplyGated(which & 1 ? view(x) : x.t, which & 2 ? view(w) : w.t, nullptr, hv.t);
+                expectClose(hv, doubles(h), 1e-6);
+            }
+        }
+}
+
 TEST_GPU(transformer_layer_backward_at_once_and_input_by_input) {
     // the executor's pass (all gradients of a node from one call) against the nodes' own, input by input; and one variable as queries, keys
     // and values, whose three gradients add up

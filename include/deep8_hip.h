@@ -481,8 +481,8 @@ int d8_avgpool2d_grad_overwrite(int dtype, void *dx, const void *dy, int B, int 
  *                        pre (may be NULL): [rows][2 * cols], receives g and u for the gradients.  Refused: 128 rows of x (all, if they
  *                        are fewer) or 32 rows of w (Float16, more than 64 rows of x: 64) of more than 2 GiB.
  * d8_matmul_gated_grad   dx (bit 0 of overwrite) and dw (bit 1) from dh, with pre as the forward call left it.
- *     scratch: d8_matmul_gated_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.  It counts on x and w at
- *     multiples of 16 bytes; elsewhere the forward call asks for a copy of each, rows padded to 16 bytes (its error says how much). */
+ *     scratch: d8_matmul_gated_scratch_bytes, which = 0 forward with x and w at multiples of 16 bytes, 2 forward wherever they lie
+ *     (room for a copy of each, rows padded to 16 bytes, unless which = 0 has it), 1 gradients; 16-byte aligned. */
 #define D8_GATE_SILU    0 /* a sigmoid(a)                 */
 #define D8_GATE_GELU    1 /* a (1 + erf(a / sqrt 2)) / 2  */
 #define D8_GATE_RELU    2
