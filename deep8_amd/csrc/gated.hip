@@ -19,15 +19,21 @@ using attention::desc_t;
 using attention::load_to_lds;
 using attention::swizzle;
 
+// the sigmoid of a and what it is short of 1, the sigmoid of -a (a difference would leave none of its bits far above 0)
+__device__ __forceinline__ void both_sigmoids(float a, float &s, float &rest) {
+    const float power = expf(-fabsf(a)), large = 1.f / (1.f + power), small = power * large;
+    s = a < 0.f ? small : large, rest = a < 0.f ? large : small;
+}
+
 // activation and its slope
 template <class T>
 __device__ __forceinline__ void activation_slope(float a, int act, float &f, float &df) {
+    float s, rest;
     switch (act) {
-        case D8_GATE_SILU: {
-            const float s = 1.f / (1.f + expf(-a));
-            f = a * s, df = s * (1.f + a * (1.f - s));
+        case D8_GATE_SILU:
+            both_sigmoids(a, s, rest);
+            f = a * s, df = s * (1.f + a * rest);
             break;
-        }
         case D8_GATE_GELU: {
             const float p = normal_integral<T>(a);
             f = a * p, df = p + a * 0.39894228f * expf(-0.5f * a * a);
@@ -36,10 +42,9 @@ __device__ __forceinline__ void activation_slope(float a, int act, float &f, flo
         case D8_GATE_RELU:
             f = a > 0.f ? a : 0.f, df = a > 0.f ? 1.f : 0.f;
             break;
-        default: {
-            const float s = 1.f / (1.f + expf(-a));
-            f = s, df = s * (1.f - s);
-        }
+        default:
+            both_sigmoids(a, s, rest);
+            f = s, df = s * rest;
     }
 }
 
