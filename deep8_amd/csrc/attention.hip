@@ -6,8 +6,9 @@
 // One pass over the keys with the running maximum and sum of the softmax (fp32).  A workgroup has 128 rows, each of its four waves
 // 32 of them; the scores are computed transposed (keys x rows), so that a row's scores lie in one lane (and its partner 32 lanes on),
 // maximum and sum are lane arithmetic, and the probabilities are the right operand of the product with the values where they are.
-// In half the probabilities, at most 1 relative to the running maximum, are rounded to half for that product: an error of 2^-12 a
-// term, which the terms' different signs and the division by a sum of the unrounded ones leave below the rounding of o itself.
+// In half the probabilities, at most 1 relative to the running maximum (up to 2^8 where it lags), are rounded to half for that product,
+// the type that the matrix instruction takes at full rate: as much error again as the rounding of o where values have random signs, 2.6 (prompts)
+// to 2.9 10^-4 (single queries over thousands of keys) for 2.1.  Maxima, sums and o are fp32, the sum that of the unrounded ones.
 #include "attention.h"
 
 namespace d8 {
@@ -117,8 +118,9 @@ __device__ __forceinline__ float exponent_scale(const Args &a) { return fmaxf(fa
 
 // Large outputs.  128 rows a workgroup, keys in tiles of 64 (32 where a row takes more than 256 bytes) that go from memory straight into one of
 // two stages of LDS, the next tile's while this one is worked on; one barrier a tile.  Two workgroups a compute unit, so that
-// one's products run under the other's exponentials.  Half, causal, sequences of 7290, 7240 and 1854, 16 + 4 heads of 128: 480 us = 930 TFLOP/s
-// (a large product 1320).  Bound by power: fragments read four products ahead take 5 % of the cycles away and the clock falls by as much.
+// one's products run under the other's exponentials.  Half, causal, sequences of 7290, 7240 and 1854, 16 + 4 heads of 128: 480 us at the least,
+// 530 in the mean of 40 calls in a row, 930 and 840 TFLOP/s (a large product 1320).  Bound by power: 7.3 M cycles at 1.89 GHz, where a kernel that waits
+// for memory runs at 2.5; fragments read four products ahead take 5 % of the cycles away and the clock falls by as much.
 template <class T, int DP>
 __global__ __launch_bounds__(256, (DP * (int)sizeof(T) <= 256 ? 2 : 1)) void attention_rows_kernel(Args a) {
     typedef Type<T> M;

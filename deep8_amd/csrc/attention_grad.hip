@@ -37,7 +37,7 @@ __device__ __forceinline__ float wave_max(float v) {
 __device__ __forceinline__ float finite(float v) { return fabsf(v) <= 3.4e38f ? v : 0.f; }
 
 // delta = sum of do o of each row; a group of lanes has a row, 16 bytes a lane.  In half also the norms of the rows of do and of v.
-// Bound by bytes: 56 MB (6144 tokens, 16 + 4 heads of 128 halves) in 19 us; four rows' loads at once took 2 us off that
+// Bound by bytes: 56 MB (6144 tokens, 16 + 4 heads of 128 halves) in 20 us; four rows' loads at once took 2 us off that
 // and added as much to small calls.
 template <class T>
 __global__ __launch_bounds__(256) void attention_delta_kernel(Args a, int lanes) {
@@ -330,8 +330,8 @@ __device__ __forceinline__ void store_sums(T *to, const f32x16 (&x)[DP / 32], fl
 // worked on.  A wave has 32 keys (rows) of its own, whose fragments and sums stay in registers.  SPLIT = 1: four waves, 128 keys
 // (rows) a workgroup, each walks every tile; SPLIT = 2, where that would leave compute units idle: 64, two waves have the same
 // 32 and take every other tile, and their sums are joined through LDS at the end.  Half, causal, sequences of 2010, 1461 and 2673, 16 + 4 heads of
-// 128: dk and dv 195 us + 20 for the join (four products, 560 TFLOP/s: two waves of a SIMD with every register taken wait for LDS and
-// barriers), dq 115 us (three, 710 TFLOP/s).  Single, 2048 tokens in four sequences, 8 heads of 64: 83 and 63 us (52 TFLOP/s).
+// 128: dk and dv 191 to 214 us + 20 for the join (four products, 570 TFLOP/s at the least time: two waves of a SIMD with every register taken wait for
+// LDS and barriers, at 2.36 GHz), dq 110 to 117 us (three, 740 TFLOP/s).  Single, 2048 tokens in four sequences, 8 heads of 64: 83 and 63 us (52 TFLOP/s).
 template <class T, int DP, int SPLIT>
 struct Shape {
     static constexpr int PB = row_bytes<T, DP>(), OWN = 128 / SPLIT, BLOCKS = PB <= 256 || SPLIT == 2 ? 2 : 1;
@@ -344,7 +344,8 @@ struct Shape {
     // whose answers wait behind the tiles on their way (waits are in order); so some fragments of the values stay in LDS, where
     // the two waves of SPLIT = 2 share them (one more there than would fit twice: 388 -> 379 us for the whole gradient above).  SPLIT = 1, at 64
     // halves too, is still three registers short: 12 bytes of scratch memory a thread (a fragment more in LDS, which 64 halves have room for, leaves
-    // that as it is: 741 -> 748 us for 2 x 4096 tokens of 32 + 8 heads).  Heads above 128 in single are 130 to 390 registers short in all kernels.
+    // that as it is: 741 -> 748 us for 2 x 4096 tokens of 32 + 8 heads).  Heads above 128 in single are 221 (dk, dv) and 386 (dq) registers
+    // short, attention.hip's kernels 109 and 143: they are right, and slow (no shape for them was looked for).
     static constexpr int SPARE = DP == 128 && sizeof(T) == 2 ? (SPLIT == 2 ? 4 : 3) : 0;
     static_assert(LOADS >= 1 && 4 * TILE_BYTES <= 160 * 1024, "a tile is at least a load of every wave, and two stages fit");
 };

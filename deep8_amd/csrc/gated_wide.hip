@@ -2,7 +2,8 @@
 // are 128 of the gate and the same 128 of the factor, arranged so that each wave has 64 of both: what a wave's lanes fetch decides it,
 // LDS layout, fragments and the order of the products are the plain product's.  The epilogue forms h from the accumulators.
 //
-// Bound by the matrix pipe's power like the plain product: 8192 x 4096 x 2 * 8192 in 840 us = 1310 TFLOP/s (a large plain product 1320).  The
+// Bound by the matrix pipe's power like the plain product: 8192 x 4096 x 2 * 8192 in 840 us at the least = 1310 TFLOP/s (a large plain product 1320), 890
+// in the mean of 40 calls in a row, at 1.86 GHz.  The
 // epilogue reads no memory and writes h, and g and u for training, 16 bytes a lane in whole 128-byte lines.
 #include "gated.h"
 #include "gemm_wide_kernel.h"

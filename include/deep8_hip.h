@@ -442,10 +442,12 @@ int d8_avgpool2d_grad_overwrite(int dtype, void *dx, const void *dy, int B, int 
                                 int FH, int FW, int covered, int sy, int sx, void *stream);
 
 /* ---- a transformer layer --------------------------------------------------------------------------
- * What such a layer needs besides MatrixMultiply and Add; no counterpart in the reference.  Float16 and Float32.  Rows
+ * Three operators of such a layer, to stand beside MatrixMultiply and Add; no counterpart in the reference.  Float16 and Float32.  Rows
  * (tokens) of several heads lie `ld` elements apart, the heads of a row next to each other, so that queries, keys and values
  * may be parts of one product's rows.  Gradients are added to what their destination holds unless their bit of `overwrite` is set.
- * Sums, statistics of norms and softmax are fp32; results are rounded once.
+ * Sums, statistics of norms and softmax are fp32; results are rounded once.  Between two products Float16 calls hold halves: d8_attention its
+ * probabilities, d8_attention_grad these and the scores' gradients, d8_matmul_gated_grad the gradients of g and u.  Each adds about as much
+ * error as the result's rounding (2.6 to 3 10^-4 of a result's norm in all, where the rounding alone is 2.1).
  *
  * d8_rotary_table        table[p][i] = (cos, sin)(p f_i) in fp32, i < rotary / 2, positions p < positions, f_i = base^(-2 i / rotary);
  *                        angles in fp64.  For contexts longer than a model was trained on, factor > 1 slows the rotation down:
@@ -472,10 +474,9 @@ int d8_avgpool2d_grad_overwrite(int dtype, void *dx, const void *dy, int B, int 
  *                        query's sequence never reach it.  Inside it a hidden key's weight is 0, as if written out: NaN or infinity
  *                        in that key's row of v (gradients: of k, v, and of the query's q, dout) can still make 0 times it, NaN.
  * d8_attention_grad      the gradients of q (bit 0 of overwrite), k (bit 1) and v (bit 2) from those of o (dout), with o and lse as the
- *                        forward call left them.  The same bits every time.  Float16: probabilities and the scores' gradients are halves in the
- *                        products, the latter relative to the largest that they can be: in a row of dq its own and its keys', in a key's dk that of
- *                        the rows (same sequence, heads that share the key) and keys beside it.  A term keeps its bits down to 2^-28 of
- *                        that and is lost below 2^-39.
+ *                        forward call left them.  The same bits every time.  Float16: a score's gradient is held relative to the largest that it can be,
+ *                        in a row of dq by that row and its keys, in a key's dk by the rows (same sequence, heads that share the key) and keys of
+ *                        its workgroup.  A term keeps its bits down to 2^-28 of that and is lost below 2^-39.
  *     scratch: d8_attention_scratch_bytes, which = 0 forward, 1 gradients; 16-byte aligned.
  * d8_matmul_gated        h = act(g) * u with (g | u) = x w: w is [inner][2 * cols], its first `cols` columns the gate's.  act: D8_GATE_*.
  *                        pre (may be NULL): [rows][2 * cols], receives g and u for the gradients.  Refused: 128 rows of x (all, if they
