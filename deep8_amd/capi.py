@@ -130,6 +130,9 @@ SIGNATURES = {
     "d8_matmul_gated_scratch_bytes": (_Z, [_I] * 5),
     "d8_matmul_gated": (_I, [_I, _P, _I, _I, _P, _I, _I, _P, _P, _P, _Z, _P]),
     "d8_matmul_gated_grad": (_I, [_I, _P, _P, _I, _I, _P, _P, _I, _I, _P, _P, _I, _P, _Z, _P]),
+    "d8_layer_norm": (_I, [_I, _P, _L, _P, _P, _P, _L, _I, _I, _F, _P]),
+    "d8_layer_norm_grad_scratch_bytes": (_Z, [_I] * 3),
+    "d8_layer_norm_grad": (_I, [_I, _P, _L, _P, _P, _L, _P, _L, _P, _P, _I, _I, _F, _I, _P, _Z, _P]),
     "d8_gemm_phase_record": (_I, [_P, _Z]),
     "d8_mfma_stream_out_bytes": (_Z, []),
     "d8_mfma_stream": (_I, [_I, _P, _Z, _P, _I, ctypes.POINTER(ctypes.c_double), _P]),

@@ -1,0 +1,437 @@
+// Norm of whole rows, and the way back.
+//
+//   m = mean(x),  r = 1 / sqrt(mean((x - m)^2) + epsilon),  u = (x - m) r,  y = u w + b
+//   back: g = dy,  dx = r (w g - mean(w g) - u mean(w g u)),  dw = sum over rows of g u,  db = sum over rows of g
+//
+// Bound by memory: x is read and y written once (back: x and dy read, dx written); a row stays in the registers of its team of 64, 256
+// or 1024 threads between the sums and the result.  A thread has up to 16 elements of a row: more would leave too few waves to keep the
+// loads coming.  The spread is taken about the mean that was found, not from the sum of squares, which would cancel in rows whose mean is
+// far from zero, and what that mean is off by (its sum is rounded) is taken out with the same pass: sum (x - m) is it.
+//
+// The way back keeps the columns' sums of dw and db in registers while a workgroup goes down its rows (the next row's loads are on their
+// way meanwhile), adds its teams' through LDS, and leaves one row of them in scratch; a second launch adds those in a fixed order.  One
+// workgroup of 1024 threads a compute unit: twice as many would write and read twice as many sums, 8 % of all bytes at 8192 x 4096 already.
+//
+// Sums are fp32; results are rounded once.
+#include <type_traits>
+
+#include "common.h"
+
+namespace d8 {
+namespace {
+
+enum { MOST_HELD = 16384 };  // elements of a row that a team holds
+
+struct NormArgs {
+    const void *x, *dy, *weight, *bias;
+    void *out;  // y, or dx
+    void *dweight, *dbias;
+    float *partial;  // gradient: [groups][dw, db][cols]
+    long ldx, lddy, ldout;
+    int rows, cols, groups, overwrite;
+    float epsilon;
+};
+
+template <class T, int V>
+struct Vec {
+    typedef T type __attribute__((ext_vector_type(V)));
+};
+template <class T>
+struct Vec<T, 1> {
+    typedef T type;
+};
+
+// E elements of a row of T in one thread, in pieces of V: piece i is number t + TEAM * i of the row.
+template <class T, int V, int TEAM, int E>
+struct Held {
+    static constexpr int P = E / V;
+    typedef typename Vec<T, V>::type vec;
+    vec raw[P];
+    __device__ __forceinline__ void load(const T *row, int t, int cols) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int c = (t + TEAM * i) * V;
+            if (c < cols) raw[i] = *(const vec *)(row + c);
+            else raw[i] = vec{};
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[E]) const {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if constexpr (V == 1) {
+                v[i] = (float)raw[i];
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[i * V + e] = (float)raw[i][e];
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(T *row, int t, int cols, const float (&v)[E]) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int c = (t + TEAM * i) * V;
+            if (c >= cols) continue;
+            vec w;
+            if constexpr (V == 1) {
+                w = (T)v[i];
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) w[e] = (T)v[i * V + e];
+            }
+            *(vec *)(row + c) = w;
+        }
+    }
+};
+
+// The sum of two values over a team.  Several waves: through LDS, a slot that the call before last used (two places in turn: the barrier
+// of the call between keeps a wave from writing what another still reads).
+template <int TEAM>
+__device__ __forceinline__ void team_sum(float &a, float &b, float2 *slots, int &turn) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
+    if constexpr (TEAM > 64) {
+        const int wave = threadIdx.x >> 6;
+        float2 *s = slots + turn * 16;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) s[wave] = make_float2(a, b);
+        __syncthreads();
+        constexpr int N = TEAM / 64;
+        s += wave / N * N;
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) a += s[i].x, b += s[i].y;
+    }
+}
+
+// (E values of which those beyond the row are 0) centred in place, 0 there again; the reciprocal of the spread
+template <int V, int TEAM, int E>
+__device__ __forceinline__ float centre(float (&v)[E], int t, int cols, float epsilon, float2 *slots, int &turn) {
+    const float n = 1.f / cols;
+    float sum = 0.f, rest = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += v[e];
+    team_sum<TEAM>(sum, rest, slots, turn);
+    const float mean = sum * n;
+    float off = 0.f, squares = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        v[e] = (t + TEAM * (e / V)) * V < cols ? v[e] - mean : 0.f;
+        off += v[e], squares += v[e] * v[e];
+    }
+    team_sum<TEAM>(off, squares, slots, turn);
+    off *= n;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = (t + TEAM * (e / V)) * V < cols ? v[e] - off : 0.f;
+    return 1.f / sqrtf(fmaxf(squares * n - off * off, 0.f) + epsilon);
+}
+
+constexpr int forward_threads(int team) { return team < 256 ? 256 : team; }
+
+template <class T, int V, int TEAM, int E>
+__global__ __launch_bounds__(forward_threads(TEAM)) void layer_norm_kernel(NormArgs a) {
+    __shared__ float2 slots[2 * 16];
+    constexpr int TEAMS = forward_threads(TEAM) / TEAM;
+    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    typedef Held<T, V, TEAM, E> H;
+    float w[E], b[E];
+    {
+        H h;
+        if (a.weight) h.load((const T *)a.weight, t, a.cols), h.get(w);
+        else for (int e = 0; e < E; ++e) w[e] = 1.f;
+        if (a.bias) h.load((const T *)a.bias, t, a.cols), h.get(b);
+        else for (int e = 0; e < E; ++e) b[e] = 0.f;
+    }
+    int turn = 0;
+    H x;
+    long row = (long)blockIdx.x * TEAMS + team;
+    const long step = (long)gridDim.x * TEAMS;
+    if (row < a.rows) x.load((const T *)a.x + row * a.ldx, t, a.cols);
+    for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += step, row += step) {  // (all teams take part in the barriers)
+        float v[E];
+        x.get(v);
+        if (row + step < a.rows) x.load((const T *)a.x + (row + step) * a.ldx, t, a.cols);
+        const float r = centre<V, TEAM, E>(v, t, a.cols, a.epsilon, slots, turn);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = v[e] * r * w[e] + b[e];
+        if (row < a.rows) H::store((T *)a.out + row * a.ldout, t, a.cols, v);
+    }
+}
+
+// Threads of a gradient workgroup: as many as hold what they need in registers (single precision with 16 elements a thread: half).
+constexpr int grad_threads(int team, int bytes) { return team == 1024 || bytes <= 32 ? 1024 : 512; }
+
+template <class T, int V, int TEAM, int E>
+__global__ __launch_bounds__(grad_threads(TEAM, E * sizeof(T))) void layer_norm_grad_kernel(NormArgs a) {
+    constexpr int THREADS = grad_threads(TEAM, E * sizeof(T)), TEAMS = THREADS / TEAM;
+    constexpr bool AHEAD = E * sizeof(T) <= 32;  // the next row's loads on their way
+    __shared__ float2 slots[2 * 16];
+    __shared__ float sums[TEAMS > 1 ? THREADS : 1];
+    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    typedef Held<T, V, TEAM, E> H;
+    H w, x, dy;
+    if (a.weight) w.load((const T *)a.weight, t, a.cols);
+    float dw[E], db[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
+    int turn = 0;
+    const float n = 1.f / a.cols;
+    long row = (long)blockIdx.x * TEAMS + team;
+    const long step = (long)gridDim.x * TEAMS;
+    auto fetch = [&](long at) {
+        if (at < a.rows) x.load((const T *)a.x + at * a.ldx, t, a.cols), dy.load((const T *)a.dy + at * a.lddy, t, a.cols);
+    };
+    fetch(row);
+    for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += step, row += step) {  // (all teams take part in the barriers)
+        float u[E], g[E];
+        x.get(u), dy.get(g);
+        if (AHEAD) fetch(row + step);
+        const float r = centre<V, TEAM, E>(u, t, a.cols, a.epsilon, slots, turn);
+        float wg[E], s0 = 0.f, s1 = 0.f;
+        if (a.weight) w.get(wg);
+        const bool mine = row < a.rows;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            u[e] *= r;
+            if (mine) dw[e] += g[e] * u[e], db[e] += g[e];
+            wg[e] = a.weight ? wg[e] * g[e] : g[e];
+            s0 += wg[e], s1 += wg[e] * u[e];
+        }
+        team_sum<TEAM>(s0, s1, slots, turn);
+        s0 *= n, s1 *= n;
+#pragma unroll
+        for (int e = 0; e < E; ++e) u[e] = r * (wg[e] - s0 - u[e] * s1);
+        if (mine && a.out) {
+            T *to = (T *)a.out + row * a.ldout;
+            if (!(a.overwrite & 1)) {
+                H old;
+                old.load(to, t, a.cols);
+                old.get(wg);
+#pragma unroll
+                for (int e = 0; e < E; ++e) u[e] += wg[e];
+            }
+            H::store(to, t, a.cols, u);
+        }
+        if (!AHEAD) fetch(row + step);
+    }
+    if (!a.partial) return;  // uniform over the workgroup
+    float *to = a.partial + (long)blockIdx.x * 2 * a.cols;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int c = (t + TEAM * (e / V)) * V + e % V;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float s = k ? db[e] : dw[e];
+            if constexpr (TEAMS > 1) {
+                __syncthreads();
+                sums[threadIdx.x] = s;
+                __syncthreads();
+                s = 0.f;
+                if (team == 0)
+                    for (int i = 0; i < TEAMS; ++i) s += sums[i * TEAM + t];
+            }
+            if (team == 0 && c < a.cols) to[(long)k * a.cols + c] = s;
+        }
+    }
+}
+
+// ---- rows that no team holds: a workgroup a row, read as often as it takes ------------------------------------------
+template <class T>
+__device__ __forceinline__ void long_row(const T *x, int cols, float epsilon, float2 *slots, int &turn, float &mean, float &off, float &r) {
+    float sum = 0.f, rest = 0.f;
+    for (int c = threadIdx.x; c < cols; c += 1024) sum += (float)x[c];
+    team_sum<1024>(sum, rest, slots, turn);
+    mean = sum / cols;
+    float squares = 0.f;
+    off = 0.f;
+    for (int c = threadIdx.x; c < cols; c += 1024) {
+        const float v = (float)x[c] - mean;
+        off += v, squares += v * v;
+    }
+    team_sum<1024>(off, squares, slots, turn);
+    off /= cols;  // (kept beside the mean, whose last bit may be as large)
+    r = 1.f / sqrtf(fmaxf(squares / cols - off * off, 0.f) + epsilon);
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void layer_norm_long_kernel(NormArgs a) {
+    __shared__ float2 slots[2 * 16];
+    int turn = 0;
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = (const T *)a.x + row * a.ldx;
+        T *y = (T *)a.out + row * a.ldout;
+        float mean, off, r;
+        long_row<T>(x, a.cols, a.epsilon, slots, turn, mean, off, r);
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float w = a.weight ? (float)((const T *)a.weight)[c] : 1.f, b = a.bias ? (float)((const T *)a.bias)[c] : 0.f;
+            y[c] = (T)(((float)x[c] - mean - off) * r * w + b);
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(NormArgs a) {
+    __shared__ float2 slots[2 * 16];
+    int turn = 0;
+    float *to = a.partial ? a.partial + (long)blockIdx.x * 2 * a.cols : nullptr;
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = (const T *)a.x + row * a.ldx, *dy = (const T *)a.dy + row * a.lddy, *w = (const T *)a.weight;
+        T *dx = a.out ? (T *)a.out + row * a.ldout : nullptr;
+        float mean, off, r, s0 = 0.f, s1 = 0.f;
+        long_row<T>(x, a.cols, a.epsilon, slots, turn, mean, off, r);
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float u = ((float)x[c] - mean - off) * r, g = (float)dy[c], wg = w ? (float)w[c] * g : g;
+            s0 += wg, s1 += wg * u;
+            if (to) {  // (a column's sums belong to one thread, whichever row it is at)
+                const bool fresh = row == blockIdx.x;
+                to[c] = (fresh ? 0.f : to[c]) + g * u;
+                to[a.cols + c] = (fresh ? 0.f : to[a.cols + c]) + g;
+            }
+        }
+        team_sum<1024>(s0, s1, slots, turn);
+        s0 /= a.cols, s1 /= a.cols;
+        if (!dx) continue;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float u = ((float)x[c] - mean - off) * r, g = (float)dy[c], wg = w ? (float)w[c] * g : g;
+            const float d = r * (wg - s0 - u * s1);
+            dx[c] = (T)(a.overwrite & 1 ? d : d + (float)dx[c]);
+        }
+    }
+}
+
+// 64 of the columns of dw (blockIdx.y 0) or db: each of 16 waves adds every 16th workgroup's sums, then the waves' are added in order
+template <class T>
+__global__ __launch_bounds__(1024) void layer_norm_sums_kernel(NormArgs a) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, k = blockIdx.y;
+    T *to = (T *)(k ? a.dbias : a.dweight);
+    if (!to) return;
+    float s = 0.f;
+    if (c < a.cols) {
+        const float *from = a.partial + (long)k * a.cols + c;
+#pragma unroll 8
+        for (int g = wave; g < a.groups; g += 16) s += from[(long)g * 2 * a.cols];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave || c >= a.cols) return;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += sums[i][lane];
+    to[c] = (T)(a.overwrite & 2 ? s : s + (float)to[c]);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+// fn<V, TEAM, E> for the smallest team that holds a row; rows that do not start at multiples of 16 bytes go element by element
+template <class T, class F>
+void with_team(bool vec, int cols, F &&fn) {
+    constexpr int V = 16 / sizeof(T);
+#define D8_TEAM(V_, TEAM_, E_) fn(std::integral_constant<int, V_>(), std::integral_constant<int, TEAM_>(), std::integral_constant<int, E_>())
+    if (!vec) {
+        if (cols <= 1024) D8_TEAM(1, 64, 16);
+        else if (cols <= 4096) D8_TEAM(1, 256, 16);
+        else D8_TEAM(1, 1024, 16);
+    } else if (cols <= 512) D8_TEAM(V, 64, 8);
+    else if (cols <= 1024) D8_TEAM(V, 64, 16);
+    else if (cols <= 2048) D8_TEAM(V, 256, 8);
+    else if (cols <= 4096) D8_TEAM(V, 256, 16);
+    else if (cols <= 8192) D8_TEAM(V, 1024, 8);
+    else D8_TEAM(V, 1024, 16);
+#undef D8_TEAM
+}
+
+bool in_pieces(const NormArgs &a, int dtype) {
+    const int v = 16 / (int)dtype_bytes(dtype);
+    const size_t all = (size_t)a.x | (size_t)a.dy | (size_t)a.weight | (size_t)a.bias | (size_t)a.out;
+    return (all & 15) == 0 && a.cols % v == 0 && a.ldx % v == 0 && a.lddy % v == 0 && a.ldout % v == 0;
+}
+
+int check(const NormArgs &a, int dtype, bool grad) {
+    const char *name = grad ? "layer_norm_grad" : "layer_norm";
+    if (dtype != D8_FLOAT16 && dtype != D8_FLOAT32) return fail(D8_ERR_DTYPE, "%s: type %d is not support", name, dtype);
+    D8_REQUIRE(a.rows >= 0 && a.cols >= 1 && a.cols < (1 << 30), "%s: %d rows of %d", name, a.rows, a.cols);
+    D8_REQUIRE(a.epsilon >= 0.f, "%s: epsilon %g", name, (double)a.epsilon);
+    if (!a.rows) return 0;
+    D8_REQUIRE(a.x && (grad ? a.dy != nullptr : a.out != nullptr), "%s: null tensor", name);
+    D8_REQUIRE(a.ldx >= a.cols && (!a.out || a.ldout >= a.cols) && (!grad || a.lddy >= a.cols), "%s: rows of %d elements do not fit their leading dimension", name, a.cols);
+    return 0;
+}
+
+template <class T>
+void launch_forward(const NormArgs &a, bool vec, hipStream_t stream) {
+    if (a.cols > MOST_HELD) {
+        hipLaunchKernelGGL(layer_norm_long_kernel<T>, dim3(a.rows < 4096 ? a.rows : 4096), dim3(1024), 0, stream, a);
+        return;
+    }
+    with_team<T>(vec, a.cols, [&](auto v, auto team, auto e) {
+        constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = forward_threads(TEAM);
+        // four rounds of the chip's waves at most: a team that goes down several rows reads weight and bias once
+        const long want = ((long)a.rows * TEAM + THREADS - 1) / THREADS, most = 2048L / THREADS * cu_count();
+        hipLaunchKernelGGL((layer_norm_kernel<T, V, TEAM, E>), dim3((unsigned)(want < most ? want : most)), dim3(THREADS), 0, stream, a);
+    });
+}
+
+template <class T>
+void launch_grad(NormArgs &a, bool vec, hipStream_t stream) {
+    if (a.cols > MOST_HELD) {
+        a.groups = a.rows < cu_count() ? a.rows : cu_count();
+        hipLaunchKernelGGL(layer_norm_grad_long_kernel<T>, dim3(a.groups), dim3(1024), 0, stream, a);
+        return;
+    }
+    with_team<T>(vec, a.cols, [&](auto v, auto team, auto e) {
+        constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = grad_threads(TEAM, E * sizeof(T));
+        const long want = ((long)a.rows * TEAM + THREADS - 1) / THREADS, most = 1024L / THREADS * cu_count();
+        a.groups = (int)(want < most ? want : most);
+        hipLaunchKernelGGL((layer_norm_grad_kernel<T, V, TEAM, E>), dim3((unsigned)a.groups), dim3(THREADS), 0, stream, a);
+    });
+}
+
+}  // namespace
+}  // namespace d8
+
+using namespace d8;
+
+extern "C" int d8_layer_norm(int dtype, const void *x, long ldx, const void *weight, const void *bias, void *y, long ldy, int rows, int cols, float epsilon,
+                             void *stream) {
+    NormArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x = x, a.ldx = ldx, a.weight = weight, a.bias = bias, a.out = y, a.ldout = ldy, a.rows = rows, a.cols = cols, a.epsilon = epsilon;
+    if (int rc = check(a, dtype, false)) return rc;
+    if (!rows) return 0;
+    if (dtype == D8_FLOAT16) launch_forward<f16>(a, in_pieces(a, dtype), as_stream(stream));
+    else launch_forward<float>(a, in_pieces(a, dtype), as_stream(stream));
+    D8_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" size_t d8_layer_norm_grad_scratch_bytes(int dtype, int rows, int cols) {
+    if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || rows < 0 || cols < 1 || cols >= (1 << 30)) return 0;
+    const int groups = rows < 2 * cu_count() ? rows : 2 * cu_count();
+    return sizeof(float) * 2 * (size_t)(groups ? groups : 1) * cols;
+}
+
+extern "C" int d8_layer_norm_grad(int dtype, const void *x, long ldx, const void *weight, const void *dy, long lddy, void *dx, long lddx, void *dweight,
+                                  void *dbias, int rows, int cols, float epsilon, int overwrite, void *scratch, size_t scratch_bytes, void *stream) {
+    NormArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x = x, a.ldx = ldx, a.weight = weight, a.dy = dy, a.lddy = lddy, a.out = dx, a.ldout = dx ? lddx : 0, a.dweight = dweight, a.dbias = dbias;
+    a.rows = rows, a.cols = cols, a.epsilon = epsilon, a.overwrite = overwrite;
+    if (int rc = check(a, dtype, true)) return rc;
+    const bool sums = dweight || dbias;
+    if (sums) {
+        const size_t need = d8_layer_norm_grad_scratch_bytes(dtype, rows, cols);
+        D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "layer_norm_grad: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
+        a.partial = (float *)scratch;
+    }
+    if (rows && (sums || dx)) {
+        if (dtype == D8_FLOAT16) launch_grad<f16>(a, in_pieces(a, dtype), as_stream(stream));
+        else launch_grad<float>(a, in_pieces(a, dtype), as_stream(stream));
+        D8_LAUNCH_CHECK();
+    }
+    if (sums) {  // (without a row the sums are zero)
+        const dim3 grid(ceil_div(cols, 64), 2);
+        if (dtype == D8_FLOAT16) hipLaunchKernelGGL(layer_norm_sums_kernel<f16>, grid, dim3(1024), 0, as_stream(stream), a);
+        else hipLaunchKernelGGL(layer_norm_sums_kernel<float>, grid, dim3(1024), 0, as_stream(stream), a);
+        D8_LAUNCH_CHECK();
+    }
+    return 0;
+}

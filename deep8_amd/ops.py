@@ -764,3 +764,31 @@ def matmul_gated_grad(x, w, pre, dh, act="silu", into=None):
     ws = _scratch(nb)
     check(lib.d8_matmul_gated_grad(dt, xi.ptr, dx_.ptr, rows, inner, wi.ptr, dw_.ptr, cols, GATES[act], pi.ptr, gi.ptr, 0 if into else 3, ws.ptr, nb, None))
     return dx_.numpy(), dw_.numpy()
+
+
+# ---- norm of a layer's rows ------------------------------------------------------------------------------------------
+def layer_norm(x, weight=None, bias=None, epsilon=1e-5, pad=0, in_place=False, stream=None):
+    """normed rows of x (rows, cols)"""
+    lib = capi.init()
+    dt = capi.dtype_id(x.dtype)
+    xi, (w, b) = _Rows(x, pad), _side(x, weight, bias)
+    y = xi if in_place else _Rows(np.zeros_like(x), pad)
+    check(lib.d8_layer_norm(dt, *xi.args, w and w.ptr, b and b.ptr, *y.args, *x.shape, epsilon, stream))
+    capi.sync(stream)
+    return y.numpy()
+
+
+def layer_norm_grad(x, dy, weight=None, epsilon=1e-5, pad=0, into=None, wanted=(True, True, True), stream=None):
+    """(dx, dweight, dbias), added to `into` (the three) if given; None where not wanted"""
+    lib = capi.init()
+    dt = _same_dtype(x, dy)
+    (rows, cols), (w,) = x.shape, _side(x, weight)
+    old = into or (np.full_like(x, np.nan), np.full(cols, np.nan), np.full(cols, np.nan))
+    xi, g, dx = _Rows(x, pad), _Rows(dy, pad), _Rows(old[0], pad) if wanted[0] else None
+    dw, db = (d if want else None for d, want in zip(_side(x, *old[1:]), wanted[1:]))
+    nb = lib.d8_layer_norm_grad_scratch_bytes(dt, rows, cols)
+    ws = _scratch(nb)
+    check(lib.d8_layer_norm_grad(dt, *xi.args, w and w.ptr, *g.args, *(dx.args if dx else (None, 0)), dw and dw.ptr, db and db.ptr, rows, cols, epsilon,
+                                 0 if into else 3, ws.ptr, nb, stream))
+    capi.sync(stream)
+    return tuple(d and d.numpy() for d in (dx, dw, db))

@@ -515,6 +515,22 @@ int d8_matmul_gated(int dtype, const void *x, int rows, int inner, const void *w
 int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner, const void *w, void *dw, int cols, int act,
                          const void *pre, const void *dh, int overwrite, void *scratch, size_t scratch_bytes, void *stream);
 
+/* ---- a transformer layer: the norm of its rows, and what it takes to serve it in 8 bits ---------------------
+ * No counterpart in the reference.  Float16 and Float32 (of x, q, k, v and results; sums, statistics and scales are fp32).
+ *
+ * d8_layer_norm          each row x of `cols` elements becomes (x - m) / sqrt(mean((x - m)^2) + epsilon) * weight + bias, m = mean(x) (weight, bias:
+ *                        cols elements, or NULL for ones and zeros).  Rows lie ldx and ldy elements apart; y may be x.
+ * d8_layer_norm_grad     from x and the gradient of y (dy) those of x (bit 0 of overwrite; NULL: not wanted) and of weight and bias (bit 1; NULL: not
+ *                        wanted); gradients are added to what their destination holds unless their bit of `overwrite` is set.  dx may be dy or x.
+ *                        The same bits every time.  scratch: d8_layer_norm_grad_scratch_bytes, 16-byte aligned; none if neither weight's nor bias'
+ *                        gradient is wanted.
+ */
+int d8_layer_norm(int dtype, const void *x, long ldx, const void *weight, const void *bias, void *y, long ldy, int rows, int cols, float epsilon,
+                  void *stream);
+size_t d8_layer_norm_grad_scratch_bytes(int dtype, int rows, int cols);
+int d8_layer_norm_grad(int dtype, const void *x, long ldx, const void *weight, const void *dy, long lddy, void *dx, long lddx, void *dweight,
+                       void *dbias, int rows, int cols, float epsilon, int overwrite, void *scratch, size_t scratch_bytes, void *stream);
+
 /* ---- measurement aid (no counterpart in the reference) ---------------------------------------
  * d8_mfma_stream issues the GEMM kernels' MFMA instruction for `dtype` (D8_FLOAT16, D8_FLOAT32 or
  * D8_FLOAT64) back to back on operands taken from `operands` (any device buffer; 16-byte aligned)
