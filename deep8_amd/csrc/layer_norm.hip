@@ -20,7 +20,8 @@
 namespace d8 {
 namespace {
 
-enum { MOST_HELD = 16384 };  // elements of a row that a team holds
+// Elements of a row that a team holds (16 a thread of 1024 do not leave the gradient enough registers in single precision).
+constexpr int most_held(bool vec, int bytes) { return vec && bytes == 2 ? 16384 : 8192; }
 
 struct NormArgs {
     const void *x, *dy, *weight, *bias;
@@ -55,16 +56,22 @@ struct Held {
             else raw[i] = vec{};
         }
     }
+    __device__ __forceinline__ void ones() {
+#pragma unroll
+        for (int i = 0; i < P; ++i) raw[i] = vec{} + (T)1;
+    }
+    __device__ __forceinline__ float at(int e) const {
+        if constexpr (V == 1) return (float)raw[e];
+        else return (float)raw[e / V][e % V];
+    }
     __device__ __forceinline__ void get(float (&v)[E]) const {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            if constexpr (V == 1) {
-                v[i] = (float)raw[i];
-            } else {
+        for (int e = 0; e < E; ++e) v[e] = at(e);
+    }
+    // the same values, but not to the compiler: what it made of them before is not kept
+    __device__ __forceinline__ void renew() {
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[i * V + e] = (float)raw[i][e];
-            }
-        }
+        for (int i = 0; i < P; ++i) asm volatile("" : "+v"(raw[i]));
     }
     static __device__ __forceinline__ void store(T *row, int t, int cols, const float (&v)[E]) {
 #pragma unroll
@@ -157,19 +164,21 @@ __global__ __launch_bounds__(forward_threads(TEAM)) void layer_norm_kernel(NormA
     }
 }
 
-// Threads of a gradient workgroup: as many as hold what they need in registers (single precision with 16 elements a thread: half).
-constexpr int grad_threads(int team, int bytes) { return team == 1024 || bytes <= 32 ? 1024 : 512; }
+// Threads of a gradient workgroup: 1024 where what a thread keeps (its columns' sums, weights, this row's and the next one's elements) fits in
+// the 128 registers that leaves it, else 512.
+constexpr int grad_threads(int team, int v, int bytes) { return team == 1024 || (v > 1 && bytes <= 32) ? 1024 : 512; }
 
 template <class T, int V, int TEAM, int E>
-__global__ __launch_bounds__(grad_threads(TEAM, E * sizeof(T))) void layer_norm_grad_kernel(NormArgs a) {
-    constexpr int THREADS = grad_threads(TEAM, E * sizeof(T)), TEAMS = THREADS / TEAM;
-    constexpr bool AHEAD = E * sizeof(T) <= 32;  // the next row's loads on their way
+__global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T))) void layer_norm_grad_kernel(NormArgs a) {
+    constexpr int THREADS = grad_threads(TEAM, V, E * sizeof(T)), TEAMS = THREADS / TEAM;
+    constexpr bool AHEAD = TEAM < 1024 || E == 8;  // the next row's loads on their way
     __shared__ float2 slots[2 * 16];
     __shared__ float sums[TEAMS > 1 ? THREADS : 1];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     typedef Held<T, V, TEAM, E> H;
     H w, x, dy;
     if (a.weight) w.load((const T *)a.weight, t, a.cols);
+    else w.ones();
     float dw[E], db[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
@@ -182,32 +191,39 @@ __global__ __launch_bounds__(grad_threads(TEAM, E * sizeof(T))) void layer_norm_
     };
     fetch(row);
     for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += step, row += step) {  // (all teams take part in the barriers)
-        float u[E], g[E];
-        x.get(u), dy.get(g);
+        float u[E], s0 = 0.f, s1 = 0.f;
+        H g = dy;
+        x.get(u);
         if (AHEAD) fetch(row + step);
         const float r = centre<V, TEAM, E>(u, t, a.cols, a.epsilon, slots, turn);
-        float wg[E], s0 = 0.f, s1 = 0.f;
-        if (a.weight) w.get(wg);
-        const bool mine = row < a.rows;
+        const bool mine = __builtin_amdgcn_readfirstlane(row < a.rows);  // (a team is whole waves)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
+            const float ge = g.at(e), wg = w.at(e) * ge;
             u[e] *= r;
-            if (mine) dw[e] += g[e] * u[e], db[e] += g[e];
-            wg[e] = a.weight ? wg[e] * g[e] : g[e];
-            s0 += wg[e], s1 += wg[e] * u[e];
+            s0 += wg, s1 += wg * u[e];
+            if (V > 1 && e % V == V - 1) asm volatile("" : "+v"(s0), "+v"(s1));  // piece by piece: one at a time is held in fp32
+        }
+        // (w and dy as they were loaded, converted again for each use: kept as fp32 they would take the registers of the next row)
+        g.renew(), w.renew();
+        if (mine) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) dw[e] += g.at(e) * u[e], db[e] += g.at(e);
+            g.renew();
         }
         team_sum<TEAM>(s0, s1, slots, turn);
         s0 *= n, s1 *= n;
 #pragma unroll
-        for (int e = 0; e < E; ++e) u[e] = r * (wg[e] - s0 - u[e] * s1);
+        for (int e = 0; e < E; ++e) {
+            u[e] = r * (w.at(e) * g.at(e) - s0 - u[e] * s1);
+            if (V > 1 && e % V == V - 1) asm volatile("" : "+v"(s0), "+v"(s1));
+        }
         if (mine && a.out) {
             T *to = (T *)a.out + row * a.ldout;
             if (!(a.overwrite & 1)) {
-                H old;
-                old.load(to, t, a.cols);
-                old.get(wg);
+                g.load(to, t, a.cols);
 #pragma unroll
-                for (int e = 0; e < E; ++e) u[e] += wg[e];
+                for (int e = 0; e < E; ++e) u[e] += g.at(e);
             }
             H::store(to, t, a.cols, u);
         }
@@ -329,13 +345,13 @@ void with_team(bool vec, int cols, F &&fn) {
     if (!vec) {
         if (cols <= 1024) D8_TEAM(1, 64, 16);
         else if (cols <= 4096) D8_TEAM(1, 256, 16);
-        else D8_TEAM(1, 1024, 16);
+        else D8_TEAM(1, 1024, 8);
     } else if (cols <= 512) D8_TEAM(V, 64, 8);
     else if (cols <= 1024) D8_TEAM(V, 64, 16);
     else if (cols <= 2048) D8_TEAM(V, 256, 8);
     else if (cols <= 4096) D8_TEAM(V, 256, 16);
     else if (cols <= 8192) D8_TEAM(V, 1024, 8);
-    else D8_TEAM(V, 1024, 16);
+    else if constexpr (sizeof(T) == 2) D8_TEAM(V, 1024, 16);
 #undef D8_TEAM
 }
 
@@ -358,7 +374,7 @@ int check(const NormArgs &a, int dtype, bool grad) {
 
 template <class T>
 void launch_forward(const NormArgs &a, bool vec, hipStream_t stream) {
-    if (a.cols > MOST_HELD) {
+    if (a.cols > most_held(vec, sizeof(T))) {
         hipLaunchKernelGGL(layer_norm_long_kernel<T>, dim3(a.rows < 4096 ? a.rows : 4096), dim3(1024), 0, stream, a);
         return;
     }
@@ -372,13 +388,13 @@ void launch_forward(const NormArgs &a, bool vec, hipStream_t stream) {
 
 template <class T>
 void launch_grad(NormArgs &a, bool vec, hipStream_t stream) {
-    if (a.cols > MOST_HELD) {
+    if (a.cols > most_held(vec, sizeof(T))) {
         a.groups = a.rows < cu_count() ? a.rows : cu_count();
         hipLaunchKernelGGL(layer_norm_grad_long_kernel<T>, dim3(a.groups), dim3(1024), 0, stream, a);
         return;
     }
     with_team<T>(vec, a.cols, [&](auto v, auto team, auto e) {
-        constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = grad_threads(TEAM, E * sizeof(T));
+        constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = grad_threads(TEAM, V, E * sizeof(T));
         const long want = ((long)a.rows * TEAM + THREADS - 1) / THREADS, most = 1024L / THREADS * cu_count();
         a.groups = (int)(want < most ? want : most);
         hipLaunchKernelGGL((layer_norm_grad_kernel<T, V, TEAM, E>), dim3((unsigned)a.groups), dim3(THREADS), 0, stream, a);
