@@ -133,6 +133,11 @@ SIGNATURES = {
     "d8_layer_norm": (_I, [_I, _P, _L, _P, _P, _P, _L, _I, _I, _F, _P]),
     "d8_layer_norm_grad_scratch_bytes": (_Z, [_I] * 3),
     "d8_layer_norm_grad": (_I, [_I, _P, _L, _P, _P, _L, _P, _L, _P, _P, _I, _I, _F, _I, _P, _Z, _P]),
+    "d8_int8_pitch": (_I, [_I]),
+    "d8_quantize_rows": (_I, [_I, _P, _L, _I, _I, _P, _P, _P]),
+    "d8_quantize_columns": (_I, [_I, _P, _L, _I, _I, _P, _P, _P]),
+    "d8_matmul_int8_scratch_bytes": (_Z, [_I] * 3),
+    "d8_matmul_int8": (_I, [_I, _P, _P, _I, _I, _P, _P, _I, _P, _L, _P, _Z, _P]),
     "d8_gemm_phase_record": (_I, [_P, _Z]),
     "d8_mfma_stream_out_bytes": (_Z, []),
     "d8_mfma_stream": (_I, [_I, _P, _Z, _P, _I, ctypes.POINTER(ctypes.c_double), _P]),

@@ -192,10 +192,13 @@ struct Operand {
 // with both operands changing every time.  (Each block still sums its k values in the same order.)
 #define WIDE_BI(m) ((m) >> 3)
 #define WIDE_BJ(m) ((((m) >> 3) & 1) ? 7 - ((m) & 7) : ((m) & 7))
+// (a policy whose operands are something else in the same bytes has its own: matmul_int8_wide.hip)
+template <class Policy>
 __device__ __forceinline__ void mfma(f32x4 &acc, const f16x8 &a, const f16x8 &b) {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 // a tile's first MFMA into a block: the sum starts at zero (no pass over the accumulators to clear them)
+template <class Policy>
 __device__ __forceinline__ void mfma_first(f32x4 &acc, const f16x8 &a, const f16x8 &b) {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=a"(acc) : "v"(a), "v"(b));
 }
@@ -304,8 +307,8 @@ __device__ __forceinline__ void k_loop(const TileOperands<A_KC, B_KC> &T, char *
         // half 0
 #pragma unroll
         for (int m = 0; m < 64; ++m) {
-            if constexpr (first) mfma_first(acc[WIDE_BI(m)][WIDE_BJ(m)], fa[0][WIDE_BI(m)], fb[0][WIDE_BJ(m)]);
-            else mfma(acc[WIDE_BI(m)][WIDE_BJ(m)], fa[0][WIDE_BI(m)], fb[0][WIDE_BJ(m)]);
+            if constexpr (first) mfma_first<Policy>(acc[WIDE_BI(m)][WIDE_BJ(m)], fa[0][WIDE_BI(m)], fb[0][WIDE_BJ(m)]);
+            else mfma<Policy>(acc[WIDE_BI(m)][WIDE_BJ(m)], fa[0][WIDE_BI(m)], fb[0][WIDE_BJ(m)]);
             if constexpr (Policy::FRAGMENT_READS) {
                 if (m % 3 == 0 && m < 48) {
                     const int e = m / 3;  // 16 reads: the B fragments first (all needed by the first row)
@@ -325,7 +328,7 @@ __device__ __forceinline__ void k_loop(const TileOperands<A_KC, B_KC> &T, char *
                     else ob.template aim_round<cur * STAGE_BYTES + OPERAND_BYTES, (m >> 2) - 8>(wave_base);
                 }
             }
-            mfma(acc[WIDE_BI(m)][WIDE_BJ(m)], fa[1][WIDE_BI(m)], fb[1][WIDE_BJ(m)]);
+            mfma<Policy>(acc[WIDE_BI(m)][WIDE_BJ(m)], fa[1][WIDE_BI(m)], fb[1][WIDE_BJ(m)]);
             if constexpr (Policy::LOADS) {
                 if constexpr ((m & 3) == 0) {
                     // 16 loads into the stage every wave has finished with, one per 4 MFMAs: a load

@@ -1,0 +1,259 @@
+// z = (x w) times a scale of each row of x and one of each column of w, x and w in 8-bit integers: sums in int32 are exact, in whatever order
+// they are added, so a reduction can be cut into parts freely.
+//
+// Three ways, by size:
+//   few rows (64 at most)      bound by memory, the weight: no LDS on its way, a wave reads 16 codes a lane straight into the operand
+//                              of v_mfma_i32_16x16x64_i8 (32 columns of w as left operand, all rows of x as right one); eight waves
+//                              share out the steps of the reduction and join through LDS
+//   many rows and columns      matmul_int8_wide.hip
+//   between                    tiles of 128 x 128 or 64 x 64 through LDS, cut along the reduction where they leave compute units idle
+// In all three w is the left operand, so a lane ends up with four columns of a row side by side.
+#include "int8.h"
+
+namespace d8 {
+namespace int8 {
+namespace {
+
+__device__ __forceinline__ void mma(i32x4 &acc, const i32x4 &a, const i32x4 &b) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc, 0, 0, 0); }
+
+// four sums of row m, columns n .. n + 3: scaled into z, or as they are into part number `part`
+template <class T>
+__device__ __forceinline__ void put(const Args &a, int part, int m, int n, const i32x4 &sum) {
+    if (m >= a.rows || n >= a.cols) return;
+    if (a.parts > 1) {  // (rows of parts are whole pieces)
+        *(i32x4 *)(a.part + ((long)part * a.rows + m) * a.part_ld + n) = sum;
+        return;
+    }
+    T *z = (T *)a.z + (long)m * a.ldz + n;
+    const float s = a.x_scales[m];
+    if (a.vec && n + 4 <= a.cols) {
+        typedef T quad __attribute__((ext_vector_type(4)));
+        quad out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = scaled<T>(sum[e], s, a.w_scales[n + e]);
+        *(quad *)z = out;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < a.cols) z[e] = scaled<T>(sum[e], s, a.w_scales[n + e]);
+    }
+}
+
+// the parts' sums of four columns of a row
+template <class T>
+__global__ __launch_bounds__(256) void int8_join_kernel(Args a) {
+    const long quads = (a.cols + 3) / 4, i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= quads * a.rows) return;
+    const int m = (int)(i / quads), n = (int)(i - m * quads) * 4;
+    i32x4 sum = {0, 0, 0, 0};
+    for (int p = 0; p < a.parts; ++p) sum += *(const i32x4 *)(a.part + ((long)p * a.rows + m) * a.part_ld + n);
+    a.parts = 1;
+    put<T>(a, 0, m, n, sum);
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------------
+enum { ROWS_WAVES = 8, ROWS_COLS = 32 };
+
+// RT tiles of 16 rows
+template <class T, int RT>
+__global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
+    __shared__ i32x4 sums[ROWS_WAVES][2 * RT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int blocks = (a.cols + ROWS_COLS - 1) / ROWS_COLS, part = blockIdx.x / blocks, n0 = (blockIdx.x - part * blocks) * ROWS_COLS;
+    const int first = (int)((long)a.steps * part / a.parts), end = (int)((long)a.steps * (part + 1) / a.parts);
+    // a lane's 16 bytes of a step of 128: columns (rows) lane % 16 of each tile, bytes 16 (lane / 16) .. of both halves.  Beyond the last
+    // column or row the last one is read again; what comes of it is not stored.
+    const int r = lane & 15, at = (lane >> 4) * 16;
+    const signed char *w[2], *x[RT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = a.w + (long)min(n0 + 16 * i + r, a.cols - 1) * a.pitch + at;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) x[j] = a.x + (long)min(16 * j + r, a.rows - 1) * a.pitch + at;
+    i32x4 acc[2][RT] = {};
+#pragma unroll 4
+    for (int s = first + wave; s < end; s += ROWS_WAVES) {
+        const long k = (long)s * STEP;
+        i32x4 fw[2][2], fx[RT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) fw[i][h] = *(const i32x4 *)(w[i] + k + 64 * h);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) fx[j][h] = *(const i32x4 *)(x[j] + k + 64 * h);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) mma(acc[i][j], fw[i][h], fx[j][h]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) sums[wave][i * RT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int q = wave; q < 2 * RT; q += ROWS_WAVES) {
+        i32x4 sum = sums[0][q][lane];
+#pragma unroll
+        for (int k = 1; k < ROWS_WAVES; ++k) sum += sums[k][q][lane];
+        put<T>(a, part, 16 * (q % RT) + r, n0 + 16 * (q / RT) + (lane >> 4) * 4, sum);
+    }
+}
+
+// ---- tiles ----------------------------------------------------------------------------------------------------------
+// B x B of z a workgroup, four waves of B / 2 x B / 2.  Two stages of LDS; a step of the reduction is fetched into registers while the one before is computed.
+// Rows of 128 bytes, 16-byte piece c of row r at position c ^ (r / 2 % 8): the 16 rows of a fragment then take all banks in turn.
+template <class T, int B>
+__global__ __launch_bounds__(256) void int8_tile_kernel(Args a) {
+    constexpr int F = B / 32, PIECES = B * STEP / 16 / 256;
+    __shared__ __attribute__((aligned(16))) signed char lds[2][2][B * STEP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+    const int tilesM = (a.rows + B - 1) / B, tilesN = (a.cols + B - 1) / B;
+    int id = blockIdx.x;
+    const int part = id / (tilesM * tilesN);
+    id -= part * tilesM * tilesN;
+    const int m0 = id % tilesM * B, n0 = id / tilesM * B;
+    const int first = (int)((long)a.steps * part / a.parts), end = (int)((long)a.steps * (part + 1) / a.parts);
+    const signed char *from[2][PIECES];
+    int to[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int p = tid + 256 * i, row = p >> 3, c = p & 7;
+        from[0][i] = a.w + (long)min(n0 + row, a.cols - 1) * a.pitch + c * 16;  // (rows beyond the last: it again, not stored)
+        from[1][i] = a.x + (long)min(m0 + row, a.rows - 1) * a.pitch + c * 16;
+        to[i] = row * STEP + ((c ^ (row >> 1 & 7)) << 4);
+    }
+    i32x4 ahead[2][PIECES], acc[F][F] = {};
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) ahead[o][i] = *(const i32x4 *)(from[o][i] + (long)s * STEP);
+    };
+    auto stage = [&](int at) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) *(i32x4 *)(lds[at][o] + to[i]) = ahead[o][i];
+    };
+    const int r = lane & 15, j = lane >> 4, sw = r >> 1 & 7;
+    if (first < end) {
+        fetch(first);
+        stage(0);
+        if (first + 1 < end) fetch(first + 1);
+        __syncthreads();
+        for (int s = first, at = 0; s < end; ++s, at ^= 1) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                i32x4 fw[F], fx[F];
+                const int c = ((j + 4 * h) ^ sw) << 4;
+#pragma unroll
+                for (int i = 0; i < F; ++i) {
+                    fw[i] = *(const i32x4 *)(lds[at][0] + (wn * (B / 2) + 16 * i + r) * STEP + c);
+                    fx[i] = *(const i32x4 *)(lds[at][1] + (wm * (B / 2) + 16 * i + r) * STEP + c);
+                }
+#pragma unroll
+                for (int i = 0; i < F; ++i)
+#pragma unroll
+                    for (int k = 0; k < F; ++k) mma(acc[i][k], fw[i], fx[k]);
+            }
+            if (s + 1 < end) stage(at ^ 1);
+            if (s + 2 < end) fetch(s + 2);
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int k = 0; k < F; ++k) put<T>(a, part, m0 + wm * (B / 2) + 16 * k + r, n0 + wn * (B / 2) + 16 * i + j * 4, acc[i][k]);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+enum { FEW_ROWS = 64 };
+
+// How a call runs.
+struct Plan {
+    enum { ROWS, TILES } way;
+    int tile, parts;
+    long part_ld;
+    size_t bytes(int rows) const { return parts > 1 ? sizeof(int) * (size_t)parts * rows * part_ld : 0; }
+};
+
+Plan plan_of(int rows, int inner, int cols) {
+    Plan p;
+    const long steps = pitch_of(inner) / STEP, cus = cu_count();
+    p.part_ld = (cols + 3L) / 4 * 4;
+    p.tile = 0;
+    long groups, most;
+    if (rows <= FEW_ROWS) {
+        p.way = Plan::ROWS;
+        groups = ceil_div(cols, ROWS_COLS), most = steps / (2 * ROWS_WAVES);
+    } else {
+        p.way = Plan::TILES;
+        const long big = (long)ceil_div(rows, 128) * ceil_div(cols, 128);
+        p.tile = big >= cus ? 128 : 64;
+        groups = (long)ceil_div(rows, p.tile) * ceil_div(cols, p.tile), most = steps / 4;
+    }
+    long parts = groups >= cus ? 1 : (2 * cus) / groups;
+    parts = parts > most ? most : parts;
+    p.parts = (int)(parts < 1 ? 1 : parts);
+    return p;
+}
+
+template <class T>
+int launch(Args a, const Plan &p, hipStream_t stream) {
+    a.parts = p.parts, a.part_ld = p.part_ld;
+    a.vec = a.ldz % 4 == 0 && ((size_t)a.z & (4 * sizeof(T) - 1)) == 0;
+    if (p.way == Plan::ROWS) {
+        const dim3 grid((unsigned)(ceil_div(a.cols, ROWS_COLS) * (long)p.parts)), threads(ROWS_WAVES * 64);
+        if (a.rows <= 16) hipLaunchKernelGGL((int8_rows_kernel<T, 1>), grid, threads, 0, stream, a);
+        else if (a.rows <= 32) hipLaunchKernelGGL((int8_rows_kernel<T, 2>), grid, threads, 0, stream, a);
+        else hipLaunchKernelGGL((int8_rows_kernel<T, 4>), grid, threads, 0, stream, a);
+    } else {
+        const dim3 grid((unsigned)((long)ceil_div(a.rows, p.tile) * ceil_div(a.cols, p.tile) * p.parts));
+        if (p.tile == 128) hipLaunchKernelGGL((int8_tile_kernel<T, 128>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((int8_tile_kernel<T, 64>), grid, dim3(256), 0, stream, a);
+    }
+    D8_LAUNCH_CHECK();
+    if (p.parts > 1) {
+        hipLaunchKernelGGL(int8_join_kernel<T>, dim3(ceil_div((long)a.rows * ((a.cols + 3) / 4), 256)), dim3(256), 0, stream, a);
+        D8_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+bool sizes(int rows, int inner, int cols) { return rows >= 0 && inner >= 1 && inner <= MOST_INNER && cols >= 0 && (long)rows * ceil_div(cols, 4) < (1L << 37); }
+
+}  // namespace
+}  // namespace int8
+}  // namespace d8
+
+using namespace d8;
+
+extern "C" size_t d8_matmul_int8_scratch_bytes(int rows, int inner, int cols) {
+    if (!int8::sizes(rows, inner, cols) || !rows || !cols) return 0;
+    return int8::plan_of(rows, inner, cols).bytes(rows);
+}
+
+extern "C" int d8_matmul_int8(int dtype, const signed char *x, const float *x_scales, int rows, int inner, const signed char *w, const float *w_scales, int cols,
+                              void *z, long ldz, void *scratch, size_t scratch_bytes, void *stream) {
+    if (dtype != D8_FLOAT16 && dtype != D8_FLOAT32) return fail(D8_ERR_DTYPE, "matmul_int8: type %d is not support", dtype);
+    D8_REQUIRE(rows >= 0 && inner >= 1 && cols >= 0, "matmul_int8: %d x %d times %d x %d", rows, inner, inner, cols);
+    D8_REQUIRE(inner <= int8::MOST_INNER, "matmul_int8: a sum has at most %d terms, not %d", (int)int8::MOST_INNER, inner);
+    if (!rows || !cols) return 0;
+    D8_REQUIRE(int8::sizes(rows, inner, cols), "matmul_int8: a result of %d x %d is too large", rows, cols);
+    D8_REQUIRE(x && x_scales && w && w_scales && z, "matmul_int8: null tensor");
+    D8_REQUIRE(ldz >= cols, "matmul_int8: rows of %d elements do not fit their leading dimension", cols);
+    D8_REQUIRE((((size_t)x | (size_t)w) & 15) == 0, "matmul_int8: codes must be 16-byte aligned");
+    int8::Args a;
+    memset(&a, 0, sizeof(a));
+    a.x = x, a.w = w, a.x_scales = x_scales, a.w_scales = w_scales, a.z = z, a.ldz = ldz, a.rows = rows, a.cols = cols, a.parts = 1;
+    a.pitch = int8::pitch_of(inner), a.steps = (int)(a.pitch / int8::STEP);
+    if (int8::wide_eligible(a)) return dtype == D8_FLOAT16 ? int8::wide_launch<f16>(a, as_stream(stream)) : int8::wide_launch<float>(a, as_stream(stream));
+    const int8::Plan p = int8::plan_of(rows, inner, cols);
+    const size_t need = p.bytes(rows);
+    D8_REQUIRE(!need || (scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0), "matmul_int8: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
+    a.part = (int *)scratch;
+    return dtype == D8_FLOAT16 ? int8::launch<f16>(a, p, as_stream(stream)) : int8::launch<float>(a, p, as_stream(stream));
+}

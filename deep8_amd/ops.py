@@ -792,3 +792,41 @@ def layer_norm_grad(x, dy, weight=None, epsilon=1e-5, pad=0, into=None, wanted=(
                                  0 if into else 3, ws.ptr, nb, stream))
     capi.sync(stream)
     return tuple(d and d.numpy() for d in (dx, dw, db))
+
+
+# ---- products in 8-bit integers --------------------------------------------------------------------------------------
+def quantize_rows(x, pad=0, stream=None):
+    """(codes (rows, pitch) int8, scales (rows,)) of x (rows, cols)"""
+    lib = capi.init()
+    xi, (rows, cols) = _Rows(x, pad), x.shape
+    codes = DeviceArray.from_numpy(np.full((rows, lib.d8_int8_pitch(cols)), 85, np.int8))
+    scales = DeviceArray.from_numpy(np.full(rows, np.nan, np.float32))
+    check(lib.d8_quantize_rows(capi.dtype_id(x.dtype), *xi.args, rows, cols, codes.ptr, scales.ptr, stream))
+    capi.sync(stream)
+    return codes.numpy(), scales.numpy()
+
+
+def quantize_columns(w, pad=0, stream=None):
+    """(codes (cols, pitch) int8, scales (cols,)) of w (rows, cols)"""
+    lib = capi.init()
+    wi, (rows, cols) = _Rows(w, pad), w.shape
+    codes = DeviceArray.from_numpy(np.full((cols, lib.d8_int8_pitch(rows)), 85, np.int8))
+    scales = DeviceArray.from_numpy(np.full(cols, np.nan, np.float32))
+    check(lib.d8_quantize_columns(capi.dtype_id(w.dtype), *wi.args, rows, cols, codes.ptr, scales.ptr, stream))
+    capi.sync(stream)
+    return codes.numpy(), scales.numpy()
+
+
+def matmul_int8(x, x_scales, w, w_scales, inner, dtype=np.float32, pad=0, stream=None):
+    """(rows, cols) from codes x (rows, pitch) and w (cols, pitch) with their scales"""
+    lib = capi.init()
+    (rows, pitch), cols = x.shape, w.shape[0]
+    if pitch != lib.d8_int8_pitch(inner) or w.shape[1] != pitch:
+        raise capi.Deep8HipError("rows of %d codes take %d bytes, not %d and %d" % (inner, lib.d8_int8_pitch(inner), pitch, w.shape[1]))
+    d = [DeviceArray.from_numpy(a) for a in (x, np.asarray(x_scales, np.float32), w, np.asarray(w_scales, np.float32))]
+    z = _Rows(np.full((rows, cols), np.nan, dtype), pad)
+    nb = lib.d8_matmul_int8_scratch_bytes(rows, inner, cols)
+    ws = _scratch(nb)
+    check(lib.d8_matmul_int8(capi.dtype_id(dtype), d[0].ptr, d[1].ptr, rows, inner, d[2].ptr, d[3].ptr, cols, *z.args, ws.ptr, nb, stream))
+    capi.sync(stream)
+    return z.numpy()

@@ -524,12 +524,28 @@ int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner
  *                        wanted); gradients are added to what their destination holds unless their bit of `overwrite` is set.  dx may be dy or x.
  *                        The same bits every time.  scratch: d8_layer_norm_grad_scratch_bytes, 16-byte aligned; none if neither weight's nor bias'
  *                        gradient is wanted.
+ *
+ * Products in 8-bit integers.  A matrix of codes has its reduction axis along memory: a row of x, or a column of w, takes d8_int8_pitch(inner) bytes
+ * (`inner` rounded up to 128), codes of -128 to 127 and behind them zeros, which take part in the sums.  16-byte aligned.  inner <= 131071.
+ * d8_quantize_rows       each row of x (cols elements, ldx apart): scale = max |x| / 127 (in fp32; at least 2^-100), codes x / scale rounded to the nearest
+ *                        whole number, halves to the even one, from the exact quotient.  A row with NaN or an infinity: scale NaN, codes 0.
+ * d8_quantize_columns    the same for each column of w [rows][cols] (rows ldw apart), whose codes become a row: for weights, laid out once.
+ * d8_matmul_int8         z[i][j] = x_scales[i] w_scales[j] sum over k of x[i][k] w[j][k], rows of z ldz apart: x (rows) and w (cols) as above, sums exact,
+ *                        scaled in fp32, rounded once to the element type.
+ *     scratch: d8_matmul_int8_scratch_bytes, 16-byte aligned.
  */
 int d8_layer_norm(int dtype, const void *x, long ldx, const void *weight, const void *bias, void *y, long ldy, int rows, int cols, float epsilon,
                   void *stream);
 size_t d8_layer_norm_grad_scratch_bytes(int dtype, int rows, int cols);
 int d8_layer_norm_grad(int dtype, const void *x, long ldx, const void *weight, const void *dy, long lddy, void *dx, long lddx, void *dweight,
                        void *dbias, int rows, int cols, float epsilon, int overwrite, void *scratch, size_t scratch_bytes, void *stream);
+
+int d8_int8_pitch(int inner);
+int d8_quantize_rows(int dtype, const void *x, long ldx, int rows, int cols, signed char *codes, float *scales, void *stream);
+int d8_quantize_columns(int dtype, const void *w, long ldw, int rows, int cols, signed char *codes, float *scales, void *stream);
+size_t d8_matmul_int8_scratch_bytes(int rows, int inner, int cols);
+int d8_matmul_int8(int dtype, const signed char *x, const float *x_scales, int rows, int inner, const signed char *w, const float *w_scales, int cols,
+                   void *z, long ldz, void *scratch, size_t scratch_bytes, void *stream);
 
 /* ---- measurement aid (no counterpart in the reference) ---------------------------------------
  * d8_mfma_stream issues the GEMM kernels' MFMA instruction for `dtype` (D8_FLOAT16, D8_FLOAT32 or
