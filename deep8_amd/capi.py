@@ -14,6 +14,7 @@ FLOAT16 = 10
 FLOAT32 = 11
 FLOAT64 = 12
 STATIC_SCRATCH_BYTES = 32 << 20  # D8_STATIC_SCRATCH_BYTES of include/deep8_hip.h
+CACHE_PAGE = 64  # D8_CACHE_PAGE
 
 c_int, c_long, c_size_t, c_float, c_void_p = (ctypes.c_int, ctypes.c_long, ctypes.c_size_t, ctypes.c_float,
                                               ctypes.c_void_p)
@@ -138,6 +139,10 @@ SIGNATURES = {
     "d8_quantize_columns": (_I, [_I, _P, _L, _I, _I, _P, _P, _P]),
     "d8_matmul_int8_scratch_bytes": (_Z, [_I] * 3),
     "d8_matmul_int8": (_I, [_I, _P, _P, _I, _I, _P, _P, _I, _P, _L, _P, _Z, _P]),
+    "d8_cache_append": (_I, [_I] + [_P, _L] * 2 + [_P] * 7 + [_I] * 6 + [_P]),
+    "d8_cache_read": (_I, [_I] + [_P, _L] * 2 + [_P] * 7 + [_I] * 6 + [_P]),
+    "d8_attention_cache_scratch_bytes": (_Z, [_I] * 7),
+    "d8_attention_cache": (_I, [_I, _P, _L] + [_P] * 4 + [_P, _L, _P] + [_P] * 3 + [_I] * 7 + [_F, _I, _P, _Z, _P]),
     "d8_gemm_phase_record": (_I, [_P, _Z]),
     "d8_mfma_stream_out_bytes": (_Z, []),
     "d8_mfma_stream": (_I, [_I, _P, _Z, _P, _I, ctypes.POINTER(ctypes.c_double), _P]),

@@ -1,0 +1,588 @@
+// Attention over a cache in 8-bit pages (cache.h).
+//
+//   o = softmax(scale q k^T) v,  k = codes * k_scale,  v = codes * v_scale;  the pages' scales go into the scores and the sums, not into the codes:
+//   s = (q . codes) (k_scale scale),  o = sum over pages of v_scale (p . codes)
+//
+// Rows.  The queries of all heads that share keys are one matrix, row r of a sequence query r / group of the kv head's head r % group.
+//
+// Products.  Both are formed transposed (keys x rows, elements x rows) with 16 x 16 accumulators: lane l has row l % 16, and with it its
+// maximum, sum and limit; the probabilities are the next product's right operand where they are.  A lane (r = l % 16, g = l / 16) of tile t of a
+// page's keys holds 16 bytes of key 16 (r / 4) + 4 t + r % 4, so that after the product lane group g has keys 16 g .. 16 g + 15 in order: the 16 bytes of
+// values [element][token] that a lane reads are then the matching left operand.  So codes go from memory to registers in 16-byte pieces, without LDS,
+// and are converted there: half in pairs, by putting the byte (its sign bit flipped) below the bits of 1024 and taking off 1024 + 128.
+//
+// Two kernels' worth of work in one: few rows (KEYS: a workgroup has 16 rows, its four waves share out the pages and join through LDS) and many
+// (ROWS: each wave has 32 rows of its own, and all four read the same pages, which the first to ask brings into the L1 cache).
+//
+// All tiles' pages, one after the other, are cut into as many equal runs as workgroups run at once, whatever sequences have how many: a workgroup
+// goes through its run and leaves, for a tile that it has not all of, sums in scratch, which a second launch joins.  Cuts are found from the
+// lengths on the device, so a call can be captured and replayed as sequences grow.
+//
+// Bound by memory where there are few rows (a page and head is 16 KB at 128 elements), by conversions and exponentials where there are many.
+//
+// Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product; every page's product starts from zero
+// and is scaled into the accumulators, so a page's scale costs nothing of another's.
+#include "cache.h"
+
+namespace d8 {
+namespace cache {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+enum { WAVES = 4 };
+
+struct AttArgs {
+    Pages c;
+    const void *q;
+    void *o;
+    float *lse;   // [heads][tokens]
+    float *part;  // [slots][kv_heads][rows of a tile][dim], then maximum and sum [slots][kv_heads][rows of a tile][2]
+    float *part_ml;
+    long ldq, ldo;
+    int heads, group, causal, vec;
+    int runs;  // workgroups of a kv head
+    float scale;
+};
+
+// One sequence: its queries' rows, how many tokens it has (`len`, which places the queries) and keys (those that the table has room for).
+struct Seq {
+    int q0, n;
+    long len;
+    int keys;
+    long tiles, pages;  // tiles of rows, pages that each goes through (1 where there is none: a result of nothing is written too)
+    __device__ __forceinline__ long cost() const { return tiles * pages; }
+};
+
+// the lane's sequence of the 64 from `first` on; top: the largest start so far (starts as in cache.hip)
+template <int R>
+__device__ __forceinline__ Seq seqs_from(const AttArgs &a, int first, int &top) {
+    const Pages &c = a.c;
+    const int lane = threadIdx.x & 63, at = min(first + lane, c.sequences), next = min(first + lane + 1, c.sequences);
+    int q0 = min(max(c.starts[at], 0), c.tokens), q1 = min(max(c.starts[next], 0), c.tokens);
+    if (__ballot(q0 < top || q1 < q0)) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int q = __shfl_up(q0, d);
+            q0 = lane >= d ? max(q0, q) : q0;
+        }
+        q0 = max(q0, top), q1 = max(q1, q0);
+    }
+    top = __builtin_amdgcn_readlane(q1, 63);
+    Seq s;
+    s.q0 = q0, s.n = q1 - q0, s.len = at < c.sequences ? max(c.lengths[at], 0) : 0;
+    s.keys = (int)min(s.len, (long)c.table_pages * PAGE);
+    s.tiles = s.n ? ((long)s.n * a.group + R - 1) / R : 0, s.pages = s.keys ? (s.keys + PAGE - 1) / PAGE : 1;
+    return s;
+}
+
+__device__ __forceinline__ long upto(long x) {  // sum over the lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long y = __shfl_up(x, d);
+        x += (threadIdx.x & 63) >= d ? y : 0;
+    }
+    return x;
+}
+__device__ __forceinline__ long from_lane(long x, int lane) { return __shfl(x, lane); }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) {
+    return (long)(((unsigned long)(unsigned)uniform((int)(x >> 32)) << 32) | (unsigned)uniform((int)x));
+}
+
+template <int R>
+__device__ __forceinline__ long total_cost(const AttArgs &a) {
+    long total = 0;
+    int top = 0;
+    for (int first = 0; first < a.c.sequences; first += 64) total += from_lane(upto(seqs_from<R>(a, first, top).cost()), 63);
+    return uniform(total);
+}
+
+// The sequence that holds item `at` of a list in which a sequence has count(seq) items; its items and tiles before it in `base` and `tile_base`.
+template <int R, class Count>
+__device__ __forceinline__ bool locate(const AttArgs &a, long at, Seq &seq, int &s, long &base, long &tile_base, long &cost_base, Count &&count) {
+    long before = 0, tiles = 0, costs = 0;
+    int top = 0;
+    for (int first = 0; first < a.c.sequences; first += 64) {
+        const Seq own = seqs_from<R>(a, first, top);
+        const long n = count(own), sum = upto(n), tsum = upto(own.tiles), csum = upto(own.cost());
+        const unsigned long long past = __ballot(before + sum > at);
+        if (past) {
+            const int l = __ffsll((long long)past) - 1;
+            s = uniform(first + l);
+            base = uniform(before + from_lane(sum - n, l)), tile_base = uniform(tiles + from_lane(tsum - own.tiles, l));
+            cost_base = uniform(costs + from_lane(csum - own.cost(), l));
+            seq.q0 = uniform(__shfl(own.q0, l)), seq.n = uniform(__shfl(own.n, l)), seq.len = uniform(from_lane(own.len, l)), seq.keys = uniform(__shfl(own.keys, l));
+            seq.tiles = uniform(from_lane(own.tiles, l)), seq.pages = uniform(from_lane(own.pages, l));
+            return true;
+        }
+        before += from_lane(sum, 63), tiles += from_lane(tsum, 63), costs += from_lane(csum, 63);
+    }
+    return false;
+}
+
+// How long the runs of a call are: equal, and four pages a wave at least, less being not worth a join.
+__device__ __forceinline__ long run_of(long total, int runs) {
+    const long even = (total + runs - 1) / runs;
+    return even < 4 * WAVES ? 4 * WAVES : even;
+}
+
+// ---- operands -------------------------------------------------------------------------------------------------------
+template <class T, int NC>
+struct Operands;
+
+// 16 codes as halves, exactly
+__device__ __forceinline__ void to_halves(const i32x4 &codes, f16x8 (&out)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        f16x2 p[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const unsigned w = (unsigned)codes[2 * i + e] ^ 0x80808080u;
+            const f16x2 off = {(f16)1152.f, (f16)1152.f};
+            p[2 * e] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - off;
+            p[2 * e + 1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off;
+        }
+        out[i] = __builtin_shufflevector(__builtin_shufflevector(p[0], p[1], 0, 1, 2, 3), __builtin_shufflevector(p[2], p[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+template <int NC>
+struct Operands<f16, NC> {
+    struct Query {
+        f16x8 f[NC * 2];
+        __device__ __forceinline__ void set(int i, float x) { f[i >> 3][i & 7] = (f16)x; }
+    };
+    struct Weights {
+        f16x8 f[2];
+        __device__ __forceinline__ void set(int i, float x) { f[i >> 3][i & 7] = (f16)x; }
+    };
+    struct Codes {
+        f16x8 f[2];
+        __device__ __forceinline__ void set(const i32x4 &codes) { to_halves(codes, f); }
+    };
+    static __device__ __forceinline__ void scores(f32x4 &acc, const Codes &k, const Query &q, int chunk) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.f[0], q.f[2 * chunk], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.f[1], q.f[2 * chunk + 1], acc, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void sums(f32x4 &acc, const Codes &v, const Weights &p) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.f[0], p.f[0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.f[1], p.f[1], acc, 0, 0, 0);
+    }
+};
+
+template <int NC>
+struct Operands<float, NC> {
+    struct Query {
+        float f[NC * 16];
+        __device__ __forceinline__ void set(int i, float x) { f[i] = x; }
+    };
+    struct Weights {
+        float f[16];
+        __device__ __forceinline__ void set(int i, float x) { f[i] = x; }
+    };
+    struct Codes {
+        i32x4 w;
+        __device__ __forceinline__ void set(const i32x4 &codes) { w = codes; }
+        __device__ __forceinline__ float at(int i) const { return (float)(signed char)(w[i >> 2] >> (8 * (i & 3))); }
+    };
+    static __device__ __forceinline__ void scores(f32x4 &acc, const Codes &k, const Query &q, int chunk) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k.at(i), q.f[chunk * 16 + i], acc, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void sums(f32x4 &acc, const Codes &v, const Weights &p) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(v.at(i), p.f[i], acc, 0, 0, 0);
+    }
+};
+
+// ---- one wave over some pages ---------------------------------------------------------------------------------------
+// RT tiles of 16 rows; NC: chunks of 64 elements of a head.
+template <class T, int NC, int RT>
+struct Wave {
+    typedef Operands<T, NC> Op;
+    typename Op::Query q[RT];
+    f32x4 o[RT][NC * 4];
+    float m[RT], sum[RT];  // of scores times log2 e; the lane's part of the sum
+    int limit[RT];         // keys that the lane's row sees
+    i32x4 kr[4][NC], vr[NC * 4];
+
+    // rows row0 .. of the sequence (those beyond `rows` are zero and see nothing)
+    __device__ __forceinline__ void begin(const AttArgs &a, const Seq &s, int head, long row0, long rows) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            const long row = row0 + 16 * j + r;
+            const bool there = row < rows;
+            const int t = there ? (int)(row / a.group) : 0, h = there ? (int)(row - (long)t * a.group) : 0;
+            const long sees = a.causal ? t + s.len - s.n + 1 : s.len;
+            limit[j] = there ? (int)min(max(sees, 0L), (long)s.keys) : 0;
+            const T *from = (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * a.group + h) * a.c.dim;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = c * 64 + g * 16;
+                constexpr int V = 16 / sizeof(T);
+                typedef T piece __attribute__((ext_vector_type(V)));
+#pragma unroll
+                for (int i = 0; i < 16; i += V) {
+                    if (a.vec && there && d + i < a.c.dim) {  // (dim is whole pieces)
+                        const piece p = *(const piece *)(from + d + i);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) q[j].set(c * 16 + i + e, (float)p[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) q[j].set(c * 16 + i + e, !a.vec && there && d + i + e < a.c.dim ? (float)from[d + i + e] : 0.f);
+                    }
+                }
+            }
+            m[j] = -INFINITY, sum[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NC * 4; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    __device__ __forceinline__ void fetch_keys(const Pages &c, int page, int head) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const signed char *from = c.k_codes + c.tile(page, head);
+        const int key = (r >> 2) * 16 + (r & 3);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int d = n * 64 + g * 16, at = d < c.pitch ? d : 0;  // (beyond the head: any codes, times zeros of q)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) kr[t][n] = *(const i32x4 *)(from + (key + 4 * t) * c.pitch + at);
+        }
+    }
+    __device__ __forceinline__ void fetch_values(const Pages &c, int page, int head) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const signed char *from = c.v_codes + c.tile(page, head) + r * PAGE + g * 16;
+#pragma unroll
+        for (int i = 0; i < NC * 4; ++i)
+            if (i * 16 < c.pitch) vr[i] = *(const i32x4 *)(from + i * 16 * PAGE);
+    }
+
+    // pages first, first + step, ... below `end` of sequence s
+    __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int end, int step) {
+        const Pages &c = a.c;
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        // (rows see more the later their queries are: the first row sees least, the last that is there most)
+        int most = 0;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) most = max(most, limit[j]);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor(most, d));
+        end = min(end, uniform((most + PAGE - 1) / PAGE));
+        const int least = uniform(limit[0]);
+        if (first >= end) return;
+        const int count = (end - first + step - 1) / step;
+        // 64 pages at a time: lane i has page, and scales, of number i
+        int ids = 0, there = 0;
+        float ks = 0.f, vs = 0.f;
+        auto list = [&](int from) {
+            const int i = from + lane, p = i < count ? c.page_of(s, first + i * step) : -1;
+            there = p >= 0, ids = max(p, 0);
+            ks = vs = 0.f;
+            if (p >= 0) ks = c.k_scales[(long)p * c.kv_heads + head], vs = c.v_scales[(long)p * c.kv_heads + head];
+        };
+        list(0);
+        int id = __builtin_amdgcn_readlane(ids, 0);
+        fetch_keys(c, id, head);
+        fetch_values(c, id, head);
+        const float by = a.scale * LOG2E;
+        for (int n = 0; n < count; ++n) {
+            const int l = n & 63, at = (first + n * step) * PAGE;
+            const bool page_there = __builtin_amdgcn_readlane(there, l) != 0;
+            const float k_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), l)) * by;
+            const float v_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), l));
+            const bool more = n + 1 < count;
+            if (more && ((n + 1) & 63) == 0) list(n + 1);
+            const int next = __builtin_amdgcn_readlane(ids, (n + 1) & 63);
+            f32x4 sc[RT][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int j = 0; j < RT; ++j) sc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    typename Op::Codes k;
+                    k.set(kr[t][i]);
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) Op::scores(sc[j][t], k, q[j], i);
+                }
+            }
+            if (more) fetch_keys(c, next, head);
+            typename Op::Weights p[RT];
+            float into[RT];  // what the page's sums are scaled by: 0 where the lane's row sees none of it
+            const bool hidden = !page_there || at + PAGE > least;
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                float x[16], top = m[j];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    x[i] = sc[j][i >> 2][i & 3] * k_scale;
+                    if (hidden) x[i] = page_there && at + g * 16 + i < limit[j] ? x[i] : -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float base = top == -INFINITY ? 0.f : top;
+                if (__ballot(top != m[j])) {
+                    const float less = __builtin_amdgcn_exp2f(m[j] - base);
+                    sum[j] *= less;
+#pragma unroll
+                    for (int i = 0; i < NC * 4; ++i) o[j][i] *= less;
+                    m[j] = top;
+                }
+                float add = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float w = __builtin_amdgcn_exp2f(x[i] - base);
+                    add += w;
+                    p[j].set(i, w);
+                }
+                sum[j] += add;
+                into[j] = hidden && !(page_there && at < limit[j]) ? 0.f : v_scale;
+            }
+#pragma unroll
+            for (int i = 0; i < NC * 4; ++i) {
+                if (i * 16 >= c.pitch) continue;
+                typename Op::Codes v;
+                v.set(vr[i]);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                    Op::sums(acc, v, p[j]);
+                    o[j][i] += acc * into[j];
+                }
+            }
+            if (more) fetch_values(c, next, head);
+        }
+    }
+};
+
+// A lane's four elements 4 g .. of a tile of 16 of row `row`'s result, divided by the sum.
+template <class T>
+__device__ __forceinline__ void put(const AttArgs &a, T *to, int d, const f32x4 &x, float by) {
+    if (d + 4 <= a.c.dim && a.vec) {
+        typedef T quad __attribute__((ext_vector_type(4)));
+        quad v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(x[e] * by);
+        *(quad *)(to + d) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < a.c.dim) to[d + e] = (T)(x[e] * by);
+    }
+}
+
+template <class T, int NC, int RT, bool ROWS>
+__global__ __launch_bounds__(WAVES * 64) void attention_cache_kernel(AttArgs a) {
+    constexpr int R = 16 * RT * (ROWS ? WAVES : 1);  // rows of a tile
+    __shared__ f32x4 others[ROWS ? 1 : WAVES][ROWS ? 1 : NC * 4][64];
+    __shared__ float2 stats[ROWS ? 1 : WAVES][16];
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), r = lane & 15, g = lane >> 4;
+    const int head = blockIdx.x % a.c.kv_heads, run = blockIdx.x / a.c.kv_heads;
+    const long total = total_cost<R>(a), length = run_of(total, a.runs);
+    const long last = min((run + 1) * length, total);
+    long at = run * length;
+    Wave<T, NC, RT> w;
+    while (at < last) {
+        Seq seq;
+        int s;
+        long base, tile_base, cost_base;
+        if (!locate<R>(a, at, seq, s, base, tile_base, cost_base, [](const Seq &x) { return x.cost(); })) return;
+        const long after = base + seq.cost();
+        while (at < last && at < after) {
+            const long tile = (at - base) / seq.pages;
+            const int first = (int)(at - base - tile * seq.pages), end = (int)min(seq.pages, first + (last - at));
+            const bool whole = first == 0 && end == seq.pages;
+            const long rows = (long)seq.n * a.group, row0 = tile * R + (ROWS ? wave * 16 * RT : 0), slot = run + tile_base + tile;
+            w.begin(a, seq, head, row0, rows);
+            if (ROWS) w.pages(a, s, head, first, end, 1);
+            else w.pages(a, s, head, first + wave, end, WAVES);
+            at += end - first;
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                w.sum[j] += __shfl_xor(w.sum[j], 16);
+                w.sum[j] += __shfl_xor(w.sum[j], 32);
+            }
+            if constexpr (!ROWS) {  // (RT is 1)
+#pragma unroll
+                for (int i = 0; i < NC * 4; ++i) others[wave][i][lane] = w.o[0][i];
+                if (g == 0) stats[wave][r] = make_float2(w.m[0], w.sum[0]);
+                __syncthreads();
+                float top = -INFINITY, by[WAVES];
+#pragma unroll
+                for (int k = 0; k < WAVES; ++k) top = fmaxf(top, stats[k][r].x);
+                const float from = top == -INFINITY ? 0.f : top;
+                w.m[0] = top, w.sum[0] = 0.f;
+#pragma unroll
+                for (int k = 0; k < WAVES; ++k) {
+                    by[k] = __builtin_amdgcn_exp2f(stats[k][r].x - from);
+                    w.sum[0] += stats[k][r].y * by[k];
+                }
+#pragma unroll
+                for (int i = 0; i < NC * 4; ++i) {
+                    if (i % WAVES != wave) continue;
+                    w.o[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < WAVES; ++k) w.o[0][i] += others[k][i][lane] * by[k];
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                const long row = row0 + 16 * j + r;
+                if (row >= rows) continue;
+                if (whole) {
+                    const int t = (int)(row / a.group), h = head * a.group + (int)(row - (long)t * a.group);
+                    T *to = (T *)a.o + (seq.q0 + (long)t) * a.ldo + (long)h * a.c.dim;
+                    const float inv = w.sum[j] == 0.f ? 0.f : 1.f / w.sum[j];
+#pragma unroll
+                    for (int i = 0; i < NC * 4; ++i)
+                        if (ROWS || i % WAVES == wave) put<T>(a, to, i * 16 + g * 4, w.o[j][i], inv);
+                    if (a.lse && g == 0 && (ROWS || wave == 0)) a.lse[(long)h * a.c.tokens + seq.q0 + t] = w.sum[j] == 0.f ? -INFINITY : (w.m[j] + log2f(w.sum[j])) * LN2;
+                } else {
+                    const long place = (slot * a.c.kv_heads + head) * R + (row - tile * R);
+                    float *to = a.part + place * a.c.dim;
+#pragma unroll
+                    for (int i = 0; i < NC * 4; ++i)
+                        if (ROWS || i % WAVES == wave)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (i * 16 + g * 4 + e < a.c.dim) to[i * 16 + g * 4 + e] = w.o[j][i][e];
+                    if (g == 0 && (ROWS || wave == 0)) *(float2 *)(a.part_ml + place * 2) = make_float2(w.m[j], w.sum[j]);
+                }
+            }
+        }
+    }
+}
+
+// The runs' sums of a tile's rows joined: a wave a row.
+template <class T, int R>
+__global__ __launch_bounds__(256) void attention_cache_join_kernel(AttArgs a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x % a.c.kv_heads;
+    const long unit = blockIdx.x / a.c.kv_heads, total = total_cost<R>(a), length = run_of(total, a.runs);
+    Seq seq;
+    int s;
+    long base, tile_base, cost_base;
+    if (!locate<R>(a, unit, seq, s, base, tile_base, cost_base, [](const Seq &x) { return x.tiles; })) return;
+    const long tile = unit - base, from = cost_base + tile * seq.pages;
+    const int first = (int)(from / length), last = (int)((from + seq.pages - 1) / length);
+    if (first == last) return;
+    const long rows = (long)seq.n * a.group, n = min((long)R, rows - tile * R), step = (long)a.c.kv_heads * R;
+    for (int row = blockIdx.y * 4 + wave; row < n; row += gridDim.y * 4) {
+        const long place = ((first + unit) * a.c.kv_heads + head) * R + row;
+        const int parts = last - first + 1;
+        float top = -INFINITY, sum = 0.f;
+        for (int i = lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[(place + i * step) * 2]);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float at = top == -INFINITY ? 0.f : top;
+        for (int i = lane; i < parts; i += 64) sum += a.part_ml[(place + i * step) * 2 + 1] * __builtin_amdgcn_exp2f(a.part_ml[(place + i * step) * 2] - at);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        const long global = tile * R + row;
+        const int t = (int)(global / a.group), h = head * a.group + (int)(global - (long)t * a.group);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        for (int d = lane; d < a.c.dim; d += 64) {
+            float x = 0.f;
+#pragma unroll 4
+            for (int i = 0; i < parts; ++i) x += a.part[(place + i * step) * a.c.dim + d] * __builtin_amdgcn_exp2f(a.part_ml[(place + i * step) * 2] - at);
+            ((T *)a.o)[(seq.q0 + (long)t) * a.ldo + (long)h * a.c.dim + d] = (T)(x * inv);
+        }
+        if (lane == 0 && a.lse) a.lse[(long)h * a.c.tokens + seq.q0 + t] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+enum { KEYS_ROWS = 16, MANY_ROWS = 128 };
+
+// How a call runs: rows of a tile, runs of a kv head, tiles of all sequences at most, and slots of partial sums (a run's and a tile's numbers added: each
+// step from piece to piece of the list is to the next run or the next tile, so no two pieces share a slot).
+struct Plan {
+    bool rows;
+    int tile, runs;
+    long units, slots;
+};
+
+Plan plan_of(int dtype, int sequences, int tokens, int table_pages, int heads, int kv_heads, int dim) {
+    Plan p;
+    const long group = heads / kv_heads, all = (long)tokens * group, some = sequences < tokens ? sequences : tokens;
+    p.rows = dtype == D8_FLOAT16 && dim <= 128 && some && all / some >= 64;
+    p.tile = p.rows ? MANY_ROWS : KEYS_ROWS;
+    p.units = all / p.tile + some;
+    const long at_once = (2L * cu_count() + kv_heads - 1) / kv_heads, most = (p.units * (table_pages ? table_pages : 1) + 4 * WAVES - 1) / (4 * WAVES);
+    p.runs = (int)(at_once < most ? at_once : most);
+    p.slots = p.units + p.runs;
+    return p;
+}
+
+size_t scratch_of(const Plan &p, int kv_heads, int dim) { return sizeof(float) * (size_t)p.slots * kv_heads * p.tile * (dim + 2); }
+
+template <class T, int NC>
+void launch(const AttArgs &a, const Plan &p, hipStream_t stream) {
+    const dim3 grid((unsigned)(p.runs * a.c.kv_heads));
+    if constexpr (sizeof(T) == 2 && NC <= 2) {
+        if (p.rows) {
+            hipLaunchKernelGGL((attention_cache_kernel<T, NC, 2, true>), grid, dim3(WAVES * 64), 0, stream, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((attention_cache_kernel<T, NC, 1, false>), grid, dim3(WAVES * 64), 0, stream, a);
+}
+
+template <class T>
+int launch_all(const AttArgs &a, const Plan &p, hipStream_t stream) {
+    if (a.c.dim <= 64) launch<T, 1>(a, p, stream);
+    else if (a.c.dim <= 128) launch<T, 2>(a, p, stream);
+    else launch<T, 4>(a, p, stream);
+    D8_LAUNCH_CHECK();
+    const dim3 join((unsigned)(p.units * a.c.kv_heads), p.rows ? 8 : 4);
+    if (p.rows) hipLaunchKernelGGL((attention_cache_join_kernel<T, MANY_ROWS>), join, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attention_cache_join_kernel<T, KEYS_ROWS>), join, dim3(256), 0, stream, a);
+    D8_LAUNCH_CHECK();
+    return 0;
+}
+
+bool sizes(int dtype, int sequences, int tokens, int heads, int kv_heads, int dim) {
+    return (dtype == D8_FLOAT16 || dtype == D8_FLOAT32) && sequences >= 0 && sequences < (1 << 24) && tokens >= 0 && kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 &&
+           dim >= 1 && dim <= MOST_DIM && (long)tokens * heads < (1L << 30);
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace d8
+
+using namespace d8;
+
+extern "C" size_t d8_attention_cache_scratch_bytes(int dtype, int sequences, int q_tokens, int table_pages, int heads, int kv_heads, int dim) {
+    if (!cache::sizes(dtype, sequences, q_tokens, heads, kv_heads, dim) || !sequences || !q_tokens || table_pages < 0 || table_pages >= (1 << 24)) return 0;
+    return cache::scratch_of(cache::plan_of(dtype, sequences, q_tokens, table_pages, heads, kv_heads, dim), kv_heads, dim);
+}
+
+extern "C" int d8_attention_cache(int dtype, const void *q, long ldq, const signed char *k_codes, const float *k_scales, const signed char *v_codes,
+                                  const float *v_scales, void *o, long ldo, float *lse, const int *starts, const int *lengths, const int *table, int sequences,
+                                  int q_tokens, int table_pages, int pages, int heads, int kv_heads, int dim, float scale, int causal, void *scratch,
+                                  size_t scratch_bytes, void *stream) {
+    cache::AttArgs a;
+    memset(&a, 0, sizeof(a));
+    a.c = {(signed char *)k_codes, (signed char *)v_codes, (float *)k_scales, (float *)v_scales, starts, lengths, table, sequences, q_tokens, pages ? table_pages : 0, pages,
+           kv_heads, dim, (int)cache::pitch_of(dim)};
+    if (int rc = cache::check(a.c, dtype, "attention_cache")) return rc;
+    D8_REQUIRE(heads >= kv_heads && heads % kv_heads == 0, "attention_cache: %d heads cannot share the keys of %d", heads, kv_heads);
+    D8_REQUIRE(cache::sizes(dtype, sequences, q_tokens, heads, kv_heads, dim), "attention_cache: too many queries");
+    D8_REQUIRE(scale == scale, "attention_cache: the scale is no number");
+    if (!sequences || !q_tokens) return 0;
+    D8_REQUIRE(q && o, "attention_cache: null tensor");
+    D8_REQUIRE(ldq >= (long)heads * dim && ldo >= (long)heads * dim, "attention_cache: rows of %ld elements do not fit their leading dimensions", (long)heads * dim);
+    const cache::Plan p = cache::plan_of(dtype, sequences, q_tokens, table_pages, heads, kv_heads, dim);
+    const size_t need = cache::scratch_of(p, kv_heads, dim);
+    D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_cache: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
+    D8_REQUIRE(p.units * kv_heads < (1L << 31), "attention_cache: too many sequences");
+    const int v = 16 / (int)dtype_bytes(dtype);
+    a.q = q, a.ldq = ldq, a.o = o, a.ldo = ldo, a.lse = lse, a.heads = heads, a.group = heads / kv_heads, a.causal = causal != 0, a.scale = scale, a.runs = p.runs;
+    a.vec = dim % v == 0 && ldq % v == 0 && ldo % v == 0 && (((size_t)q | (size_t)o) & 15) == 0;
+    a.part = (float *)scratch, a.part_ml = a.part + (size_t)p.slots * kv_heads * p.tile * dim;
+    return dtype == D8_FLOAT16 ? cache::launch_all<f16>(a, p, as_stream(stream)) : cache::launch_all<float>(a, p, as_stream(stream));
+}

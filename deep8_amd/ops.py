@@ -830,3 +830,54 @@ def matmul_int8(x, x_scales, w, w_scales, inner, dtype=np.float32, pad=0, stream
     check(lib.d8_matmul_int8(capi.dtype_id(dtype), d[0].ptr, d[1].ptr, rows, inner, d[2].ptr, d[3].ptr, cols, *z.args, ws.ptr, nb, stream))
     capi.sync(stream)
     return z.numpy()
+
+
+# ---- a cache of keys and values in 8-bit pages -----------------------------------------------------------------------
+class PagedCache:
+    """pages of capi.CACHE_PAGE tokens on the device; tables (sequences, table_pages), lengths and starts are given with each call"""
+
+    def __init__(self, pages, kv_heads, dim, fill=0):
+        self.pages, self.kv_heads, self.dim, self.pitch = pages, kv_heads, dim, (dim + 15) // 16 * 16
+        n = capi.CACHE_PAGE
+        self.k_codes = DeviceArray.from_numpy(np.full((pages, kv_heads, n, self.pitch), fill, np.int8))
+        self.v_codes = DeviceArray.from_numpy(np.full((pages, kv_heads, self.pitch, n), fill, np.int8))
+        self.k_scales, self.v_scales = (DeviceArray.from_numpy(np.full((pages, kv_heads), np.nan, np.float32)) for _ in range(2))
+
+    def _state(self):
+        return self.k_codes.ptr, self.k_scales.ptr, self.v_codes.ptr, self.v_scales.ptr
+
+    def _where(self, starts, lengths, table, rows):
+        table = np.ascontiguousarray(table, np.int32)
+        held = _ints(starts), _ints(lengths), _ints(table)
+        return held, tuple(d.ptr for d in held) + (len(lengths), rows, table.shape[1], self.pages)
+
+    def append(self, k, v, starts, lengths, table, pad=0, stream=None):
+        """rows of k and v (tokens, kv_heads, dim) into the places that lengths, which count them, end with"""
+        lib = capi.init()
+        ki, vi = _Rows(k, pad), _Rows(v, pad)
+        held, where = self._where(starts, lengths, table, k.shape[0])
+        check(lib.d8_cache_append(_same_dtype(k, v), *ki.args, *vi.args, *self._state(), *where, self.kv_heads, self.dim, stream))
+        capi.sync(stream)
+
+    def read(self, rows, starts, lengths, table, dtype=np.float32, pad=0, into=None, stream=None):
+        """(k, v) of those places; into: what the two held before"""
+        lib = capi.init()
+        old = into or tuple(np.zeros((rows, self.kv_heads, self.dim), dtype) for _ in range(2))
+        ko, vo = (_Rows(a, pad) for a in old)
+        held, where = self._where(starts, lengths, table, rows)
+        check(lib.d8_cache_read(capi.dtype_id(old[0].dtype), *ko.args, *vo.args, *self._state(), *where, self.kv_heads, self.dim, stream))
+        capi.sync(stream)
+        return ko.numpy(), vo.numpy()
+
+    def attention(self, q, starts, lengths, table, scale, causal=True, pad=0, o=None, stream=None):
+        """(o, lse) of q (queries, heads, dim); o: what the output holds before"""
+        lib = capi.init()
+        dt, (rows, heads, dim) = capi.dtype_id(q.dtype), q.shape
+        qi, oo = _Rows(q, pad), _Rows(np.zeros_like(q) if o is None else o, pad)
+        lse = DeviceArray.from_numpy(np.full((heads, rows), np.nan, np.float32))
+        held, where = self._where(starts, lengths, table, rows)
+        nb = lib.d8_attention_cache_scratch_bytes(dt, where[3], rows, where[5], heads, self.kv_heads, dim)
+        ws = _scratch(nb)
+        check(lib.d8_attention_cache(dt, *qi.args, *self._state(), *oo.args, lse.ptr, *where, heads, self.kv_heads, dim, scale, int(causal), ws.ptr, nb, stream))
+        capi.sync(stream)
+        return oo.numpy(), lse.numpy()

@@ -533,7 +533,27 @@ int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner
  * d8_matmul_int8         z[i][j] = x_scales[i] w_scales[j] sum over k of x[i][k] w[j][k], rows of z ldz apart: x (rows) and w (cols) as above, sums exact,
  *                        scaled in fp32, rounded once to the element type.
  *     scratch: d8_matmul_int8_scratch_bytes, 16-byte aligned.
+ *
+ * A cache of keys and values in 8-bit integers, in pages of D8_CACHE_PAGE tokens with a scale for each page and key head.  With pitch = dim rounded up to 16:
+ * k_codes [pages][kv_heads][token][pitch], v_codes [pages][kv_heads][pitch][token], both 16-byte aligned, k_scales and v_scales [pages][kv_heads]; a code
+ * stands for code * scale.  Which pages a sequence has: table[sequences][table_pages], on the device; entry p is the page of its tokens 64 p ..
+ * 64 p + 63, one outside 0 .. pages - 1 is no page.  lengths[sequences], on the device: how many tokens a sequence has in the cache, those
+ * that the call brings among them; rows starts[s] .. starts[s + 1] - 1 of a call (starts as d8_attention's) are its last ones.  dim <= 256.
+ * d8_cache_append        rows of k and v (kv_heads heads each) into their places.  A page's scale is a power of two, at least 2^-100: the least of which 127
+ *                        reach the largest element since the page's first token was written.  Codes are exact quotients rounded to the nearest, halves
+ *                        to the even one; where new tokens raise the scale, codes that are there are rounded again in the same way.  NaN or an infinity makes
+ *                        its page and head's scale NaN, and so everything that is read from it, until its first token is written anew.  A token whose
+ *                        place is before the first or has no page is left out.  Two sequences must not bring tokens to one page in one call;
+ *                        full pages may be in any number of tables.
+ * d8_cache_read          the values of those places into rows of k and v, zeros for a token whose place is before the first or has no page.
+ * d8_attention_cache     o = softmax(scale q k^T) v over the values that such a cache holds, head i with the keys and values of head i / (heads / kv_heads);
+ *                        scales may be any numbers.  causal != 0: query t of a sequence's n sees the keys of its places up to t + length - n, so the
+ *                        last one sees them all; 0: every key.  Keys without a page are not seen.  lse[heads][q_tokens] (may be NULL) as
+ *                        d8_attention's; a query that sees nothing gets o = 0 and lse = -infinity; rows of no sequence are left alone.  The same call
+ *                        serves a prompt's next part, a step of decoding and attention to another sequence's states.  The same bits every time.
+ *     scratch: d8_attention_cache_scratch_bytes, 16-byte aligned.
  */
+#define D8_CACHE_PAGE 64
 int d8_layer_norm(int dtype, const void *x, long ldx, const void *weight, const void *bias, void *y, long ldy, int rows, int cols, float epsilon,
                   void *stream);
 size_t d8_layer_norm_grad_scratch_bytes(int dtype, int rows, int cols);
@@ -546,6 +566,19 @@ int d8_quantize_columns(int dtype, const void *w, long ldw, int rows, int cols, 
 size_t d8_matmul_int8_scratch_bytes(int rows, int inner, int cols);
 int d8_matmul_int8(int dtype, const signed char *x, const float *x_scales, int rows, int inner, const signed char *w, const float *w_scales, int cols,
                    void *z, long ldz, void *scratch, size_t scratch_bytes, void *stream);
+
+int d8_cache_append(int dtype, const void *k, long ldk, const void *v, long ldv, signed char *k_codes, float *k_scales, signed char *v_codes,
+                    float *v_scales, const int *starts, const int *lengths, const int *table, int sequences, int tokens, int table_pages, int pages,
+                    int kv_heads, int dim, void *stream);
+int d8_cache_read(int dtype, void *k, long ldk, void *v, long ldv, const signed char *k_codes, const float *k_scales, const signed char *v_codes,
+                  const float *v_scales, const int *starts, const int *lengths, const int *table, int sequences, int tokens, int table_pages, int pages,
+                  int kv_heads, int dim, void *stream);
+
+size_t d8_attention_cache_scratch_bytes(int dtype, int sequences, int q_tokens, int table_pages, int heads, int kv_heads, int dim);
+int d8_attention_cache(int dtype, const void *q, long ldq, const signed char *k_codes, const float *k_scales, const signed char *v_codes,
+                       const float *v_scales, void *o, long ldo, float *lse, const int *starts, const int *lengths, const int *table, int sequences,
+                       int q_tokens, int table_pages, int pages, int heads, int kv_heads, int dim, float scale, int causal, void *scratch,
+                       size_t scratch_bytes, void *stream);
 
 /* ---- measurement aid (no counterpart in the reference) ---------------------------------------
  * d8_mfma_stream issues the GEMM kernels' MFMA instruction for `dtype` (D8_FLOAT16, D8_FLOAT32 or
