@@ -31,15 +31,20 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum { WAVES = 4 };
 
+struct Join;
+
 struct AttArgs {
     Pages c;
     const void *q;
     void *o;
     float *lse;   // [heads][tokens]
-    float *part;  // [slots][kv_heads][rows of a tile][dim], then maximum and sum [slots][kv_heads][rows of a tile][2]
+    float *part;  // [slots][kv_heads][rows of a tile][part_ld], then maximum and sum [slots][kv_heads][rows of a tile][2]
     float *part_ml;
+    Join *joins;  // [units]
+    long units;
     long ldq, ldo;
     int heads, group, causal, vec;
+    int part_ld;  // elements of a row of partial sums: whole pieces of four
     int runs;  // workgroups of a kv head
     float scale;
 };
@@ -89,41 +94,59 @@ __device__ __forceinline__ long uniform(long x) {
     return (long)(((unsigned long)(unsigned)uniform((int)(x >> 32)) << 32) | (unsigned)uniform((int)x));
 }
 
+// What a workgroup knows of all sequences: the lane's of the first 64 with the tiles and costs up to it, and the sums over all.
 template <int R>
-__device__ __forceinline__ long total_cost(const AttArgs &a) {
-    long total = 0;
-    int top = 0;
-    for (int first = 0; first < a.c.sequences; first += 64) total += from_lane(upto(seqs_from<R>(a, first, top).cost()), 63);
-    return uniform(total);
-}
-
-// The sequence that holds item `at` of a list in which a sequence has count(seq) items; its items and tiles before it in `base` and `tile_base`.
-template <int R, class Count>
-__device__ __forceinline__ bool locate(const AttArgs &a, long at, Seq &seq, int &s, long &base, long &tile_base, long &cost_base, Count &&count) {
-    long before = 0, tiles = 0, costs = 0;
-    int top = 0;
-    for (int first = 0; first < a.c.sequences; first += 64) {
-        const Seq own = seqs_from<R>(a, first, top);
-        const long n = count(own), sum = upto(n), tsum = upto(own.tiles), csum = upto(own.cost());
-        const unsigned long long past = __ballot(before + sum > at);
-        if (past) {
-            const int l = __ffsll((long long)past) - 1;
-            s = uniform(first + l);
-            base = uniform(before + from_lane(sum - n, l)), tile_base = uniform(tiles + from_lane(tsum - own.tiles, l));
-            cost_base = uniform(costs + from_lane(csum - own.cost(), l));
-            seq.q0 = uniform(__shfl(own.q0, l)), seq.n = uniform(__shfl(own.n, l)), seq.len = uniform(from_lane(own.len, l)), seq.keys = uniform(__shfl(own.keys, l));
-            seq.tiles = uniform(from_lane(own.tiles, l)), seq.pages = uniform(from_lane(own.pages, l));
-            return true;
+struct Scan {
+    Seq own;
+    long tiles_upto, cost_upto, tiles, cost;
+    int top;  // largest start of those 64
+    __device__ __forceinline__ void begin(const AttArgs &a) {
+        top = 0;
+        own = seqs_from<R>(a, 0, top);
+        tiles_upto = upto(own.tiles), cost_upto = upto(own.cost());
+        tiles = from_lane(tiles_upto, 63), cost = from_lane(cost_upto, 63);
+        int at = top;
+        for (int first = 64; first < a.c.sequences; first += 64) {
+            const Seq s = seqs_from<R>(a, first, at);
+            tiles += from_lane(upto(s.tiles), 63), cost += from_lane(upto(s.cost()), 63);
         }
-        before += from_lane(sum, 63), tiles += from_lane(tsum, 63), costs += from_lane(csum, 63);
+        tiles = uniform(tiles), cost = uniform(cost);
     }
-    return false;
-}
+    // the sequence of page `at` of the list: the list's pages and tiles before it
+    __device__ __forceinline__ bool locate(const AttArgs &a, long at, Seq &seq, int &s, long &cost_base, long &tile_base) const {
+        Seq x = own;
+        long t = tiles_upto, c = cost_upto, tiles_before = 0, cost_before = 0;
+        int start = top;
+        for (int first = 0; first < a.c.sequences; first += 64) {
+            if (first) {
+                x = seqs_from<R>(a, first, start);
+                t = upto(x.tiles), c = upto(x.cost());
+            }
+            const unsigned long long past = __ballot(cost_before + c > at);
+            if (past) {
+                const int l = __ffsll((long long)past) - 1;
+                s = uniform(first + l);
+                cost_base = uniform(cost_before + from_lane(c - x.cost(), l)), tile_base = uniform(tiles_before + from_lane(t - x.tiles, l));
+                seq.q0 = uniform(__shfl(x.q0, l)), seq.n = uniform(__shfl(x.n, l)), seq.len = uniform(from_lane(x.len, l)), seq.keys = uniform(__shfl(x.keys, l));
+                seq.tiles = uniform(from_lane(x.tiles, l)), seq.pages = uniform(from_lane(x.pages, l));
+                return true;
+            }
+            cost_before += from_lane(c, 63), tiles_before += from_lane(t, 63);
+        }
+        return false;
+    }
+};
 
-// How long the runs of a call are: equal, and four pages a wave at least, less being not worth a join.
+// What the second launch joins of a tile: how many runs have a part of it (0: nothing to join), the first of them, the sequence's first query, and
+// the tile's first row and those from it on.
+struct Join {
+    int parts, run, q0, row0, rows, pad[3];
+};
+
+// How long the runs of a call are: equal, and a page a wave at least.
 __device__ __forceinline__ long run_of(long total, int runs) {
     const long even = (total + runs - 1) / runs;
-    return even < 4 * WAVES ? 4 * WAVES : even;
+    return even < WAVES ? WAVES : even;
 }
 
 // ---- operands -------------------------------------------------------------------------------------------------------
@@ -259,42 +282,92 @@ struct Wave {
             if (i * 16 < c.pitch) vr[i] = *(const i32x4 *)(from + i * 16 * PAGE);
     }
 
-    // pages first, first + step, ... below `end` of sequence s
+    // Scores of a page whose first place is `at` to weights; accumulators and sums to the new maximum.  `into`: what the page's sums are scaled by, 0
+    // where the lane's row sees none of it.  hidden: some row does not see all of the page (or there is none).
+    __device__ __forceinline__ void weigh(f32x4 (&sc)[4], int j, int at, bool there, bool hidden, float k_scale, float v_scale, typename Op::Weights &p, float &into) {
+        const int g = (threadIdx.x & 63) >> 4;
+        float x[16], by = k_scale;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = sc[i >> 2][i & 3];
+        if (by < 0.f) {  // (the largest score is wanted, not the largest product)
+            by = -by;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = -x[i];
+        }
+        into = v_scale;
+        if (hidden) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = there && at + g * 16 + i < limit[j] ? x[i] * by : -INFINITY;
+            by = 1.f;
+            if (!(there && at < limit[j])) into = 0.f;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        top = fmaxf(top * by, m[j]);
+        const float base = top == -INFINITY ? 0.f : top;
+        if (__ballot(top != m[j])) {
+            const float less = __builtin_amdgcn_exp2f(m[j] - base);
+            sum[j] *= less;
+#pragma unroll
+            for (int i = 0; i < NC * 4; ++i) o[j][i] *= less;
+            m[j] = top;
+        }
+        float add = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float w = __builtin_amdgcn_exp2f(x[i] * by - base);
+            add += w;
+            p.set(i, w);
+        }
+        sum[j] += add;
+    }
+
+    // 64 pages of a sequence at a time: lane i has page, and scales, of number i
+    struct List {
+        int ids, there;
+        float ks, vs;
+        __device__ __forceinline__ void load(const Pages &c, int s, int head, int first, int count, int step, int from) {
+            const int i = from + (threadIdx.x & 63), p = i < count ? c.page_of(s, first + i * step) : -1;
+            there = p >= 0, ids = max(p, 0), ks = vs = 0.f;
+            if (p >= 0) ks = c.k_scales[(long)p * c.kv_heads + head], vs = c.v_scales[(long)p * c.kv_heads + head];
+        }
+        __device__ __forceinline__ int id(int n) const { return __builtin_amdgcn_readlane(ids, n & 63); }
+        __device__ __forceinline__ bool is(int n) const { return __builtin_amdgcn_readlane(there, n & 63) != 0; }
+        __device__ __forceinline__ float k(int n) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), n & 63)); }
+        __device__ __forceinline__ float v(int n) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), n & 63)); }
+    };
+
+    // keys that the wave's rows see at most (the later a row's query, the more)
+    __device__ __forceinline__ int most() const {
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) n = max(n, limit[j]);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) n = max(n, __shfl_xor(n, d));
+        return uniform(n);
+    }
+
+    // KEYS: pages first, first + step, ... below `end` of sequence s, by this wave alone
     __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int end, int step) {
         const Pages &c = a.c;
-        const int lane = threadIdx.x & 63, g = lane >> 4;
-        // (rows see more the later their queries are: the first row sees least, the last that is there most)
-        int most = 0;
-#pragma unroll
-        for (int j = 0; j < RT; ++j) most = max(most, limit[j]);
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor(most, d));
-        end = min(end, uniform((most + PAGE - 1) / PAGE));
+        end = min(end, (most() + PAGE - 1) / PAGE);
         const int least = uniform(limit[0]);
         if (first >= end) return;
         const int count = (end - first + step - 1) / step;
-        // 64 pages at a time: lane i has page, and scales, of number i
-        int ids = 0, there = 0;
-        float ks = 0.f, vs = 0.f;
-        auto list = [&](int from) {
-            const int i = from + lane, p = i < count ? c.page_of(s, first + i * step) : -1;
-            there = p >= 0, ids = max(p, 0);
-            ks = vs = 0.f;
-            if (p >= 0) ks = c.k_scales[(long)p * c.kv_heads + head], vs = c.v_scales[(long)p * c.kv_heads + head];
-        };
-        list(0);
-        int id = __builtin_amdgcn_readlane(ids, 0);
-        fetch_keys(c, id, head);
-        fetch_values(c, id, head);
+        List list;
+        list.load(c, s, head, first, count, step, 0);
+        fetch_keys(c, list.id(0), head);
+        fetch_values(c, list.id(0), head);
         const float by = a.scale * LOG2E;
         for (int n = 0; n < count; ++n) {
-            const int l = n & 63, at = (first + n * step) * PAGE;
-            const bool page_there = __builtin_amdgcn_readlane(there, l) != 0;
-            const float k_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), l)) * by;
-            const float v_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), l));
-            const bool more = n + 1 < count;
-            if (more && ((n + 1) & 63) == 0) list(n + 1);
-            const int next = __builtin_amdgcn_readlane(ids, (n + 1) & 63);
+            const int at = (first + n * step) * PAGE;
+            const bool there = list.is(n), more = n + 1 < count;
+            const float k_scale = list.k(n) * by, v_scale = list.v(n);
+            if (more && ((n + 1) & 63) == 0) list.load(c, s, head, first, count, step, n + 1);
+            const int next = list.id(n + 1);
             f32x4 sc[RT][4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -310,38 +383,9 @@ struct Wave {
             }
             if (more) fetch_keys(c, next, head);
             typename Op::Weights p[RT];
-            float into[RT];  // what the page's sums are scaled by: 0 where the lane's row sees none of it
-            const bool hidden = !page_there || at + PAGE > least;
+            float into[RT];
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                float x[16], top = m[j];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    x[i] = sc[j][i >> 2][i & 3] * k_scale;
-                    if (hidden) x[i] = page_there && at + g * 16 + i < limit[j] ? x[i] : -INFINITY;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float base = top == -INFINITY ? 0.f : top;
-                if (__ballot(top != m[j])) {
-                    const float less = __builtin_amdgcn_exp2f(m[j] - base);
-                    sum[j] *= less;
-#pragma unroll
-                    for (int i = 0; i < NC * 4; ++i) o[j][i] *= less;
-                    m[j] = top;
-                }
-                float add = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(x[i] - base);
-                    add += w;
-                    p[j].set(i, w);
-                }
-                sum[j] += add;
-                into[j] = hidden && !(page_there && at < limit[j]) ? 0.f : v_scale;
-            }
+            for (int j = 0; j < RT; ++j) weigh(sc[j], j, at, there, !there || at + PAGE > least, k_scale, v_scale, p[j], into[j]);
 #pragma unroll
             for (int i = 0; i < NC * 4; ++i) {
                 if (i * 16 >= c.pitch) continue;
@@ -356,6 +400,87 @@ struct Wave {
             }
             if (more) fetch_values(c, next, head);
         }
+    }
+
+    // ROWS: pages first .. end - 1 by all four waves, each with rows of its own.  A page's codes are converted once, a quarter by each wave, and
+    // go through LDS as operands, lane by lane: [keys' tile][chunk][half], then [values' tile][half], a buffer of `stage` for every other page.
+    __device__ __forceinline__ void fetch_share(const Pages &c, int page, int head, int wave) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const signed char *k = c.k_codes + c.tile(page, head) + ((r >> 2) * 16 + (r & 3) + 4 * wave) * c.pitch, *v = c.v_codes + c.tile(page, head) + r * PAGE + g * 16;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int d = n * 64 + g * 16;
+            kr[0][n] = *(const i32x4 *)(k + (d < c.pitch ? d : 0));
+            const int i = n * 4 + wave;
+            if (i * 16 < c.pitch) vr[n] = *(const i32x4 *)(v + i * 16 * PAGE);
+        }
+    }
+    __device__ __forceinline__ void stage_share(f16x8 (*stage)[64], int wave) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            f16x8 x[2];
+            to_halves(kr[0][n], x);
+            stage[(wave * NC + n) * 2][lane] = x[0], stage[(wave * NC + n) * 2 + 1][lane] = x[1];
+            to_halves(vr[n], x);
+            stage[8 * NC + (n * 4 + wave) * 2][lane] = x[0], stage[8 * NC + (n * 4 + wave) * 2 + 1][lane] = x[1];
+        }
+    }
+    __device__ __forceinline__ void pages_together(const AttArgs &a, int s, int head, int first, int end, int wave, f16x8 (*stages)[16 * NC][64]) {
+        const Pages &c = a.c;
+        const int own_end = (most() + PAGE - 1) / PAGE, least = uniform(limit[0]), count = end - first;
+        if (count <= 0) return;  // (all four waves alike)
+        List list, ahead;  // of the page that is computed, and of the one that is fetched
+        list.load(c, s, head, first, count, 1, 0);
+        ahead = list;
+        fetch_share(c, list.id(0), head, wave);
+        stage_share(stages[0], wave);
+        if (count > 1) fetch_share(c, list.id(1), head, wave);
+        const float by = a.scale * LOG2E;
+        for (int n = 0; n < count; ++n) {
+            __syncthreads();  // the page is in LDS, and nobody reads the one before it any more
+            const f16x8 (*stage)[64] = stages[n & 1];
+            const int at = (first + n) * PAGE, lane = threadIdx.x & 63;
+            const bool there = list.is(n);
+            const float k_scale = list.k(n) * by, v_scale = list.v(n);
+            if (first + n < own_end) {
+                f32x4 sc[RT][4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) sc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < 2 * NC; ++i) {
+                        const f16x8 k = stage[t * 2 * NC + i][lane];
+#pragma unroll
+                        for (int j = 0; j < RT; ++j) sc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[j].f[i], sc[j][t], 0, 0, 0);
+                    }
+                }
+                typename Op::Weights p[RT];
+                float into[RT];
+#pragma unroll
+                for (int j = 0; j < RT; ++j) weigh(sc[j], j, at, there, !there || at + PAGE > least, k_scale, v_scale, p[j], into[j]);
+#pragma unroll
+                for (int i = 0; i < NC * 4; ++i) {
+                    if (i * 16 >= c.pitch) continue;
+                    const f16x8 v0 = stage[8 * NC + 2 * i][lane], v1 = stage[8 * NC + 2 * i + 1][lane];
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) {
+                        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[j].f[0], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[j].f[1], acc, 0, 0, 0);
+                        o[j][i] += acc * into[j];
+                    }
+                }
+            }
+            if (n + 1 < count) stage_share(stages[(n + 1) & 1], wave);
+            if (n + 2 < count) {
+                if (((n + 2) & 63) == 0) ahead.load(c, s, head, first, count, 1, n + 2);
+                fetch_share(c, ahead.id(n + 2), head, wave);
+            }
+            if (((n + 1) & 63) == 0) list = ahead;
+        }
+        __syncthreads();  // (the next tile takes the same LDS)
     }
 };
 
@@ -376,30 +501,47 @@ __device__ __forceinline__ void put(const AttArgs &a, T *to, int d, const f32x4 
 }
 
 template <class T, int NC, int RT, bool ROWS>
-__global__ __launch_bounds__(WAVES * 64) void attention_cache_kernel(AttArgs a) {
+__global__ __launch_bounds__(WAVES * 64, NC == 4 || sizeof(T) == 4 ? 1 : 2) void attention_cache_kernel(AttArgs a) {
     constexpr int R = 16 * RT * (ROWS ? WAVES : 1);  // rows of a tile
+    __shared__ f16x8 stages[ROWS ? 2 : 1][ROWS ? 16 * NC : 1][64];
     __shared__ f32x4 others[ROWS ? 1 : WAVES][ROWS ? 1 : NC * 4][64];
     __shared__ float2 stats[ROWS ? 1 : WAVES][16];
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), r = lane & 15, g = lane >> 4;
     const int head = blockIdx.x % a.c.kv_heads, run = blockIdx.x / a.c.kv_heads;
-    const long total = total_cost<R>(a), length = run_of(total, a.runs);
+    Scan<R> scan;
+    scan.begin(a);
+    const long total = scan.cost, length = run_of(total, a.runs);
     const long last = min((run + 1) * length, total);
     long at = run * length;
+    if (run == 0 && head == 0)  // tiles that the launch has room for and the sequences do not have
+        for (long i = scan.tiles + threadIdx.x; i < a.units; i += WAVES * 64) a.joins[i].parts = 0;
+    if (at >= last) return;
+    Seq seq;
+    int s;
+    long base, tile_base;
+    if (!scan.locate(a, at, seq, s, base, tile_base)) return;
     Wave<T, NC, RT> w;
-    while (at < last) {
-        Seq seq;
-        int s;
-        long base, tile_base, cost_base;
-        if (!locate<R>(a, at, seq, s, base, tile_base, cost_base, [](const Seq &x) { return x.cost(); })) return;
+    for (;;) {
         const long after = base + seq.cost();
         while (at < last && at < after) {
             const long tile = (at - base) / seq.pages;
             const int first = (int)(at - base - tile * seq.pages), end = (int)min(seq.pages, first + (last - at));
             const bool whole = first == 0 && end == seq.pages;
             const long rows = (long)seq.n * a.group, row0 = tile * R + (ROWS ? wave * 16 * RT : 0), slot = run + tile_base + tile;
+            if (first == 0 && head == 0 && threadIdx.x == 0) {  // (the tile's first page: every head's parts are alike)
+                const long from = base + tile * seq.pages, to = from + seq.pages - 1;
+                const int parts = (int)(to / length - from / length) + 1;
+                a.joins[tile_base + tile] = Join{parts == 1 ? 0 : parts, run, seq.q0, (int)(tile * R), (int)(rows - tile * R), {0, 0, 0}};
+            }
             w.begin(a, seq, head, row0, rows);
-            if (ROWS) w.pages(a, s, head, first, end, 1);
-            else w.pages(a, s, head, first + wave, end, WAVES);
+            if constexpr (ROWS) {
+                // what the tile's last row sees: all four waves go through as many pages
+                const int t = (int)((min((tile + 1) * R, rows) - 1) / a.group);
+                const long sees = min(max(a.causal ? t + seq.len - seq.n + 1 : seq.len, 0L), (long)seq.keys);
+                w.pages_together(a, s, head, first, min(end, (int)((sees + PAGE - 1) / PAGE)), wave, stages);
+            } else {
+                w.pages(a, s, head, first + wave, end, WAVES);
+            }
             at += end - first;
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
@@ -444,54 +586,51 @@ __global__ __launch_bounds__(WAVES * 64) void attention_cache_kernel(AttArgs a) 
                     if (a.lse && g == 0 && (ROWS || wave == 0)) a.lse[(long)h * a.c.tokens + seq.q0 + t] = w.sum[j] == 0.f ? -INFINITY : (w.m[j] + log2f(w.sum[j])) * LN2;
                 } else {
                     const long place = (slot * a.c.kv_heads + head) * R + (row - tile * R);
-                    float *to = a.part + place * a.c.dim;
+                    float *to = a.part + place * a.part_ld;
 #pragma unroll
                     for (int i = 0; i < NC * 4; ++i)
-                        if (ROWS || i % WAVES == wave)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (i * 16 + g * 4 + e < a.c.dim) to[i * 16 + g * 4 + e] = w.o[j][i][e];
+                        if ((ROWS || i % WAVES == wave) && i * 16 + g * 4 < a.part_ld) *(f32x4 *)(to + i * 16 + g * 4) = w.o[j][i];
                     if (g == 0 && (ROWS || wave == 0)) *(float2 *)(a.part_ml + place * 2) = make_float2(w.m[j], w.sum[j]);
                 }
             }
         }
+        if (at >= last) return;
+        Scan<R> again;  // (anew: kept, it would take the registers of a wave)
+        again.begin(a);
+        if (!again.locate(a, at, seq, s, base, tile_base)) return;
     }
 }
 
-// The runs' sums of a tile's rows joined: a wave a row.
+// The runs' sums of a tile's rows joined: half a wave a row, four elements a lane.
 template <class T, int R>
 __global__ __launch_bounds__(256) void attention_cache_join_kernel(AttArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x % a.c.kv_heads;
-    const long unit = blockIdx.x / a.c.kv_heads, total = total_cost<R>(a), length = run_of(total, a.runs);
-    Seq seq;
-    int s;
-    long base, tile_base, cost_base;
-    if (!locate<R>(a, unit, seq, s, base, tile_base, cost_base, [](const Seq &x) { return x.tiles; })) return;
-    const long tile = unit - base, from = cost_base + tile * seq.pages;
-    const int first = (int)(from / length), last = (int)((from + seq.pages - 1) / length);
-    if (first == last) return;
-    const long rows = (long)seq.n * a.group, n = min((long)R, rows - tile * R), step = (long)a.c.kv_heads * R;
-    for (int row = blockIdx.y * 4 + wave; row < n; row += gridDim.y * 4) {
-        const long place = ((first + unit) * a.c.kv_heads + head) * R + row;
-        const int parts = last - first + 1;
+    const int half = threadIdx.x & 31, of = threadIdx.x >> 5, head = blockIdx.x % a.c.kv_heads, unit = blockIdx.x / a.c.kv_heads;
+    const Join join = a.joins[unit];
+    if (!join.parts) return;
+    const int n = min(R, join.rows);
+    const long step = (long)a.c.kv_heads * R;
+    for (int row = blockIdx.y * 8 + of; row < n; row += gridDim.y * 8) {
+        const long place = (((long)join.run + unit) * a.c.kv_heads + head) * R + row;
+        const float2 *ml = (const float2 *)a.part_ml + place;
         float top = -INFINITY, sum = 0.f;
-        for (int i = lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[(place + i * step) * 2]);
+        for (int i = half; i < join.parts; i += 32) top = fmaxf(top, ml[i * step].x);
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
         const float at = top == -INFINITY ? 0.f : top;
-        for (int i = lane; i < parts; i += 64) sum += a.part_ml[(place + i * step) * 2 + 1] * __builtin_amdgcn_exp2f(a.part_ml[(place + i * step) * 2] - at);
+        for (int i = half; i < join.parts; i += 32) sum += ml[i * step].y * __builtin_amdgcn_exp2f(ml[i * step].x - at);
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-        const long global = tile * R + row;
-        const int t = (int)(global / a.group), h = head * a.group + (int)(global - (long)t * a.group);
+        for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor(sum, d);
+        const int t = (join.row0 + row) / a.group, h = head * a.group + join.row0 + row - t * a.group;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        for (int d = lane; d < a.c.dim; d += 64) {
-            float x = 0.f;
+        T *to = (T *)a.o + ((long)join.q0 + t) * a.ldo + (long)h * a.c.dim;
+        for (int d = half * 4; d < a.c.dim; d += 128) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            const float *from = a.part + place * a.part_ld + d;
 #pragma unroll 4
-            for (int i = 0; i < parts; ++i) x += a.part[(place + i * step) * a.c.dim + d] * __builtin_amdgcn_exp2f(a.part_ml[(place + i * step) * 2] - at);
-            ((T *)a.o)[(seq.q0 + (long)t) * a.ldo + (long)h * a.c.dim + d] = (T)(x * inv);
+            for (int i = 0; i < join.parts; ++i) x += *(const f32x4 *)(from + i * step * a.part_ld) * __builtin_amdgcn_exp2f(ml[i * step].x - at);
+            put<T>(a, to, d, x, inv);
         }
-        if (lane == 0 && a.lse) a.lse[(long)h * a.c.tokens + seq.q0 + t] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+        if (half == 0 && a.lse) a.lse[(long)h * a.c.tokens + join.q0 + t] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
     }
 }
 
@@ -512,13 +651,16 @@ Plan plan_of(int dtype, int sequences, int tokens, int table_pages, int heads, i
     p.rows = dtype == D8_FLOAT16 && dim <= 128 && some && all / some >= 64;
     p.tile = p.rows ? MANY_ROWS : KEYS_ROWS;
     p.units = all / p.tile + some;
-    const long at_once = (2L * cu_count() + kv_heads - 1) / kv_heads, most = (p.units * (table_pages ? table_pages : 1) + 4 * WAVES - 1) / (4 * WAVES);
+    const long at_once = (2L * cu_count() + kv_heads - 1) / kv_heads, most = (p.units * (table_pages ? table_pages : 1) + WAVES - 1) / WAVES;
     p.runs = (int)(at_once < most ? at_once : most);
     p.slots = p.units + p.runs;
     return p;
 }
 
-size_t scratch_of(const Plan &p, int kv_heads, int dim) { return sizeof(float) * (size_t)p.slots * kv_heads * p.tile * (dim + 2); }
+int part_ld_of(int dim) { return (dim + 3) / 4 * 4; }
+size_t scratch_of(const Plan &p, int kv_heads, int dim) {
+    return sizeof(Join) * p.units + sizeof(float) * (size_t)p.slots * kv_heads * p.tile * (part_ld_of(dim) + 2);
+}
 
 template <class T, int NC>
 void launch(const AttArgs &a, const Plan &p, hipStream_t stream) {
@@ -538,7 +680,7 @@ int launch_all(const AttArgs &a, const Plan &p, hipStream_t stream) {
     else if (a.c.dim <= 128) launch<T, 2>(a, p, stream);
     else launch<T, 4>(a, p, stream);
     D8_LAUNCH_CHECK();
-    const dim3 join((unsigned)(p.units * a.c.kv_heads), p.rows ? 8 : 4);
+    const dim3 join((unsigned)(p.units * a.c.kv_heads), p.rows ? 4 : 2);
     if (p.rows) hipLaunchKernelGGL((attention_cache_join_kernel<T, MANY_ROWS>), join, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((attention_cache_join_kernel<T, KEYS_ROWS>), join, dim3(256), 0, stream, a);
     D8_LAUNCH_CHECK();
@@ -583,6 +725,7 @@ extern "C" int d8_attention_cache(int dtype, const void *q, long ldq, const sign
     const int v = 16 / (int)dtype_bytes(dtype);
     a.q = q, a.ldq = ldq, a.o = o, a.ldo = ldo, a.lse = lse, a.heads = heads, a.group = heads / kv_heads, a.causal = causal != 0, a.scale = scale, a.runs = p.runs;
     a.vec = dim % v == 0 && ldq % v == 0 && ldo % v == 0 && (((size_t)q | (size_t)o) & 15) == 0;
-    a.part = (float *)scratch, a.part_ml = a.part + (size_t)p.slots * kv_heads * p.tile * dim;
+    a.part_ld = cache::part_ld_of(dim), a.units = p.units;
+    a.joins = (cache::Join *)scratch, a.part = (float *)(a.joins + p.units), a.part_ml = a.part + (size_t)p.slots * kv_heads * p.tile * a.part_ld;
     return dtype == D8_FLOAT16 ? cache::launch_all<f16>(a, p, as_stream(stream)) : cache::launch_all<float>(a, p, as_stream(stream));
 }

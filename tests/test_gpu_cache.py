@@ -362,10 +362,11 @@ def test_scratch_has_room_for_every_piece(sequences, tokens, table_pages, heads,
         nb = lib.d8_attention_cache_scratch_bytes(dt, sequences, tokens, table_pages, heads, kv_heads, dim)
         many = dt == capi.FLOAT16 and dim <= 128 and tokens * group // min(sequences, tokens) >= 64
         rows = 128 if many else 16
-        slots = nb // (4 * kv_heads * rows * (dim + 2))
         units = tokens * group // rows + min(sequences, tokens)
+        per_slot = 4 * kv_heads * rows * ((dim + 3) // 4 * 4 + 2)
+        slots = (nb - 32 * units) // per_slot  # (32 bytes a tile say what is joined)
         runs = slots - units
-        assert runs >= 1 and nb == slots * 4 * kv_heads * rows * (dim + 2)
+        assert runs >= 1 and nb == 32 * units + slots * per_slot
         for _ in range(20):
             cuts = np.sort(r.integers(0, tokens + 1, sequences - 1))
             n = np.diff(np.r_[0, cuts, tokens])
@@ -373,7 +374,7 @@ def test_scratch_has_room_for_every_piece(sequences, tokens, table_pages, heads,
             tiles = -(-n * group // rows)
             assert tiles.sum() <= units
             total = int((tiles * pages).sum())
-            length = max(-(-total // runs), 16)
+            length = max(-(-total // runs), 4)
             used, at, unit = set(), 0, 0
             for t, p in zip(tiles, pages):
                 for _ in range(t):
