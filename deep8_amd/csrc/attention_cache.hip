@@ -20,8 +20,7 @@
 //
 // Bound by memory where there are few rows (a page and head is 16 KB at 128 elements), by conversions and exponentials where there are many.
 //
-// Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product; every page's product starts from zero
-// and is scaled into the accumulators, so a page's scale costs nothing of another's.
+// Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product.
 #include "cache.h"
 
 namespace d8 {
@@ -29,7 +28,7 @@ namespace cache {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-enum { WAVES = 4 };
+enum { KEYS_WAVES = 4, KEYS_ROWS = 16, ROWS_WAVES = 8, MANY_ROWS = 128 };
 
 struct Join;
 
@@ -146,7 +145,7 @@ struct Join {
 // How long the runs of a call are: equal, and a page a wave at least.
 __device__ __forceinline__ long run_of(long total, int runs) {
     const long even = (total + runs - 1) / runs;
-    return even < WAVES ? WAVES : even;
+    return even < KEYS_WAVES ? KEYS_WAVES : even;
 }
 
 // ---- operands -------------------------------------------------------------------------------------------------------
@@ -177,7 +176,14 @@ struct Operands<f16, NC> {
     };
     struct Weights {
         f16x8 f[2];
-        __device__ __forceinline__ void set(int i, float x) { f[i >> 3][i & 7] = (f16)x; }
+        __device__ __forceinline__ void set(const float (&x)[16]) {  // (two values a conversion, to nearest)
+            f16x2 p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = __builtin_convertvector((f32x2){x[2 * i], x[2 * i + 1]}, f16x2);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                f[i] = __builtin_shufflevector(__builtin_shufflevector(p[4 * i], p[4 * i + 1], 0, 1, 2, 3), __builtin_shufflevector(p[4 * i + 2], p[4 * i + 3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+        }
     };
     struct Codes {
         f16x8 f[2];
@@ -201,7 +207,10 @@ struct Operands<float, NC> {
     };
     struct Weights {
         float f[16];
-        __device__ __forceinline__ void set(int i, float x) { f[i] = x; }
+        __device__ __forceinline__ void set(const float (&x)[16]) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = x[i];
+        }
     };
     struct Codes {
         i32x4 w;
@@ -218,269 +227,260 @@ struct Operands<float, NC> {
     }
 };
 
-// ---- one wave over some pages ---------------------------------------------------------------------------------------
-// RT tiles of 16 rows; NC: chunks of 64 elements of a head.
-template <class T, int NC, int RT>
+// the larger, and the sum, of the four lanes that have a row (l, l + 16, l + 32, l + 48)
+__device__ __forceinline__ float row_max(float x) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// ---- one wave, 16 rows ----------------------------------------------------------------------------------------------
+// NC: chunks of 64 elements of a head.
+template <class T, int NC>
 struct Wave {
     typedef Operands<T, NC> Op;
-    typename Op::Query q[RT];
-    f32x4 o[RT][NC * 4];
-    float m[RT], sum[RT];  // of scores times log2 e; the lane's part of the sum
-    int limit[RT];         // keys that the lane's row sees
-    i32x4 kr[4][NC], vr[NC * 4];
+    typename Op::Query q;
+    f32x4 o[NC * 4];
+    float m, sum;  // of scores times log2 e; the lane's part of the sum
+    int limit;     // keys that the lane's row sees
 
     // rows row0 .. of the sequence (those beyond `rows` are zero and see nothing)
     __device__ __forceinline__ void begin(const AttArgs &a, const Seq &s, int head, long row0, long rows) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const long row = row0 + r;
+        const bool there = row < rows;
+        const int t = there ? (int)row / a.group : 0, h = there ? (int)row - t * a.group : 0;
+        const long sees = a.causal ? t + s.len - s.n + 1 : s.len;
+        limit = there ? (int)min(max(sees, 0L), (long)s.keys) : 0;
+        const T *from = (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * a.group + h) * a.c.dim;
 #pragma unroll
-        for (int j = 0; j < RT; ++j) {
-            const long row = row0 + 16 * j + r;
-            const bool there = row < rows;
-            const int t = there ? (int)(row / a.group) : 0, h = there ? (int)(row - (long)t * a.group) : 0;
-            const long sees = a.causal ? t + s.len - s.n + 1 : s.len;
-            limit[j] = there ? (int)min(max(sees, 0L), (long)s.keys) : 0;
-            const T *from = (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * a.group + h) * a.c.dim;
+        for (int c = 0; c < NC; ++c) {
+            const int d = c * 64 + g * 16;
+            constexpr int V = 16 / sizeof(T);
+            typedef T piece __attribute__((ext_vector_type(V)));
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int d = c * 64 + g * 16;
-                constexpr int V = 16 / sizeof(T);
-                typedef T piece __attribute__((ext_vector_type(V)));
+            for (int i = 0; i < 16; i += V) {
+                if (a.vec && there && d + i < a.c.dim) {  // (dim is whole pieces)
+                    const piece p = *(const piece *)(from + d + i);
 #pragma unroll
-                for (int i = 0; i < 16; i += V) {
-                    if (a.vec && there && d + i < a.c.dim) {  // (dim is whole pieces)
-                        const piece p = *(const piece *)(from + d + i);
+                    for (int e = 0; e < V; ++e) q.set(c * 16 + i + e, (float)p[e]);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < V; ++e) q[j].set(c * 16 + i + e, (float)p[e]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < V; ++e) q[j].set(c * 16 + i + e, !a.vec && there && d + i + e < a.c.dim ? (float)from[d + i + e] : 0.f);
-                    }
+                    for (int e = 0; e < V; ++e) q.set(c * 16 + i + e, !a.vec && there && d + i + e < a.c.dim ? (float)from[d + i + e] : 0.f);
                 }
             }
-            m[j] = -INFINITY, sum[j] = 0.f;
-#pragma unroll
-            for (int i = 0; i < NC * 4; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
+        m = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC * 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    __device__ __forceinline__ void fetch_keys(const Pages &c, int page, int head) {
-        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-        const signed char *from = c.k_codes + c.tile(page, head);
-        const int key = (r >> 2) * 16 + (r & 3);
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const int d = n * 64 + g * 16, at = d < c.pitch ? d : 0;  // (beyond the head: any codes, times zeros of q)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) kr[t][n] = *(const i32x4 *)(from + (key + 4 * t) * c.pitch + at);
-        }
+    // where a lane's operands lie in a page and head: its key's row of tile t (16 bytes of chunk n; beyond the head any codes, times zeros of q),
+    // its element's of tile i
+    static __device__ __forceinline__ const i32x4 *key_at(const Pages &c, const signed char *page, int t, int n) {
+        const int lane = threadIdx.x & 63, r = lane & 15, d = n * 64 + (lane >> 4) * 16;
+        return (const i32x4 *)(page + ((r >> 2) * 16 + (r & 3) + 4 * t) * c.pitch + (d < c.pitch ? d : 0));
     }
-    __device__ __forceinline__ void fetch_values(const Pages &c, int page, int head) {
-        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-        const signed char *from = c.v_codes + c.tile(page, head) + r * PAGE + g * 16;
-#pragma unroll
-        for (int i = 0; i < NC * 4; ++i)
-            if (i * 16 < c.pitch) vr[i] = *(const i32x4 *)(from + i * 16 * PAGE);
+    static __device__ __forceinline__ const i32x4 *value_at(const signed char *page, int i) {
+        const int lane = threadIdx.x & 63;
+        return (const i32x4 *)(page + (i * 16 + (lane & 15)) * PAGE + (lane >> 4) * 16);
     }
 
-    // Scores of a page whose first place is `at` to weights; accumulators and sums to the new maximum.  `into`: what the page's sums are scaled by, 0
-    // where the lane's row sees none of it.  hidden: some row does not see all of the page (or there is none).
-    __device__ __forceinline__ void weigh(f32x4 (&sc)[4], int j, int at, bool there, bool hidden, float k_scale, float v_scale, typename Op::Weights &p, float &into) {
+    // Scores of a page whose first place is `at` to weights; accumulators and sums to the new maximum.  hidden: some row does not see all of
+    // the page (or there is none).  `into`: what the page's sums are scaled by, 0 where the lane's row sees none of it.
+    __device__ __forceinline__ void weigh(const f32x4 (&sc)[4], int at, bool there, bool hidden, float k_scale, float v_scale, typename Op::Weights &p, float &into) {
         const int g = (threadIdx.x & 63) >> 4;
         float x[16], by = k_scale;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = sc[i >> 2][i & 3];
-        if (by < 0.f) {  // (the largest score is wanted, not the largest product)
-            by = -by;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = -x[i];
-        }
         into = v_scale;
-        if (hidden) {
+        if (hidden || by < 0.f) {  // (below, the largest score is taken for the largest product)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = there && at + g * 16 + i < limit[j] ? x[i] * by : -INFINITY;
+            for (int i = 0; i < 16; ++i) x[i] = there && at + g * 16 + i < limit ? x[i] * by : -INFINITY;
             by = 1.f;
-            if (!(there && at < limit[j])) into = 0.f;
+            into = there && at < limit ? v_scale : 0.f;
         }
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        top = fmaxf(top * by, m[j]);
+        top = fmaxf(row_max(top) * by, m);
         const float base = top == -INFINITY ? 0.f : top;
-        if (__ballot(top != m[j])) {
-            const float less = __builtin_amdgcn_exp2f(m[j] - base);
-            sum[j] *= less;
+        if (__ballot(top != m)) {
+            const float less = __builtin_amdgcn_exp2f(m - base);
+            sum *= less;
 #pragma unroll
-            for (int i = 0; i < NC * 4; ++i) o[j][i] *= less;
-            m[j] = top;
+            for (int i = 0; i < NC * 4; ++i) o[i] *= less;
+            m = top;
         }
         float add = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float w = __builtin_amdgcn_exp2f(x[i] * by - base);
-            add += w;
-            p.set(i, w);
+            x[i] = __builtin_amdgcn_exp2f(x[i] * by - base);
+            add += x[i];
         }
-        sum[j] += add;
+        p.set(x);
+        sum += add;
     }
 
-    // 64 pages of a sequence at a time: lane i has page, and scales, of number i
+    // 64 pages of a sequence: lane i has page, and scales, of number i
     struct List {
         int ids, there;
         float ks, vs;
-        __device__ __forceinline__ void load(const Pages &c, int s, int head, int first, int count, int step, int from) {
-            const int i = from + (threadIdx.x & 63), p = i < count ? c.page_of(s, first + i * step) : -1;
+        __device__ __forceinline__ void load(const Pages &c, int s, int head, int first, int count, int step) {
+            const int i = threadIdx.x & 63, p = i < count ? c.page_of(s, first + i * step) : -1;
             there = p >= 0, ids = max(p, 0), ks = vs = 0.f;
             if (p >= 0) ks = c.k_scales[(long)p * c.kv_heads + head], vs = c.v_scales[(long)p * c.kv_heads + head];
         }
-        __device__ __forceinline__ int id(int n) const { return __builtin_amdgcn_readlane(ids, n & 63); }
-        __device__ __forceinline__ bool is(int n) const { return __builtin_amdgcn_readlane(there, n & 63) != 0; }
-        __device__ __forceinline__ float k(int n) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), n & 63)); }
-        __device__ __forceinline__ float v(int n) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), n & 63)); }
+        __device__ __forceinline__ int id(int n) const { return __builtin_amdgcn_readlane(ids, n); }
+        __device__ __forceinline__ bool is(int n) const { return __builtin_amdgcn_readlane(there, n) != 0; }
+        __device__ __forceinline__ float k(int n) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), n)); }
+        __device__ __forceinline__ float v(int n) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), n)); }
     };
 
-    // keys that the wave's rows see at most (the later a row's query, the more)
+    // pages that the wave's rows see at most (the later a row's query, the more)
     __device__ __forceinline__ int most() const {
-        int n = 0;
-#pragma unroll
-        for (int j = 0; j < RT; ++j) n = max(n, limit[j]);
+        int n = limit;
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) n = max(n, __shfl_xor(n, d));
-        return uniform(n);
+        return uniform((n + PAGE - 1) / PAGE);
     }
 
-    // KEYS: pages first, first + step, ... below `end` of sequence s, by this wave alone
-    __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int end, int step) {
+    // KEYS: `count` pages, 64 at most, first, first + step, ... of sequence s, by this wave alone
+    __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int count, int step) {
         const Pages &c = a.c;
-        end = min(end, (most() + PAGE - 1) / PAGE);
-        const int least = uniform(limit[0]);
-        if (first >= end) return;
-        const int count = (end - first + step - 1) / step;
+        const int least = uniform(limit);
         List list;
-        list.load(c, s, head, first, count, step, 0);
-        fetch_keys(c, list.id(0), head);
-        fetch_values(c, list.id(0), head);
-        const float by = a.scale * LOG2E;
+        list.load(c, s, head, first, count, step);
+        i32x4 kr[4][NC], vr[NC * 4];
+        auto fetch_keys = [&](int page) {
+            const signed char *from = c.k_codes + c.tile(page, head);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int n = 0; n < NC; ++n) kr[t][n] = *key_at(c, from, t, n);
+        };
+        auto fetch_values = [&](int page) {
+            const signed char *from = c.v_codes + c.tile(page, head);
+#pragma unroll
+            for (int i = 0; i < NC * 4; ++i)
+                if (i * 16 < c.pitch) vr[i] = *value_at(from, i);
+        };
+        fetch_keys(list.id(0)), fetch_values(list.id(0));
         for (int n = 0; n < count; ++n) {
             const int at = (first + n * step) * PAGE;
             const bool there = list.is(n), more = n + 1 < count;
-            const float k_scale = list.k(n) * by, v_scale = list.v(n);
-            if (more && ((n + 1) & 63) == 0) list.load(c, s, head, first, count, step, n + 1);
-            const int next = list.id(n + 1);
-            f32x4 sc[RT][4];
+            const int next = list.id(more ? n + 1 : n);
+            f32x4 sc[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                for (int j = 0; j < RT; ++j) sc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < NC; ++i) {
                     typename Op::Codes k;
                     k.set(kr[t][i]);
-#pragma unroll
-                    for (int j = 0; j < RT; ++j) Op::scores(sc[j][t], k, q[j], i);
+                    Op::scores(sc[t], k, q, i);
                 }
             }
-            if (more) fetch_keys(c, next, head);
-            typename Op::Weights p[RT];
-            float into[RT];
-#pragma unroll
-            for (int j = 0; j < RT; ++j) weigh(sc[j], j, at, there, !there || at + PAGE > least, k_scale, v_scale, p[j], into[j]);
+            if (more) fetch_keys(next);
+            typename Op::Weights p;
+            float into;
+            weigh(sc, at, there, !there || at + PAGE > least, list.k(n) * (a.scale * LOG2E), list.v(n), p, into);
 #pragma unroll
             for (int i = 0; i < NC * 4; ++i) {
                 if (i * 16 >= c.pitch) continue;
                 typename Op::Codes v;
                 v.set(vr[i]);
-#pragma unroll
-                for (int j = 0; j < RT; ++j) {
-                    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                    Op::sums(acc, v, p[j]);
-                    o[j][i] += acc * into[j];
-                }
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                Op::sums(acc, v, p);
+                o[i] += acc * into;
             }
-            if (more) fetch_values(c, next, head);
+            if (more) fetch_values(next);
         }
     }
 
-    // ROWS: pages first .. end - 1 by all four waves, each with rows of its own.  A page's codes are converted once, a quarter by each wave, and
-    // go through LDS as operands, lane by lane: [keys' tile][chunk][half], then [values' tile][half], a buffer of `stage` for every other page.
-    __device__ __forceinline__ void fetch_share(const Pages &c, int page, int head, int wave) {
-        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-        const signed char *k = c.k_codes + c.tile(page, head) + ((r >> 2) * 16 + (r & 3) + 4 * wave) * c.pitch, *v = c.v_codes + c.tile(page, head) + r * PAGE + g * 16;
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const int d = n * 64 + g * 16;
-            kr[0][n] = *(const i32x4 *)(k + (d < c.pitch ? d : 0));
-            const int i = n * 4 + wave;
-            if (i * 16 < c.pitch) vr[n] = *(const i32x4 *)(v + i * 16 * PAGE);
-        }
-    }
-    __device__ __forceinline__ void stage_share(f16x8 (*stage)[64], int wave) {
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            f16x8 x[2];
-            to_halves(kr[0][n], x);
-            stage[(wave * NC + n) * 2][lane] = x[0], stage[(wave * NC + n) * 2 + 1][lane] = x[1];
-            to_halves(vr[n], x);
-            stage[8 * NC + (n * 4 + wave) * 2][lane] = x[0], stage[8 * NC + (n * 4 + wave) * 2 + 1][lane] = x[1];
-        }
-    }
-    __device__ __forceinline__ void pages_together(const AttArgs &a, int s, int head, int first, int end, int wave, f16x8 (*stages)[16 * NC][64]) {
+    // ROWS: `count` pages, 64 at most, from `first` on by all waves of a workgroup, each with rows of its own.  A page's codes are converted once, an
+    // eighth by each wave, and go through LDS as operands, lane by lane: [keys' tile][chunk][half], then [values' tile][half], a buffer for every other page.
+    __device__ __forceinline__ void pages_together(const AttArgs &a, int s, int head, int first, int count, int wave, f16x8 (*stages)[16 * NC][64]) {
         const Pages &c = a.c;
-        const int own_end = (most() + PAGE - 1) / PAGE, least = uniform(limit[0]), count = end - first;
-        if (count <= 0) return;  // (all four waves alike)
-        List list, ahead;  // of the page that is computed, and of the one that is fetched
-        list.load(c, s, head, first, count, 1, 0);
-        ahead = list;
-        fetch_share(c, list.id(0), head, wave);
-        stage_share(stages[0], wave);
-        if (count > 1) fetch_share(c, list.id(1), head, wave);
-        const float by = a.scale * LOG2E;
+        const int lane = threadIdx.x & 63, own_end = most(), least = uniform(limit);
+        List list;
+        list.load(c, s, head, first, count, 1);
+        i32x4 share[NC];
+        auto fetch = [&](int page) {
+            const signed char *k = c.k_codes + c.tile(page, head), *v = c.v_codes + c.tile(page, head);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                const int item = wave + ROWS_WAVES * n;
+                if (item < 4 * NC) share[n] = *key_at(c, k, item / NC, item % NC);
+                else if ((item - 4 * NC) * 16 < c.pitch) share[n] = *value_at(v, item - 4 * NC);
+            }
+        };
+        auto stage = [&](int to) {
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                f16x8 x[2];
+                to_halves(share[n], x);
+                stages[to][(wave + ROWS_WAVES * n) * 2][lane] = x[0], stages[to][(wave + ROWS_WAVES * n) * 2 + 1][lane] = x[1];
+            }
+        };
+        fetch(list.id(0));
+        stage(0);
+        if (count > 1) fetch(list.id(1));
         for (int n = 0; n < count; ++n) {
             __syncthreads();  // the page is in LDS, and nobody reads the one before it any more
-            const f16x8 (*stage)[64] = stages[n & 1];
-            const int at = (first + n) * PAGE, lane = threadIdx.x & 63;
+            const f16x8 (*from)[64] = stages[n & 1];
+            const int at = (first + n) * PAGE;
             const bool there = list.is(n);
-            const float k_scale = list.k(n) * by, v_scale = list.v(n);
             if (first + n < own_end) {
-                f32x4 sc[RT][4];
+                // fragments in groups of four, the next on their way while one is multiplied; kept in that order (left to itself the compiler reads them
+                // all at once, which takes more registers than four waves a SIMD leave)
+                f16x8 ahead[2][4];
+                auto group = [&](int k) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
+                    for (int i = 0; i < 4; ++i)
+                        ahead[k & 1][i] = from[4 * k + i][lane];
+                };
+                f32x4 sc[4];
+                group(0);
 #pragma unroll
-                    for (int j = 0; j < RT; ++j) sc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < 4; ++t) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < 2 * NC; ++i) {
-                        const f16x8 k = stage[t * 2 * NC + i][lane];
+                for (int k = 0; k < 2 * NC; ++k) {
+                    group(k + 1);
 #pragma unroll
-                        for (int j = 0; j < RT; ++j) sc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[j].f[i], sc[j][t], 0, 0, 0);
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = 4 * k + i, t = at / (2 * NC);
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[k & 1][i], q.f[at % (2 * NC)], sc[t], 0, 0, 0);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                typename Op::Weights p[RT];
-                float into[RT];
+                typename Op::Weights p;
+                float into;
+                weigh(sc, at, there, !there || at + PAGE > least, list.k(n) * (a.scale * LOG2E), list.v(n), p, into);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < RT; ++j) weigh(sc[j], j, at, there, !there || at + PAGE > least, k_scale, v_scale, p[j], into[j]);
+                for (int k = 0; k < 2 * NC; ++k) {
+                    if (k + 1 < 2 * NC) group(2 * NC + k + 1);
 #pragma unroll
-                for (int i = 0; i < NC * 4; ++i) {
-                    if (i * 16 >= c.pitch) continue;
-                    const f16x8 v0 = stage[8 * NC + 2 * i][lane], v1 = stage[8 * NC + 2 * i + 1][lane];
-#pragma unroll
-                    for (int j = 0; j < RT; ++j) {
+                    for (int i = 0; i < 2; ++i) {  // (elements beyond the head, whatever they are, are not stored)
                         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[j].f[0], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[j].f[1], acc, 0, 0, 0);
-                        o[j][i] += acc * into[j];
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[k & 1][2 * i], p.f[0], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[k & 1][2 * i + 1], p.f[1], acc, 0, 0, 0);
+                        o[k * 2 + i] += acc * into;
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (n + 1 < count) stage_share(stages[(n + 1) & 1], wave);
-            if (n + 2 < count) {
-                if (((n + 2) & 63) == 0) ahead.load(c, s, head, first, count, 1, n + 2);
-                fetch_share(c, ahead.id(n + 2), head, wave);
-            }
-            if (((n + 1) & 63) == 0) list = ahead;
+            if (n + 1 < count) stage((n + 1) & 1);
+            if (n + 2 < count) fetch(list.id(n + 2));
         }
-        __syncthreads();  // (the next tile takes the same LDS)
+        __syncthreads();  // (the next pages take the same LDS)
     }
 };
 
@@ -500,9 +500,9 @@ __device__ __forceinline__ void put(const AttArgs &a, T *to, int d, const f32x4 
     }
 }
 
-template <class T, int NC, int RT, bool ROWS>
-__global__ __launch_bounds__(WAVES * 64, NC == 4 || sizeof(T) == 4 ? 1 : 2) void attention_cache_kernel(AttArgs a) {
-    constexpr int R = 16 * RT * (ROWS ? WAVES : 1);  // rows of a tile
+template <class T, int NC, bool ROWS>
+__global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 || sizeof(T) == 4 ? 1 : ROWS ? 4 : 2) void attention_cache_kernel(AttArgs a) {
+    constexpr int WAVES = ROWS ? ROWS_WAVES : KEYS_WAVES, R = ROWS ? MANY_ROWS : KEYS_ROWS;  // rows of a tile
     __shared__ f16x8 stages[ROWS ? 2 : 1][ROWS ? 16 * NC : 1][64];
     __shared__ f32x4 others[ROWS ? 1 : WAVES][ROWS ? 1 : NC * 4][64];
     __shared__ float2 stats[ROWS ? 1 : WAVES][16];
@@ -520,14 +520,14 @@ __global__ __launch_bounds__(WAVES * 64, NC == 4 || sizeof(T) == 4 ? 1 : 2) void
     int s;
     long base, tile_base;
     if (!scan.locate(a, at, seq, s, base, tile_base)) return;
-    Wave<T, NC, RT> w;
+    Wave<T, NC> w;
     for (;;) {
         const long after = base + seq.cost();
         while (at < last && at < after) {
             const long tile = (at - base) / seq.pages;
             const int first = (int)(at - base - tile * seq.pages), end = (int)min(seq.pages, first + (last - at));
             const bool whole = first == 0 && end == seq.pages;
-            const long rows = (long)seq.n * a.group, row0 = tile * R + (ROWS ? wave * 16 * RT : 0), slot = run + tile_base + tile;
+            const long rows = (long)seq.n * a.group, row0 = tile * R + (ROWS ? wave * 16 : 0), slot = run + tile_base + tile;
             if (first == 0 && head == 0 && threadIdx.x == 0) {  // (the tile's first page: every head's parts are alike)
                 const long from = base + tile * seq.pages, to = from + seq.pages - 1;
                 const int parts = (int)(to / length - from / length) + 1;
@@ -535,63 +535,58 @@ __global__ __launch_bounds__(WAVES * 64, NC == 4 || sizeof(T) == 4 ? 1 : 2) void
             }
             w.begin(a, seq, head, row0, rows);
             if constexpr (ROWS) {
-                // what the tile's last row sees: all four waves go through as many pages
-                const int t = (int)((min((tile + 1) * R, rows) - 1) / a.group);
+                // what the tile's last row sees: all waves go through as many pages
+                const int t = ((int)min((tile + 1) * R, rows) - 1) / a.group;
                 const long sees = min(max(a.causal ? t + seq.len - seq.n + 1 : seq.len, 0L), (long)seq.keys);
-                w.pages_together(a, s, head, first, min(end, (int)((sees + PAGE - 1) / PAGE)), wave, stages);
+                const int upto = min(end, (int)((sees + PAGE - 1) / PAGE));
+                for (int i = first; i < upto; i += 64) w.pages_together(a, s, head, i, min(64, upto - i), wave, stages);
             } else {
-                w.pages(a, s, head, first + wave, end, WAVES);
+                const int upto = min(end, w.most());
+                for (int i = first + wave; i < upto; i += 64 * WAVES) w.pages(a, s, head, i, min(64, (upto - i + WAVES - 1) / WAVES), WAVES);
             }
             at += end - first;
+            w.sum = row_sum(w.sum);
+            if constexpr (!ROWS) {
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                w.sum[j] += __shfl_xor(w.sum[j], 16);
-                w.sum[j] += __shfl_xor(w.sum[j], 32);
-            }
-            if constexpr (!ROWS) {  // (RT is 1)
-#pragma unroll
-                for (int i = 0; i < NC * 4; ++i) others[wave][i][lane] = w.o[0][i];
-                if (g == 0) stats[wave][r] = make_float2(w.m[0], w.sum[0]);
+                for (int i = 0; i < NC * 4; ++i) others[wave][i][lane] = w.o[i];
+                if (g == 0) stats[wave][r] = make_float2(w.m, w.sum);
                 __syncthreads();
                 float top = -INFINITY, by[WAVES];
 #pragma unroll
                 for (int k = 0; k < WAVES; ++k) top = fmaxf(top, stats[k][r].x);
                 const float from = top == -INFINITY ? 0.f : top;
-                w.m[0] = top, w.sum[0] = 0.f;
+                w.m = top, w.sum = 0.f;
 #pragma unroll
                 for (int k = 0; k < WAVES; ++k) {
                     by[k] = __builtin_amdgcn_exp2f(stats[k][r].x - from);
-                    w.sum[0] += stats[k][r].y * by[k];
+                    w.sum += stats[k][r].y * by[k];
                 }
 #pragma unroll
                 for (int i = 0; i < NC * 4; ++i) {
                     if (i % WAVES != wave) continue;
-                    w.o[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    w.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < WAVES; ++k) w.o[0][i] += others[k][i][lane] * by[k];
+                    for (int k = 0; k < WAVES; ++k) w.o[i] += others[k][i][lane] * by[k];
                 }
                 __syncthreads();
             }
+            const long row = row0 + r;
+            if (row >= rows) continue;
+            if (whole) {
+                const int t = (int)row / a.group, h = head * a.group + (int)row - t * a.group;
+                T *to = (T *)a.o + (seq.q0 + (long)t) * a.ldo + (long)h * a.c.dim;
+                const float inv = w.sum == 0.f ? 0.f : 1.f / w.sum;
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                const long row = row0 + 16 * j + r;
-                if (row >= rows) continue;
-                if (whole) {
-                    const int t = (int)(row / a.group), h = head * a.group + (int)(row - (long)t * a.group);
-                    T *to = (T *)a.o + (seq.q0 + (long)t) * a.ldo + (long)h * a.c.dim;
-                    const float inv = w.sum[j] == 0.f ? 0.f : 1.f / w.sum[j];
+                for (int i = 0; i < NC * 4; ++i)
+                    if (ROWS || i % WAVES == wave) put<T>(a, to, i * 16 + g * 4, w.o[i], inv);
+                if (a.lse && g == 0 && (ROWS || wave == 0)) a.lse[(long)h * a.c.tokens + seq.q0 + t] = w.sum == 0.f ? -INFINITY : (w.m + log2f(w.sum)) * LN2;
+            } else {
+                const long place = (slot * a.c.kv_heads + head) * R + (row - tile * R);
+                float *to = a.part + place * a.part_ld;
 #pragma unroll
-                    for (int i = 0; i < NC * 4; ++i)
-                        if (ROWS || i % WAVES == wave) put<T>(a, to, i * 16 + g * 4, w.o[j][i], inv);
-                    if (a.lse && g == 0 && (ROWS || wave == 0)) a.lse[(long)h * a.c.tokens + seq.q0 + t] = w.sum[j] == 0.f ? -INFINITY : (w.m[j] + log2f(w.sum[j])) * LN2;
-                } else {
-                    const long place = (slot * a.c.kv_heads + head) * R + (row - tile * R);
-                    float *to = a.part + place * a.part_ld;
-#pragma unroll
-                    for (int i = 0; i < NC * 4; ++i)
-                        if ((ROWS || i % WAVES == wave) && i * 16 + g * 4 < a.part_ld) *(f32x4 *)(to + i * 16 + g * 4) = w.o[j][i];
-                    if (g == 0 && (ROWS || wave == 0)) *(float2 *)(a.part_ml + place * 2) = make_float2(w.m[j], w.sum[j]);
-                }
+                for (int i = 0; i < NC * 4; ++i)
+                    if ((ROWS || i % WAVES == wave) && i * 16 + g * 4 < a.part_ld) *(f32x4 *)(to + i * 16 + g * 4) = w.o[i];
+                if (g == 0 && (ROWS || wave == 0)) *(float2 *)(a.part_ml + place * 2) = make_float2(w.m, w.sum);
             }
         }
         if (at >= last) return;
@@ -635,8 +630,6 @@ __global__ __launch_bounds__(256) void attention_cache_join_kernel(AttArgs a) {
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
-enum { KEYS_ROWS = 16, MANY_ROWS = 128 };
-
 // How a call runs: rows of a tile, runs of a kv head, tiles of all sequences at most, and slots of partial sums (a run's and a tile's numbers added: each
 // step from piece to piece of the list is to the next run or the next tile, so no two pieces share a slot).
 struct Plan {
@@ -651,7 +644,7 @@ Plan plan_of(int dtype, int sequences, int tokens, int table_pages, int heads, i
     p.rows = dtype == D8_FLOAT16 && dim <= 128 && some && all / some >= 64;
     p.tile = p.rows ? MANY_ROWS : KEYS_ROWS;
     p.units = all / p.tile + some;
-    const long at_once = (2L * cu_count() + kv_heads - 1) / kv_heads, most = (p.units * (table_pages ? table_pages : 1) + WAVES - 1) / WAVES;
+    const long at_once = (2L * cu_count() + kv_heads - 1) / kv_heads, most = (p.units * (table_pages ? table_pages : 1) + KEYS_WAVES - 1) / KEYS_WAVES;
     p.runs = (int)(at_once < most ? at_once : most);
     p.slots = p.units + p.runs;
     return p;
@@ -667,11 +660,11 @@ void launch(const AttArgs &a, const Plan &p, hipStream_t stream) {
     const dim3 grid((unsigned)(p.runs * a.c.kv_heads));
     if constexpr (sizeof(T) == 2 && NC <= 2) {
         if (p.rows) {
-            hipLaunchKernelGGL((attention_cache_kernel<T, NC, 2, true>), grid, dim3(WAVES * 64), 0, stream, a);
+            hipLaunchKernelGGL((attention_cache_kernel<T, NC, true>), grid, dim3(ROWS_WAVES * 64), 0, stream, a);
             return;
         }
     }
-    hipLaunchKernelGGL((attention_cache_kernel<T, NC, 1, false>), grid, dim3(WAVES * 64), 0, stream, a);
+    hipLaunchKernelGGL((attention_cache_kernel<T, NC, false>), grid, dim3(KEYS_WAVES * 64), 0, stream, a);
 }
 
 template <class T>
