@@ -33,33 +33,7 @@ struct Args {
     Pages c;
     void *k, *v;
     long ldk, ldv;
-    int window;  // rows of a call whose pages a workgroup looks after
 };
-
-// Row r's sequence: the last that starts at or before it, a start that lies before an earlier one counting as that one; its place in the
-// sequence's tokens as the cache holds them, and the rows from it on that are its sequence's.  false: a row of no sequence.  All lanes take part.
-__device__ __forceinline__ bool find(const Pages &c, int r, int &s, long &place, int &rows, bool &first) {
-    const int lane = threadIdx.x & 63;
-    int top = 0;
-    for (int from = 0; from <= c.sequences; from += 64) {
-        const int at = from + lane, start = at <= c.sequences ? c.starts[at] : 0x7fffffff;
-        const unsigned long long past = __ballot(start > r);
-        const int n = past ? __ffsll((long long)past) - 1 : 64;  // starts of this piece at or before r
-        int most = lane < n ? max(start, 0) : 0;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
-        top = max(top, most);
-        if (!past) continue;
-        s = __builtin_amdgcn_readfirstlane(from + n - 1);
-        if (s < 0 || s >= c.sequences) return false;
-        const int end = min(c.starts[s + 1], c.tokens);
-        rows = __builtin_amdgcn_readfirstlane(end - r);
-        place = (long)max(c.lengths[s], 0) - rows;
-        first = r == __builtin_amdgcn_readfirstlane(top);
-        return true;
-    }
-    return false;
-}
 
 __device__ __forceinline__ unsigned size_of(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
@@ -87,42 +61,47 @@ template <class T>
 struct Piece<T, 1> {
     typedef T type;
 };
-template <class T, int V>
-__device__ __forceinline__ void load(const T *p, float (&x)[V]) {
-    const typename Piece<T, V>::type v = *(const typename Piece<T, V>::type *)p;
-    if constexpr (V == 1) {
-        x[0] = (float)v;
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = (float)v[e];
-    }
-}
-
 __device__ __forceinline__ unsigned code_of(float x, float back) { return (unsigned)(int)rintf(x * back) & 255u; }  // (exact but for the rounding)
 
 enum { WORDS = 17 };  // words of LDS between two elements' 16 of tokens: four elements of one token in different banks
 
 // Rows r .. r + rows - 1 of the call are places slot .. of `page`, which holds `slot` tokens already (or none that count).  V: elements of a 16-byte
-// piece, or 1 where rows cannot be moved in such.
+// piece, or 1 where rows cannot be moved in such.  An item is a piece of four tokens, of keys and of values: a word of codes of each of its elements.
 template <class T, int V>
 __device__ __forceinline__ void append(const Args &a, int r, int rows, int slot, int page, int head, unsigned *sizes, unsigned *words) {
     const Pages &c = a.c;
-    const int tid = threadIdx.x, pieces = c.dim / V;
+    typedef typename Piece<T, V>::type piece;
+    const int tid = threadIdx.x, pieces = c.dim / V, first = slot >> 2, items = (((slot + rows - 1) >> 2) - first + 1) * pieces;
     const T *k = (const T *)a.k + (long)r * a.ldk + (long)head * c.dim, *v = (const T *)a.v + (long)r * a.ldv + (long)head * c.dim;
     float *ks = c.k_scales + (long)page * c.kv_heads + head, *vs = c.v_scales + (long)page * c.kv_heads + head;
-    // the largest of both
-    unsigned k_size = 0, v_size = 0;
-    for (int i = tid; i < rows * pieces; i += 256) {
-        const int row = i / pieces, d = (i - row * pieces) * V;
-        float x[V], y[V];
-        load<T, V>(k + row * a.ldk + d, x), load<T, V>(v + row * a.ldv + d, y);
+    piece kx[4], vx[4];
+    auto load = [&](int i) {  // (rows that are not there: zeros)
+        const int word = i / pieces, d = (i - word * pieces) * V, row = (first + word) * 4 - slot;
 #pragma unroll
-        for (int e = 0; e < V; ++e) k_size = max(k_size, size_of(x[e])), v_size = max(v_size, size_of(y[e]));
+        for (int j = 0; j < 4; ++j) {
+            kx[j] = vx[j] = piece{};
+            if (row + j >= 0 && row + j < rows) kx[j] = *(const piece *)(k + (row + j) * a.ldk + d), vx[j] = *(const piece *)(v + (row + j) * a.ldv + d);
+        }
+    };
+    auto at = [&](const piece &x, int e) {
+        if constexpr (V == 1) return (float)x;
+        else return (float)x[e];
+    };
+    // the largest of both; a thread's last item stays in its registers
+    unsigned k_size = 0, v_size = 0;
+    int held = -1;
+    for (int i = tid; i < items; i += 256) {
+        load(i);
+        held = i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) k_size = max(k_size, size_of(at(kx[j], e))), v_size = max(v_size, size_of(at(vx[j], e)));
     }
+    if (tid == 0) sizes[8] = slot ? __float_as_uint(*ks) : 0u, sizes[9] = slot ? __float_as_uint(*vs) : 0u;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) k_size = max(k_size, (unsigned)__shfl_xor((int)k_size, d)), v_size = max(v_size, (unsigned)__shfl_xor((int)v_size, d));
     if ((tid & 63) == 0) sizes[tid >> 6] = k_size, sizes[4 + (tid >> 6)] = v_size;
-    if (tid == 0) sizes[8] = slot ? __float_as_uint(*ks) : 0u, sizes[9] = slot ? __float_as_uint(*vs) : 0u;
     for (int i = tid; i < c.pitch * WORDS; i += 256) words[i] = 0;
     __syncthreads();
     const float k_old = __uint_as_float(sizes[8]), v_old = __uint_as_float(sizes[9]);
@@ -133,35 +112,30 @@ __device__ __forceinline__ void append(const Args &a, int r, int rows, int slot,
     const float v_scale = v_need != v_need || v_old != v_old ? __uint_as_float(0x7fc00000u) : fmaxf(v_need, v_old);
     if (tid == 0) *ks = k_scale, *vs = v_scale;
     const float k_back = k_scale == k_scale ? 1.f / k_scale : 0.f, v_back = v_scale == v_scale ? 1.f / v_scale : 0.f;
+    const bool k_good = k_size < 0x7f800000u, v_good = v_size < 0x7f800000u;
     signed char *k_to = c.k_codes + c.tile(page, head), *v_to = c.v_codes + c.tile(page, head);
-    // values' words of four tokens: thread by piece and word; keys beside them
-    const int first = slot >> 2, last = (slot + rows - 1) >> 2;
-    for (int i = tid; i < (last - first + 1) * pieces; i += 256) {
+    for (int i = held; i >= 0; i -= 256) {
+        if (i != held) load(i);
         const int word = i / pieces, d = (i - word * pieces) * V;
         unsigned w[V] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int at = (first + word) * 4 + j, row = at - slot;
-            if (row < 0 || row >= rows) continue;
-            float x[V];
-            load<T, V>(k + row * a.ldk + d, x);
-            signed char *to = k_to + at * c.pitch + d;
+            const int place = (first + word) * 4 + j;
+            if (v_good)
+#pragma unroll
+                for (int e = 0; e < V; ++e) w[e] |= code_of(at(vx[j], e), v_back) << (8 * j);
+            if (place < slot || place >= slot + rows) continue;
+            signed char *to = k_to + place * c.pitch + d;
             if constexpr (V == 1) {
-                *to = (signed char)(k_size < 0x7f800000u ? code_of(x[0], k_back) : 0u);
+                *to = (signed char)(k_good ? code_of(at(kx[j], 0), k_back) : 0u);
             } else {
                 unsigned q[V / 4];
 #pragma unroll
-                for (int e = 0; e < V; e += 4) {
-                    q[e / 4] = code_of(x[e], k_back) | code_of(x[e + 1], k_back) << 8 | code_of(x[e + 2], k_back) << 16 | code_of(x[e + 3], k_back) << 24;
-                    if (k_size >= 0x7f800000u) q[e / 4] = 0;
-                }
+                for (int e = 0; e < V; e += 4)
+                    q[e / 4] = !k_good ? 0u : code_of(at(kx[j], e), k_back) | code_of(at(kx[j], e + 1), k_back) << 8 | code_of(at(kx[j], e + 2), k_back) << 16 | code_of(at(kx[j], e + 3), k_back) << 24;
                 if constexpr (V == 8) *(uint2 *)to = make_uint2(q[0], q[1]);
                 else *(unsigned *)to = q[0];
             }
-            load<T, V>(v + row * a.ldv + d, x);
-            if (v_size < 0x7f800000u)
-#pragma unroll
-                for (int e = 0; e < V; ++e) w[e] |= code_of(x[e], v_back) << (8 * j);
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) words[(d + e) * WORDS + first + word] = w[e];
@@ -197,35 +171,63 @@ __device__ __forceinline__ void append(const Args &a, int r, int rows, int slot,
         }
         *(i32x4 *)(v_to + i * 16) = w;
     }
-    __syncthreads();  // (the next page takes the same LDS)
 }
 
-// body(row, rows, slot, page, head) for the pages that begin in a workgroup's rows of the call, or go on there from what the cache held: each
-// is one workgroup's; page -1: none.
-template <class Body>
-__device__ __forceinline__ void for_pages(const Args &a, Body &&body) {
-    const int head = blockIdx.x % a.c.kv_heads, from = blockIdx.x / a.c.kv_heads * a.window, to = min(from + a.window, a.c.tokens);
-    for (int r = from; r < to;) {
-        int s, rows;
-        long place;
-        bool first;
-        if (!find(a.c, r, s, place, rows, first)) {
-            ++r;
-            continue;
+// The workgroup's share of a call: rows row .. row + rows - 1 are places slot .. of `page` (-1: none) of one sequence, all that the call brings to it.
+struct Share {
+    int row, rows, slot, page;
+};
+
+// Share number `id` of the call, sequence by sequence and page by page; false beyond the last.  A start that lies before an earlier one counts
+// as that one.  All lanes of a wave take part, 64 sequences at a time.
+__device__ __forceinline__ bool share_of(const Pages &c, int id, Share &share) {
+    const int lane = threadIdx.x & 63;
+    int before = 0, top = 0;
+    for (int from = 0; from < c.sequences; from += 64) {
+        const int at = min(from + lane, c.sequences), next = min(from + lane + 1, c.sequences);
+        int first = min(max(c.starts[at], 0), c.tokens), end = min(max(c.starts[next], 0), c.tokens);
+        const long length = at < c.sequences ? max(c.lengths[at], 0) : 0;
+        if (__ballot(first < top || end < first)) {
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int other = __shfl_up(first, d);
+                first = lane >= d ? max(first, other) : first;
+            }
+            first = max(first, top), end = max(end, first);
         }
-        const int slot = (int)(place & (PAGE - 1)), n = min(PAGE - slot, rows);
-        if (first || slot == 0) body(r, n, slot, place >> 6 < a.c.table_pages ? a.c.page_of(s, place < 0 ? -1 : (int)(place >> 6)) : -1, head);
-        r += n;
+        top = __builtin_amdgcn_readlane(end, 63);
+        const int n = end - first;
+        const long place = length - n;  // of the first row; before 0 where the cache holds fewer tokens than the call brings
+        const int pages = n ? (int)((place & (PAGE - 1)) + n + PAGE - 1) / PAGE : 0;
+        int upto = pages;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int other = __shfl_up(upto, d);
+            upto += lane >= d ? other : 0;
+        }
+        const unsigned long long past = __ballot(before + upto > id);
+        if (past) {
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)past) - 1), s = from + l;
+            const int number = id - before - __builtin_amdgcn_readlane(upto - pages, l), slot0 = __builtin_amdgcn_readlane((int)(place & (PAGE - 1)), l);
+            const int page0 = __builtin_amdgcn_readlane((int)(place >> 6), l), rows = __builtin_amdgcn_readlane(n, l);
+            const int skipped = number ? number * PAGE - slot0 : 0;
+            share.row = __builtin_amdgcn_readlane(first, l) + skipped;
+            share.slot = number ? 0 : slot0;
+            share.rows = min(PAGE - share.slot, rows - skipped);
+            share.page = c.page_of(s, page0 + number);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
+    return false;
 }
 
 template <class T, int V>
 __global__ __launch_bounds__(256) void cache_append_kernel(Args a) {
     __shared__ unsigned sizes[10];  // of four waves' keys and values, and the scales before
     __shared__ unsigned words[MOST_DIM * WORDS];
-    for_pages(a, [&](int r, int rows, int slot, int page, int head) {
-        if (page >= 0) append<T, V>(a, r, rows, slot, page, head, sizes, words);
-    });
+    Share s;
+    if (share_of(a.c, blockIdx.x / a.c.kv_heads, s) && s.page >= 0) append<T, V>(a, s.row, s.rows, s.slot, s.page, blockIdx.x % a.c.kv_heads, sizes, words);
 }
 
 template <class T, int V>
@@ -268,6 +270,7 @@ __device__ __forceinline__ void read(const Args &a, int r, int rows, int slot, i
         }
         __syncthreads();
     }
+#pragma unroll 4
     for (int i = tid; i < rows * pieces; i += 256) {
         const int row = i / pieces, d = (i - row * pieces) * V, t = slot + row;
         float x[V] = {}, y[V] = {};
@@ -285,20 +288,19 @@ __device__ __forceinline__ void read(const Args &a, int r, int rows, int slot, i
         }
         store<T, V>(k + row * a.ldk + d, x), store<T, V>(v + row * a.ldv + d, y);
     }
-    __syncthreads();  // (the next page takes the same LDS)
 }
 
 template <class T, int V>
 __global__ __launch_bounds__(256) void cache_read_kernel(Args a) {
     __shared__ unsigned words[MOST_DIM * WORDS];
-    for_pages(a, [&](int r, int rows, int slot, int page, int head) { read<T, V>(a, r, rows, slot, page, head, words); });
+    Share s;
+    if (share_of(a.c, blockIdx.x / a.c.kv_heads, s)) read<T, V>(a, s.row, s.rows, s.slot, s.page, blockIdx.x % a.c.kv_heads, words);
 }
 
-// A workgroup looks after a quarter of a sequence's rows in the mean, 16 at most: with one it would be mostly looking for its sequence where pages
-// are filled, and with many go through many pages one after the other where they get a token each.
-int window_of(const Pages &c) {
-    const int mean = c.tokens / c.sequences / 4;
-    return mean < 1 ? 1 : mean > 16 ? 16 : mean;
+// Workgroups of a call: n rows of a sequence reach (n + 62) / 64 + 1 pages at most, and each at least one.
+dim3 grid_of(const Pages &c) {
+    const long some = c.sequences < c.tokens ? c.sequences : c.tokens, shares = (c.tokens + 62 * some) / 64 + some;
+    return dim3((unsigned)((shares < c.tokens ? shares : c.tokens) * c.kv_heads));
 }
 
 int check_rows(const Args &a, const char *name) {
@@ -336,13 +338,12 @@ extern "C" int d8_cache_append(int dtype, const void *k, long ldk, const void *v
                                float *v_scales, const int *starts, const int *lengths, const int *table, int sequences, int tokens, int table_pages, int pages,
                                int kv_heads, int dim, void *stream) {
     cache::Args a = {{k_codes, v_codes, k_scales, v_scales, starts, lengths, table, sequences, tokens, table_pages, pages, kv_heads, dim, (int)cache::pitch_of(dim)},
-                     (void *)k, (void *)v, ldk, ldv, 1};
+                     (void *)k, (void *)v, ldk, ldv};
     if (int rc = cache::check(a.c, dtype, "cache_append")) return rc;
     if (!sequences || !tokens) return 0;
     if (int rc = cache::check_rows(a, "cache_append")) return rc;
     if (!pages || !table_pages) return 0;
-    a.window = cache::window_of(a.c);
-    const dim3 grid((unsigned)(ceil_div(tokens, a.window) * (long)kv_heads));
+    const dim3 grid = cache::grid_of(a.c);
     if (dtype == D8_FLOAT16) cache::launch_append<f16>(a, grid, as_stream(stream));
     else cache::launch_append<float>(a, grid, as_stream(stream));
     D8_LAUNCH_CHECK();
@@ -354,12 +355,11 @@ extern "C" int d8_cache_read(int dtype, void *k, long ldk, void *v, long ldv, co
                              int kv_heads, int dim, void *stream) {
     cache::Args a = {{(signed char *)k_codes, (signed char *)v_codes, (float *)k_scales, (float *)v_scales, starts, lengths, table, sequences, tokens, table_pages, pages,
                       kv_heads, dim, (int)cache::pitch_of(dim)},
-                     k, v, ldk, ldv, 1};
+                     k, v, ldk, ldv};
     if (int rc = cache::check(a.c, dtype, "cache_read")) return rc;
     if (!sequences || !tokens) return 0;
     if (int rc = cache::check_rows(a, "cache_read")) return rc;
-    a.window = cache::window_of(a.c);
-    const dim3 grid((unsigned)(ceil_div(tokens, a.window) * (long)kv_heads));
+    const dim3 grid = cache::grid_of(a.c);
     if (dtype == D8_FLOAT16) cache::launch_read<f16>(a, grid, as_stream(stream));
     else cache::launch_read<float>(a, grid, as_stream(stream));
     D8_LAUNCH_CHECK();

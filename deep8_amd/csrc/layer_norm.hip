@@ -93,7 +93,7 @@ __global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T))) void layer_no
     constexpr int THREADS = grad_threads(TEAM, V, E * sizeof(T)), TEAMS = THREADS / TEAM;
     constexpr bool AHEAD = TEAM < 1024 || E == 8;  // the next row's loads on their way
     __shared__ float2 slots[2 * 16];
-    __shared__ float sums[TEAMS > 1 ? THREADS : 1];
+    __shared__ float sums[TEAMS > 1 ? THREADS * E : 1];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     typedef Held<T, V, TEAM, E> H;
     H w, x, dy;
@@ -152,20 +152,24 @@ __global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T))) void layer_no
     if (!a.partial) return;  // uniform over the workgroup
     float *to = a.partial + (long)blockIdx.x * 2 * a.cols;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = (t + TEAM * (e / V)) * V + e % V;
+    for (int k = 0; k < 2; ++k) {
+        if constexpr (TEAMS == 1) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float s = k ? db[e] : dw[e];
-            if constexpr (TEAMS > 1) {
-                __syncthreads();
-                sums[threadIdx.x] = s;
-                __syncthreads();
-                s = 0.f;
-                if (team == 0)
-                    for (int i = 0; i < TEAMS; ++i) s += sums[i * TEAM + t];
+            for (int e = 0; e < E; ++e) {
+                const int c = (t + TEAM * (e / V)) * V + e % V;
+                if (c < a.cols) to[(long)k * a.cols + c] = k ? db[e] : dw[e];
             }
-            if (team == 0 && c < a.cols) to[(long)k * a.cols + c] = s;
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e) sums[team * (TEAM * E) + (t + TEAM * (e / V)) * V + e % V] = k ? db[e] : dw[e];
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.cols; c += THREADS) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < TEAMS; ++i) s += sums[i * (TEAM * E) + c];
+                to[(long)k * a.cols + c] = s;
+            }
         }
     }
 }
