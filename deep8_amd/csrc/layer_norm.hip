@@ -86,10 +86,10 @@ __global__ __launch_bounds__(forward_threads(TEAM)) void layer_norm_kernel(NormA
 
 // Threads of a gradient workgroup: 1024 where what a thread keeps (its columns' sums, weights, this row's and the next one's elements) fits in
 // the 128 registers that leaves it, else 512.
-constexpr int grad_threads(int team, int v, int bytes) { return team == 1024 || (v > 1 && bytes <= 32) ? 1024 : 512; }
+constexpr int grad_threads(int team, int v, int bytes) { return team == 1024 ? 1024 : 512; }
 
 template <class T, int V, int TEAM, int E>
-__global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T))) void layer_norm_grad_kernel(NormArgs a) {
+__global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T)), V > 1 && E * sizeof(T) <= 32 ? 4 : 1) void layer_norm_grad_kernel(NormArgs a) {
     constexpr int THREADS = grad_threads(TEAM, V, E * sizeof(T)), TEAMS = THREADS / TEAM;
     constexpr bool AHEAD = TEAM < 1024 || E == 8;  // the next row's loads on their way
     __shared__ float2 slots[2 * 16];
@@ -300,8 +300,8 @@ void launch_grad(NormArgs &a, bool vec, hipStream_t stream) {
         return;
     }
     with_team<T>(vec, a.cols, [&](auto v, auto team, auto e) {
-        constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = grad_threads(TEAM, V, E * sizeof(T));
-        const long want = ((long)a.rows * TEAM + THREADS - 1) / THREADS, most = 1024L / THREADS * cu_count();
+        constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = grad_threads(TEAM, V, E * sizeof(T)), AT_ONCE = THREADS == 1024 || V == 1 || E * sizeof(T) > 32 ? 1 : 2;
+        const long want = ((long)a.rows * TEAM + THREADS - 1) / THREADS, most = (long)AT_ONCE * cu_count();
         a.groups = (int)(want < most ? want : most);
         hipLaunchKernelGGL((layer_norm_grad_kernel<T, V, TEAM, E>), dim3((unsigned)a.groups), dim3(THREADS), 0, stream, a);
     });
