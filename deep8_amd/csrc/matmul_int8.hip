@@ -6,8 +6,8 @@
 //                              of v_mfma_i32_16x16x64_i8 (32 columns of w as left operand, all rows of x as right one); eight waves
 //                              share out the steps of the reduction and join through LDS
 //   many rows and columns      matmul_int8_wide.hip
-//   between                    tiles of 128 x 128 or 64 x 64 through LDS, cut along the reduction where they leave compute units idle
-// In all three w is the left operand, so a lane ends up with four columns of a row side by side.
+//   between                    tiles of 64 x 64 through LDS, cut along the reduction where they leave compute units idle and it is long
+// Where w is the left operand, a lane ends up with four columns of a row side by side.
 #include "int8.h"
 
 namespace d8 {
@@ -70,23 +70,32 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < RT; ++j) x[j] = a.x + (long)min(16 * j + r, a.rows - 1) * a.pitch + at;
     i32x4 acc[2][RT] = {};
-#pragma unroll 4
-    for (int s = first + wave; s < end; s += ROWS_WAVES) {
-        const long k = (long)s * STEP;
-        i32x4 fw[2][2], fx[RT][2];
+    // the loads of several steps at once (those beyond the last: it again, not multiplied)
+    constexpr int U = RT == 1 ? 4 : 2;
+    for (int s = first + wave; s < end; s += ROWS_WAVES * U) {
+        i32x4 fw[U][2][2], fx[U][RT][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int u = 0; u < U; ++u) {
+            const long k = (long)min(s + ROWS_WAVES * u, end - 1) * STEP;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) fw[i][h] = *(const i32x4 *)(w[i] + k + 64 * h);
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int j = 0; j < RT; ++j) fx[j][h] = *(const i32x4 *)(x[j] + k + 64 * h);
+                for (int i = 0; i < 2; ++i) fw[u][i][h] = *(const i32x4 *)(w[i] + k + 64 * h);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) fx[u][j][h] = *(const i32x4 *)(x[j] + k + 64 * h);
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int u = 0; u < U; ++u) {
+            if (s + ROWS_WAVES * u >= end) break;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < RT; ++j) mma(acc[i][j], fw[i][h], fx[j][h]);
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) mma(acc[i][j], fw[u][i][h], fx[u][j][h]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -102,11 +111,18 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
 }
 
 // ---- tiles ----------------------------------------------------------------------------------------------------------
-// B x B of z a workgroup, four waves of B / 2 x B / 2.  Two stages of LDS; a step of the reduction is fetched into registers while the one before is computed.
-// Rows of 128 bytes, 16-byte piece c of row r at position c ^ (r / 2 % 8): the 16 rows of a fragment then take all banks in turn.
-template <class T, int B>
+// 64 x 64 of z a workgroup, four waves of 32 x 32.  Two stages of LDS; the three steps of the reduction after the next are on their way into registers: a
+// workgroup alone on its compute unit would else take as long as memory answers for each (65 x 4096 x 4096: 13.2 us, 16.3 with one ahead).
+// Rows of 128 bytes, 16-byte piece c of row r at position c ^ (r / 2 % 8): the 16 rows of a fragment then take all banks in turn.  Bound by LDS where
+// there are many tiles: two fragments read for each two products, 1000 TOP/s (1024 x 4096 x 4096 in 33 us; tiles of 128 x 128, of which fewer fit a compute
+// unit: 35, and 14 for 8.5 at 777 x 1024 x 1352).
+// QUADS: w is the left operand, a lane has four columns of a row; else x is, and 16 lanes have a row's columns side by side, which is what rows of z that cannot
+// be stored four elements at a time want (777 x 1000 x 1351 in single: 64 separate words a store before, 11 us for 9.2).
+enum { TILE = 64 };
+
+template <class T, bool QUADS>
 __global__ __launch_bounds__(256) void int8_tile_kernel(Args a) {
-    constexpr int F = B / 32, PIECES = B * STEP / 16 / 256;
+    constexpr int B = TILE, F = B / 32, PIECES = B * STEP / 16 / 256;
     __shared__ __attribute__((aligned(16))) signed char lds[2][2][B * STEP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
     const int tilesM = (a.rows + B - 1) / B, tilesN = (a.cols + B - 1) / B;
@@ -124,49 +140,69 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(Args a) {
         from[1][i] = a.x + (long)min(m0 + row, a.rows - 1) * a.pitch + c * 16;
         to[i] = row * STEP + ((c ^ (row >> 1 & 7)) << 4);
     }
-    i32x4 ahead[2][PIECES], acc[F][F] = {};
-    auto fetch = [&](int s) {
+    constexpr int D = 3;
+    i32x4 ahead[D][2][PIECES], acc[F][F] = {};
+    auto fetch = [&](i32x4 (&to)[2][PIECES], int s) {
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) ahead[o][i] = *(const i32x4 *)(from[o][i] + (long)s * STEP);
+            for (int i = 0; i < PIECES; ++i) to[o][i] = *(const i32x4 *)(from[o][i] + (long)s * STEP);
     };
-    auto stage = [&](int at) {
+    auto stage = [&](const i32x4 (&x)[2][PIECES], int at) {
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) *(i32x4 *)(lds[at][o] + to[i]) = ahead[o][i];
+            for (int i = 0; i < PIECES; ++i) *(i32x4 *)(lds[at][o] + to[i]) = x[o][i];
     };
     const int r = lane & 15, j = lane >> 4, sw = r >> 1 & 7;
-    if (first < end) {
-        fetch(first);
-        stage(0);
-        if (first + 1 < end) fetch(first + 1);
-        __syncthreads();
-        for (int s = first, at = 0; s < end; ++s, at ^= 1) {
+    // step s, which is in LDS; step s + 1 from `next` into LDS, step s + 1 + D on its way there
+    auto step = [&](int s, i32x4 (&next)[2][PIECES]) {
+        const int at = (s - first) & 1;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                i32x4 fw[F], fx[F];
-                const int c = ((j + 4 * h) ^ sw) << 4;
+        for (int h = 0; h < 2; ++h) {
+            i32x4 fw[F], fx[F];
+            const int c = ((j + 4 * h) ^ sw) << 4;
 #pragma unroll
-                for (int i = 0; i < F; ++i) {
-                    fw[i] = *(const i32x4 *)(lds[at][0] + (wn * (B / 2) + 16 * i + r) * STEP + c);
-                    fx[i] = *(const i32x4 *)(lds[at][1] + (wm * (B / 2) + 16 * i + r) * STEP + c);
-                }
-#pragma unroll
-                for (int i = 0; i < F; ++i)
-#pragma unroll
-                    for (int k = 0; k < F; ++k) mma(acc[i][k], fw[i], fx[k]);
+            for (int i = 0; i < F; ++i) {
+                fw[i] = *(const i32x4 *)(lds[at][0] + (wn * (B / 2) + 16 * i + r) * STEP + c);
+                fx[i] = *(const i32x4 *)(lds[at][1] + (wm * (B / 2) + 16 * i + r) * STEP + c);
             }
-            if (s + 1 < end) stage(at ^ 1);
-            if (s + 2 < end) fetch(s + 2);
-            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int k = 0; k < F; ++k) mma(acc[i][k], QUADS ? fw[i] : fx[k], QUADS ? fx[k] : fw[i]);
         }
+        // (steps beyond the last: it again, not computed.  Without conditions the compiler knows how many loads are on their way and waits for no more
+        // than it needs.)
+        stage(next, at ^ 1);
+        fetch(next, min(s + 1 + D, end - 1));
+        __syncthreads();
+    };
+    if (first < end) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) fetch(ahead[d], min(first + d, end - 1));
+        stage(ahead[0], 0);
+        fetch(ahead[0], min(first + D, end - 1));
+        __syncthreads();
+        int s = first;
+        for (; s + D <= end; s += D) step(s, ahead[1]), step(s + 1, ahead[2]), step(s + 2, ahead[0]);
+        if (s < end) step(s, ahead[1]);
+        if (s + 1 < end) step(s + 1, ahead[2]);
     }
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
-        for (int k = 0; k < F; ++k) put<T>(a, part, m0 + wm * (B / 2) + 16 * k + r, n0 + wn * (B / 2) + 16 * i + j * 4, acc[i][k]);
+        for (int k = 0; k < F; ++k) {
+            const int m = m0 + wm * (B / 2) + 16 * k, n = n0 + wn * (B / 2) + 16 * i;
+            if constexpr (QUADS) {
+                put<T>(a, part, m + r, n + j * 4, acc[i][k]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (m + j * 4 + e < a.rows && n + r < a.cols)
+                        ((T *)a.z)[(long)(m + j * 4 + e) * a.ldz + n + r] = scaled<T>(acc[i][k][e], a.x_scales[m + j * 4 + e], a.w_scales[n + r]);
+            }
+        }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -174,29 +210,22 @@ enum { FEW_ROWS = 64 };
 
 // How a call runs.
 struct Plan {
-    enum { ROWS, TILES } way;
-    int tile, parts;
+    bool few;
+    int parts;
     long part_ld;
     size_t bytes(int rows) const { return parts > 1 ? sizeof(int) * (size_t)parts * rows * part_ld : 0; }
 };
 
+// Parts where workgroups are fewer than compute units, of 16 steps at least: a join costs 3 us and more, as much as some ten steps take (64 x 64 tiles, one part
+// and two: 512 x 1024 x 1024 6.5 and 9.3 us, 256 x 2048 x 2048 8.6 and 10.2, 65 x 4096 x 4096 13.2 and 12.2).
 Plan plan_of(int rows, int inner, int cols) {
     Plan p;
     const long steps = pitch_of(inner) / STEP, cus = cu_count();
     p.part_ld = (cols + 3L) / 4 * 4;
-    p.tile = 0;
-    long groups, most;
-    if (rows <= FEW_ROWS) {
-        p.way = Plan::ROWS;
-        groups = ceil_div(cols, ROWS_COLS), most = steps / (2 * ROWS_WAVES);
-    } else {
-        p.way = Plan::TILES;
-        const long big = (long)ceil_div(rows, 128) * ceil_div(cols, 128);
-        p.tile = big >= cus ? 128 : 64;
-        groups = (long)ceil_div(rows, p.tile) * ceil_div(cols, p.tile), most = steps / 4;
-    }
+    p.few = rows <= FEW_ROWS;
+    const long groups = p.few ? ceil_div(cols, ROWS_COLS) : (long)ceil_div(rows, TILE) * ceil_div(cols, TILE);
     long parts = groups >= cus ? 1 : (2 * cus) / groups;
-    parts = parts > most ? most : parts;
+    parts = parts > steps / 16 ? steps / 16 : parts;
     p.parts = (int)(parts < 1 ? 1 : parts);
     return p;
 }
@@ -205,15 +234,16 @@ template <class T>
 int launch(Args a, const Plan &p, hipStream_t stream) {
     a.parts = p.parts, a.part_ld = p.part_ld;
     a.vec = a.ldz % 4 == 0 && ((size_t)a.z & (4 * sizeof(T) - 1)) == 0;
-    if (p.way == Plan::ROWS) {
+    if (p.few) {
         const dim3 grid((unsigned)(ceil_div(a.cols, ROWS_COLS) * (long)p.parts)), threads(ROWS_WAVES * 64);
         if (a.rows <= 16) hipLaunchKernelGGL((int8_rows_kernel<T, 1>), grid, threads, 0, stream, a);
         else if (a.rows <= 32) hipLaunchKernelGGL((int8_rows_kernel<T, 2>), grid, threads, 0, stream, a);
         else hipLaunchKernelGGL((int8_rows_kernel<T, 4>), grid, threads, 0, stream, a);
     } else {
-        const dim3 grid((unsigned)((long)ceil_div(a.rows, p.tile) * ceil_div(a.cols, p.tile) * p.parts));
-        if (p.tile == 128) hipLaunchKernelGGL((int8_tile_kernel<T, 128>), grid, dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((int8_tile_kernel<T, 64>), grid, dim3(256), 0, stream, a);
+        const long groups = (long)ceil_div(a.rows, TILE) * ceil_div(a.cols, TILE) * p.parts;
+        D8_REQUIRE(groups < (1L << 31), "matmul_int8: a result of %d x %d is too large", a.rows, a.cols);
+        if (a.vec || a.parts > 1) hipLaunchKernelGGL((int8_tile_kernel<T, true>), dim3((unsigned)groups), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((int8_tile_kernel<T, false>), dim3((unsigned)groups), dim3(256), 0, stream, a);
     }
     D8_LAUNCH_CHECK();
     if (p.parts > 1) {

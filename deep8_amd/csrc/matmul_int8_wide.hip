@@ -36,13 +36,31 @@ struct WideArgs {
     }
 };
 
-// The scales of what a lane stores: its eight columns', and its 32 rows' (row 16 i + 4 t + lane / 16 of the wave's 128).
+typedef wide::TileOperands<true, true> WideOperands;
+
+// The operands of the tile at `w`, from arguments that the compiler takes for new ones: per tile, not once and kept.  Scalar registers are short, and
+// one that is brought back from a vector register right before a load into LDS, which is asm, comes too late for it (the built code is tested for that).
+__device__ __forceinline__ void wide_operands(WideOperands &T, const WideArgs &all, const wide::Where &w, int wave, int lane) {
+    WideArgs a = all;
+    asm volatile("" : "+s"(a.a.rows), "+s"(a.a.cols), "+s"(a.a.steps), "+s"(a.a.pitch), "+v"(lane));
+    T.init<wide::Int8>(a.product().p[0], w, wave, lane);
+}
+
+// The eight columns of a row that a lane stores, of a wave's 128: half, eight side by side, 16 bytes; single, four and the four 64 further on, so that
+// in either a store instruction has whole lines.
+template <class T>
+__device__ __forceinline__ int column(int l15, int e) {
+    return sizeof(T) == 2 ? l15 * 8 + e : l15 * 4 + (e >> 2) * 64 + (e & 3);
+}
+
+// The scales of what a lane stores: its columns', and its 32 rows' (row 16 i + 4 t + lane / 16 of the wave's 128).
+template <class T>
 struct Scales {
     float w[8], x[32];
     __device__ __forceinline__ void load(const Args &a, const wide::Where &at, int wave, int lane) {
-        const int n = at.n0 + (wave & 1) * 128 + (lane & 15) * 8, m = at.m0 + (wave >> 1) * 128 + (lane >> 4);
+        const int n = at.n0 + (wave & 1) * 128, m = at.m0 + (wave >> 1) * 128 + (lane >> 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = a.w_scales[n + e];
+        for (int e = 0; e < 8; ++e) w[e] = a.w_scales[n + column<T>(lane & 15, e)];
 #pragma unroll
         for (int e = 0; e < 32; ++e) x[e] = a.x_scales[m + e * 4];
     }
@@ -55,34 +73,48 @@ struct Scales {
     }
 };
 
-// A finished tile on its way out, as wide::store_tile.  INTERIOR: every lane stores all its 32 pieces (single precision: 64 stores).
+// A finished tile on its way out, as wide::store_tile.  INTERIOR: every lane stores all its 32 pieces (single precision: 64).  Else element by element, 16
+// lanes along a row.
 template <class T, bool INTERIOR>
-__device__ __forceinline__ void store_scaled(const Args &a, const wide::Where &w, const Scales &by, float *patch, int wave, int lane, f32x4 (&acc)[8][8]) {
+__device__ __forceinline__ void store_scaled(const Args &a, const wide::Where &w, const Scales<T> &by, float *patch, int wave, int lane, f32x4 (&acc)[8][8]) {
     asm volatile("" : "+v"(lane));
     const int wm = wave >> 1, wn = wave & 1, l15 = lane & 15, l4 = lane >> 4;
-    const int n = w.n0 + wn * 128 + l15 * 8;
+    const int n = w.n0 + wn * 128;
     unsigned wr[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) wr[q] = (unsigned)(size_t)WIDE_LDS(float, patch) + 4u * ((4 * l4) * 128 + ((q ^ l4) * 16 + l15));
+    float along[8];  // scales of columns lane % 16 + 16 k
+#pragma unroll
+    for (int k = 0; k < 8; ++k) along[k] = INTERIOR ? 0.f : a.w_scales[n + l15 + k * 16];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         wide::write_slab<0>(wr, acc[i]);
+        if (INTERIOR) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int row = t * 4 + l4, cc = (l15 * 8) ^ (t * 16), m = w.m0 + wm * 128 + i * 16 + row;
-            const i32x4 lo = *(const i32x4 *)(patch + row * 128 + cc), hi = *(const i32x4 *)(patch + row * 128 + cc + 4);
-            T out[8];
+            for (int t = 0; t < 4; ++t) {
+                const int row = t * 4 + l4, m = w.m0 + wm * 128 + i * 16 + row;
+                i32x4 part[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) out[e] = scaled<T>(e < 4 ? lo[e & 3] : hi[e & 3], by.x[i * 4 + t], by.w[e]);
-            T *z = (T *)a.z + (long)m * a.ldz + n;
-            typedef T piece __attribute__((ext_vector_type(16 / sizeof(T))));
-            if (INTERIOR) {
+                for (int h = 0; h < 2; ++h) part[h] = *(const i32x4 *)(patch + row * 128 + (column<T>(l15, 4 * h) ^ (t * 16)));
+                T out[8];
 #pragma unroll
-                for (int e = 0; e < 8; e += 16 / sizeof(T)) __builtin_nontemporal_store(*(const piece *)(out + e), (piece *)(z + e));
-            } else {
+                for (int e = 0; e < 8; ++e) out[e] = scaled<T>(part[e >> 2][e & 3], by.x[i * 4 + t], by.w[e]);
+                typedef T piece __attribute__((ext_vector_type(16 / sizeof(T))));
+                T *z = (T *)a.z + (long)m * a.ldz + n;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (m >= w.m_own && n + e >= w.n_own) z[e] = out[e];
+                for (int e = 0; e < 8; e += 16 / sizeof(T)) __builtin_nontemporal_store(*(const piece *)(out + e), (piece *)(z + column<T>(l15, e)));
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int row = t * 4 + l4, m = w.m0 + wm * 128 + i * 16 + row;
+                int sums[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sums[k] = __float_as_int(patch[row * 128 + ((k * 16 + l15) ^ (t * 16))]);
+                T *z = (T *)a.z + (long)m * a.ldz + n + l15;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (m >= w.m_own && n + l15 + k * 16 >= w.n_own) z[k * 16] = scaled<T>(sums[k], by.x[i * 4 + t], along[k]);
             }
         }
     }
@@ -100,8 +132,8 @@ __global__ __launch_bounds__(256) void int8_wide_kernel(WideArgs wa) {
     int idx = blockIdx.x;
     Where cur = locate(wa.product(), idx);
     {
-        TileOperands<true, true> T_;
-        T_.template init<Int8>(wa.product().p[0], cur, wave, lane);
+        WideOperands T_;
+        wide_operands(T_, wa, cur, wave, lane);
         T_.issue_first_steps(wave_base);
     }
     __builtin_amdgcn_s_waitcnt(0x4f70);  // vmcnt(16): the first stage has landed
@@ -110,17 +142,17 @@ __global__ __launch_bounds__(256) void int8_wide_kernel(WideArgs wa) {
         const int nidx = idx + gridDim.x;
         const bool more = nidx < wa.total;
         const Where nxt = more ? locate(wa.product(), nidx) : cur;
-        Scales by;  // on their way during the loop
+        Scales<T> by;  // on their way during the loop
         by.load(wa.a, cur, wave, lane);
         {
-            TileOperands<true, true> T_;
-            T_.template init<Int8>(wa.product().p[0], cur, wave, lane);
+            WideOperands T_;
+            wide_operands(T_, wa, cur, wave, lane);
             k_loop<Int8, true, true>(T_, lds, wave_base, acc);
         }
         by.arrive();
         if (more) {  // the next tile's first two steps set out before this tile's epilogue: 32 loads a wave
-            TileOperands<true, true> T_;
-            T_.template init<Int8>(wa.product().p[0], nxt, wave, lane);
+            WideOperands T_;
+            wide_operands(T_, wa, nxt, wave, lane);
             T_.issue_first_steps(wave_base);
         }
         const bool interior = wa.a.vec && cur.m0 == cur.m_own && cur.n0 == cur.n_own;
@@ -136,11 +168,14 @@ __global__ __launch_bounds__(256) void int8_wide_kernel(WideArgs wa) {
     }
 }
 
+// Where these tiles are estimated to be through before those of 64 x 64: a step of 128 codes takes 1.05 us, a call 8 us beside them; the others go at 1000 TOP/s
+// after 5 us.  (us here / there: 1024 x 4096 x 4096 40 / 34, 2048 x 4096 x 4096 39 / 66, 4096 x 1024 x 4096 19 / 36, 3000 x 256 x 1024 11 / 7.)
 bool wide_eligible(const Args &a) {
     if (a.rows < 256 || a.cols < 256) return false;
     if (a.rows * a.pitch >= (1L << 31) || a.cols * a.pitch >= (1L << 31)) return false;
-    const long tiles = (long)ceil_div(a.rows, 256) * ceil_div(a.cols, 256);
-    return 4 * tiles >= 3L * cu_count() && tiles < (1L << 30);
+    const long tiles = (long)ceil_div(a.rows, 256) * ceil_div(a.cols, 256), cus = cu_count();
+    const float here = 8.f + 1.05f * a.steps * ((tiles + cus - 1) / cus), there = 5.f + 2e-9f * a.rows * a.cols * a.steps * STEP;
+    return here < there && tiles < (1L << 30);
 }
 
 template <class T>
