@@ -98,6 +98,7 @@ Variable &headNormRotary(Variable &x, Variable &weight, Variable &positions, Var
 Variable &headRotary(Variable &x, Variable &positions, Variable &table, int heads, bool interleaved = false);
 Variable &attention(Variable &q, Variable &k, Variable &v, Variable &qStarts, Variable &kStarts, int heads, int kvHeads, float scale = 0, bool causal = true);
 Variable &matrixMultiplyGated(Variable &x, Variable &w, Math::GateType act = Math::GateType::SiLU);
+Variable &layerNorm(Variable &x, Variable &weight, Variable &bias, float epsilon = 1e-5f);  // the node LayerNorm
 Variable &operator-(Variable &x, Variable &y);  // Minus, with broadcasting
 Variable &minus(Variable &x, Variable &y);
 Variable &l1Norm(Variable &x);

@@ -156,6 +156,36 @@ void MatrixMultiplyGated(const Tensor &x, const Tensor &w, Tensor *pre, Tensor &
 void MatrixMultiplyGatedGrad(const Tensor &x, Tensor &dx, const Tensor &w, Tensor &dw, const Tensor &pre, const Tensor &h, const Tensor &dh,
                              GateType act = GateType::SiLU);
 
+/** y = (x - mean) / sqrt(mean((x - mean)^2) + epsilon) * weight + bias along each row of x [rows, cols] (weight, bias [cols], null: ones
+ *  and zeros); d8_layer_norm, no counterpart in the reference.  y may be x */
+void LayerNorm(const Tensor &x, const Tensor *weight, const Tensor *bias, Tensor &y, float epsilon = 1e-5f);
+/** dx, dweight, dbias (null: not wanted) += */
+void LayerNormGrad(const Tensor &x, Tensor *dx, const Tensor *weight, Tensor *dweight, Tensor *dbias, const Tensor &dy, float epsilon = 1e-5f);
+
+// Serving in 8-bit integers (d8_quantize_rows, d8_matmul_int8, d8_cache_append, d8_attention_cache; no counterpart in the reference).
+/** bytes of a row of codes: `inner` rounded up */
+size_t Int8Pitch(size_t inner);
+/** x [rows, cols] as codes (Int8 [rows, Int8Pitch(cols)]) and scales (Float32 [rows]); columns: w [rows, cols] column by column, codes Int8
+ *  [cols, Int8Pitch(rows)], scales [cols] */
+void QuantizeRows(const Tensor &x, Tensor &codes, Tensor &scales);
+void QuantizeColumns(const Tensor &w, Tensor &codes, Tensor &scales);
+/** z [rows, cols] = x w, x as QuantizeRows and w as QuantizeColumns left them, `inner` terms a sum */
+void MatrixMultiplyInt8(const Tensor &x, const Tensor &xScales, const Tensor &w, const Tensor &wScales, size_t inner, Tensor &z);
+/** pages of CACHE_PAGE tokens: codes Int8 [pages, kvHeads, CACHE_PAGE, pitch] of keys and [pages, kvHeads, pitch, CACHE_PAGE] of values, pitch = dim
+ *  rounded up to 16; scales Float32 [pages, kvHeads] */
+enum { CACHE_PAGE = 64 };
+struct PagedCache {
+    Tensor kCodes, kScales, vCodes, vScales;
+};
+/** k and v [tokens, kvHeads * dim]: rows starts[s] .. starts[s + 1] - 1 are the last of the lengths[s] tokens of sequence s, whose pages are row s of
+ *  table (Int32 [sequences, pages of a sequence at most]) */
+void CacheAppend(const Tensor &k, const Tensor &v, PagedCache &cache, const Tensor &starts, const Tensor &lengths, const Tensor &table, int kvHeads);
+/** ... and their values again */
+void CacheRead(Tensor &k, Tensor &v, const PagedCache &cache, const Tensor &starts, const Tensor &lengths, const Tensor &table, int kvHeads);
+/** o = softmax(scale q k^T) v over the cache, q and o [tokens, heads * dim]; causal and lse as Attention's */
+void AttentionCache(const Tensor &q, const PagedCache &cache, Tensor &o, Tensor *lse, const Tensor &starts, const Tensor &lengths, const Tensor &table,
+                    int heads, int kvHeads, float scale, bool causal = true);
+
 }  // namespace Math
 }  // namespace Deep8
 

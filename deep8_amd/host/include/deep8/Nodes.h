@@ -105,6 +105,8 @@ public:
     Variable &headRotary(Variable &positions, Variable &table, int heads, bool interleaved = false);
     Variable &attention(Variable &k, Variable &v, Variable &qStarts, Variable &kStarts, int heads, int kvHeads, float scale = 0, bool causal = true);
     Variable &matrixMultiplyGated(Variable &w, Math::GateType act = Math::GateType::SiLU);
+    // each row's norm, times weight, plus bias (the node LayerNorm)
+    Variable &layerNorm(Variable &weight, Variable &bias, float epsilon = 1e-5f);
     // what a loss needs (deep8/src/nodes/Variable.cpp:342-346,461-465,521-535)
     Variable &minus(Variable &y);
     Variable &l1Norm();
@@ -121,7 +123,7 @@ public:
 };
 
 enum class FunctionType { Unkown = 0, Conv2d, DeConv2d, MatrixMultiply, Add, ReLu, Minus, L1Norm, L2Norm, ReduceMean, MaxPooling2d, AvgPooling2d,
-                          MatrixMultiplyBiasReLu, Conv2dBiasReLu, HeadNormRotary, Attention, MatrixMultiplyGated };
+                          MatrixMultiplyBiasReLu, Conv2dBiasReLu, HeadNormRotary, Attention, MatrixMultiplyGated, LayerNorm };
 
 class Function : public Node {
 protected:
@@ -297,6 +299,21 @@ public:
 protected:
     Tensor pre;
     void run(const std::vector<const Tensor *> &inputs, Tensor *output, bool keep);
+};
+
+// (x - mean) / sqrt(mean((x - mean)^2) + epsilon) * weight + bias along each row.  Inputs: x [rows, cols], weight and bias [cols].
+class LayerNorm : public Function {
+public:
+    float epsilon;
+
+    explicit LayerNorm(std::vector<Node *> &inputs, float epsilon = 1e-5f);
+    Shape checkShape(std::vector<Shape> &inputShapes) override;
+    ElementType checkElementType(std::vector<ElementType> &inputTypes) override;
+    void forward(const std::vector<const Tensor *> &inputs, Tensor *output) override;
+    void backward(const std::vector<const Tensor *> &inputs, const Tensor *output, const Tensor *outputGradient,
+                  size_t index, Tensor *iGradient) override;
+    using Function::forward;
+    void backward() override;  // all gradients through one Math call
 };
 
 // z = x - y under the same broadcasting rule (deep8/include/nodes/Minus.h, deep8/src/nodes/Minus.cpp:6-39)

@@ -271,5 +271,6 @@ Variable &attention(Variable &q, Variable &k, Variable &v, Variable &qStarts, Va
     return q.attention(k, v, qStarts, kStarts, heads, kvHeads, scale, causal);
 }
 Variable &matrixMultiplyGated(Variable &x, Variable &w, Math::GateType act) { return x.matrixMultiplyGated(w, act); }
+Variable &layerNorm(Variable &x, Variable &weight, Variable &bias, float epsilon) { return x.layerNorm(weight, bias, epsilon); }
 
 }  // namespace Deep8

@@ -978,5 +978,148 @@ void MatrixMultiplyGatedGrad(const Tensor &x, Tensor &dx, const Tensor &w, Tenso
                                   ws.bytes, nullptr));
 }
 
+// ---- the norm of a layer's rows ------------------------------------------------------------------------------------------
+namespace {
+void checkNorm(const Tensor &x, const Tensor *weight, const Tensor *bias, const Tensor &like) {
+    checkSame(x, like);
+    DEEP8_ARGUMENT_CHECK(2 == x.nDims() && x.shape == like.shape, "the shape must be same");
+    for (const Tensor *t : {weight, bias}) {
+        if (nullptr == t) continue;
+        checkSame(x, *t);
+        DEEP8_ARGUMENT_CHECK(t->size() == x.col(), "weight and bias must have one value per element of a row");
+    }
+    requireGPU(x);
+}
+}  // namespace
+
+void LayerNorm(const Tensor &x, const Tensor *weight, const Tensor *bias, Tensor &y, float epsilon) {
+    checkNorm(x, weight, bias, y);
+    const void *from = x.raw();  // (first: y may be x)
+    y.takeZero();
+    D8_CHECK(d8_layer_norm(dtypeOf(x), from, (long)x.col(), weight ? weight->raw() : nullptr, bias ? bias->raw() : nullptr, y.raw(), (long)y.col(), rowsOf(x),
+                           (int)x.col(), epsilon, nullptr));
+}
+
+void LayerNormGrad(const Tensor &x, Tensor *dx, const Tensor *weight, Tensor *dweight, Tensor *dbias, const Tensor &dy, float epsilon) {
+    checkNorm(x, weight, nullptr, dy);
+    if (dx) checkNorm(x, dweight, dbias, *dx);
+    else checkNorm(x, dweight, dbias, dy);
+    const int dt = dtypeOf(x), rows = rowsOf(x), cols = (int)x.col();
+    bool fresh[2] = {dweight && dweight->takeZero(), dbias && dbias->takeZero()};
+    if (fresh[0] != fresh[1] && dweight && dbias) {  // (one bit says both: the deferred fill of the one that has it)
+        if (fresh[0]) dweight->zero();
+        else dbias->zero();
+        fresh[0] = fresh[1] = false;
+    }
+    const int overwrite = (dx && dx->takeZero() ? 1 : 0) | (fresh[0] || fresh[1] ? 2 : 0);
+    PoolScratch ws(x.device(), d8_layer_norm_grad_scratch_bytes(dt, rows, cols));
+    D8_CHECK(d8_layer_norm_grad(dt, x.raw(), cols, weight ? weight->raw() : nullptr, dy.raw(), cols, dx ? dx->raw() : nullptr, cols, dweight ? dweight->raw() : nullptr,
+                                dbias ? dbias->raw() : nullptr, rows, cols, epsilon, overwrite, ws.ptr, ws.bytes, nullptr));
+}
+
+// ---- serving in 8-bit integers ---------------------------------------------------------------------------------------------
+namespace {
+void checkCodes(const Tensor &codes, const Tensor &scales, size_t rows, size_t inner) {
+    requireGPU(codes), requireGPU(scales);
+    DEEP8_ARGUMENT_CHECK(DType::Int8 == codes.elementType.id && DType::Float32 == scales.elementType.id, "codes must be Int8, scales Float32");
+    DEEP8_ARGUMENT_CHECK(2 == codes.nDims() && (size_t)rowsOf(codes) == rows && codes.col() == Int8Pitch(inner) && scales.size() == rows,
+                         "codes must be [" << rows << ", " << Int8Pitch(inner) << "], with a scale for each row");
+}
+
+// Sequences' pages: the table's rows, and how many pages the cache has.
+struct Where {
+    const int *starts, *lengths, *table;
+    int sequences, tablePages, pages, dim;
+};
+
+Where checkCache(const Tensor &rows, const PagedCache &c, const Tensor &starts, const Tensor &lengths, const Tensor &table, int heads, int kvHeads) {
+    DEEP8_ARGUMENT_CHECK(kvHeads >= 1 && heads >= 1 && 0 == heads % kvHeads, "the heads must be a multiple of the heads of keys");
+    DEEP8_ARGUMENT_CHECK(2 == rows.nDims() && 0 == rows.col() % heads, "a row must hold whole heads");
+    requireGPU(rows);
+    const size_t dim = rows.col() / heads, pitch = (dim + 15) / 16 * 16, n = lengths.size(), pages = c.kScales.size() / kvHeads;
+    for (const Tensor *t : {&c.kCodes, &c.vCodes}) {
+        requireGPU(*t);
+        DEEP8_ARGUMENT_CHECK(DType::Int8 == t->elementType.id && t->size() == pages * kvHeads * CACHE_PAGE * pitch, "the codes must be Int8, " << CACHE_PAGE << " tokens of " << pitch << " for each page and head");
+    }
+    for (const Tensor *t : {&c.kScales, &c.vScales}) {
+        requireGPU(*t);
+        DEEP8_ARGUMENT_CHECK(DType::Float32 == t->elementType.id && t->size() == pages * kvHeads, "the scales must be Float32, one for each page and head");
+    }
+    DEEP8_ARGUMENT_CHECK(n >= 1 && 0 == table.size() % n, "the table must have a row for each sequence");
+    return Where{indices(&starts, n + 1, "starts"), indices(&lengths, n, "lengths"), indices(&table, n, "table"), (int)n, (int)(table.size() / n), (int)pages, (int)dim};
+}
+
+void checkKeys(const Tensor &k, const Tensor &v) {
+    checkSame(k, v);
+    DEEP8_ARGUMENT_CHECK(k.shape == v.shape, "each key needs its value");
+}
+}  // namespace
+
+size_t Int8Pitch(size_t inner) {
+    const int pitch = inner < (1u << 30) ? d8_int8_pitch((int)inner) : 0;
+    DEEP8_ARGUMENT_CHECK(pitch > 0, "a sum has 1 to 131071 terms, not " << inner);
+    return (size_t)pitch;
+}
+
+void QuantizeRows(const Tensor &x, Tensor &codes, Tensor &scales) {
+    DEEP8_ARGUMENT_CHECK(2 == x.nDims(), "the shape is error");
+    checkCodes(codes, scales, (size_t)rowsOf(x), x.col());
+    requireGPU(x);
+    codes.takeZero(), scales.takeZero();
+    D8_CHECK(d8_quantize_rows(dtypeOf(x), x.raw(), (long)x.col(), rowsOf(x), (int)x.col(), (signed char *)codes.raw(), (float *)scales.raw(), nullptr));
+}
+
+void QuantizeColumns(const Tensor &w, Tensor &codes, Tensor &scales) {
+    DEEP8_ARGUMENT_CHECK(2 == w.nDims() && 1 == w.batch(), "the shape is error");
+    checkCodes(codes, scales, w.col(), w.row());
+    requireGPU(w);
+    codes.takeZero(), scales.takeZero();
+    D8_CHECK(d8_quantize_columns(dtypeOf(w), w.raw(), (long)w.col(), (int)w.row(), (int)w.col(), (signed char *)codes.raw(), (float *)scales.raw(), nullptr));
+}
+
+void MatrixMultiplyInt8(const Tensor &x, const Tensor &xScales, const Tensor &w, const Tensor &wScales, size_t inner, Tensor &z) {
+    DEEP8_ARGUMENT_CHECK(2 == z.nDims(), "the shape is error");
+    checkCodes(x, xScales, (size_t)rowsOf(z), inner), checkCodes(w, wScales, z.col(), inner);
+    requireGPU(z);
+    const int rows = rowsOf(z), cols = (int)z.col();
+    PoolScratch ws(z.device(), d8_matmul_int8_scratch_bytes(rows, (int)inner, cols));
+    z.takeZero();
+    D8_CHECK(d8_matmul_int8(dtypeOf(z), (const signed char *)x.raw(), (const float *)xScales.raw(), rows, (int)inner, (const signed char *)w.raw(),
+                            (const float *)wScales.raw(), cols, z.raw(), cols, ws.ptr, ws.bytes, nullptr));
+}
+
+void CacheAppend(const Tensor &k, const Tensor &v, PagedCache &c, const Tensor &starts, const Tensor &lengths, const Tensor &table, int kvHeads) {
+    checkKeys(k, v);
+    const Where w = checkCache(k, c, starts, lengths, table, kvHeads, kvHeads);
+    D8_CHECK(d8_cache_append(dtypeOf(k), k.raw(), (long)k.col(), v.raw(), (long)v.col(), (signed char *)c.kCodes.raw(), (float *)c.kScales.raw(),
+                             (signed char *)c.vCodes.raw(), (float *)c.vScales.raw(), w.starts, w.lengths, w.table, w.sequences, rowsOf(k), w.tablePages, w.pages,
+                             kvHeads, w.dim, nullptr));
+}
+
+void CacheRead(Tensor &k, Tensor &v, const PagedCache &c, const Tensor &starts, const Tensor &lengths, const Tensor &table, int kvHeads) {
+    checkKeys(k, v);
+    const Where w = checkCache(k, c, starts, lengths, table, kvHeads, kvHeads);
+    // (rows of no sequence keep what the outputs hold: a deferred zero fill is performed)
+    D8_CHECK(d8_cache_read(dtypeOf(k), k.raw(), (long)k.col(), v.raw(), (long)v.col(), (const signed char *)c.kCodes.raw(), (const float *)c.kScales.raw(),
+                           (const signed char *)c.vCodes.raw(), (const float *)c.vScales.raw(), w.starts, w.lengths, w.table, w.sequences, rowsOf(k), w.tablePages,
+                           w.pages, kvHeads, w.dim, nullptr));
+}
+
+void AttentionCache(const Tensor &q, const PagedCache &c, Tensor &o, Tensor *lse, const Tensor &starts, const Tensor &lengths, const Tensor &table, int heads,
+                    int kvHeads, float scale, bool causal) {
+    checkSame(q, o);
+    DEEP8_ARGUMENT_CHECK(q.shape == o.shape, "the shape must be same");
+    const Where w = checkCache(q, c, starts, lengths, table, heads, kvHeads);
+    if (lse) {
+        requireGPU(*lse);
+        DEEP8_ARGUMENT_CHECK(DType::Float32 == lse->elementType.id && lse->size() == (size_t)heads * rowsOf(q), "the lse must be Float32, one value per query and head");
+    }
+    const int dt = dtypeOf(q);
+    PoolScratch ws(q.device(), d8_attention_cache_scratch_bytes(dt, w.sequences, rowsOf(q), w.tablePages, heads, kvHeads, w.dim));
+    D8_CHECK(d8_attention_cache(dt, q.raw(), (long)q.col(), (const signed char *)c.kCodes.raw(), (const float *)c.kScales.raw(), (const signed char *)c.vCodes.raw(),
+                                (const float *)c.vScales.raw(), o.raw(), (long)o.col(), lse ? (float *)lse->raw() : nullptr, w.starts, w.lengths, w.table, w.sequences,
+                                rowsOf(q), w.tablePages, w.pages, heads, kvHeads, w.dim, scale, causal ? 1 : 0, ws.ptr, ws.bytes, nullptr));
+}
+
 }  // namespace Math
 }  // namespace Deep8

@@ -209,6 +209,12 @@ Variable &Variable::matrixMultiplyGated(Variable &w, Math::GateType act) {
     return *executor->addFunction(new MatrixMultiplyGated(in, act));
 }
 
+Variable &Variable::layerNorm(Variable &weight, Variable &bias, float epsilon) {
+    DEEP8_ARGUMENT_CHECK(nullptr != executor, "the Variable does not belong to an Executor");
+    std::vector<Node *> in = {this, &weight, &bias};
+    return *executor->addFunction(new LayerNorm(in, epsilon));
+}
+
 Variable &Variable::minus(Variable &y) {
     DEEP8_ARGUMENT_CHECK(nullptr != executor, "the Variable does not belong to an Executor");
     std::vector<Node *> in = {this, &y};
@@ -783,6 +789,41 @@ void MatrixMultiplyGated::backward() {
     Variable *out = nullptr;
     std::vector<const Tensor *> in = gatherInputs(this, out);
     Math::MatrixMultiplyGatedGrad(*in[0], x->gradient, *in[1], w->gradient, pre, out->value, out->gradient, act);
+}
+
+LayerNorm::LayerNorm(std::vector<Node *> &in, float e) : Function(in), epsilon(e) {
+    DEEP8_ARGUMENT_CHECK(3 == inputs.size(), "the LayerNorm Function needs x, a weight and a bias");
+    DEEP8_ARGUMENT_CHECK(epsilon >= 0, "the epsilon must >= 0");
+}
+
+Shape LayerNorm::checkShape(std::vector<Shape> &shapes) {
+    DEEP8_ARGUMENT_CHECK(3 == shapes.size(), "the input count must be 3");
+    DEEP8_ARGUMENT_CHECK(2 == shapes[0].nDims, "the inputs dimensions is error");
+    for (size_t i = 1; i < 3; ++i) DEEP8_ARGUMENT_CHECK(shapes[i].size() == shapes[0].col(), "weight and bias must have one value per element of a row");
+    return shapes[0];
+}
+
+ElementType LayerNorm::checkElementType(std::vector<ElementType> &types) {
+    DEEP8_ARGUMENT_CHECK(3 == types.size(), "the input count must be 3");
+    return checkTypes(types, 3, 0);
+}
+
+void LayerNorm::forward(const std::vector<const Tensor *> &in, Tensor *output) { Math::LayerNorm(*in[0], in[1], in[2], *output, epsilon); }
+
+void LayerNorm::backward(const std::vector<const Tensor *> &in, const Tensor *, const Tensor *outputGradient, size_t index, Tensor *iGradient) {
+    DEEP8_ARGUMENT_CHECK(index < 3, "the index is error");
+    Math::LayerNormGrad(*in[0], 0 == index ? iGradient : nullptr, in[1], 1 == index ? iGradient : nullptr, 2 == index ? iGradient : nullptr, *outputGradient, epsilon);
+}
+
+void LayerNorm::backward() {
+    Variable *v[3];
+    for (size_t i = 0; i < 3; ++i) v[i] = (Variable *)inputs[i];
+    if (v[0] == v[1] || v[0] == v[2] || v[1] == v[2]) return Function::backward();  // (their gradients add up one after the other)
+    Variable *out = nullptr;
+    std::vector<const Tensor *> in = gatherInputs(this, out);
+    Tensor *d[3];
+    for (size_t i = 0; i < 3; ++i) d[i] = v[i]->updateGradient ? &v[i]->gradient : nullptr;
+    if (d[0] || d[1] || d[2]) Math::LayerNormGrad(*in[0], d[0], in[1], d[1], d[2], out->gradient, epsilon);
 }
 
 // ---- Add / ReLu -------------------------------------------------------------------------------------------------

@@ -1263,6 +1263,145 @@ TEST_GPU(transformer_layer_backward_at_once_and_input_by_input) {
     executor.clearInterimNodes();
 }
 
+TEST_GPU(layer_norm_node) {
+    const int rows = 6, cols = 20;
+    for (DType id : {DType::Float32, DType::Float16}) {
+        const ElementType type = ElementType::from(id);
+        HostTensor x = normalTensor(type, 2, {rows / 2, cols}), w = normalTensor(type, 1, {cols}), b = normalTensor(type, 1, {cols});
+        Variable v0 = placeholder(type), v1 = placeholder(type), v2 = placeholder(type);
+        std::vector<Node *> nodes = {&v0, &v1, &v2};
+        LayerNorm node(nodes, 1e-3f);
+        auto f = [&](const std::vector<Doubles> &in) {
+            Doubles y = in[0];
+            for (int r = 0; r < rows; ++r) {
+                double *v = &y[r * cols], mean = 0, square = 0;
+                for (int c = 0; c < cols; ++c) mean += v[c] / cols;
+                for (int c = 0; c < cols; ++c) square += (v[c] - mean) * (v[c] - mean) / cols;
+                for (int c = 0; c < cols; ++c) v[c] = (v[c] - mean) / std::sqrt(square + 1e-3f) * in[1][c] + in[2][c];
+            }
+            return y;
+        };
+        layerCase(node, {&x, &w, &b}, 3, f);
+    }
+}
+
+TEST_GPU(layer_norm_backward_at_once_and_input_by_input) {
+    EagerExecutor executor;
+    Variable &x = parameter(&executor, {5, 24}), &w = parameter(&executor, {24}), &b = parameter(&executor, {24}), &one = parameter(&executor, {1, 24});
+    for (Variable *v : {&x, &w, &b, &one}) {
+        std::vector<float> h(v->shape().size());
+        std::normal_distribution<float> nd;
+        for (float &f : h) f = nd(rng);
+        v->feed(h.data());
+    }
+    auto gradient = [&](Variable &v) {
+        std::vector<float> h(v.shape().size());
+        v.gradient.device()->copyFromGPUToCPU(v.gradient.raw(), h.data(), h.size() * 4);
+        return h;
+    };
+    Variable &y = layerNorm(x, w, b), &twice = layerNorm(one, one, b);  // (the second: one variable as rows and weight)
+    EXPECT(y.shape() == x.shape());
+    backward(y.l2NormLoss() + twice.l2NormLoss(), false);
+    const std::vector<float> g[] = {gradient(x), gradient(w), gradient(b), gradient(one)};
+    for (Variable *v : {&x, &w, &b, &one}) v->zeroGradient();
+    LayerNorm *node = (LayerNorm *)y.inputs[0], *second = (LayerNorm *)twice.inputs[0];
+    std::vector<const Tensor *> in = {&x.value, &w.value, &b.value}, in2 = {&one.value, &one.value, &b.value};
+    Tensor *to[] = {&x.gradient, &w.gradient, &b.gradient}, *to2[] = {&one.gradient, &one.gradient, &b.gradient};
+    for (size_t i = 0; i < 3; ++i) node->backward(in, &y.value, &y.gradient, i, to[i]), second->backward(in2, &twice.value, &twice.gradient, i, to2[i]);
+    const std::vector<float> s[] = {gradient(x), gradient(w), gradient(b), gradient(one)};
+    for (size_t k = 0; k < 4; ++k) {
+        double num = 0, den = 0;
+        for (size_t i = 0; i < g[k].size(); ++i) num += (double)(g[k][i] - s[k][i]) * (g[k][i] - s[k][i]), den += (double)s[k][i] * s[k][i];
+        EXPECT(den > 0 && std::sqrt(num / den) <= 1e-6);  // (the same sums, added to the gradient in another order)
+    }
+    EXPECT(throws<std::invalid_argument>([&] { node->backward(in, &y.value, &y.gradient, 3, &x.gradient); }));
+    EXPECT(throws<std::invalid_argument>([&] { Math::LayerNorm(x.value, &x.value, nullptr, y.value); }));
+    EXPECT(throws<std::invalid_argument>([&] { Math::LayerNorm(x.value, &w.value, &b.value, twice.value); }));
+    executor.clearInterimNodes();
+}
+
+TEST_GPU(serving_in_8_bits) {
+    // a product with quantised operands, and attention over a cache of two sequences (70 and 3 tokens), each against its formula on what the codes stand for
+    const size_t rows = 3, inner = 40, cols = 10, pitch = Math::Int8Pitch(inner);
+    const ElementType f32 = ElementType::from<float>(), i8 = ElementType::from(DType::Int8);
+    auto make = [&](ElementType type, std::vector<size_t> dims) { return makeTensor(gpu(), type, 1, dims); };
+    HostTensor x = normalTensor(f32, 1, {rows, inner}), w = normalTensor(f32, 1, {inner, cols}), z = normalTensor(f32, 1, {rows, cols});
+    Tensor xc = make(i8, {rows, pitch}), wc = make(i8, {cols, pitch}), xs = make(f32, {rows}), ws = make(f32, {cols});
+    Math::QuantizeRows(x.t, xc, xs), Math::QuantizeColumns(w.t, wc, ws);
+    Math::MatrixMultiplyInt8(xc, xs, wc, ws, inner, z.t);
+    Doubles want(rows * cols);
+    for (size_t r = 0; r < rows; ++r)
+        for (size_t c = 0; c < cols; ++c) {
+            float a = 0, b = 0;
+            for (size_t k = 0; k < inner; ++k) a = std::max(a, std::fabs(x.host[r * inner + k])), b = std::max(b, std::fabs(w.host[k * cols + c]));
+            const double sa = a / 127.f, sb = b / 127.f;
+            for (size_t k = 0; k < inner; ++k) want[r * cols + c] += sa * std::nearbyint(x.host[r * inner + k] / sa) * sb * std::nearbyint(w.host[k * cols + c] / sb);
+        }
+    expectClose(z, want, 1e-6);
+    EXPECT(throws<std::invalid_argument>([&] { Math::MatrixMultiplyInt8(xc, xs, wc, ws, 200, z.t); }));
+    EXPECT(throws<std::invalid_argument>([&] { Math::MatrixMultiplyInt8(xc, ws, wc, ws, inner, z.t); }));
+    EXPECT(throws<std::invalid_argument>([&] { Math::QuantizeRows(w.t, xc, xs); }));
+
+    const int heads = 4, kvHeads = 2, pages = 3;
+    const size_t dim = 8, tokens = 73, queries = 4;
+    Math::PagedCache cache{make(i8, {pages, kvHeads, 64, 16}), make(f32, {pages, kvHeads}), make(i8, {pages, kvHeads, 16, 64}), make(f32, {pages, kvHeads})};
+    HostTensor k = normalTensor(f32, 1, {tokens, kvHeads * dim}), v = normalTensor(f32, 1, {tokens, kvHeads * dim}), kb = normalTensor(f32, 1, {tokens, kvHeads * dim}), vb = normalTensor(f32, 1, {tokens, kvHeads * dim});
+    HostTensor q = normalTensor(f32, 1, {queries, heads * dim}), o = normalTensor(f32, 1, {queries, heads * dim});
+    const std::vector<int> held = {70, 3}, qs = {0, 3, 4};
+    HostTensor starts = intTensor({0, 70, 73}), lengths = intTensor(held), table = intTensor({2, 0, 1, -1}), queryStarts = intTensor(qs);
+    Math::CacheAppend(k.t, v.t, cache, starts.t, lengths.t, table.t, kvHeads);
+    Math::CacheRead(kb.t, vb.t, cache, starts.t, lengths.t, table.t, kvHeads);
+    download(kb), download(vb);
+    float largest = 0, off = 0;
+    for (size_t i = 0; i < k.host.size(); ++i) {
+        largest = std::max(largest, std::max(std::fabs(k.host[i]), std::fabs(v.host[i])));
+        off = std::max(off, std::max(std::fabs(k.host[i] - kb.host[i]), std::fabs(v.host[i] - vb.host[i])));
+    }
+    EXPECT(off > 0 && off <= largest / 127 * 1.0001f);  // half a step, and a step is a power of two of which 127 reach the page's largest: at most 2 / 127 of it
+    Math::AttentionCache(q.t, cache, o.t, nullptr, queryStarts.t, lengths.t, table.t, heads, kvHeads, 0.3f);
+    Doubles seen(queries * heads * dim, 0.0);
+    for (size_t s = 0; s < 2; ++s)
+        for (int t = qs[s]; t < qs[s + 1]; ++t)
+            for (int h = 0; h < heads; ++h) {
+                double sum = 0, *to = &seen[(t * heads + h) * dim];
+                for (int j = 0; j <= held[s] - (qs[s + 1] - t); ++j) {
+                    const size_t at = ((s ? 70 : 0) + j) * kvHeads * dim + h / 2 * dim;
+                    double score = 0;
+                    for (size_t e = 0; e < dim; ++e) score += 0.3f * q.host[(t * heads + h) * dim + e] * kb.host[at + e];
+                    sum += std::exp(score);
+                    for (size_t e = 0; e < dim; ++e) to[e] += std::exp(score) * vb.host[at + e];
+                }
+                for (size_t e = 0; e < dim; ++e) to[e] /= sum;
+            }
+    expectClose(o, seen, 1e-5);
+    EXPECT(throws<std::invalid_argument>([&] { Math::CacheAppend(k.t, q.t, cache, starts.t, lengths.t, table.t, kvHeads); }));
+    EXPECT(throws<std::invalid_argument>([&] { Math::CacheAppend(k.t, v.t, cache, lengths.t, lengths.t, table.t, kvHeads); }));          // starts too short
+    EXPECT(throws<std::invalid_argument>([&] { Math::CacheAppend(k.t, v.t, cache, starts.t, lengths.t, starts.t, kvHeads); }));          // three entries for two sequences
+    EXPECT(throws<std::invalid_argument>([&] { Math::AttentionCache(q.t, cache, o.t, nullptr, queryStarts.t, lengths.t, table.t, heads, 4, 1.f); }));  // a cache of two heads
+}
+
+TEST_CPU(layer_norm_shape_inference) {
+    const ElementType f32 = ElementType::from<float>(), h16 = ElementType::from<half>();
+    struct Probe : Variable {
+        Probe() : Variable(0, "", nullptr) {}
+    } a, b, c;
+    std::vector<Node *> two = {&a, &b}, three = {&a, &b, &c};
+    EXPECT(throws<std::invalid_argument>([&] { LayerNorm n(two); }));
+    EXPECT(throws<std::invalid_argument>([&] { LayerNorm n(three, -1.f); }));
+    LayerNorm n(three);
+    std::vector<Shape> s = {Shape(2, {5, 32}), Shape(1, {32}), Shape(1, {32})};
+    EXPECT(n.checkShape(s) == Shape(2, {5, 32}));
+    for (size_t i = 0; i < 3; ++i) {
+        std::vector<Shape> t = s;
+        t[i] = Shape(1, {31});
+        EXPECT(throws<std::invalid_argument>([&] { n.checkShape(t); }));
+    }
+    std::vector<ElementType> t = {h16, h16, h16};
+    EXPECT(n.checkElementType(t) == h16);
+    t[2] = f32;
+    EXPECT(throws<std::invalid_argument>([&] { n.checkElementType(t); }));
+}
+
 TEST_CPU(transformer_layer_shape_inference) {
     const ElementType f32 = ElementType::from<float>(), h16 = ElementType::from<half>(), i32 = ElementType::from(DType::Int32);
     struct Probe : Variable {
