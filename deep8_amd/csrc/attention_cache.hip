@@ -149,9 +149,6 @@ __device__ __forceinline__ long run_of(long total, int runs) {
 }
 
 // ---- operands -------------------------------------------------------------------------------------------------------
-template <class T, int NC>
-struct Operands;
-
 // 16 codes as halves, exactly
 __device__ __forceinline__ void to_halves(const i32x4 &codes, f16x8 (&out)[2]) {
 #pragma unroll
@@ -168,64 +165,46 @@ __device__ __forceinline__ void to_halves(const i32x4 &codes, f16x8 (&out)[2]) {
     }
 }
 
-template <int NC>
-struct Operands<f16, NC> {
-    struct Query {
-        f16x8 f[NC * 2];
-        __device__ __forceinline__ void set(int i, float x) { f[i >> 3][i & 7] = (f16)x; }
-    };
-    struct Weights {
-        f16x8 f[2];
-        __device__ __forceinline__ void set(const float (&x)[16]) {  // (two values a conversion, to nearest)
-            f16x2 p[8];
+// sixteen numbers as halves, two a conversion, to nearest
+__device__ __forceinline__ void round_halves(const float (&x)[16], f16x8 (&out)[2]) {
+    f16x2 p[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = __builtin_convertvector((f32x2){x[2 * i], x[2 * i + 1]}, f16x2);
+    for (int i = 0; i < 8; ++i) p[i] = __builtin_convertvector((f32x2){x[2 * i], x[2 * i + 1]}, f16x2);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                f[i] = __builtin_shufflevector(__builtin_shufflevector(p[4 * i], p[4 * i + 1], 0, 1, 2, 3), __builtin_shufflevector(p[4 * i + 2], p[4 * i + 3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-    };
-    struct Codes {
-        f16x8 f[2];
-        __device__ __forceinline__ void set(const i32x4 &codes) { to_halves(codes, f); }
-    };
-    static __device__ __forceinline__ void scores(f32x4 &acc, const Codes &k, const Query &q, int chunk) {
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.f[0], q.f[2 * chunk], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.f[1], q.f[2 * chunk + 1], acc, 0, 0, 0);
-    }
-    static __device__ __forceinline__ void sums(f32x4 &acc, const Codes &v, const Weights &p) {
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.f[0], p.f[0], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.f[1], p.f[1], acc, 0, 0, 0);
-    }
+    for (int i = 0; i < 2; ++i)
+        out[i] = __builtin_shufflevector(__builtin_shufflevector(p[4 * i], p[4 * i + 1], 0, 1, 2, 3), __builtin_shufflevector(p[4 * i + 2], p[4 * i + 3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// What meets the codes in a product: a query's elements, or a page's probabilities.  Codes are halves exactly, so single precision runs on the same
+// instructions, its numbers as sums of halves, each what the ones before leave: queries of three (33 bits, all of them), probabilities of two (22 bits: off by
+// 2^-22 each at most, which the sum over keys averages).  Single precision's own matrix instructions take eight times as long as half's for a product: 16
+// queries over 131072 keys, 32 + 8 heads of 128, in 161 us.
+template <class T>
+struct Precision;
+template <>
+struct Precision<f16> {
+    static constexpr int QUERY = 1, WEIGHT = 1;
+    static constexpr float LIFT = 0.f;
+};
+// So that what is left stays in half's range too, a row of queries is brought to 2^13 .. 2^14 by a power of two, and probabilities by LIFT.
+template <>
+struct Precision<float> {
+    static constexpr int QUERY = 3, WEIGHT = 2;
+    static constexpr float LIFT = 14.f;
 };
 
-template <int NC>
-struct Operands<float, NC> {
-    struct Query {
-        float f[NC * 16];
-        __device__ __forceinline__ void set(int i, float x) { f[i] = x; }
-    };
-    struct Weights {
-        float f[16];
-        __device__ __forceinline__ void set(const float (&x)[16]) {
+template <int PARTS>
+__device__ __forceinline__ void split(float (&x)[16], f16x8 (&out)[PARTS][2]) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = x[i];
-        }
-    };
-    struct Codes {
-        i32x4 w;
-        __device__ __forceinline__ void set(const i32x4 &codes) { w = codes; }
-        __device__ __forceinline__ float at(int i) const { return (float)(signed char)(w[i >> 2] >> (8 * (i & 3))); }
-    };
-    static __device__ __forceinline__ void scores(f32x4 &acc, const Codes &k, const Query &q, int chunk) {
+    for (int p = 0; p < PARTS; ++p) {
+        round_halves(x, out[p]);
+        if (p + 1 < PARTS)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k.at(i), q.f[chunk * 16 + i], acc, 0, 0, 0);
+            for (int i = 0; i < 16; ++i) x[i] -= (float)out[p][i >> 3][i & 7];
     }
-    static __device__ __forceinline__ void sums(f32x4 &acc, const Codes &v, const Weights &p) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(v.at(i), p.f[i], acc, 0, 0, 0);
-    }
-};
+}
+
+__device__ __forceinline__ f32x4 mma(const f16x8 &a, const f16x8 &b, const f32x4 &c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // the larger, and the sum, of the four lanes that have a row (l, l + 16, l + 32, l + 48)
 __device__ __forceinline__ float row_max(float x) {
@@ -244,8 +223,9 @@ __device__ __forceinline__ float row_sum(float x) {
 // NC: chunks of 64 elements of a head.
 template <class T, int NC>
 struct Wave {
-    typedef Operands<T, NC> Op;
-    typename Op::Query q;
+    typedef Precision<T> P;
+    f16x8 q[NC][P::QUERY][2];
+    float q_scale;  // of the lane's row (single precision)
     f32x4 o[NC * 4];
     float m, sum;  // of scores times log2 e; the lane's part of the sum
     int limit;     // keys that the lane's row sees
@@ -259,6 +239,7 @@ struct Wave {
         const long sees = a.causal ? t + s.len - s.n + 1 : s.len;
         limit = there ? (int)min(max(sees, 0L), (long)s.keys) : 0;
         const T *from = (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * a.group + h) * a.c.dim;
+        float x[NC][16], largest = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = c * 64 + g * 16;
@@ -269,13 +250,30 @@ struct Wave {
                 if (a.vec && there && d + i < a.c.dim) {  // (dim is whole pieces)
                     const piece p = *(const piece *)(from + d + i);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) q.set(c * 16 + i + e, (float)p[e]);
+                    for (int e = 0; e < V; ++e) x[c][i + e] = (float)p[e];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) q.set(c * 16 + i + e, !a.vec && there && d + i + e < a.c.dim ? (float)from[d + i + e] : 0.f);
+                    for (int e = 0; e < V; ++e) x[c][i + e] = !a.vec && there && d + i + e < a.c.dim ? (float)from[d + i + e] : 0.f;
                 }
             }
+            if (P::QUERY > 1)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) largest = fmaxf(largest, fabsf(x[c][i]));
         }
+        q_scale = 1.f;
+        if (P::QUERY > 1) {
+            largest = row_max(largest);
+            // 2^(e - 13) of a largest element 1.f 2^e, at least 2^-100; 1 for rows of zeros, infinities and NaN
+            const int e = max((int)(__float_as_uint(largest) >> 23) - 13, 27);
+            if (largest > 0.f && largest < INFINITY) q_scale = __uint_as_float((unsigned)e << 23);
+            const float back = 1.f / q_scale;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[c][i] *= back;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) split<P::QUERY>(x[c], q[c]);
         m = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NC * 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -294,9 +292,10 @@ struct Wave {
 
     // Scores of a page whose first place is `at` to weights; accumulators and sums to the new maximum.  hidden: some row does not see all of
     // the page (or there is none).  `into`: what the page's sums are scaled by, 0 where the lane's row sees none of it.
-    __device__ __forceinline__ void weigh(const f32x4 (&sc)[4], int at, bool there, bool hidden, float k_scale, float v_scale, typename Op::Weights &p, float &into) {
+    __device__ __forceinline__ void weigh(const f32x4 (&sc)[4], int at, bool there, bool hidden, float k_scale, float v_scale, f16x8 (&p)[P::WEIGHT][2], float &into) {
+#pragma clang fp contract(off)  // (a fused product less its rounded maximum can be anything but small where scores are large)
         const int g = (threadIdx.x & 63) >> 4;
-        float x[16], by = k_scale;
+        float x[16], by = P::QUERY > 1 ? k_scale * q_scale : k_scale;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = sc[i >> 2][i & 3];
         into = v_scale;
@@ -321,10 +320,14 @@ struct Wave {
         float add = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_amdgcn_exp2f(x[i] * by - base);
+            x[i] = __builtin_amdgcn_exp2f(x[i] * by - (base - P::LIFT));
             add += x[i];
         }
-        p.set(x);
+        split<P::WEIGHT>(x, p);
+        if (P::LIFT != 0.f) {
+            constexpr float LOWER = 1.f / 16384.f;
+            add *= LOWER, into *= LOWER;
+        }
         sum += add;
     }
 
@@ -382,22 +385,24 @@ struct Wave {
                 sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < NC; ++i) {
-                    typename Op::Codes k;
-                    k.set(kr[t][i]);
-                    Op::scores(sc[t], k, q, i);
+                    f16x8 k[2];
+                    to_halves(kr[t][i], k);
+#pragma unroll
+                    for (int e = 0; e < P::QUERY; ++e) sc[t] = mma(k[1], q[i][e][1], mma(k[0], q[i][e][0], sc[t]));
                 }
             }
             if (more) fetch_keys(next);
-            typename Op::Weights p;
+            f16x8 p[P::WEIGHT][2];
             float into;
             weigh(sc, at, there, !there || at + PAGE > least, list.k(n) * (a.scale * LOG2E), list.v(n), p, into);
 #pragma unroll
             for (int i = 0; i < NC * 4; ++i) {
                 if (i * 16 >= c.pitch) continue;
-                typename Op::Codes v;
-                v.set(vr[i]);
+                f16x8 v[2];
+                to_halves(vr[i], v);
                 f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                Op::sums(acc, v, p);
+#pragma unroll
+                for (int e = 0; e < P::WEIGHT; ++e) acc = mma(v[1], p[e][1], mma(v[0], p[e][0], acc));
                 o[i] += acc * into;
             }
             if (more) fetch_values(next);
@@ -455,12 +460,13 @@ struct Wave {
                     group(k + 1);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int at = 4 * k + i, t = at / (2 * NC);
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[k & 1][i], q.f[at % (2 * NC)], sc[t], 0, 0, 0);
+                        const int at = 4 * k + i, t = at / (2 * NC), c = at % (2 * NC);
+#pragma unroll
+                        for (int e = 0; e < P::QUERY; ++e) sc[t] = mma(ahead[k & 1][i], q[c >> 1][e][c & 1], sc[t]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                typename Op::Weights p;
+                f16x8 p[P::WEIGHT][2];
                 float into;
                 weigh(sc, at, there, !there || at + PAGE > least, list.k(n) * (a.scale * LOG2E), list.v(n), p, into);
                 __builtin_amdgcn_sched_barrier(0);
@@ -470,8 +476,8 @@ struct Wave {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {  // (elements beyond the head, whatever they are, are not stored)
                         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[k & 1][2 * i], p.f[0], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[k & 1][2 * i + 1], p.f[1], acc, 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < P::WEIGHT; ++e) acc = mma(ahead[k & 1][2 * i + 1], p[e][1], mma(ahead[k & 1][2 * i], p[e][0], acc));
                         o[k * 2 + i] += acc * into;
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -501,7 +507,7 @@ __device__ __forceinline__ void put(const AttArgs &a, T *to, int d, const f32x4 
 }
 
 template <class T, int NC, bool ROWS>
-__global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 || sizeof(T) == 4 ? 1 : ROWS ? 4 : 2) void attention_cache_kernel(AttArgs a) {
+__global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 : ROWS && sizeof(T) == 2 ? 4 : 2) void attention_cache_kernel(AttArgs a) {
     constexpr int WAVES = ROWS ? ROWS_WAVES : KEYS_WAVES, R = ROWS ? MANY_ROWS : KEYS_ROWS;  // rows of a tile
     __shared__ f16x8 stages[ROWS ? 2 : 1][ROWS ? 16 * NC : 1][64];
     __shared__ f32x4 others[ROWS ? 1 : WAVES][ROWS ? 1 : NC * 4][64];
@@ -638,10 +644,10 @@ struct Plan {
     long units, slots;
 };
 
-Plan plan_of(int dtype, int sequences, int tokens, int table_pages, int heads, int kv_heads, int dim) {
+Plan plan_of(int sequences, int tokens, int table_pages, int heads, int kv_heads, int dim) {
     Plan p;
     const long group = heads / kv_heads, all = (long)tokens * group, some = sequences < tokens ? sequences : tokens;
-    p.rows = dtype == D8_FLOAT16 && dim <= 128 && some && all / some >= 64;
+    p.rows = dim <= 128 && some && all / some >= 64;
     p.tile = p.rows ? MANY_ROWS : KEYS_ROWS;
     p.units = all / p.tile + some;
     const long at_once = (2L * cu_count() + kv_heads - 1) / kv_heads, most = (p.units * (table_pages ? table_pages : 1) + KEYS_WAVES - 1) / KEYS_WAVES;
@@ -658,7 +664,7 @@ size_t scratch_of(const Plan &p, int kv_heads, int dim) {
 template <class T, int NC>
 void launch(const AttArgs &a, const Plan &p, hipStream_t stream) {
     const dim3 grid((unsigned)(p.runs * a.c.kv_heads));
-    if constexpr (sizeof(T) == 2 && NC <= 2) {
+    if constexpr (NC <= 2) {
         if (p.rows) {
             hipLaunchKernelGGL((attention_cache_kernel<T, NC, true>), grid, dim3(ROWS_WAVES * 64), 0, stream, a);
             return;
@@ -693,7 +699,7 @@ using namespace d8;
 
 extern "C" size_t d8_attention_cache_scratch_bytes(int dtype, int sequences, int q_tokens, int table_pages, int heads, int kv_heads, int dim) {
     if (!cache::sizes(dtype, sequences, q_tokens, heads, kv_heads, dim) || !sequences || !q_tokens || table_pages < 0 || table_pages >= (1 << 24)) return 0;
-    return cache::scratch_of(cache::plan_of(dtype, sequences, q_tokens, table_pages, heads, kv_heads, dim), kv_heads, dim);
+    return cache::scratch_of(cache::plan_of(sequences, q_tokens, table_pages, heads, kv_heads, dim), kv_heads, dim);
 }
 
 extern "C" int d8_attention_cache(int dtype, const void *q, long ldq, const signed char *k_codes, const float *k_scales, const signed char *v_codes,
@@ -711,7 +717,7 @@ extern "C" int d8_attention_cache(int dtype, const void *q, long ldq, const sign
     if (!sequences || !q_tokens) return 0;
     D8_REQUIRE(q && o, "attention_cache: null tensor");
     D8_REQUIRE(ldq >= (long)heads * dim && ldo >= (long)heads * dim, "attention_cache: rows of %ld elements do not fit their leading dimensions", (long)heads * dim);
-    const cache::Plan p = cache::plan_of(dtype, sequences, q_tokens, table_pages, heads, kv_heads, dim);
+    const cache::Plan p = cache::plan_of(sequences, q_tokens, table_pages, heads, kv_heads, dim);
     const size_t need = cache::scratch_of(p, kv_heads, dim);
     D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_cache: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
     D8_REQUIRE(p.units * kv_heads < (1L << 31), "attention_cache: too many sequences");

@@ -245,6 +245,27 @@ def test_pages_out_of_scale_beside_others(nq, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [6, 96])
+def test_queries_of_any_size(n):
+    """rows of 1e-37 to 1e37, elements of different sizes in a row, rows of zeros; one with an infinity and one with NaN, which stay theirs alone"""
+    r = rng(12)
+    cache, table, pages, (kv, vv) = _filled([200], 1, 64, r)
+    q = r.standard_normal((n, 1, 64))
+    size = np.array([1e-37, 1e-20, 1.0, 1e20, 1e37, 0.0])
+    q = (q * size[np.arange(n) % 6][:, None, None]).astype(np.float32)
+    q[2] *= np.exp2(-r.integers(0, 40, 64))
+    want, lse = so.attention_cache(q, kv, vv, [0, n], [200], table, pages, 0.125, False)
+    got, got_lse = cache.attention(q, [0, n], [200], table, 0.125, False)
+    _near(got, want, FP32_TOL)
+    assert (np.abs(got_lse - lse) <= 1e-5 * np.maximum(1, np.abs(lse))).all()
+    q[3, 0, 5], q[5, 0, 9] = np.inf, np.nan
+    bad, _ = cache.attention(q, [0, n], [200], table, 0.125, False)
+    rest = np.ones(n, bool)
+    rest[[3, 5]] = False
+    assert np.array_equal(bad[rest], got[rest]) and np.isnan(bad[[3, 5]]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("nq", [[1, 1, 1], [40, 3, 90]])
 def test_steps_captured_and_replayed(nq):
     """an append and the attention after it, captured once; lengths, tokens and queries change between the replays, eager calls run between them"""
@@ -360,7 +381,7 @@ def test_scratch_has_room_for_every_piece(sequences, tokens, table_pages, heads,
     lib, group, r = capi.load(), heads // kv_heads, rng(tokens)
     for dt in (capi.FLOAT16, capi.FLOAT32):
         nb = lib.d8_attention_cache_scratch_bytes(dt, sequences, tokens, table_pages, heads, kv_heads, dim)
-        many = dt == capi.FLOAT16 and dim <= 128 and tokens * group // min(sequences, tokens) >= 64
+        many = dim <= 128 and tokens * group // min(sequences, tokens) >= 64
         rows = 128 if many else 16
         units = tokens * group // rows + min(sequences, tokens)
         per_slot = 4 * kv_heads * rows * ((dim + 3) // 4 * 4 + 2)
