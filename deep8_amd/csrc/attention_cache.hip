@@ -8,17 +8,22 @@
 // Products.  Both are formed transposed (keys x rows, elements x rows) with 16 x 16 accumulators: lane l has row l % 16, and with it its
 // maximum, sum and limit; the probabilities are the next product's right operand where they are.  A lane (r = l % 16, g = l / 16) of tile t of a
 // page's keys holds 16 bytes of key 16 (r / 4) + 4 t + r % 4, so that after the product lane group g has keys 16 g .. 16 g + 15 in order: the 16 bytes of
-// values [element][token] that a lane reads are then the matching left operand.  So codes go from memory to registers in 16-byte pieces, without LDS,
-// and are converted there: half in pairs, by putting the byte (its sign bit flipped) below the bits of 1024 and taking off 1024 + 128.
+// values [element][token] that a lane reads are then the matching left operand.  So codes go from memory to registers in 16-byte pieces, and are
+// converted there: half in pairs, by putting the byte (its sign bit flipped) below the bits of 1024 and taking off 1024 + 128.
 //
-// Two kernels' worth of work in one: few rows (KEYS: a workgroup has 16 rows, its four waves share out the pages and join through LDS) and many
-// (ROWS: each wave has 32 rows of its own, and all four read the same pages, which the first to ask brings into the L1 cache).
+// KEYS, for few rows: a workgroup has 16 rows, its four waves share out the pages, each by itself and a page ahead, and join through LDS.
+// ROWS, from 64 rows a sequence on and for heads of 128 elements at most: eight waves have 16 rows each and go through the pages together; a page's codes
+// are converted once and go through LDS as operands, in two buffers.  (4 x 128 queries of 32 heads over 32768 keys of 8: 320 us with every wave converting
+// for itself, 137 so.)
 //
 // All tiles' pages, one after the other, are cut into as many equal runs as workgroups run at once, whatever sequences have how many: a workgroup
 // goes through its run and leaves, for a tile that it has not all of, sums in scratch, which a second launch joins.  Cuts are found from the
 // lengths on the device, so a call can be captured and replayed as sequences grow.
 //
-// Bound by memory where there are few rows (a page and head is 16 KB at 128 elements), by conversions and exponentials where there are many.
+// KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 66 us, 4.1 TB/s, where
+// a large copy moves 5.2; single precision 77 us.  ROWS by conversions, exponentials and matrix instructions, which share an issue slot: 1 x 2048 queries
+// of 32 heads over 8192 keys take 365 us, 660 TFLOP/s, where a large product of the library makes 1200.  Short calls are bound by latency: a wave's
+// way from the first length to its last store is 10 us, and the join 4.
 //
 // Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product.
 #include "cache.h"
@@ -55,6 +60,12 @@ struct Seq {
     int keys;
     long tiles, pages;  // tiles of rows, pages that each goes through (1 where there is none: a result of nothing is written too)
     __device__ __forceinline__ long cost() const { return tiles * pages; }
+    template <int R>
+    __device__ __forceinline__ void set(const AttArgs &a, int first, int rows, int length) {
+        q0 = first, n = rows, len = max(length, 0);
+        keys = (int)min(len, (long)a.c.table_pages * PAGE);
+        tiles = n ? ((long)n * a.group + R - 1) / R : 0, pages = keys ? (keys + PAGE - 1) / PAGE : 1;
+    }
 };
 
 // the lane's sequence of the 64 from `first` on; top: the largest start so far (starts as in cache.hip)
@@ -73,19 +84,17 @@ __device__ __forceinline__ Seq seqs_from(const AttArgs &a, int first, int &top) 
     }
     top = __builtin_amdgcn_readlane(q1, 63);
     Seq s;
-    s.q0 = q0, s.n = q1 - q0, s.len = at < c.sequences ? max(c.lengths[at], 0) : 0;
-    s.keys = (int)min(s.len, (long)c.table_pages * PAGE);
-    s.tiles = s.n ? ((long)s.n * a.group + R - 1) / R : 0, s.pages = s.keys ? (s.keys + PAGE - 1) / PAGE : 1;
+    s.set<R>(a, q0, q1 - q0, at < c.sequences ? c.lengths[at] : 0);
     return s;
 }
 
-__device__ __forceinline__ long upto(long x) {  // sum over the lanes up to this one
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long y = __shfl_up(x, d);
-        x += (threadIdx.x & 63) >= d ? y : 0;
+// sums over the lanes up to this one, of which `most` are not 0
+__device__ __forceinline__ void sum_upto(long &x, long &y, int most) {
+    for (int d = 1; d < 64 && d < most; d <<= 1) {
+        const long u = __shfl_up(x, d), v = __shfl_up(y, d);
+        const bool add = (threadIdx.x & 63) >= d;
+        x += add ? u : 0, y += add ? v : 0;
     }
-    return x;
 }
 __device__ __forceinline__ long from_lane(long x, int lane) { return __shfl(x, lane); }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -102,12 +111,16 @@ struct Scan {
     __device__ __forceinline__ void begin(const AttArgs &a) {
         top = 0;
         own = seqs_from<R>(a, 0, top);
-        tiles_upto = upto(own.tiles), cost_upto = upto(own.cost());
-        tiles = from_lane(tiles_upto, 63), cost = from_lane(cost_upto, 63);
+        tiles_upto = own.tiles, cost_upto = own.cost();
+        sum_upto(tiles_upto, cost_upto, a.c.sequences);
+        const int last = min(a.c.sequences, 64) - 1;
+        tiles = from_lane(tiles_upto, last), cost = from_lane(cost_upto, last);
         int at = top;
         for (int first = 64; first < a.c.sequences; first += 64) {
             const Seq s = seqs_from<R>(a, first, at);
-            tiles += from_lane(upto(s.tiles), 63), cost += from_lane(upto(s.cost()), 63);
+            long t = s.tiles, c = s.cost();
+            sum_upto(t, c, 64);
+            tiles += from_lane(t, 63), cost += from_lane(c, 63);
         }
         tiles = uniform(tiles), cost = uniform(cost);
     }
@@ -119,9 +132,10 @@ struct Scan {
         for (int first = 0; first < a.c.sequences; first += 64) {
             if (first) {
                 x = seqs_from<R>(a, first, start);
-                t = upto(x.tiles), c = upto(x.cost());
+                t = x.tiles, c = x.cost();
+                sum_upto(t, c, 64);
             }
-            const unsigned long long past = __ballot(cost_before + c > at);
+            const unsigned long long past = __ballot(first + (int)(threadIdx.x & 63) < a.c.sequences && cost_before + c > at);
             if (past) {
                 const int l = __ffsll((long long)past) - 1;
                 s = uniform(first + l);
@@ -130,11 +144,26 @@ struct Scan {
                 seq.tiles = uniform(from_lane(x.tiles, l)), seq.pages = uniform(from_lane(x.pages, l));
                 return true;
             }
-            cost_before += from_lane(c, 63), tiles_before += from_lane(t, 63);
+            const int last = min(a.c.sequences - first, 64) - 1;
+            cost_before += from_lane(c, last), tiles_before += from_lane(t, last);
         }
         return false;
     }
 };
+
+// The next sequence that has queries, after `seq`, number s; false beyond the last.
+template <int R>
+__device__ __forceinline__ bool advance(const AttArgs &a, Seq &seq, int &s) {
+    int end = seq.q0 + seq.n;
+    while (++s < a.c.sequences) {
+        const int first = end;
+        end = uniform(max(first, min(a.c.starts[s + 1], a.c.tokens)));
+        if (end == first) continue;
+        seq.set<R>(a, first, end - first, uniform(a.c.lengths[s]));
+        return true;
+    }
+    return false;
+}
 
 // What the second launch joins of a tile: how many runs have a part of it (0: nothing to join), the first of them, the sequence's first query, and
 // the tile's first row and those from it on.
@@ -142,10 +171,13 @@ struct Join {
     int parts, run, q0, row0, rows, pad[3];
 };
 
-// How long the runs of a call are: equal, and a page a wave at least.
-__device__ __forceinline__ long run_of(long total, int runs) {
-    const long even = (total + runs - 1) / runs;
-    return even < KEYS_WAVES ? KEYS_WAVES : even;
+// How long the runs of a call are: equal, but not so short that a tile's many pieces cost more to join than is gained: KEYS stays at a tile, or a page a
+// wave, ROWS at a quarter of a tile, or four pages.  (One token over 8000 keys of 8 heads: 17 us so, 22 with runs of a page; 256 queries of 8 heads over
+// 4096 keys in single, 38 and 50.  Runs longer than a tile go through short sequences one after the other: 16 of 100 keys took 24 us with four pages, 17 so.)
+template <int R>
+__device__ __forceinline__ long run_of(long total, long tiles, int runs) {
+    const long even = (total + runs - 1) / runs, mean = (total + tiles - 1) / max(tiles, 1L);
+    return max(even, min(R == KEYS_ROWS ? mean : mean / 4, 4L));
 }
 
 // ---- operands -------------------------------------------------------------------------------------------------------
@@ -230,15 +262,24 @@ struct Wave {
     float m, sum;  // of scores times log2 e; the lane's part of the sum
     int limit;     // keys that the lane's row sees
 
+    const T *from;  // the lane's row of queries, null for none
+
     // rows row0 .. of the sequence (those beyond `rows` are zero and see nothing)
     __device__ __forceinline__ void begin(const AttArgs &a, const Seq &s, int head, long row0, long rows) {
-        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-        const long row = row0 + r;
+        const long row = row0 + (threadIdx.x & 15);
         const bool there = row < rows;
         const int t = there ? (int)row / a.group : 0, h = there ? (int)row - t * a.group : 0;
         const long sees = a.causal ? t + s.len - s.n + 1 : s.len;
         limit = there ? (int)min(max(sees, 0L), (long)s.keys) : 0;
-        const T *from = (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * a.group + h) * a.c.dim;
+        from = there ? (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * a.group + h) * a.c.dim : nullptr;
+        m = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC * 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    __device__ __forceinline__ void load_queries(const AttArgs &a) {
+        const int g = (threadIdx.x & 63) >> 4;
+        const bool there = from != nullptr;
         float x[NC][16], largest = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -274,9 +315,6 @@ struct Wave {
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) split<P::QUERY>(x[c], q[c]);
-        m = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < NC * 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
     // where a lane's operands lie in a page and head: its key's row of tile t (16 bytes of chunk n; beyond the head any codes, times zeros of q),
@@ -354,8 +392,8 @@ struct Wave {
         return uniform((n + PAGE - 1) / PAGE);
     }
 
-    // KEYS: `count` pages, 64 at most, first, first + step, ... of sequence s, by this wave alone
-    __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int count, int step) {
+    // KEYS: `count` pages, 64 at most, first, first + step, ... of sequence s, by this wave alone.  fresh: load the queries too
+    __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int count, int step, bool fresh) {
         const Pages &c = a.c;
         const int least = uniform(limit);
         List list;
@@ -375,6 +413,7 @@ struct Wave {
                 if (i * 16 < c.pitch) vr[i] = *value_at(from, i);
         };
         fetch_keys(list.id(0)), fetch_values(list.id(0));
+        if (fresh) load_queries(a);
         for (int n = 0; n < count; ++n) {
             const int at = (first + n * step) * PAGE;
             const bool there = list.is(n), more = n + 1 < count;
@@ -509,6 +548,9 @@ __device__ __forceinline__ void put(const AttArgs &a, T *to, int d, const f32x4 
 template <class T, int NC, bool ROWS>
 __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 : ROWS && sizeof(T) == 2 ? 4 : 2) void attention_cache_kernel(AttArgs a) {
     constexpr int WAVES = ROWS ? ROWS_WAVES : KEYS_WAVES, R = ROWS ? MANY_ROWS : KEYS_ROWS;  // rows of a tile
+    // Queries are loaded once a tile's first page has set out, where registers leave room for both: 16 queries over 131072 keys took 1 us less so (in single,
+    // or with more elements, 3 us more).
+    constexpr bool LATE = !ROWS && sizeof(T) == 2 && NC <= 2;
     __shared__ f16x8 stages[ROWS ? 2 : 1][ROWS ? 16 * NC : 1][64];
     __shared__ f32x4 others[ROWS ? 1 : WAVES][ROWS ? 1 : NC * 4][64];
     __shared__ float2 stats[ROWS ? 1 : WAVES][16];
@@ -516,7 +558,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
     const int head = blockIdx.x % a.c.kv_heads, run = blockIdx.x / a.c.kv_heads;
     Scan<R> scan;
     scan.begin(a);
-    const long total = scan.cost, length = run_of(total, a.runs);
+    const long total = scan.cost, length = run_of<R>(total, scan.tiles, a.runs);
     const long last = min((run + 1) * length, total);
     long at = run * length;
     if (run == 0 && head == 0)  // tiles that the launch has room for and the sequences do not have
@@ -540,6 +582,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
                 a.joins[tile_base + tile] = Join{parts == 1 ? 0 : parts, run, seq.q0, (int)(tile * R), (int)(rows - tile * R), {0, 0, 0}};
             }
             w.begin(a, seq, head, row0, rows);
+            if (!LATE) w.load_queries(a);
             if constexpr (ROWS) {
                 // what the tile's last row sees: all waves go through as many pages
                 const int t = ((int)min((tile + 1) * R, rows) - 1) / a.group;
@@ -548,7 +591,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
                 for (int i = first; i < upto; i += 64) w.pages_together(a, s, head, i, min(64, upto - i), wave, stages);
             } else {
                 const int upto = min(end, w.most());
-                for (int i = first + wave; i < upto; i += 64 * WAVES) w.pages(a, s, head, i, min(64, (upto - i + WAVES - 1) / WAVES), WAVES);
+                for (int i = first + wave; i < upto; i += 64 * WAVES) w.pages(a, s, head, i, min(64, (upto - i + WAVES - 1) / WAVES), WAVES, LATE && i == first + wave);
             }
             at += end - first;
             w.sum = row_sum(w.sum);
@@ -596,9 +639,8 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
             }
         }
         if (at >= last) return;
-        Scan<R> again;  // (anew: kept, it would take the registers of a wave)
-        again.begin(a);
-        if (!again.locate(a, at, seq, s, base, tile_base)) return;
+        base = after, tile_base += seq.tiles;
+        if (!advance<R>(a, seq, s)) return;
     }
 }
 
@@ -644,13 +686,14 @@ struct Plan {
     long units, slots;
 };
 
-Plan plan_of(int sequences, int tokens, int table_pages, int heads, int kv_heads, int dim) {
+Plan plan_of(int dtype, int sequences, int tokens, int table_pages, int heads, int kv_heads, int dim) {
     Plan p;
     const long group = heads / kv_heads, all = (long)tokens * group, some = sequences < tokens ? sequences : tokens;
     p.rows = dim <= 128 && some && all / some >= 64;
     p.tile = p.rows ? MANY_ROWS : KEYS_ROWS;
     p.units = all / p.tile + some;
-    const long at_once = (2L * cu_count() + kv_heads - 1) / kv_heads, most = (p.units * (table_pages ? table_pages : 1) + KEYS_WAVES - 1) / KEYS_WAVES;
+    const int held = dim > 128 || (p.rows && dtype == D8_FLOAT32) ? 1 : 2;  // workgroups whose registers a compute unit holds
+    const long at_once = ((long)held * cu_count() + kv_heads - 1) / kv_heads, most = p.units * (table_pages ? table_pages : 1);
     p.runs = (int)(at_once < most ? at_once : most);
     p.slots = p.units + p.runs;
     return p;
@@ -699,7 +742,7 @@ using namespace d8;
 
 extern "C" size_t d8_attention_cache_scratch_bytes(int dtype, int sequences, int q_tokens, int table_pages, int heads, int kv_heads, int dim) {
     if (!cache::sizes(dtype, sequences, q_tokens, heads, kv_heads, dim) || !sequences || !q_tokens || table_pages < 0 || table_pages >= (1 << 24)) return 0;
-    return cache::scratch_of(cache::plan_of(sequences, q_tokens, table_pages, heads, kv_heads, dim), kv_heads, dim);
+    return cache::scratch_of(cache::plan_of(dtype, sequences, q_tokens, table_pages, heads, kv_heads, dim), kv_heads, dim);
 }
 
 extern "C" int d8_attention_cache(int dtype, const void *q, long ldq, const signed char *k_codes, const float *k_scales, const signed char *v_codes,
@@ -717,7 +760,7 @@ extern "C" int d8_attention_cache(int dtype, const void *q, long ldq, const sign
     if (!sequences || !q_tokens) return 0;
     D8_REQUIRE(q && o, "attention_cache: null tensor");
     D8_REQUIRE(ldq >= (long)heads * dim && ldo >= (long)heads * dim, "attention_cache: rows of %ld elements do not fit their leading dimensions", (long)heads * dim);
-    const cache::Plan p = cache::plan_of(sequences, q_tokens, table_pages, heads, kv_heads, dim);
+    const cache::Plan p = cache::plan_of(dtype, sequences, q_tokens, table_pages, heads, kv_heads, dim);
     const size_t need = cache::scratch_of(p, kv_heads, dim);
     D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_cache: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
     D8_REQUIRE(p.units * kv_heads < (1L << 31), "attention_cache: too many sequences");

@@ -395,7 +395,8 @@ def test_scratch_has_room_for_every_piece(sequences, tokens, table_pages, heads,
             tiles = -(-n * group // rows)
             assert tiles.sum() <= units
             total = int((tiles * pages).sum())
-            length = max(-(-total // runs), 4)
+            mean = -(-total // int(tiles.sum()))
+            length = max(-(-total // runs), min(mean // 4 if many else mean, 4))
             used, at, unit = set(), 0, 0
             for t, p in zip(tiles, pages):
                 for _ in range(t):
