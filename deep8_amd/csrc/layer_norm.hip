@@ -3,14 +3,17 @@
 //   m = mean(x),  r = 1 / sqrt(mean((x - m)^2) + epsilon),  u = (x - m) r,  y = u w + b
 //   back: g = dy,  dx = r (w g - mean(w g) - u mean(w g u)),  dw = sum over rows of g u,  db = sum over rows of g
 //
-// Bound by memory: x is read and y written once (back: x and dy read, dx written); a row stays in the registers of its team of 64, 256
-// or 1024 threads between the sums and the result.  A thread has up to 16 elements of a row: more would leave too few waves to keep the
+// Bound by memory: x is read and y written once (back: x and dy read, dx written); a row stays in the registers of its team of 16 to 1024 threads
+// (row_team.h) between the sums and the result.  A thread has up to 16 elements of a row: more would leave too few waves to keep the
 // loads coming.  The spread is taken about the mean that was found, not from the sum of squares, which would cancel in rows whose mean is
 // far from zero, and what that mean is off by (its sum is rounded) is taken out with the same pass: sum (x - m) is it.
 //
 // The way back keeps the columns' sums of dw and db in registers while a workgroup goes down its rows (the next row's loads are on their
-// way meanwhile), adds its teams' through LDS, and leaves one row of them in scratch; a second launch adds those in a fixed order.  One
-// workgroup of 1024 threads a compute unit: twice as many would write and read twice as many sums, 8 % of all bytes at 8192 x 4096 already.
+// way meanwhile), adds its teams' through LDS, and leaves one row of them in scratch; a second launch adds those in a fixed order.  Two
+// workgroups of 512 threads a compute unit, so that one loads while the other adds; more would write and read more such rows.
+//
+// Half: 16384 x 4096 forward 53 us, 5.0 TB/s, where a large copy moves 5.2; 8192 x 4096 back 49 us (44 and 4 for the sums), 4.1 TB/s.  Single, 8192 x 4096 forward
+// 50 us, back 82 us: 5.3 and 4.9 TB/s.
 //
 // Sums are fp32; results are rounded once.
 #include "row_team.h"
@@ -31,7 +34,7 @@ struct NormArgs {
 };
 
 // (E values of which those beyond the row are 0) centred in place, 0 there again; the reciprocal of the spread
-template <int V, int TEAM, int E>
+template <class H, int TEAM, int E>
 __device__ __forceinline__ float centre(float (&v)[E], int t, int cols, float epsilon, float2 *slots, int &turn) {
     const float n = 1.f / cols;
     float sum = 0.f, rest = 0.f;
@@ -42,30 +45,30 @@ __device__ __forceinline__ float centre(float (&v)[E], int t, int cols, float ep
     float off = 0.f, squares = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        v[e] = (t + TEAM * (e / V)) * V < cols ? v[e] - mean : 0.f;
+        v[e] = H::has(e, t, cols) ? v[e] - mean : 0.f;
         off += v[e], squares += v[e] * v[e];
     }
     team_sum<TEAM>(off, squares, slots, turn);
     off *= n;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = (t + TEAM * (e / V)) * V < cols ? v[e] - off : 0.f;
+    for (int e = 0; e < E; ++e) v[e] = H::has(e, t, cols) ? v[e] - off : 0.f;
     return 1.f / sqrtf(fmaxf(squares * n - off * off, 0.f) + epsilon);
 }
 
 constexpr int forward_threads(int team) { return team < 256 ? 256 : team; }
 
-template <class T, int V, int TEAM, int E>
+template <class T, int V, int TEAM, int E, bool ODD>
 __global__ __launch_bounds__(forward_threads(TEAM)) void layer_norm_kernel(NormArgs a) {
     __shared__ float2 slots[2 * 16];
     constexpr int TEAMS = forward_threads(TEAM) / TEAM;
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    typedef Held<T, V, TEAM, E> H;
+    typedef Held<T, V, TEAM, E, ODD> H;
     float w[E], b[E];
     {
         H h;
-        if (a.weight) h.load((const T *)a.weight, t, a.cols), h.get(w);
+        if (a.weight) h.load((const T *)a.weight, t, a.cols), h.settle(t, a.cols), h.get(w);
         else for (int e = 0; e < E; ++e) w[e] = 1.f;
-        if (a.bias) h.load((const T *)a.bias, t, a.cols), h.get(b);
+        if (a.bias) h.load((const T *)a.bias, t, a.cols), h.settle(t, a.cols), h.get(b);
         else for (int e = 0; e < E; ++e) b[e] = 0.f;
     }
     int turn = 0;
@@ -75,29 +78,30 @@ __global__ __launch_bounds__(forward_threads(TEAM)) void layer_norm_kernel(NormA
     if (row < a.rows) x.load((const T *)a.x + row * a.ldx, t, a.cols);
     for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += step, row += step) {  // (all teams take part in the barriers)
         float v[E];
-        x.get(v);
+        x.settle(t, a.cols), x.get(v);
         if (row + step < a.rows) x.load((const T *)a.x + (row + step) * a.ldx, t, a.cols);
-        const float r = centre<V, TEAM, E>(v, t, a.cols, a.epsilon, slots, turn);
+        const float r = centre<H, TEAM, E>(v, t, a.cols, a.epsilon, slots, turn);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = v[e] * r * w[e] + b[e];
         if (row < a.rows) H::store((T *)a.out + row * a.ldout, t, a.cols, v);
     }
 }
 
-// Threads of a gradient workgroup: 1024 where what a thread keeps (its columns' sums, weights, this row's and the next one's elements) fits in
-// the 128 registers that leaves it, else 512.
-constexpr int grad_threads(int team, int v, int bytes) { return team == 1024 ? 1024 : 512; }
+// Threads of a gradient workgroup, whole teams.
+constexpr int grad_threads(int team) { return team == 1024 ? 1024 : 512; }
+// Waves a SIMD: four where what a thread keeps (its columns' sums, weights, this row's and the next one's elements) fits in the 128 registers that leaves it.
+constexpr int grad_waves(int elements, int bytes, bool odd) { return elements == 8 || (bytes == 2 && !odd) ? 4 : 1; }
 
-template <class T, int V, int TEAM, int E>
-__global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T)), V > 1 && E * sizeof(T) <= 32 ? 4 : 1) void layer_norm_grad_kernel(NormArgs a) {
-    constexpr int THREADS = grad_threads(TEAM, V, E * sizeof(T)), TEAMS = THREADS / TEAM;
+template <class T, int V, int TEAM, int E, bool ODD>
+__global__ __launch_bounds__(grad_threads(TEAM), grad_waves(E, sizeof(T), ODD)) void layer_norm_grad_kernel(NormArgs a) {
+    constexpr int THREADS = grad_threads(TEAM), TEAMS = THREADS / TEAM;
     constexpr bool AHEAD = TEAM < 1024 || E == 8;  // the next row's loads on their way
     __shared__ float2 slots[2 * 16];
     __shared__ float sums[TEAMS > 1 ? THREADS * E : 1];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    typedef Held<T, V, TEAM, E> H;
+    typedef Held<T, V, TEAM, E, ODD> H;
     H w, x, dy;
-    if (a.weight) w.load((const T *)a.weight, t, a.cols);
+    if (a.weight) w.load((const T *)a.weight, t, a.cols), w.settle(t, a.cols);
     else w.ones();
     float dw[E], db[E];
 #pragma unroll
@@ -112,17 +116,18 @@ __global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T)), V > 1 && E * 
     fetch(row);
     for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += step, row += step) {  // (all teams take part in the barriers)
         float u[E], s0 = 0.f, s1 = 0.f;
+        x.settle(t, a.cols), dy.settle(t, a.cols);
         H g = dy;
         x.get(u);
         if (AHEAD) fetch(row + step);
-        const float r = centre<V, TEAM, E>(u, t, a.cols, a.epsilon, slots, turn);
-        const bool mine = __builtin_amdgcn_readfirstlane(row < a.rows);  // (a team is whole waves)
+        const float r = centre<H, TEAM, E>(u, t, a.cols, a.epsilon, slots, turn);
+        const bool mine = TEAM < 64 ? row < a.rows : __builtin_amdgcn_readfirstlane(row < a.rows);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float ge = g.at(e), wg = w.at(e) * ge;
             u[e] *= r;
             s0 += wg, s1 += wg * u[e];
-            if (V > 1 && e % V == V - 1) asm volatile("" : "+v"(s0), "+v"(s1));  // piece by piece: one at a time is held in fp32
+            if (e % V == V - 1) asm volatile("" : "+v"(s0), "+v"(s1));  // piece by piece: one at a time is held in fp32
         }
         // (w and dy as they were loaded, converted again for each use: kept as fp32 they would take the registers of the next row)
         g.renew(), w.renew();
@@ -136,12 +141,12 @@ __global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T)), V > 1 && E * 
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             u[e] = r * (w.at(e) * g.at(e) - s0 - u[e] * s1);
-            if (V > 1 && e % V == V - 1) asm volatile("" : "+v"(s0), "+v"(s1));
+            if (e % V == V - 1) asm volatile("" : "+v"(s0), "+v"(s1));
         }
         if (mine && a.out) {
             T *to = (T *)a.out + row * a.ldout;
             if (!(a.overwrite & 1)) {
-                g.load(to, t, a.cols);
+                g.load(to, t, a.cols), g.settle(t, a.cols);
 #pragma unroll
                 for (int e = 0; e < E; ++e) u[e] += g.at(e);
             }
@@ -157,7 +162,7 @@ __global__ __launch_bounds__(grad_threads(TEAM, V, E * sizeof(T)), V > 1 && E * 
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int c = (t + TEAM * (e / V)) * V + e % V;
-                if (c < a.cols) to[(long)k * a.cols + c] = k ? db[e] : dw[e];
+                if (H::has(e, t, a.cols)) to[(long)k * a.cols + c] = k ? db[e] : dw[e];
             }
         } else {
             __syncthreads();
@@ -279,31 +284,32 @@ int check(const NormArgs &a, int dtype, bool grad) {
 }
 
 template <class T>
-void launch_forward(const NormArgs &a, bool vec, hipStream_t stream) {
-    if (a.cols > most_held(vec, sizeof(T))) {
+void launch_forward(const NormArgs &a, bool whole, hipStream_t stream) {
+    if (a.cols > most_held(sizeof(T), false)) {
         hipLaunchKernelGGL(layer_norm_long_kernel<T>, dim3(a.rows < 4096 ? a.rows : 4096), dim3(1024), 0, stream, a);
         return;
     }
-    with_team<T>(vec, a.cols, [&](auto v, auto team, auto e) {
+    with_team<T, false>(whole, a.cols, [&](auto v, auto team, auto e, auto odd) {
         constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = forward_threads(TEAM);
         // four rounds of the chip's waves at most: a team that goes down several rows reads weight and bias once
         const long want = ((long)a.rows * TEAM + THREADS - 1) / THREADS, most = 2048L / THREADS * cu_count();
-        hipLaunchKernelGGL((layer_norm_kernel<T, V, TEAM, E>), dim3((unsigned)(want < most ? want : most)), dim3(THREADS), 0, stream, a);
+        hipLaunchKernelGGL((layer_norm_kernel<T, V, TEAM, E, decltype(odd)::value>), dim3((unsigned)(want < most ? want : most)), dim3(THREADS), 0, stream, a);
     });
 }
 
 template <class T>
-void launch_grad(NormArgs &a, bool vec, hipStream_t stream) {
-    if (a.cols > most_held(vec, sizeof(T))) {
+void launch_grad(NormArgs &a, bool whole, hipStream_t stream) {
+    if (a.cols > most_held(sizeof(T), true)) {
         a.groups = a.rows < cu_count() ? a.rows : cu_count();
         hipLaunchKernelGGL(layer_norm_grad_long_kernel<T>, dim3(a.groups), dim3(1024), 0, stream, a);
         return;
     }
-    with_team<T>(vec, a.cols, [&](auto v, auto team, auto e) {
-        constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = grad_threads(TEAM, V, E * sizeof(T)), AT_ONCE = THREADS == 1024 || V == 1 || E * sizeof(T) > 32 ? 1 : 2;
+    with_team<T, true>(whole, a.cols, [&](auto v, auto team, auto e, auto odd) {
+        constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = grad_threads(TEAM),
+                      AT_ONCE = grad_waves(E, sizeof(T), decltype(odd)::value) * 256 / THREADS > 1 ? 2 : 1;
         const long want = ((long)a.rows * TEAM + THREADS - 1) / THREADS, most = (long)AT_ONCE * cu_count();
         a.groups = (int)(want < most ? want : most);
-        hipLaunchKernelGGL((layer_norm_grad_kernel<T, V, TEAM, E>), dim3((unsigned)a.groups), dim3(THREADS), 0, stream, a);
+        hipLaunchKernelGGL((layer_norm_grad_kernel<T, V, TEAM, E, decltype(odd)::value>), dim3((unsigned)a.groups), dim3(THREADS), 0, stream, a);
     });
 }
 

@@ -71,7 +71,7 @@ struct QuantizeArgs {
 template <int TEAM>
 __device__ __forceinline__ unsigned team_max(unsigned m, unsigned *slots, int &turn) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+    for (int d = 1; d < (TEAM < 64 ? TEAM : 64); d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
     if constexpr (TEAM > 64) {
         unsigned *s = slots + turn * 16;
         turn ^= 1;
@@ -88,15 +88,15 @@ __device__ __forceinline__ unsigned team_max(unsigned m, unsigned *slots, int &t
 
 constexpr int rows_threads(int team) { return team < 256 ? 256 : team; }
 
-template <class T, int V, int TEAM, int E>
+template <class T, int V, int TEAM, int E, bool ODD>
 __global__ __launch_bounds__(rows_threads(TEAM)) void quantize_rows_kernel(QuantizeArgs a) {
     __shared__ unsigned slots[2 * 16];
     constexpr int TEAMS = rows_threads(TEAM) / TEAM;
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     int turn = 0;
     const long row = (long)blockIdx.x * TEAMS + team;
-    Held<T, V, TEAM, E> x;
-    if (row < a.rows) x.load((const T *)a.x + row * a.ldx, t, a.cols);
+    Held<T, V, TEAM, E, ODD> x;
+    if (row < a.rows) x.load((const T *)a.x + row * a.ldx, t, a.cols), x.settle(t, a.cols);
     unsigned size = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) size = max(size, row < a.rows ? size_of(x.at(e)) : 0u);
@@ -180,15 +180,15 @@ __global__ __launch_bounds__(256) void quantize_columns_kernel(QuantizeArgs a) {
 template <class T>
 void launch_rows(const QuantizeArgs &a, hipStream_t stream) {
     const int v = 16 / (int)sizeof(T);
-    const bool vec = ((size_t)a.x & 15) == 0 && a.cols % v == 0 && a.ldx % v == 0;
-    if (a.cols > most_held(vec, sizeof(T))) {
+    const bool whole = ((size_t)a.x & 15) == 0 && a.cols % v == 0 && a.ldx % v == 0;
+    if (a.cols > most_held(sizeof(T), false)) {
         hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3(a.rows < 4096 ? a.rows : 4096), dim3(1024), 0, stream, a);
         return;
     }
-    with_team<T>(vec, a.cols, [&](auto v, auto team, auto e) {
+    with_team<T, false>(whole, a.cols, [&](auto v, auto team, auto e, auto odd) {
         constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = rows_threads(TEAM);
         const long groups = ((long)a.rows * TEAM + THREADS - 1) / THREADS;
-        hipLaunchKernelGGL((quantize_rows_kernel<T, V, TEAM, E>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a);
+        hipLaunchKernelGGL((quantize_rows_kernel<T, V, TEAM, E, decltype(odd)::value>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a);
     });
 }
 

@@ -1,5 +1,4 @@
-// Rows that a team of 64, 256 or 1024 threads holds in registers: how they are loaded and stored, and which team a row takes (layer_norm.hip,
-// quantize.hip).
+// Rows that a team of 16 to 1024 threads holds in registers: how they are loaded and stored, and which team a row takes (layer_norm.hip, quantize.hip).
 #ifndef DEEP8_AMD_ROW_TEAM_H
 #define DEEP8_AMD_ROW_TEAM_H
 
@@ -10,40 +9,48 @@
 namespace d8 {
 namespace row_team {
 
-// Elements of a row that a team holds (16 a thread of 1024 do not leave the gradient enough registers in single precision).
-constexpr int most_held(bool vec, int bytes) { return vec && bytes == 2 ? 16384 : 8192; }
+// Elements of a row that a team holds: 16 a thread of 1024, which in single precision do not leave a gradient enough registers.
+constexpr int most_held(int bytes, bool grad) { return bytes == 4 && grad ? 8192 : 16384; }
 
-template <class T, int V>
-struct Vec {
-    typedef T type __attribute__((ext_vector_type(V)));
-};
-template <class T>
-struct Vec<T, 1> {
-    typedef T type;
-};
-
-// E elements of a row of T in one thread, in pieces of V: piece i is number t + TEAM * i of the row.
-template <class T, int V, int TEAM, int E>
+// E elements of a row of T in one thread, in pieces of V: piece i is number t + TEAM * i of the row.  ODD: the row, of V elements at least, starts
+// anywhere, and may end within a piece, for which the row's last V are read; settle() then moves them down.  (Norm of 16384 rows of 1001 in half: 15 us, 32
+// element by element.  A load that branches where the row ends keeps the next row's from running ahead: gradients of 4096 rows of 4095 took 51 us
+// so, and 34 with this.)
+template <class T, int V, int TEAM, int E, bool ODD>
 struct Held {
     static constexpr int P = E / V;
-    typedef typename Vec<T, V>::type vec;
+    typedef T vec __attribute__((ext_vector_type(V)));
+    typedef T odd_vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    typedef std::conditional_t<ODD, odd_vec, vec> there;
     vec raw[P];
+    // whether element e of the thread's is one of the row's
+    static __device__ __forceinline__ bool has(int e, int t, int cols) { return (t + TEAM * (e / V)) * V + (ODD ? e % V : 0) < cols; }
     __device__ __forceinline__ void load(const T *row, int t, int cols) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int c = (t + TEAM * i) * V;
-            if (c < cols) raw[i] = *(const vec *)(row + c);
+            if constexpr (ODD) raw[i] = *(const there *)(row + min(c, cols - V));
+            else if (c < cols) raw[i] = *(const vec *)(row + c);
             else raw[i] = vec{};
+        }
+    }
+    // after a load, before its elements are used: those beyond the row are 0
+    __device__ __forceinline__ void settle(int t, int cols) {
+        if constexpr (ODD) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int beyond = (t + TEAM * i) * V - (cols - V);
+                if (beyond <= 0) continue;
+                typedef unsigned _BitInt(8 * V * sizeof(T)) bits;
+                raw[i] = beyond < V ? __builtin_bit_cast(vec, (bits)(__builtin_bit_cast(bits, raw[i]) >> (8 * (int)sizeof(T) * beyond))) : vec{};
+            }
         }
     }
     __device__ __forceinline__ void ones() {
 #pragma unroll
         for (int i = 0; i < P; ++i) raw[i] = vec{} + (T)1;
     }
-    __device__ __forceinline__ float at(int e) const {
-        if constexpr (V == 1) return (float)raw[e];
-        else return (float)raw[e / V][e % V];
-    }
+    __device__ __forceinline__ float at(int e) const { return (float)raw[e / V][e % V]; }
     __device__ __forceinline__ void get(float (&v)[E]) const {
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = at(e);
@@ -51,21 +58,21 @@ struct Held {
     // the same values, but not to the compiler: what it made of them before is not kept
     __device__ __forceinline__ void renew() {
 #pragma unroll
-        for (int i = 0; i < P; ++i) asm volatile("" : "+v"(raw[i]));
+        for (int i = 0; i < P; ++i)
+            if constexpr (V > 1) asm volatile("" : "+v"(raw[i]));
     }
     static __device__ __forceinline__ void store(T *row, int t, int cols, const float (&v)[E]) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int c = (t + TEAM * i) * V;
-            if (c >= cols) continue;
             vec w;
-            if constexpr (V == 1) {
-                w = (T)v[i];
-            } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) w[e] = (T)v[i * V + e];
-            }
-            *(vec *)(row + c) = w;
+            for (int e = 0; e < V; ++e) w[e] = (T)v[i * V + e];
+            if (ODD ? c + V <= cols : c < cols) *(there *)(row + c) = w;
+            else if (ODD && c < cols)
+#pragma unroll
+                for (int e = 0; e < V - 1; ++e)
+                    if (c + e < cols) row[c + e] = w[e];
         }
     }
 };
@@ -75,7 +82,7 @@ struct Held {
 template <int TEAM>
 __device__ __forceinline__ void team_sum(float &a, float &b, float2 *slots, int &turn) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
+    for (int d = 1; d < (TEAM < 64 ? TEAM : 64); d <<= 1) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
     if constexpr (TEAM > 64) {
         const int wave = threadIdx.x >> 6;
         float2 *s = slots + turn * 16;
@@ -90,24 +97,28 @@ __device__ __forceinline__ void team_sum(float &a, float &b, float2 *slots, int 
     }
 }
 
-// fn<V, TEAM, E> for the smallest team that holds a row; rows that do not start at multiples of 16 bytes go element by element
-template <class T, class F>
-void with_team(bool vec, int cols, F &&fn) {
+// fn(V, TEAM, E, ODD) for the smallest team that holds a row; whole: every row is whole pieces of 16 bytes.  Short rows share a wave (65536 of 96 in half:
+// norm 9 us, 21 with a wave each); 16 elements a thread of 512 are better than 8 of 1024, of whose workgroups a compute unit has half as many to change
+// between (8192 rows of 5120: 43 us and 78).
+template <class T, bool GRAD, class F>
+void with_team(bool whole, int cols, F &&fn) {
     constexpr int V = 16 / sizeof(T);
-#define D8_TEAM(V_, TEAM_, E_) fn(std::integral_constant<int, V_>(), std::integral_constant<int, TEAM_>(), std::integral_constant<int, E_>())
-    if (!vec) {
-        if (cols <= 1024) D8_TEAM(1, 64, 16);
-        else if (cols <= 4096) D8_TEAM(1, 256, 16);
-        else D8_TEAM(1, 1024, 8);
-    } else if (cols <= 512) D8_TEAM(V, 64, 8);
-    else if (cols <= 1024) D8_TEAM(V, 64, 16);
-    else if (cols <= 2048) D8_TEAM(V, 256, 8);
-    else if (cols <= 4096) D8_TEAM(V, 256, 16);
-    else if (cols <= 8192) D8_TEAM(V, 1024, 8);
-    else if constexpr (sizeof(T) == 2) D8_TEAM(V, 1024, 16);
+    if (cols < V) return fn(std::integral_constant<int, 1>(), std::integral_constant<int, 16>(), std::integral_constant<int, 8>(), std::true_type());
+    auto in = [&](auto odd) {
+#define D8_TEAM(TEAM_, E_) fn(std::integral_constant<int, V>(), std::integral_constant<int, TEAM_>(), std::integral_constant<int, E_>(), odd)
+        if (cols <= 128) D8_TEAM(16, 8);
+        else if (cols <= 512) D8_TEAM(64, 8);
+        else if (cols <= 1024) D8_TEAM(64, 16);
+        else if (cols <= 2048) D8_TEAM(256, 8);
+        else if (cols <= 4096) D8_TEAM(256, 16);
+        else if constexpr (most_held(sizeof(T), GRAD) == 8192) D8_TEAM(1024, 8);
+        else if (cols <= 8192) D8_TEAM(512, 16);
+        else D8_TEAM(1024, 16);
 #undef D8_TEAM
+    };
+    if (whole) in(std::false_type());
+    else in(std::true_type());
 }
-
 
 }  // namespace row_team
 }  // namespace d8

@@ -4,7 +4,7 @@ Tolerances, element by element.  HALF: the result's own rounding, half a step of
 step E = 2^-24): an element's distance from the mean is good to E of itself and, by the mean, to a few E of the spread; the spread's square is a
 sum of at most 16 terms a lane in a row, then 6 + 2 levels of lanes and waves: 24 roundings; the reciprocal of its root three more.  32 E of what is added up covers
 it.  dx adds two more such sums: 64 E.  dw and db: a row's term as above, then sums of at most 20 rows a lane, 16 teams, 16 workgroups a wave and
-16 waves: 68 roundings more, 128 E in all."""
+16 waves (teams of 16 threads: a row, 32 teams, 9 workgroups, 16 waves): 68 roundings more, 128 E in all."""
 import numpy as np
 import pytest
 
@@ -15,9 +15,10 @@ HALF = {np.float16: 2.0 ** -11, np.float32: 2.0 ** -24}
 E = 2.0 ** -24
 TINY = {np.float16: 2.0 ** -25, np.float32: 0.0}  # half a step of the smallest numbers
 
-# rows, cols, pad: teams of 64, 256 and 1024 threads with 8 and 16 elements each, rows in 16-byte pieces and not, rows that no team holds
+# rows, cols, pad: teams of 16, 64, 256, 512 and 1024 threads with 8 and 16 elements each, rows in 16-byte pieces and not, shorter than one, rows that no team holds
 CASES = [(1, 1, 0), (3, 7, 1), (5, 64, 0), (2, 512, 8), (9, 520, 0), (33, 1000, 0), (3, 1024, 3), (7, 1025, 0), (5, 2048, 0), (3, 2056, 8), (6, 4096, 0),
-         (2, 4097, 0), (3, 8192, 0), (2, 8200, 8), (3, 16384, 0), (2, 16384, 1), (3, 16385, 0), (2, 20000, 8), (700, 96, 0), (4099, 100, 0), (1030, 1000, 24)]
+         (2, 4097, 0), (3, 8192, 0), (2, 8200, 8), (3, 16384, 0), (2, 16384, 1), (3, 16385, 0), (2, 20000, 8), (700, 96, 0), (4099, 100, 0), (1030, 1000, 24),
+         (700, 3, 0), (65, 8, 0), (33, 9, 1), (70, 128, 0), (33, 127, 1), (9, 129, 3), (4, 2047, 0), (300, 4095, 5), (2, 5120, 0), (3, 8191, 2), (2, 8193, 0), (2, 11111, 0)]
 
 
 def _inputs(rows, cols, dtype, seed, shift=0.0):
