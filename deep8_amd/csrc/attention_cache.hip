@@ -14,15 +14,15 @@
 // KEYS, for few rows: a workgroup has 16 rows, its four waves share out the pages, each by itself and a page ahead, and join through LDS.
 // ROWS, from 64 rows a sequence on and for heads of 128 elements at most: eight waves have 16 rows each and go through the pages together; a page's codes
 // are converted once and go through LDS as operands, in two buffers.  (4 x 128 queries of 32 heads over 32768 keys of 8: 320 us with every wave converting
-// for itself, 137 so.)
+// for itself, 131 so.)
 //
 // All tiles' pages, one after the other, are cut into as many equal runs as workgroups run at once, whatever sequences have how many: a workgroup
 // goes through its run and leaves, for a tile that it has not all of, sums in scratch, which a second launch joins.  Cuts are found from the
 // lengths on the device, so a call can be captured and replayed as sequences grow.
 //
-// KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 66 us, 4.1 TB/s, where
-// a large copy moves 5.2; single precision 77 us.  ROWS by conversions, exponentials and matrix instructions, which share an issue slot: 1 x 2048 queries
-// of 32 heads over 8192 keys take 365 us, 660 TFLOP/s, where a large product of the library makes 1200.  Short calls are bound by latency: a wave's
+// KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 65 us, 4.1 TB/s, where
+// a large copy moves 5.2; single precision 66 us.  ROWS by conversions, exponentials and matrix instructions, which share an issue slot: 1 x 2048 queries
+// of 32 heads over 8192 keys take 355 us, 680 TFLOP/s, where a large product of the library makes 1200.  Short calls are bound by latency: a wave's
 // way from the first length to its last store is 10 us, and the join 4.
 //
 // Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product.
@@ -239,20 +239,35 @@ __device__ __forceinline__ void split(float (&x)[16], f16x8 (&out)[PARTS][2]) {
 __device__ __forceinline__ f32x4 mma(const f16x8 &a, const f16x8 &b, const f32x4 &c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // the larger, and the sum, of the four lanes that have a row (l, l + 16, l + 32, l + 48)
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x2 half_rows(float x) { return __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false)); }
+__device__ __forceinline__ u32x2 halves(float x) { return __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false)); }
 __device__ __forceinline__ float row_max(float x) {
-    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-    u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
-    x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-    y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    u32x2 y = half_rows(x);
+    y = halves(fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])));
     return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 __device__ __forceinline__ float row_sum(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    u32x2 y = half_rows(x);
+    y = halves(__uint_as_float(y[0]) + __uint_as_float(y[1]));
+    return __uint_as_float(y[0]) + __uint_as_float(y[1]);
 }
 
 // ---- one wave, 16 rows ----------------------------------------------------------------------------------------------
 // NC: chunks of 64 elements of a head.
+// The lane, and a number that all lanes have, to the compiler others at every tile: what depends on them (addresses, comparisons with a head's elements,
+// reciprocals of divisors) would be kept for the whole launch in registers that the products need: 16 queries over 131072 keys in single, 75 us with and 66 so.
+__device__ __forceinline__ int fresh_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+template <class N>
+__device__ __forceinline__ N fresh(N x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
 template <class T, int NC>
 struct Wave {
     typedef Precision<T> P;
@@ -266,20 +281,21 @@ struct Wave {
 
     // rows row0 .. of the sequence (those beyond `rows` are zero and see nothing)
     __device__ __forceinline__ void begin(const AttArgs &a, const Seq &s, int head, long row0, long rows) {
-        const long row = row0 + (threadIdx.x & 15);
+        const long row = row0 + (fresh_lane() & 15);
         const bool there = row < rows;
-        const int t = there ? (int)row / a.group : 0, h = there ? (int)row - t * a.group : 0;
+        const int group = fresh(a.group), t = there ? (int)row / group : 0, h = there ? (int)row - t * group : 0;
         const long sees = a.causal ? t + s.len - s.n + 1 : s.len;
         limit = there ? (int)min(max(sees, 0L), (long)s.keys) : 0;
-        from = there ? (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * a.group + h) * a.c.dim : nullptr;
+        from = there ? (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * group + h) * a.c.dim : nullptr;
         m = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NC * 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
     __device__ __forceinline__ void load_queries(const AttArgs &a) {
-        const int g = (threadIdx.x & 63) >> 4;
+        const int g = fresh_lane() >> 4;
         const bool there = from != nullptr;
+        const int dim = fresh(a.c.dim);
         float x[NC][16], largest = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -288,13 +304,13 @@ struct Wave {
             typedef T piece __attribute__((ext_vector_type(V)));
 #pragma unroll
             for (int i = 0; i < 16; i += V) {
-                if (a.vec && there && d + i < a.c.dim) {  // (dim is whole pieces)
+                if (a.vec && there && d + i < dim) {  // (dim is whole pieces)
                     const piece p = *(const piece *)(from + d + i);
 #pragma unroll
                     for (int e = 0; e < V; ++e) x[c][i + e] = (float)p[e];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) x[c][i + e] = !a.vec && there && d + i + e < a.c.dim ? (float)from[d + i + e] : 0.f;
+                    for (int e = 0; e < V; ++e) x[c][i + e] = !a.vec && there && d + i + e < dim ? (float)from[d + i + e] : 0.f;
                 }
             }
             if (P::QUERY > 1)
@@ -319,20 +335,18 @@ struct Wave {
 
     // where a lane's operands lie in a page and head: its key's row of tile t (16 bytes of chunk n; beyond the head any codes, times zeros of q),
     // its element's of tile i
-    static __device__ __forceinline__ const i32x4 *key_at(const Pages &c, const signed char *page, int t, int n) {
-        const int lane = threadIdx.x & 63, r = lane & 15, d = n * 64 + (lane >> 4) * 16;
+    static __device__ __forceinline__ const i32x4 *key_at(const Pages &c, const signed char *page, int lane, int t, int n) {
+        const int r = lane & 15, d = n * 64 + (lane >> 4) * 16;
         return (const i32x4 *)(page + ((r >> 2) * 16 + (r & 3) + 4 * t) * c.pitch + (d < c.pitch ? d : 0));
     }
-    static __device__ __forceinline__ const i32x4 *value_at(const signed char *page, int i) {
-        const int lane = threadIdx.x & 63;
+    static __device__ __forceinline__ const i32x4 *value_at(const signed char *page, int lane, int i) {
         return (const i32x4 *)(page + (i * 16 + (lane & 15)) * PAGE + (lane >> 4) * 16);
     }
 
     // Scores of a page whose first place is `at` to weights; accumulators and sums to the new maximum.  hidden: some row does not see all of
     // the page (or there is none).  `into`: what the page's sums are scaled by, 0 where the lane's row sees none of it.
-    __device__ __forceinline__ void weigh(const f32x4 (&sc)[4], int at, bool there, bool hidden, float k_scale, float v_scale, f16x8 (&p)[P::WEIGHT][2], float &into) {
+    __device__ __forceinline__ void weigh(const f32x4 (&sc)[4], int g, int at, bool there, bool hidden, float k_scale, float v_scale, f16x8 (&p)[P::WEIGHT][2], float &into) {
 #pragma clang fp contract(off)  // (a fused product less its rounded maximum can be anything but small where scores are large)
-        const int g = (threadIdx.x & 63) >> 4;
         float x[16], by = P::QUERY > 1 ? k_scale * q_scale : k_scale;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = sc[i >> 2][i & 3];
@@ -395,7 +409,7 @@ struct Wave {
     // KEYS: `count` pages, 64 at most, first, first + step, ... of sequence s, by this wave alone.  fresh: load the queries too
     __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int count, int step, bool fresh) {
         const Pages &c = a.c;
-        const int least = uniform(limit);
+        const int lane = fresh_lane(), least = uniform(limit);
         List list;
         list.load(c, s, head, first, count, step);
         i32x4 kr[4][NC], vr[NC * 4];
@@ -404,13 +418,13 @@ struct Wave {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int n = 0; n < NC; ++n) kr[t][n] = *key_at(c, from, t, n);
+                for (int n = 0; n < NC; ++n) kr[t][n] = *key_at(c, from, lane, t, n);
         };
         auto fetch_values = [&](int page) {
             const signed char *from = c.v_codes + c.tile(page, head);
 #pragma unroll
             for (int i = 0; i < NC * 4; ++i)
-                if (i * 16 < c.pitch) vr[i] = *value_at(from, i);
+                if (i * 16 < c.pitch) vr[i] = *value_at(from, lane, i);
         };
         fetch_keys(list.id(0)), fetch_values(list.id(0));
         if (fresh) load_queries(a);
@@ -433,7 +447,7 @@ struct Wave {
             if (more) fetch_keys(next);
             f16x8 p[P::WEIGHT][2];
             float into;
-            weigh(sc, at, there, !there || at + PAGE > least, list.k(n) * (a.scale * LOG2E), list.v(n), p, into);
+            weigh(sc, lane >> 4, at, there, !there || at + PAGE > least, list.k(n) * (a.scale * LOG2E), list.v(n), p, into);
 #pragma unroll
             for (int i = 0; i < NC * 4; ++i) {
                 if (i * 16 >= c.pitch) continue;
@@ -452,7 +466,7 @@ struct Wave {
     // eighth by each wave, and go through LDS as operands, lane by lane: [keys' tile][chunk][half], then [values' tile][half], a buffer for every other page.
     __device__ __forceinline__ void pages_together(const AttArgs &a, int s, int head, int first, int count, int wave, f16x8 (*stages)[16 * NC][64]) {
         const Pages &c = a.c;
-        const int lane = threadIdx.x & 63, own_end = most(), least = uniform(limit);
+        const int lane = fresh_lane(), own_end = most(), least = uniform(limit);
         List list;
         list.load(c, s, head, first, count, 1);
         i32x4 share[NC];
@@ -461,8 +475,8 @@ struct Wave {
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
                 const int item = wave + ROWS_WAVES * n;
-                if (item < 4 * NC) share[n] = *key_at(c, k, item / NC, item % NC);
-                else if ((item - 4 * NC) * 16 < c.pitch) share[n] = *value_at(v, item - 4 * NC);
+                if (item < 4 * NC) share[n] = *key_at(c, k, lane, item / NC, item % NC);
+                else if ((item - 4 * NC) * 16 < c.pitch) share[n] = *value_at(v, lane, item - 4 * NC);
             }
         };
         auto stage = [&](int to) {
@@ -507,7 +521,7 @@ struct Wave {
                 }
                 f16x8 p[P::WEIGHT][2];
                 float into;
-                weigh(sc, at, there, !there || at + PAGE > least, list.k(n) * (a.scale * LOG2E), list.v(n), p, into);
+                weigh(sc, lane >> 4, at, there, !there || at + PAGE > least, list.k(n) * (a.scale * LOG2E), list.v(n), p, into);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int k = 0; k < 2 * NC; ++k) {
@@ -554,7 +568,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
     __shared__ f16x8 stages[ROWS ? 2 : 1][ROWS ? 16 * NC : 1][64];
     __shared__ f32x4 others[ROWS ? 1 : WAVES][ROWS ? 1 : NC * 4][64];
     __shared__ float2 stats[ROWS ? 1 : WAVES][16];
-    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), r = lane & 15, g = lane >> 4;
+    const int wave = uniform((int)(threadIdx.x >> 6));
     const int head = blockIdx.x % a.c.kv_heads, run = blockIdx.x / a.c.kv_heads;
     Scan<R> scan;
     scan.begin(a);
@@ -570,22 +584,23 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
     if (!scan.locate(a, at, seq, s, base, tile_base)) return;
     Wave<T, NC> w;
     for (;;) {
-        const long after = base + seq.cost();
-        while (at < last && at < after) {
-            const long tile = (at - base) / seq.pages;
-            const int first = (int)(at - base - tile * seq.pages), end = (int)min(seq.pages, first + (last - at));
+        const long after = base + seq.cost(), stop = min(fresh(last), after);
+        while (at < stop) {
+            const long tile = (at - base) / fresh(seq.pages);
+            const int first = (int)(at - base - tile * seq.pages), end = (int)min(seq.pages, first + (stop - at));
             const bool whole = first == 0 && end == seq.pages;
             const long rows = (long)seq.n * a.group, row0 = tile * R + (ROWS ? wave * 16 : 0), slot = run + tile_base + tile;
             if (first == 0 && head == 0 && threadIdx.x == 0) {  // (the tile's first page: every head's parts are alike)
                 const long from = base + tile * seq.pages, to = from + seq.pages - 1;
-                const int parts = (int)(to / length - from / length) + 1;
+                const long run_length = fresh(length);
+                const int parts = (int)(to / run_length - from / run_length) + 1;
                 a.joins[tile_base + tile] = Join{parts == 1 ? 0 : parts, run, seq.q0, (int)(tile * R), (int)(rows - tile * R), {0, 0, 0}};
             }
             w.begin(a, seq, head, row0, rows);
             if (!LATE) w.load_queries(a);
             if constexpr (ROWS) {
                 // what the tile's last row sees: all waves go through as many pages
-                const int t = ((int)min((tile + 1) * R, rows) - 1) / a.group;
+                const int t = ((int)min((tile + 1) * R, rows) - 1) / fresh(a.group);
                 const long sees = min(max(a.causal ? t + seq.len - seq.n + 1 : seq.len, 0L), (long)seq.keys);
                 const int upto = min(end, (int)((sees + PAGE - 1) / PAGE));
                 for (int i = first; i < upto; i += 64) w.pages_together(a, s, head, i, min(64, upto - i), wave, stages);
@@ -593,6 +608,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
                 const int upto = min(end, w.most());
                 for (int i = first + wave; i < upto; i += 64 * WAVES) w.pages(a, s, head, i, min(64, (upto - i + WAVES - 1) / WAVES), WAVES, LATE && i == first + wave);
             }
+            const int lane = fresh_lane(), r = lane & 15, g = lane >> 4;
             at += end - first;
             w.sum = row_sum(w.sum);
             if constexpr (!ROWS) {
@@ -622,7 +638,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
             const long row = row0 + r;
             if (row >= rows) continue;
             if (whole) {
-                const int t = (int)row / a.group, h = head * a.group + (int)row - t * a.group;
+                const int group = fresh(a.group), t = (int)row / group, h = head * group + (int)row - t * group;
                 T *to = (T *)a.o + (seq.q0 + (long)t) * a.ldo + (long)h * a.c.dim;
                 const float inv = w.sum == 0.f ? 0.f : 1.f / w.sum;
 #pragma unroll
@@ -638,7 +654,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
                 if (g == 0 && (ROWS || wave == 0)) *(float2 *)(a.part_ml + place * 2) = make_float2(w.m, w.sum);
             }
         }
-        if (at >= last) return;
+        if (at >= fresh(last)) return;
         base = after, tile_base += seq.tiles;
         if (!advance<R>(a, seq, s)) return;
     }
