@@ -5,6 +5,8 @@ step E = 2^-24): an element's distance from the mean is good to E of itself and,
 sum of at most 16 terms a lane in a row, then 6 + 2 levels of lanes and waves: 24 roundings; the reciprocal of its root three more.  32 E of what is added up covers
 it.  dx adds two more such sums: 64 E.  dw and db: a row's term as above, then sums of at most 20 rows a lane, 16 teams, 16 workgroups a wave and
 16 waves (teams of 16 threads: a row, 32 teams, 9 workgroups, 16 waves): 68 roundings more, 128 E in all."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -144,6 +146,40 @@ def test_no_rows():
     old = (x, np.ones(24, np.float32), np.full(24, 2, np.float32))
     _, dw, db = ops.layer_norm_grad(x, x, into=old)
     assert (dw == 1).all() and (db == 2).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("rows,cols", [(40, 96), (300, 1001), (1000, 4096), (5, 17000)])
+def test_captured_and_replayed(rows, cols, dtype):
+    """both directions on a stream of the caller's, captured: the bits of the eager calls at every replay, with eager calls of other sizes between them"""
+    from deep8_amd import capi, ops
+    lib = capi.init()
+    code = capi.FLOAT16 if dtype == np.float16 else capi.FLOAT32
+    x, w, b, dy = _inputs(rows, cols, dtype, rows)
+    want = (ops.layer_norm(x, w, b), *ops.layer_norm_grad(x, dy, w))
+    d = [capi.DeviceArray.from_numpy(a) for a in (x, w, b, dy)]
+    out = [capi.DeviceArray.from_numpy(np.full(a.shape, 7, dtype)) for a in want]
+    nb = lib.d8_layer_norm_grad_scratch_bytes(code, rows, cols)
+    scratch = capi.DeviceArray((nb,), np.uint8)
+    stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    capi.check(lib.d8_stream_create(ctypes.byref(stream)))
+    capi.sync()
+    capi.check(lib.d8_graph_begin(stream))
+    rcs = (lib.d8_layer_norm(code, d[0].ptr, cols, d[1].ptr, d[2].ptr, out[0].ptr, cols, rows, cols, 1e-5, stream),
+           lib.d8_layer_norm_grad(code, d[0].ptr, cols, d[1].ptr, d[3].ptr, cols, out[1].ptr, cols, out[2].ptr, out[3].ptr, rows, cols, 1e-5, 3, scratch.ptr, nb, stream))
+    capi.check(lib.d8_graph_end(stream, ctypes.byref(graph)))
+    for rc in rcs:
+        capi.check(rc)
+    for _ in range(3):
+        for o in out:
+            o.copy_from(np.full(o.shape, 7, dtype))
+        capi.check(lib.d8_graph_launch(graph, stream))
+        capi.sync(stream)
+        assert all(np.array_equal(o.numpy(), a) for o, a in zip(out, want))
+        ops.layer_norm_grad(x[: rows // 2], dy[: rows // 2], w)
+    capi.check(lib.d8_graph_destroy(graph))
+    capi.check(lib.d8_stream_destroy(stream))
 
 
 def test_refusals():
