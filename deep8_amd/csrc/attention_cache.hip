@@ -21,8 +21,10 @@
 // lengths on the device, so a call can be captured and replayed as sequences grow.
 //
 // KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 65 us, 4.1 TB/s, where
-// a large copy moves 5.2; single precision 66 us.  ROWS by conversions, exponentials and matrix instructions, which share an issue slot: 1 x 2048 queries
-// of 32 heads over 8192 keys take 355 us, 680 TFLOP/s, where a large product of the library makes 1200.  Short calls are bound by latency: a wave's
+// a large copy moves 5.2; single precision 66 us.  ROWS by no unit alone: 1 x 2048 queries of 32 heads over
+// 8192 keys take 355 us, 680 TFLOP/s, where a large product of the library makes 1200; the vector units are busy for 38 % of the time with
+// what lies between the products, the matrix units for 30 %, LDS for 39 %, and a workgroup's waves are mostly at the same of them.  (Two sets of rows a wave,
+// which halve what LDS reads and leave two waves a SIMD: 155 us in place of 133.)  Short calls are bound by latency: a wave's
 // way from the first length to its last store is 10 us, and the join 4.
 //
 // Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product.
@@ -779,7 +781,7 @@ extern "C" int d8_attention_cache(int dtype, const void *q, long ldq, const sign
     const cache::Plan p = cache::plan_of(dtype, sequences, q_tokens, table_pages, heads, kv_heads, dim);
     const size_t need = cache::scratch_of(p, kv_heads, dim);
     D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "attention_cache: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
-    D8_REQUIRE(p.units * kv_heads < (1L << 31), "attention_cache: too many sequences");
+    D8_REQUIRE(p.units * kv_heads < (1L << 24), "attention_cache: too many tokens and sequences for a launch");
     const int v = 16 / (int)dtype_bytes(dtype);
     a.q = q, a.ldq = ldq, a.o = o, a.ldo = ldo, a.lse = lse, a.heads = heads, a.group = heads / kv_heads, a.causal = causal != 0, a.scale = scale, a.runs = p.runs;
     a.vec = dim % v == 0 && ldq % v == 0 && ldo % v == 0 && (((size_t)q | (size_t)o) & 15) == 0;

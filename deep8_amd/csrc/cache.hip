@@ -297,16 +297,17 @@ __global__ __launch_bounds__(256) void cache_read_kernel(Args a) {
     if (share_of(a.c, blockIdx.x / a.c.kv_heads, s)) read<T, V>(a, s.row, s.rows, s.slot, s.page, blockIdx.x % a.c.kv_heads, words);
 }
 
-// Workgroups of a call: n rows of a sequence reach (n + 62) / 64 + 1 pages at most, and each at least one.
-dim3 grid_of(const Pages &c) {
+// Workgroups of a call, for each head: n rows of a sequence reach (n + 62) / 64 + 1 pages at most, and each at least one.
+long shares_of(const Pages &c) {
     const long some = c.sequences < c.tokens ? c.sequences : c.tokens, shares = (c.tokens + 62 * some) / 64 + some;
-    return dim3((unsigned)((shares < c.tokens ? shares : c.tokens) * c.kv_heads));
+    return shares < c.tokens ? shares : c.tokens;
 }
 
 int check_rows(const Args &a, const char *name) {
     const long row = (long)a.c.kv_heads * a.c.dim;
     D8_REQUIRE(a.k && a.v, "%s: null tensor", name);
     D8_REQUIRE(a.ldk >= row && a.ldv >= row, "%s: rows of %ld elements do not fit their leading dimensions", name, row);
+    D8_REQUIRE(shares_of(a.c) * a.c.kv_heads < (1L << 24), "%s: too many tokens and sequences for a launch", name);
     return 0;
 }
 
@@ -343,7 +344,7 @@ extern "C" int d8_cache_append(int dtype, const void *k, long ldk, const void *v
     if (!sequences || !tokens) return 0;
     if (int rc = cache::check_rows(a, "cache_append")) return rc;
     if (!pages || !table_pages) return 0;
-    const dim3 grid = cache::grid_of(a.c);
+    const dim3 grid((unsigned)(cache::shares_of(a.c) * kv_heads));
     if (dtype == D8_FLOAT16) cache::launch_append<f16>(a, grid, as_stream(stream));
     else cache::launch_append<float>(a, grid, as_stream(stream));
     D8_LAUNCH_CHECK();
@@ -359,7 +360,7 @@ extern "C" int d8_cache_read(int dtype, void *k, long ldk, void *v, long ldv, co
     if (int rc = cache::check(a.c, dtype, "cache_read")) return rc;
     if (!sequences || !tokens) return 0;
     if (int rc = cache::check_rows(a, "cache_read")) return rc;
-    const dim3 grid = cache::grid_of(a.c);
+    const dim3 grid((unsigned)(cache::shares_of(a.c) * kv_heads));
     if (dtype == D8_FLOAT16) cache::launch_read<f16>(a, grid, as_stream(stream));
     else cache::launch_read<float>(a, grid, as_stream(stream));
     D8_LAUNCH_CHECK();

@@ -94,28 +94,30 @@ __global__ __launch_bounds__(rows_threads(TEAM)) void quantize_rows_kernel(Quant
     constexpr int TEAMS = rows_threads(TEAM) / TEAM;
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     int turn = 0;
-    const long row = (long)blockIdx.x * TEAMS + team;
-    Held<T, V, TEAM, E, ODD> x;
-    if (row < a.rows) x.load((const T *)a.x + row * a.ldx, t, a.cols), x.settle(t, a.cols);
-    unsigned size = 0;
+    for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += (long)gridDim.x * TEAMS) {  // (once, but for more rows than a launch has threads)
+        const long row = first + team;
+        Held<T, V, TEAM, E, ODD> x;
+        if (row < a.rows) x.load((const T *)a.x + row * a.ldx, t, a.cols), x.settle(t, a.cols);
+        unsigned size = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) size = max(size, row < a.rows ? size_of(x.at(e)) : 0u);
-    size = team_max<TEAM>(size, slots, turn);
-    if (row >= a.rows) return;
-    const float scale = scale_of(size), back = finite(size) ? 1.f / scale : 0.f;
-    signed char *to = a.codes + row * a.pitch;
+        for (int e = 0; e < E; ++e) size = max(size, row < a.rows ? size_of(x.at(e)) : 0u);
+        size = team_max<TEAM>(size, slots, turn);
+        if (row >= a.rows) continue;
+        const float scale = scale_of(size), back = finite(size) ? 1.f / scale : 0.f;
+        signed char *to = a.codes + row * a.pitch;
 #pragma unroll
-    for (int i = 0; i < E / V; ++i) {
-        const int c = (t + TEAM * i) * V;
-        if (c >= a.pitch) continue;
-        float v[V];
-        int code[V];
+        for (int i = 0; i < E / V; ++i) {
+            const int c = (t + TEAM * i) * V;
+            if (c >= a.pitch) continue;
+            float v[V];
+            int code[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = finite(size) ? x.at(i * V + e) : 0.f;
-        codes_of<V>(v, scale, back, code);
-        store_codes<V>(to + c, code);
+            for (int e = 0; e < V; ++e) v[e] = finite(size) ? x.at(i * V + e) : 0.f;
+            codes_of<V>(v, scale, back, code);
+            store_codes<V>(to + c, code);
+        }
+        if (t == 0) a.scales[row] = scale;
     }
-    if (t == 0) a.scales[row] = scale;
 }
 
 template <class T>
@@ -187,7 +189,7 @@ void launch_rows(const QuantizeArgs &a, hipStream_t stream) {
     }
     with_team<T, false>(whole, a.cols, [&](auto v, auto team, auto e, auto odd) {
         constexpr int V = decltype(v)::value, TEAM = decltype(team)::value, E = decltype(e)::value, THREADS = rows_threads(TEAM);
-        const long groups = ((long)a.rows * TEAM + THREADS - 1) / THREADS;
+        const long want = ((long)a.rows * TEAM + THREADS - 1) / THREADS, most = (1L << 31) / THREADS, groups = want < most ? want : most;
         hipLaunchKernelGGL((quantize_rows_kernel<T, V, TEAM, E, decltype(odd)::value>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a);
     });
 }

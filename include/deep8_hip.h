@@ -543,8 +543,8 @@ int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner
  *                        reach the largest element since the page's first token was written.  Codes are exact quotients rounded to the nearest, halves
  *                        to the even one; where new tokens raise the scale, codes that are there are rounded again in the same way.  NaN or an infinity makes
  *                        its page and head's scale NaN, and so everything that is read from it, until its first token is written anew.  A token whose
- *                        place is before the first or has no page is left out.  Two sequences must not bring tokens to one page in one call;
- *                        full pages may be in any number of tables.
+ *                        place is before the first or has no page is left out.  Two sequences must not bring tokens to one page in one
+ *                        call, nor one sequence to a page that stands twice in its table; full pages may be in any number of tables.
  * d8_cache_read          the values of those places into rows of k and v, zeros for a token whose place is before the first or has no page.
  * d8_attention_cache     o = softmax(scale q k^T) v over the values that such a cache holds, head i with the keys and values of head i / (heads / kv_heads);
  *                        scales may be any numbers.  causal != 0: query t of a sequence's n sees the keys of its places up to t + length - n, so the

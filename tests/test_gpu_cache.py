@@ -365,10 +365,12 @@ def test_refusals():
         refused(fn, rows, [(1, None), (2, 63), (3, None), (4, 63), (5, None), (5, 72), (6, None), (7, None), (7, 8), (8, None), (9, None), (10, None), (11, None), (12, -1), (13, -1), (14, -1),
                            (15, -1), (16, 0), (17, 0), (17, 257), (12, 1 << 24), (14, 1 << 24), (13, 1 << 30)])
         refused(fn, rows, [(0, capi.FLOAT64), (0, 3)], 10002)
+        assert fn(*rows[:12], 1 << 23, 1 << 23, *rows[14:]) == 10001  # 2^24 pages and heads, of 256 threads each
     att = (capi.FLOAT16, p, 128, p, p, p, p, p, 128, p, p, p, p, 2, 3, 4, 5, 4, 2, 32, 0.5, 1, p, big, None)
     refused(lib.d8_attention_cache, att, [(1, None), (2, 127), (3, None), (3, 72), (4, None), (5, None), (6, None), (7, None), (8, 127), (10, None), (11, None), (12, None), (13, -1), (14, -1), (15, -1),
                                           (16, -1), (17, 3), (17, 1), (18, 0), (19, 0), (19, 257), (20, float("nan")), (22, None), (22, 72), (23, 0)])
     refused(lib.d8_attention_cache, att, [(0, capi.FLOAT64)], 10002)
+    assert lib.d8_attention_cache(*att[:13], 1 << 23, 1 << 23, *att[15:]) == 10001
     size = lib.d8_attention_cache_scratch_bytes
     assert size(capi.FLOAT16, 2, 3, 4, 4, 2, 32) > 0
     assert [size(*a) for a in ((capi.FLOAT64, 2, 3, 4, 4, 2, 32), (capi.FLOAT16, 2, 3, 4, 3, 2, 32), (capi.FLOAT16, 2, 3, -1, 4, 2, 32), (capi.FLOAT16, 2, 3, 4, 4, 2, 300))] == [0] * 4
