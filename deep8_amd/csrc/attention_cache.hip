@@ -13,7 +13,7 @@
 //
 // KEYS, for few rows: a workgroup has 16 rows, its four waves share out the pages, each by itself and a page ahead, and join through LDS.
 // ROWS, from 64 rows a sequence on and for heads of 128 elements at most: eight waves have 16 rows each and go through the pages together; a page's codes
-// are converted once and go through LDS as operands, in two buffers.  (4 x 128 queries of 32 heads over 32768 keys of 8: 320 us with every wave converting
+// are converted once and go through LDS as operands, in two buffers.  (512 queries of 4 sequences and 32 heads over 32768 keys of 8: 320 us with every wave converting
 // for itself, 131 so.)
 //
 // All tiles' pages, one after the other, are cut into as many equal runs as workgroups run at once, whatever sequences have how many: a workgroup
@@ -21,7 +21,7 @@
 // lengths on the device, so a call can be captured and replayed as sequences grow.
 //
 // KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 65 us, 4.1 TB/s, where
-// a large copy moves 5.2; single precision 66 us.  ROWS by no unit alone: 1 x 2048 queries of 32 heads over
+// a large copy moves 5.2; single precision too.  ROWS by no unit alone: 1 x 2048 queries of 32 heads over
 // 8192 keys take 355 us, 680 TFLOP/s, where a large product of the library makes 1200; the vector units are busy for 38 % of the time with
 // what lies between the products, the matrix units for 30 %, LDS for 39 %, and a workgroup's waves are mostly at the same of them.  (Two sets of rows a wave,
 // which halve what LDS reads and leave two waves a SIMD: 155 us in place of 133.)  Short calls are bound by latency: a wave's
@@ -258,7 +258,7 @@ __device__ __forceinline__ float row_sum(float x) {
 // ---- one wave, 16 rows ----------------------------------------------------------------------------------------------
 // NC: chunks of 64 elements of a head.
 // The lane, and a number that all lanes have, to the compiler others at every tile: what depends on them (addresses, comparisons with a head's elements,
-// reciprocals of divisors) would be kept for the whole launch in registers that the products need: 16 queries over 131072 keys in single, 75 us with and 66 so.
+// reciprocals of divisors) would be kept for the whole launch in registers that the products need: 16 queries over 131072 keys in single, 75 us with and 66 without.
 __device__ __forceinline__ int fresh_lane() {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
@@ -408,7 +408,8 @@ struct Wave {
         return uniform((n + PAGE - 1) / PAGE);
     }
 
-    // KEYS: `count` pages, 64 at most, first, first + step, ... of sequence s, by this wave alone.  fresh: load the queries too
+    // KEYS: `count` pages, 64 at most, first, first + step, ... of sequence s, by this wave alone.  fresh: the first of a tile's, whose queries
+    // are loaded once the first page's loads have set out (16 queries over 131072 keys: 1 us less; ROWS, short of registers, loads them before)
     __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int count, int step, bool fresh) {
         const Pages &c = a.c;
         const int lane = fresh_lane(), least = uniform(limit);
@@ -564,9 +565,6 @@ __device__ __forceinline__ void put(const AttArgs &a, T *to, int d, const f32x4 
 template <class T, int NC, bool ROWS>
 __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 : ROWS && sizeof(T) == 2 ? 4 : 2) void attention_cache_kernel(AttArgs a) {
     constexpr int WAVES = ROWS ? ROWS_WAVES : KEYS_WAVES, R = ROWS ? MANY_ROWS : KEYS_ROWS;  // rows of a tile
-    // Queries are loaded once a tile's first page has set out, where registers leave room for both: 16 queries over 131072 keys took 1 us less so (in single,
-    // or with more elements, 3 us more).
-    constexpr bool LATE = !ROWS && sizeof(T) == 2 && NC <= 2;
     __shared__ f16x8 stages[ROWS ? 2 : 1][ROWS ? 16 * NC : 1][64];
     __shared__ f32x4 others[ROWS ? 1 : WAVES][ROWS ? 1 : NC * 4][64];
     __shared__ float2 stats[ROWS ? 1 : WAVES][16];
@@ -599,7 +597,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
                 a.joins[tile_base + tile] = Join{parts == 1 ? 0 : parts, run, seq.q0, (int)(tile * R), (int)(rows - tile * R), {0, 0, 0}};
             }
             w.begin(a, seq, head, row0, rows);
-            if (!LATE) w.load_queries(a);
+            if (ROWS) w.load_queries(a);
             if constexpr (ROWS) {
                 // what the tile's last row sees: all waves go through as many pages
                 const int t = ((int)min((tile + 1) * R, rows) - 1) / fresh(a.group);
@@ -608,7 +606,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
                 for (int i = first; i < upto; i += 64) w.pages_together(a, s, head, i, min(64, upto - i), wave, stages);
             } else {
                 const int upto = min(end, w.most());
-                for (int i = first + wave; i < upto; i += 64 * WAVES) w.pages(a, s, head, i, min(64, (upto - i + WAVES - 1) / WAVES), WAVES, LATE && i == first + wave);
+                for (int i = first + wave; i < upto; i += 64 * WAVES) w.pages(a, s, head, i, min(64, (upto - i + WAVES - 1) / WAVES), WAVES, i == first + wave);
             }
             const int lane = fresh_lane(), r = lane & 15, g = lane >> 4;
             at += end - first;
