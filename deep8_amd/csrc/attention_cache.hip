@@ -20,8 +20,8 @@
 // goes through its run and leaves, for a tile that it has not all of, sums in scratch, which a second launch joins.  Cuts are found from the
 // lengths on the device, so a call can be captured and replayed as sequences grow.
 //
-// KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 65 us, 4.1 TB/s, where
-// a large copy moves 5.2; single precision too.  ROWS by no unit alone: 1 x 2048 queries of 32 heads over
+// KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 63 us, 4.2 TB/s, where
+// a large copy moves 5.2; single precision 66 us.  ROWS by no unit alone: 1 x 2048 queries of 32 heads over
 // 8192 keys take 355 us, 680 TFLOP/s, where a large product of the library makes 1200; the vector units are busy for 38 % of the time with
 // what lies between the products, the matrix units for 30 %, LDS for 39 %, and a workgroup's waves are mostly at the same of them.  (Two sets of rows a wave,
 // which halve what LDS reads and leave two waves a SIMD: 155 us in place of 133.)  Short calls are bound by latency: a wave's
@@ -98,11 +98,11 @@ __device__ __forceinline__ void sum_upto(long &x, long &y, int most) {
         x += add ? u : 0, y += add ? v : 0;
     }
 }
-__device__ __forceinline__ long from_lane(long x, int lane) { return __shfl(x, lane); }
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long uniform(long x) {
-    return (long)(((unsigned long)(unsigned)uniform((int)(x >> 32)) << 32) | (unsigned)uniform((int)x));
+__device__ __forceinline__ int from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }  // (`lane` as all lanes have it)
+__device__ __forceinline__ long from_lane(long x, int lane) {
+    return (long)((unsigned long)(unsigned)from_lane((int)(x >> 32), lane) << 32 | (unsigned)from_lane((int)x, lane));
 }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // What a workgroup knows of all sequences: the lane's of the first 64 with the tiles and costs up to it, and the sums over all.
 template <int R>
@@ -124,7 +124,6 @@ struct Scan {
             sum_upto(t, c, 64);
             tiles += from_lane(t, 63), cost += from_lane(c, 63);
         }
-        tiles = uniform(tiles), cost = uniform(cost);
     }
     // the sequence of page `at` of the list: the list's pages and tiles before it
     __device__ __forceinline__ bool locate(const AttArgs &a, long at, Seq &seq, int &s, long &cost_base, long &tile_base) const {
@@ -141,9 +140,9 @@ struct Scan {
             if (past) {
                 const int l = __ffsll((long long)past) - 1;
                 s = uniform(first + l);
-                cost_base = uniform(cost_before + from_lane(c - x.cost(), l)), tile_base = uniform(tiles_before + from_lane(t - x.tiles, l));
-                seq.q0 = uniform(__shfl(x.q0, l)), seq.n = uniform(__shfl(x.n, l)), seq.len = uniform(from_lane(x.len, l)), seq.keys = uniform(__shfl(x.keys, l));
-                seq.tiles = uniform(from_lane(x.tiles, l)), seq.pages = uniform(from_lane(x.pages, l));
+                cost_base = cost_before + from_lane(c - x.cost(), l), tile_base = tiles_before + from_lane(t - x.tiles, l);
+                seq.q0 = from_lane(x.q0, l), seq.n = from_lane(x.n, l), seq.len = from_lane(x.len, l), seq.keys = from_lane(x.keys, l);
+                seq.tiles = from_lane(x.tiles, l), seq.pages = from_lane(x.pages, l);
                 return true;
             }
             const int last = min(a.c.sequences - first, 64) - 1;
@@ -174,7 +173,7 @@ struct Join {
 };
 
 // How long the runs of a call are: equal, but not so short that a tile's many pieces cost more to join than is gained: KEYS stays at a tile, or a page a
-// wave, ROWS at a quarter of a tile, or four pages.  (One token over 8000 keys of 8 heads: 17 us so, 22 with runs of a page; 256 queries of 8 heads over
+// wave, ROWS at a quarter of a tile, or four pages.  (One token over 8000 keys of 8 heads: 15 us so, 20 with runs of a page; 256 queries of 8 heads over
 // 4096 keys in single, 38 and 50.  Runs longer than a tile go through short sequences one after the other: 16 of 100 keys took 24 us with four pages, 17 so.)
 template <int R>
 __device__ __forceinline__ long run_of(long total, long tiles, int runs) {
@@ -279,16 +278,17 @@ struct Wave {
     float m, sum;  // of scores times log2 e; the lane's part of the sum
     int limit;     // keys that the lane's row sees
 
-    const T *from;  // the lane's row of queries, null for none
+    const T *from;  // the lane's row of queries, or another's where it has none
+    bool there;
 
     // rows row0 .. of the sequence (those beyond `rows` are zero and see nothing)
     __device__ __forceinline__ void begin(const AttArgs &a, const Seq &s, int head, long row0, long rows) {
         const long row = row0 + (fresh_lane() & 15);
-        const bool there = row < rows;
+        there = row < rows;
         const int group = fresh(a.group), t = there ? (int)row / group : 0, h = there ? (int)row - t * group : 0;
         const long sees = a.causal ? t + s.len - s.n + 1 : s.len;
         limit = there ? (int)min(max(sees, 0L), (long)s.keys) : 0;
-        from = there ? (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * group + h) * a.c.dim : nullptr;
+        from = (const T *)a.q + (s.q0 + (long)t) * a.ldq + ((long)head * group + h) * a.c.dim;
         m = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NC * 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -296,24 +296,24 @@ struct Wave {
 
     __device__ __forceinline__ void load_queries(const AttArgs &a) {
         const int g = fresh_lane() >> 4;
-        const bool there = from != nullptr;
         const int dim = fresh(a.c.dim);
         float x[NC][16], largest = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = c * 64 + g * 16;
-            constexpr int V = 16 / sizeof(T);
-            typedef T piece __attribute__((ext_vector_type(V)));
+            if (a.vec) {  // (dim is whole pieces; where there are none, the first is loaded for nothing)
+                constexpr int V = 16 / sizeof(T);
+                typedef T piece __attribute__((ext_vector_type(V)));
 #pragma unroll
-            for (int i = 0; i < 16; i += V) {
-                if (a.vec && there && d + i < dim) {  // (dim is whole pieces)
-                    const piece p = *(const piece *)(from + d + i);
+                for (int i = 0; i < 16; i += V) {
+                    const bool some = there && d + i < dim;
+                    const piece p = *(const piece *)(from + (some ? d + i : 0));
 #pragma unroll
-                    for (int e = 0; e < V; ++e) x[c][i + e] = (float)p[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[c][i + e] = !a.vec && there && d + i + e < dim ? (float)from[d + i + e] : 0.f;
+                    for (int e = 0; e < V; ++e) x[c][i + e] = some ? (float)p[e] : 0.f;
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[c][i] = there && d + i < dim ? (float)from[d + i] : 0.f;
             }
             if (P::QUERY > 1)
 #pragma unroll
@@ -408,8 +408,7 @@ struct Wave {
         return uniform((n + PAGE - 1) / PAGE);
     }
 
-    // KEYS: `count` pages, 64 at most, first, first + step, ... of sequence s, by this wave alone.  fresh: the first of a tile's, whose queries
-    // are loaded once the first page's loads have set out (16 queries over 131072 keys: 1 us less; ROWS, short of registers, loads them before)
+    // KEYS: `count` pages, 64 at most, first, first + step, ... of sequence s, by this wave alone.  fresh: load the queries too
     __device__ __forceinline__ void pages(const AttArgs &a, int s, int head, int first, int count, int step, bool fresh) {
         const Pages &c = a.c;
         const int lane = fresh_lane(), least = uniform(limit);
@@ -565,6 +564,9 @@ __device__ __forceinline__ void put(const AttArgs &a, T *to, int d, const f32x4 
 template <class T, int NC, bool ROWS>
 __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 : ROWS && sizeof(T) == 2 ? 4 : 2) void attention_cache_kernel(AttArgs a) {
     constexpr int WAVES = ROWS ? ROWS_WAVES : KEYS_WAVES, R = ROWS ? MANY_ROWS : KEYS_ROWS;  // rows of a tile
+    // Queries are loaded once the loads of a tile's first page have set out, where registers leave room for both: 16 queries over 131072 keys take 1 us less so
+    // in half, and 4 us more in single.
+    constexpr bool LATE = !ROWS && sizeof(T) == 2;
     __shared__ f16x8 stages[ROWS ? 2 : 1][ROWS ? 16 * NC : 1][64];
     __shared__ f32x4 others[ROWS ? 1 : WAVES][ROWS ? 1 : NC * 4][64];
     __shared__ float2 stats[ROWS ? 1 : WAVES][16];
@@ -586,18 +588,17 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
     for (;;) {
         const long after = base + seq.cost(), stop = min(fresh(last), after);
         while (at < stop) {
-            const long tile = (at - base) / fresh(seq.pages);
+            const long ahead = at - base, tile = ahead < seq.pages ? 0 : ahead / fresh(seq.pages);
             const int first = (int)(at - base - tile * seq.pages), end = (int)min(seq.pages, first + (stop - at));
             const bool whole = first == 0 && end == seq.pages;
             const long rows = (long)seq.n * a.group, row0 = tile * R + (ROWS ? wave * 16 : 0), slot = run + tile_base + tile;
             if (first == 0 && head == 0 && threadIdx.x == 0) {  // (the tile's first page: every head's parts are alike)
-                const long from = base + tile * seq.pages, to = from + seq.pages - 1;
-                const long run_length = fresh(length);
-                const int parts = (int)(to / run_length - from / run_length) + 1;
+                const long to = at + seq.pages - 1, run_length = fresh(length);
+                const int parts = to < (run + 1) * run_length ? 1 : (int)(to / run_length) - run + 1;
                 a.joins[tile_base + tile] = Join{parts == 1 ? 0 : parts, run, seq.q0, (int)(tile * R), (int)(rows - tile * R), {0, 0, 0}};
             }
             w.begin(a, seq, head, row0, rows);
-            if (ROWS) w.load_queries(a);
+            if (!LATE) w.load_queries(a);
             if constexpr (ROWS) {
                 // what the tile's last row sees: all waves go through as many pages
                 const int t = ((int)min((tile + 1) * R, rows) - 1) / fresh(a.group);
@@ -606,7 +607,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
                 for (int i = first; i < upto; i += 64) w.pages_together(a, s, head, i, min(64, upto - i), wave, stages);
             } else {
                 const int upto = min(end, w.most());
-                for (int i = first + wave; i < upto; i += 64 * WAVES) w.pages(a, s, head, i, min(64, (upto - i + WAVES - 1) / WAVES), WAVES, i == first + wave);
+                for (int i = first + wave; i < upto; i += 64 * WAVES) w.pages(a, s, head, i, min(64, (upto - i + WAVES - 1) / WAVES), WAVES, LATE && i == first + wave);
             }
             const int lane = fresh_lane(), r = lane & 15, g = lane >> 4;
             at += end - first;
