@@ -7,7 +7,8 @@
 // one fma has exactly (scale is normal and x a number of 24 bits), says on which side the quotient is.  A row of 16384 halves meets that
 // three times.  A row that holds NaN or an infinity gets the scale NaN and codes 0, so its results are NaN.
 //
-// Rows: bound by memory, x read once (a team of threads holds a row: row_team.h) and a byte written for each element.  Columns are laid out once
+// Rows: bound by memory, x read once (a team of threads holds a row: row_team.h) and a byte written for each element: 8192 x 4096
+// halves in 22 us, 4.6 TB/s, where a large copy moves 5.2.  Columns are laid out once
 // when a model is loaded: a workgroup goes down 64 columns twice (the second time mostly out of cache) and transposes through LDS.
 #include "int8.h"
 #include "row_team.h"
