@@ -235,13 +235,15 @@ int launch(Args a, const Plan &p, hipStream_t stream) {
     a.parts = p.parts, a.part_ld = p.part_ld;
     a.vec = a.ldz % 4 == 0 && ((size_t)a.z & (4 * sizeof(T) - 1)) == 0;
     if (p.few) {
-        const dim3 grid((unsigned)(ceil_div(a.cols, ROWS_COLS) * (long)p.parts)), threads(ROWS_WAVES * 64);
+        const long groups = ceil_div(a.cols, ROWS_COLS) * (long)p.parts;
+        D8_REQUIRE(groups < (1L << 23), "matmul_int8: a result of %d x %d is too large", a.rows, a.cols);
+        const dim3 grid((unsigned)groups), threads(ROWS_WAVES * 64);
         if (a.rows <= 16) hipLaunchKernelGGL((int8_rows_kernel<T, 1>), grid, threads, 0, stream, a);
         else if (a.rows <= 32) hipLaunchKernelGGL((int8_rows_kernel<T, 2>), grid, threads, 0, stream, a);
         else hipLaunchKernelGGL((int8_rows_kernel<T, 4>), grid, threads, 0, stream, a);
     } else {
         const long groups = (long)ceil_div(a.rows, TILE) * ceil_div(a.cols, TILE) * p.parts;
-        D8_REQUIRE(groups < (1L << 31), "matmul_int8: a result of %d x %d is too large", a.rows, a.cols);
+        D8_REQUIRE(groups < (1L << 24), "matmul_int8: a result of %d x %d is too large", a.rows, a.cols);
         if (a.vec || a.parts > 1) hipLaunchKernelGGL((int8_tile_kernel<T, true>), dim3((unsigned)groups), dim3(256), 0, stream, a);
         else hipLaunchKernelGGL((int8_tile_kernel<T, false>), dim3((unsigned)groups), dim3(256), 0, stream, a);
     }

@@ -219,4 +219,6 @@ def test_refusals():
     refused(lib.d8_matmul_int8, product, [(1, None), (1, 72), (2, None), (3, -1), (4, 0), (4, 131072), (5, None), (5, 65), (6, None), (7, -1), (8, None), (9, 7), (10, None), (10, 72),
                                           (11, 0)])
     refused(lib.d8_matmul_int8, product, [(0, capi.FLOAT64)], 10002)
+    for rows, cols in ((1, 1 << 28), (100, 1 << 30)):  # more than the threads of a launch
+        assert lib.d8_matmul_int8(capi.FLOAT16, p, p, rows, 128, p, p, cols, p, cols, p, 1 << 40, None) == 10001
     assert lib.d8_matmul_int8_scratch_bytes(4, 131072, 8) == 0 and lib.d8_matmul_int8_scratch_bytes(-1, 8, 8) == 0
