@@ -136,3 +136,37 @@ def test_a_layer_captured_and_replayed(dtype):
             assert np.array_equal(getattr(live.cache, name).numpy(), getattr(eager.cache, name).numpy(), equal_nan=True)
     capi.check(live.lib.d8_graph_destroy(graph))
     capi.check(live.lib.d8_stream_destroy(stream))
+
+
+def test_two_layers_at_once():
+    """two caches served on two streams, calls of both on their way together: the bits of each alone"""
+    from deep8_amd import capi
+    layers, alone, r = [_Layer(np.float16, [260, 140]) for _ in range(2)], _Layer(np.float16, [260, 140]), rng(24)
+    streams = [ctypes.c_void_p() for _ in layers]
+    for s in streams:
+        capi.check(layers[0].lib.d8_stream_create(ctypes.byref(s)))
+    calls, held = [], np.zeros(2, np.int64)
+    for new in ([250, 130], [1, 1], [1, 2], [1, 1]):
+        held = held + new
+        x = r.standard_normal((2, sum(new), WIDTH)).astype(np.float16)
+        rooms = [layer.room(sum(new), 2) for layer in layers]
+        for layer, b, rows in zip(layers, rooms, x):
+            layer.feed(b, rows, new, held)
+        calls.append((new, held, x, rooms))
+    capi.sync()
+    for new, held, x, rooms in calls:
+        for layer, b, s in zip(layers, rooms, streams):
+            layer.step(b, layer.cache, s)
+    for s in streams:
+        capi.sync(s)
+    for i in range(2):
+        if i:
+            alone = _Layer(np.float16, [260, 140])
+        for new, held, x, rooms in calls:
+            b = alone.room(sum(new), 2)
+            alone.feed(b, x[i], new, held)
+            alone.step(b, alone.cache)
+            capi.sync()
+            assert all(np.array_equal(b[name].numpy(), rooms[i][name].numpy()) for name in ("n", "nc", "q", "k", "v", "o", "lse", "oc", "y"))
+    for s in streams:
+        capi.check(layers[0].lib.d8_stream_destroy(s))
