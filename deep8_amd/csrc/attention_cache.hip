@@ -14,7 +14,7 @@
 // KEYS, for few rows: a workgroup has 16 rows, its four waves share out the pages, each by itself and a page ahead, and join through LDS.
 // ROWS, from 64 rows a sequence on and for heads of 128 elements at most: eight waves have 16 rows each and go through the pages together; a page's codes
 // are converted once and go through LDS as operands, in two buffers.  (512 queries of 4 sequences and 32 heads over 32768 keys of 8: 320 us with every wave converting
-// for itself, 131 so.)
+// for itself, 126 so.)
 //
 // All tiles' pages, one after the other, are cut into as many equal runs as workgroups run at once, whatever sequences have how many: a workgroup
 // goes through its run and leaves, for a tile that it has not all of, sums in scratch, which a second launch joins.  Cuts are found from the
@@ -22,9 +22,10 @@
 //
 // KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 63 us, 4.2 TB/s, where
 // a large copy moves 5.2; single precision 66 us.  ROWS by no unit alone: 1 x 2048 queries of 32 heads over
-// 8192 keys take 355 us, 680 TFLOP/s, where a large product of the library makes 1200; the vector units are busy for 38 % of the time with
-// what lies between the products, the matrix units for 30 %, LDS for 39 %, and a workgroup's waves are mostly at the same of them.  (Two sets of rows a wave,
-// which halve what LDS reads and leave two waves a SIMD: 155 us in place of 133.)  Short calls are bound by latency: a wave's
+// 8192 keys take 355 us, 680 TFLOP/s, where a large product of the library makes 1200; counters have the vector units, matrix
+// instructions' issue among it, busy for 68 % of the time, the matrix units for 30 %, LDS for 39 %.  What takes vector instructions away helps, as long as no
+// register more is needed.  (Two sets of rows a wave, which halve what LDS reads and leave two waves a SIMD: 155 us in place of 133; half the waves a phase behind
+// the others, no gain; accumulators in units of the pages' scales: 139 for 126.)  Short calls are bound by latency: a wave's
 // way from the first length to its last store is 10 us, and the join 4.
 //
 // Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product.
@@ -243,10 +244,16 @@ __device__ __forceinline__ f32x4 mma(const f16x8 &a, const f16x8 &b, const f32x4
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u32x2 half_rows(float x) { return __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false)); }
 __device__ __forceinline__ u32x2 halves(float x) { return __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false)); }
+// (asm: fmaxf quiets each operand first that the compiler cannot tell to be a quiet NaN or none)
+__device__ __forceinline__ float larger(float a, float b) {
+    float c;
+    asm("v_max_f32 %0, %1, %2" : "=v"(c) : "v"(a), "v"(b));
+    return c;
+}
 __device__ __forceinline__ float row_max(float x) {
     u32x2 y = half_rows(x);
-    y = halves(fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])));
-    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    y = halves(larger(__uint_as_float(y[0]), __uint_as_float(y[1])));
+    return larger(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 __device__ __forceinline__ float row_sum(float x) {
     u32x2 y = half_rows(x);
@@ -348,7 +355,9 @@ struct Wave {
     // Scores of a page whose first place is `at` to weights; accumulators and sums to the new maximum.  hidden: some row does not see all of
     // the page (or there is none).  `into`: what the page's sums are scaled by, 0 where the lane's row sees none of it.
     __device__ __forceinline__ void weigh(const f32x4 (&sc)[4], int g, int at, bool there, bool hidden, float k_scale, float v_scale, f16x8 (&p)[P::WEIGHT][2], float &into) {
-#pragma clang fp contract(off)  // (a fused product less its rounded maximum can be anything but small where scores are large)
+#pragma clang fp contract(off)  // (a fused product less its rounded maximum is off by half a step of that, which sum and result
+        // share: 2^-15 at most below LARGE, but anything where scores are larger)
+        constexpr float LARGE = 1024.f;
         float x[16], by = P::QUERY > 1 ? k_scale * q_scale : k_scale;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = sc[i >> 2][i & 3];
@@ -372,9 +381,14 @@ struct Wave {
             m = top;
         }
         float add = 0.f;
+        if (__ballot(fabsf(base) >= LARGE)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] *= by;
+            by = 1.f;
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_amdgcn_exp2f(x[i] * by - (base - P::LIFT));
+            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by, P::LIFT - base));
             add += x[i];
         }
         split<P::WEIGHT>(x, p);
