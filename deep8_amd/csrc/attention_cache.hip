@@ -675,40 +675,54 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
     }
 }
 
-// The runs' sums of a tile's rows joined: half a wave a row, four elements a lane.
+// The runs' sums of a tile's rows joined: half a wave a row, four elements a lane.  The first parts' sums are loaded before their maxima are known.
 template <class T, int R>
 __global__ __launch_bounds__(256) void attention_cache_join_kernel(AttArgs a) {
-    const int half = threadIdx.x & 31, of = threadIdx.x >> 5, head = blockIdx.x % a.c.kv_heads, unit = blockIdx.x / a.c.kv_heads;
+    const int half = threadIdx.x & 31, head = blockIdx.x % a.c.kv_heads, unit = blockIdx.x / a.c.kv_heads, row = blockIdx.y * 8 + (threadIdx.x >> 5);
     const Join join = a.joins[unit];
-    if (!join.parts) return;
-    const int n = min(R, join.rows);
-    const long step = (long)a.c.kv_heads * R;
-    for (int row = blockIdx.y * 8 + of; row < n; row += gridDim.y * 8) {
-        const long place = (((long)join.run + unit) * a.c.kv_heads + head) * R + row;
-        const float2 *ml = (const float2 *)a.part_ml + place;
-        float top = -INFINITY, sum = 0.f;
-        for (int i = half; i < join.parts; i += 32) top = fmaxf(top, ml[i * step].x);
+    const int parts = join.parts;
+    if (!parts || row >= min(R, join.rows)) return;
+    const long step = (long)a.c.kv_heads * R, place = (((long)join.run + unit) * a.c.kv_heads + head) * R + row;
+    const float2 *ml = (const float2 *)a.part_ml + place;
+    const float *from = a.part + place * a.part_ld;
+    constexpr int BATCH = 8;
+    f32x4 batch[BATCH];
+    auto load = [&](int i, int d) {  // parts i .. (those beyond the last: it again, for weights of 0)
+        const float *of = from + (d + half * 4 < a.part_ld ? d + half * 4 : 0);
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        const float at = top == -INFINITY ? 0.f : top;
-        for (int i = half; i < join.parts; i += 32) sum += ml[i * step].y * __builtin_amdgcn_exp2f(ml[i * step].x - at);
+        for (int k = 0; k < BATCH; ++k) batch[k] = *(const f32x4 *)(of + min(i + k, parts - 1) * step * a.part_ld);
+    };
+    load(0, 0);
+    const float2 mine = half < parts ? ml[half * step] : make_float2(-INFINITY, 0.f);
+    float top = mine.x;
+    for (int i = half + 32; i < parts; i += 32) top = fmaxf(top, ml[i * step].x);
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor(sum, d);
-        const int t = (join.row0 + row) / a.group, h = head * a.group + join.row0 + row - t * a.group;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        T *to = (T *)a.o + ((long)join.q0 + t) * a.ldo + (long)h * a.c.dim;
-        for (int d = half * 4; d < a.c.dim; d += 128) {
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            const float *from = a.part + place * a.part_ld + d;
-#pragma unroll 4
-            for (int i = 0; i < join.parts; ++i) x += *(const f32x4 *)(from + i * step * a.part_ld) * __builtin_amdgcn_exp2f(ml[i * step].x - at);
-            put<T>(a, to, d, x, inv);
+    for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float at = top == -INFINITY ? 0.f : top, weight = __builtin_amdgcn_exp2f(mine.x - at);
+    float sum = mine.y * weight;
+    for (int i = half + 32; i < parts; i += 32) sum += ml[i * step].y * __builtin_amdgcn_exp2f(ml[i * step].x - at);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor(sum, d);
+    const int t = (join.row0 + row) / a.group, h = head * a.group + join.row0 + row - t * a.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T *to = (T *)a.o + ((long)join.q0 + t) * a.ldo + (long)h * a.c.dim;
+    for (int d = 0; d < a.c.dim; d += 128) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        float w = weight;
+        for (int i = 0; i < parts; i += BATCH) {
+            if (i && !(i & 31)) w = i + half < parts ? __builtin_amdgcn_exp2f(ml[(i + half) * step].x - at) : 0.f;
+            if (i || d) load(i, d);
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                const float by = __shfl(w, (i & 31) + k, 32);
+                if (i + k < parts) x += batch[k] * by;
+            }
         }
-        if (half == 0 && a.lse) a.lse[(long)h * a.c.tokens + join.q0 + t] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+        if (d + half * 4 < a.c.dim) put<T>(a, to, d + half * 4, x, inv);
     }
+    if (half == 0 && a.lse) a.lse[(long)h * a.c.tokens + join.q0 + t] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-// ---- host -----------------------------------------------------------------------------------------------------------
 // How a call runs: rows of a tile, runs of a kv head, tiles of all sequences at most, and slots of partial sums (a run's and a tile's numbers added: each
 // step from piece to piece of the list is to the next run or the next tile, so no two pieces share a slot).
 struct Plan {
@@ -753,7 +767,7 @@ int launch_all(const AttArgs &a, const Plan &p, hipStream_t stream) {
     else if (a.c.dim <= 128) launch<T, 2>(a, p, stream);
     else launch<T, 4>(a, p, stream);
     D8_LAUNCH_CHECK();
-    const dim3 join((unsigned)(p.units * a.c.kv_heads), p.rows ? 4 : 2);
+    const dim3 join((unsigned)(p.units * a.c.kv_heads), p.tile / 8);
     if (p.rows) hipLaunchKernelGGL((attention_cache_join_kernel<T, MANY_ROWS>), join, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((attention_cache_join_kernel<T, KEYS_ROWS>), join, dim3(256), 0, stream, a);
     D8_LAUNCH_CHECK();
