@@ -12,7 +12,7 @@
 // converted there: half in pairs, by putting the byte (its sign bit flipped) below the bits of 1024 and taking off 1024 + 128.
 //
 // KEYS, for few rows: a workgroup has 16 rows, its four waves share out the pages, each by itself and a page ahead, and join through LDS.
-// ROWS, from 64 rows a sequence on and for heads of 128 elements at most: eight waves have 16 rows each and go through the pages together; a page's codes
+// ROWS, for more, and heads of 128 elements at most: eight waves have 16 rows each and go through the pages together; a page's codes
 // are converted once and go through LDS as operands, in two buffers.  (512 queries of 4 sequences and 32 heads over 32768 keys of 8: 320 us with every wave converting
 // for itself, 126 so.)
 //
@@ -734,7 +734,10 @@ struct Plan {
 Plan plan_of(int dtype, int sequences, int tokens, int table_pages, int heads, int kv_heads, int dim) {
     Plan p;
     const long group = heads / kv_heads, all = (long)tokens * group, some = sequences < tokens ? sequences : tokens;
-    p.rows = dim <= 128 && some && all / some >= 64;
+    // Rows of a sequence in the mean from which on ROWS is faster (us with and without: half, 48 over 4000 keys of 8 heads 16 / 18, 64 over 8192 of 4 sequences and
+    // 8 heads 39 / 45, 32 over 16384 of 8 heads 25 / 22; single, whose ROWS leave two waves a SIMD, 64 as above 57 / 48, 80 over 16000 of 8 heads of 64 25 / 25).
+    const int from = dtype == D8_FLOAT16 ? 33 : 96;
+    p.rows = dim <= 128 && some && all / some >= from;
     p.tile = p.rows ? MANY_ROWS : KEYS_ROWS;
     p.units = all / p.tile + some;
     const int held = dim > 128 || (p.rows && dtype == D8_FLOAT32) ? 1 : 2;  // workgroups whose registers a compute unit holds

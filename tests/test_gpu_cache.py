@@ -383,7 +383,7 @@ def test_scratch_has_room_for_every_piece(sequences, tokens, table_pages, heads,
     lib, group, r = capi.load(), heads // kv_heads, rng(tokens)
     for dt in (capi.FLOAT16, capi.FLOAT32):
         nb = lib.d8_attention_cache_scratch_bytes(dt, sequences, tokens, table_pages, heads, kv_heads, dim)
-        many = dim <= 128 and tokens * group // min(sequences, tokens) >= 64
+        many = dim <= 128 and tokens * group // min(sequences, tokens) >= (33 if dt == capi.FLOAT16 else 96)
         rows = 128 if many else 16
         units = tokens * group // rows + min(sequences, tokens)
         per_slot = 4 * kv_heads * rows * ((dim + 3) // 4 * 4 + 2)
