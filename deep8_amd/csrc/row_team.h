@@ -107,6 +107,7 @@ void with_team(bool whole, int cols, F &&fn) {
     auto in = [&](auto odd) {
 #define D8_TEAM(TEAM_, E_) fn(std::integral_constant<int, V>(), std::integral_constant<int, TEAM_>(), std::integral_constant<int, E_>(), odd)
         if (cols <= 128) D8_TEAM(16, 8);
+        else if (cols <= 256) D8_TEAM(32, 8);
         else if (cols <= 512) D8_TEAM(64, 8);
         else if (cols <= 1024) D8_TEAM(64, 16);
         else if (cols <= 2048) D8_TEAM(256, 8);

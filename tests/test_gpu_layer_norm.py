@@ -17,10 +17,10 @@ HALF = {np.float16: 2.0 ** -11, np.float32: 2.0 ** -24}
 E = 2.0 ** -24
 TINY = {np.float16: 2.0 ** -25, np.float32: 0.0}  # half a step of the smallest numbers
 
-# rows, cols, pad: teams of 16, 64, 256, 512 and 1024 threads with 8 and 16 elements each, rows in 16-byte pieces and not, shorter than one, rows that no team holds
+# rows, cols, pad: teams of 16, 32, 64, 256, 512 and 1024 threads with 8 and 16 elements each, rows in 16-byte pieces and not, shorter than one, rows that no team holds
 CASES = [(1, 1, 0), (3, 7, 1), (5, 64, 0), (2, 512, 8), (9, 520, 0), (33, 1000, 0), (3, 1024, 3), (7, 1025, 0), (5, 2048, 0), (3, 2056, 8), (6, 4096, 0),
          (2, 4097, 0), (3, 8192, 0), (2, 8200, 8), (3, 16384, 0), (2, 16384, 1), (3, 16385, 0), (2, 20000, 8), (700, 96, 0), (4099, 100, 0), (1030, 1000, 24),
-         (700, 3, 0), (65, 8, 0), (33, 9, 1), (70, 128, 0), (33, 127, 1), (9, 129, 3), (4, 2047, 0), (300, 4095, 5), (2, 5120, 0), (3, 8191, 2), (2, 8193, 0), (2, 11111, 0)]
+         (700, 3, 0), (65, 8, 0), (33, 9, 1), (70, 128, 0), (33, 127, 1), (9, 129, 3), (301, 200, 0), (40, 256, 8), (33, 255, 1), (3, 257, 0), (4, 2047, 0), (300, 4095, 5), (2, 5120, 0), (3, 8191, 2), (2, 8193, 0), (2, 11111, 0)]
 
 
 def _inputs(rows, cols, dtype, seed, shift=0.0):
