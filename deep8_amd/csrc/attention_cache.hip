@@ -30,6 +30,7 @@
 //
 // Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product.
 #include "cache.h"
+#include "lanes.h"
 
 namespace d8 {
 namespace cache {
@@ -417,8 +418,7 @@ struct Wave {
     // pages that the wave's rows see at most (the later a row's query, the more)
     __device__ __forceinline__ int most() const {
         int n = limit;
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) n = max(n, __shfl_xor(n, d));
+        n = over_lanes<16>(n, [](int x, int y) { return max(x, y); });
         return uniform((n + PAGE - 1) / PAGE);
     }
 
@@ -696,13 +696,11 @@ __global__ __launch_bounds__(256) void attention_cache_join_kernel(AttArgs a) {
     const float2 mine = half < parts ? ml[half * step] : make_float2(-INFINITY, 0.f);
     float top = mine.x;
     for (int i = half + 32; i < parts; i += 32) top = fmaxf(top, ml[i * step].x);
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    top = over_lanes<32>(top, larger);
     const float at = top == -INFINITY ? 0.f : top, weight = __builtin_amdgcn_exp2f(mine.x - at);
     float sum = mine.y * weight;
     for (int i = half + 32; i < parts; i += 32) sum += ml[i * step].y * __builtin_amdgcn_exp2f(ml[i * step].x - at);
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor(sum, d);
+    sum = over_lanes<32>(sum, [](float x, float y) { return x + y; });
     const int t = (join.row0 + row) / a.group, h = head * a.group + join.row0 + row - t * a.group;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T *to = (T *)a.o + ((long)join.q0 + t) * a.ldo + (long)h * a.c.dim;

@@ -11,6 +11,7 @@
 // by memory where pages are filled (8192 tokens of 8 heads of 128 halves: 13 us written, 11 read back, 3.8 and 4.6 TB/s), by the chain of its loads
 // (sequence, page, scale, codes) where they get a token each: 5 us.
 #include "cache.h"
+#include "lanes.h"
 
 namespace d8 {
 namespace cache {
@@ -100,8 +101,8 @@ __device__ __forceinline__ void append(const Args &a, int r, int rows, int slot,
             for (int e = 0; e < V; ++e) k_size = max(k_size, size_of(at(kx[j], e))), v_size = max(v_size, size_of(at(vx[j], e)));
     }
     if (tid == 0) sizes[8] = slot ? __float_as_uint(*ks) : 0u, sizes[9] = slot ? __float_as_uint(*vs) : 0u;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) k_size = max(k_size, (unsigned)__shfl_xor((int)k_size, d)), v_size = max(v_size, (unsigned)__shfl_xor((int)v_size, d));
+    const auto larger = [](unsigned x, unsigned y) { return max(x, y); };
+    k_size = over_lanes<64>(k_size, larger), v_size = over_lanes<64>(v_size, larger);
     if ((tid & 63) == 0) sizes[tid >> 6] = k_size, sizes[4 + (tid >> 6)] = v_size;
     for (int i = tid; i < c.pitch * WORDS; i += 256) words[i] = 0;
     __syncthreads();

@@ -71,8 +71,7 @@ struct QuantizeArgs {
 
 template <int TEAM>
 __device__ __forceinline__ unsigned team_max(unsigned m, unsigned *slots, int &turn) {
-#pragma unroll
-    for (int d = 1; d < (TEAM < 64 ? TEAM : 64); d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+    m = over_lanes<TEAM>(m, [](unsigned x, unsigned y) { return max(x, y); });
     if constexpr (TEAM > 64) {
         unsigned *s = slots + turn * 16;
         turn ^= 1;

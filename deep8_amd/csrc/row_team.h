@@ -4,7 +4,7 @@
 
 #include <type_traits>
 
-#include "common.h"
+#include "lanes.h"
 
 namespace d8 {
 namespace row_team {
@@ -81,8 +81,8 @@ struct Held {
 // of the call between keeps a wave from writing what another still reads).
 template <int TEAM>
 __device__ __forceinline__ void team_sum(float &a, float &b, float2 *slots, int &turn) {
-#pragma unroll
-    for (int d = 1; d < (TEAM < 64 ? TEAM : 64); d <<= 1) a += __shfl_xor(a, d), b += __shfl_xor(b, d);
+    const auto add = [](float x, float y) { return x + y; };
+    a = over_lanes<TEAM>(a, add), b = over_lanes<TEAM>(b, add);
     if constexpr (TEAM > 64) {
         const int wave = threadIdx.x >> 6;
         float2 *s = slots + turn * 16;
