@@ -92,14 +92,6 @@ __device__ __forceinline__ Seq seqs_from(const AttArgs &a, int first, int &top) 
     return s;
 }
 
-// sums over the lanes up to this one, of which `most` are not 0
-__device__ __forceinline__ void sum_upto(long &x, long &y, int most) {
-    for (int d = 1; d < 64 && d < most; d <<= 1) {
-        const long u = __shfl_up(x, d), v = __shfl_up(y, d);
-        const bool add = (threadIdx.x & 63) >= d;
-        x += add ? u : 0, y += add ? v : 0;
-    }
-}
 __device__ __forceinline__ int from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }  // (`lane` as all lanes have it)
 __device__ __forceinline__ long from_lane(long x, int lane) {
     return (long)((unsigned long)(unsigned)from_lane((int)(x >> 32), lane) << 32 | (unsigned)from_lane((int)x, lane));
@@ -116,15 +108,13 @@ struct Scan {
         top = 0;
         own = seqs_from<R>(a, 0, top);
         tiles_upto = own.tiles, cost_upto = own.cost();
-        sum_upto(tiles_upto, cost_upto, a.c.sequences);
+        if (a.c.sequences > 1) tiles_upto = sum_upto_lane(tiles_upto), cost_upto = sum_upto_lane(cost_upto);
         const int last = min(a.c.sequences, 64) - 1;
         tiles = from_lane(tiles_upto, last), cost = from_lane(cost_upto, last);
         int at = top;
         for (int first = 64; first < a.c.sequences; first += 64) {
             const Seq s = seqs_from<R>(a, first, at);
-            long t = s.tiles, c = s.cost();
-            sum_upto(t, c, 64);
-            tiles += from_lane(t, 63), cost += from_lane(c, 63);
+            tiles += from_lane(sum_upto_lane(s.tiles), 63), cost += from_lane(sum_upto_lane(s.cost()), 63);
         }
     }
     // the sequence of page `at` of the list: the list's pages and tiles before it
@@ -135,8 +125,7 @@ struct Scan {
         for (int first = 0; first < a.c.sequences; first += 64) {
             if (first) {
                 x = seqs_from<R>(a, first, start);
-                t = x.tiles, c = x.cost();
-                sum_upto(t, c, 64);
+                t = sum_upto_lane(x.tiles), c = sum_upto_lane(x.cost());
             }
             const unsigned long long past = __ballot(first + (int)(threadIdx.x & 63) < a.c.sequences && cost_before + c > at);
             if (past) {

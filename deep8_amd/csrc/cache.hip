@@ -201,12 +201,7 @@ __device__ __forceinline__ bool share_of(const Pages &c, int id, Share &share) {
         const int n = end - first;
         const long place = length - n;  // of the first row; before 0 where the cache holds fewer tokens than the call brings
         const int pages = n ? (int)((place & (PAGE - 1)) + n + PAGE - 1) / PAGE : 0;
-        int upto = pages;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int other = __shfl_up(upto, d);
-            upto += lane >= d ? other : 0;
-        }
+        const int upto = sum_upto_lane(pages);
         const unsigned long long past = __ballot(before + upto > id);
         if (past) {
             const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)past) - 1), s = from + l;

@@ -35,6 +35,21 @@ __device__ __forceinline__ N over_lanes(N x, F op) {
     return x;
 }
 
+// the sum over the lanes up to this one: within sixteens, then what the sixteens, and the halves, before have
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved_or_0(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long moved_or_0(long x) {
+    return (long)((unsigned long)(unsigned)moved_or_0<CTRL, ROWS>((int)(x >> 32)) << 32 | (unsigned)moved_or_0<CTRL, ROWS>((int)x));
+}
+template <class N>
+__device__ __forceinline__ N sum_upto_lane(N x) {
+    x += moved_or_0<0x111, 0xf>(x), x += moved_or_0<0x112, 0xf>(x), x += moved_or_0<0x114, 0xf>(x), x += moved_or_0<0x118, 0xf>(x);  // lanes 1, 2, 4, 8 before
+    x += moved_or_0<0x142, 0xa>(x);  // the last lane of a sixteen, into all of the next: second and fourth
+    x += moved_or_0<0x143, 0xc>(x);  // lane 31, into the other half
+    return x;
+}
+
 }  // namespace d8
 
 #endif
