@@ -8,7 +8,7 @@
 //
 // One workgroup writes the tokens that a call brings to one page of one head: the elements are read twice (the largest, then the codes; the
 // second time out of cache), values are transposed through LDS, and a page that holds tokens already is read and written whole.  Bound
-// by memory where pages are filled (8192 tokens of 8 heads of 128 halves: 13 us written, 11 read back, 3.8 and 4.6 TB/s), by the chain of its loads
+// by memory where pages are filled (8192 tokens of 8 heads of 128 halves: 13 us written, 11.5 read back, 3.9 and 4.4 TB/s), by the chain of its loads
 // (sequence, page, scale, codes) where they get a token each: 5 us.
 #include "cache.h"
 #include "lanes.h"

@@ -12,8 +12,8 @@
 // way meanwhile), adds its teams' through LDS, and leaves one row of them in scratch; a second launch adds those in a fixed order.  Two
 // workgroups of 512 threads a compute unit, so that one loads while the other adds; more would write and read more such rows.
 //
-// Half: 16384 x 4096 forward 53 us, 5.0 TB/s, where a large copy moves 5.2; 8192 x 4096 back 49 us (44 and 4 for the sums), 4.1 TB/s.  Single, 8192 x 4096 forward
-// 50 us, back 82 us: 5.3 and 4.9 TB/s.
+// Half: 16384 x 4096 forward 53 us, 5.05 TB/s, where a large copy moves 5.2; 8192 x 4096 back 47 us (43 and 4 for the sums), 4.3 TB/s.  Single, 8192 x 4096
+// forward 50 us, back 81 us: 5.4 and 5.0 TB/s.
 //
 // Sums are fp32; results are rounded once.
 #include "row_team.h"

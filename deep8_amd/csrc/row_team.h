@@ -15,7 +15,7 @@ constexpr int most_held(int bytes, bool grad) { return bytes == 4 && grad ? 8192
 // E elements of a row of T in one thread, in pieces of V: piece i is number t + TEAM * i of the row.  ODD: the row, of V elements at least, starts
 // anywhere, and may end within a piece, for which the row's last V are read; settle() then moves them down.  (Norm of 16384 rows of 1001 in half: 15 us, 32
 // element by element.  A load that branches where the row ends keeps the next row's from running ahead: gradients of 4096 rows of 4095 took 51 us
-// so, and 34 with this.)
+// so, and 31 with this.)
 template <class T, int V, int TEAM, int E, bool ODD>
 struct Held {
     static constexpr int P = E / V;
@@ -99,7 +99,7 @@ __device__ __forceinline__ void team_sum(float &a, float &b, float2 *slots, int 
 
 // fn(V, TEAM, E, ODD) for the smallest team that holds a row; whole: every row is whole pieces of 16 bytes.  Short rows share a wave (65536 of 96 in half:
 // norm 9 us, 21 with a wave each); 16 elements a thread of 512 are better than 8 of 1024, of whose workgroups a compute unit has half as many to change
-// between (8192 rows of 5120: 43 us and 78).
+// between (8192 rows of 5120: 40 us and 78).
 template <class T, bool GRAD, class F>
 void with_team(bool whole, int cols, F &&fn) {
     constexpr int V = 16 / sizeof(T);
