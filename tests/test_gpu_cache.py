@@ -245,6 +245,36 @@ def test_pages_out_of_scale_beside_others(nq, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("n", [16, 130])
+def test_scores_small_and_large_side_by_side(n, dtype):
+    """rows whose largest scores are 1, some hundred, some thousand and 2^24 and more, in turn.  A score, a sum of 64 products, is off by 64 E of the products'
+    absolute sum at most, E = 2^-24, and a weight by the exponential of twice that: rows where that says nothing are the ones with one key far above all
+    others, whose weights are 1 and 0 in any case"""
+    r = rng(31)
+    cache, table, pages, (kv, vv) = _filled([300], 1, 64, r)
+    size = np.array([1, 300, 900, 1100, 5000])[np.arange(n) % 5]
+    q = r.standard_normal((n, 1, 64)) * (size / 20)[:, None, None]
+    q = q.astype(np.float16).astype(dtype)
+    scale = 0.125
+    if dtype == np.float32:
+        q[7] *= 2.0 ** 16
+    want, lse = so.attention_cache(q, kv, vv, [0, n], [300], table, pages, scale, False)
+    got, got_lse = cache.attention(q, [0, n], [300], table, scale, False)
+    got = f(got)[:, 0].astype(np.float64)
+    keys = np.concatenate([kv[p, 0] for p in table[0]])[:300]
+    values = np.concatenate([vv[p, 0] for p in table[0]])[:300]
+    terms = scale * (np.abs(f(q)[:, 0].astype(np.float64)) @ np.abs(keys).T)
+    off = np.expm1(np.minimum(2 * 64 * 2.0 ** -24 * terms.max(1), 1.0))
+    score = np.sort(scale * (f(q)[:, 0].astype(np.float64) @ keys.T), 1)
+    alone = score[:, -1] - score[:, -2] > 40 + 4 * 64 * 2.0 ** -24 * terms.max(1)
+    bound = np.where(alone, 0, 2 * off * np.abs(values).max()) + 4 * TOL[dtype] * np.abs(values).max()
+    assert np.isfinite(got).all() and np.isfinite(got_lse).all()
+    assert (np.abs(got - want[:, 0]).max(1) <= bound).all()
+    assert (np.abs(got_lse - lse) <= 64 * 2.0 ** -24 * terms.max(1) + 1e-5 * np.maximum(1, np.abs(lse))).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [6, 96])
 def test_queries_of_any_size(n):
     """rows of 1e-37 to 1e37, elements of different sizes in a row, rows of zeros; one with an infinity and one with NaN, which stay theirs alone"""
