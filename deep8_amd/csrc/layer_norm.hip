@@ -285,7 +285,7 @@ int check(const NormArgs &a, int dtype, bool grad) {
 
 template <class T>
 void launch_forward(const NormArgs &a, bool whole, hipStream_t stream) {
-    if (a.cols > most_held(sizeof(T), false)) {
+    if (a.cols > MOST_HELD) {
         hipLaunchKernelGGL(layer_norm_long_kernel<T>, dim3(a.rows < 4096 ? a.rows : 4096), dim3(1024), 0, stream, a);
         return;
     }
@@ -299,7 +299,7 @@ void launch_forward(const NormArgs &a, bool whole, hipStream_t stream) {
 
 template <class T>
 void launch_grad(NormArgs &a, bool whole, hipStream_t stream) {
-    if (a.cols > most_held(sizeof(T), true)) {
+    if (a.cols > MOST_HELD) {
         a.groups = a.rows < cu_count() ? a.rows : cu_count();
         hipLaunchKernelGGL(layer_norm_grad_long_kernel<T>, dim3(a.groups), dim3(1024), 0, stream, a);
         return;

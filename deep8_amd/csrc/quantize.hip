@@ -183,7 +183,7 @@ template <class T>
 void launch_rows(const QuantizeArgs &a, hipStream_t stream) {
     const int v = 16 / (int)sizeof(T);
     const bool whole = ((size_t)a.x & 15) == 0 && a.cols % v == 0 && a.ldx % v == 0;
-    if (a.cols > most_held(sizeof(T), false)) {
+    if (a.cols > MOST_HELD) {
         hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3(a.rows < 4096 ? a.rows : 4096), dim3(1024), 0, stream, a);
         return;
     }

@@ -9,8 +9,8 @@
 namespace d8 {
 namespace row_team {
 
-// Elements of a row that a team holds: 16 a thread of 1024, which in single precision do not leave a gradient enough registers.
-constexpr int most_held(int bytes, bool grad) { return bytes == 4 && grad ? 8192 : 16384; }
+// Elements of a row that a team holds at most, 16 a thread of 1024.
+enum { MOST_HELD = 16384 };
 
 // E elements of a row of T in one thread, in pieces of V: piece i is number t + TEAM * i of the row.  ODD: the row, of V elements at least, starts
 // anywhere, and may end within a piece, for which the row's last V are read; settle() then moves them down.  (Norm of 16384 rows of 1001 in half: 15 us, 32
@@ -22,6 +22,9 @@ struct Held {
     typedef T vec __attribute__((ext_vector_type(V)));
     typedef T odd_vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     typedef std::conditional_t<ODD, odd_vec, vec> there;
+    // Whether pieces beyond the row read its last V too and are cleared when used, in place of a load that may not be made: fewer registers (gradients of
+    // 1024 rows of 16384 in single: 61 us, 107 without), but 2 % more time in single where there are enough.
+    static constexpr bool CLAMPED = ODD || TEAM == 1024;
     vec raw[P];
     // whether element e of the thread's is one of the row's
     static __device__ __forceinline__ bool has(int e, int t, int cols) { return (t + TEAM * (e / V)) * V + (ODD ? e % V : 0) < cols; }
@@ -29,20 +32,22 @@ struct Held {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int c = (t + TEAM * i) * V;
-            if constexpr (ODD) raw[i] = *(const there *)(row + min(c, cols - V));
+            if constexpr (CLAMPED) raw[i] = *(const there *)(row + min(c, cols - V));
             else if (c < cols) raw[i] = *(const vec *)(row + c);
             else raw[i] = vec{};
         }
     }
     // after a load, before its elements are used: those beyond the row are 0
     __device__ __forceinline__ void settle(int t, int cols) {
-        if constexpr (ODD) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int beyond = (t + TEAM * i) * V - (cols - V);
-                if (beyond <= 0) continue;
+        for (int i = 0; i < P; ++i) {
+            const int beyond = (t + TEAM * i) * V - (cols - V);
+            if (!CLAMPED || beyond <= 0) continue;
+            if constexpr (ODD) {
                 typedef unsigned _BitInt(8 * V * sizeof(T)) bits;
                 raw[i] = beyond < V ? __builtin_bit_cast(vec, (bits)(__builtin_bit_cast(bits, raw[i]) >> (8 * (int)sizeof(T) * beyond))) : vec{};
+            } else {
+                raw[i] = vec{};
             }
         }
     }
@@ -112,8 +117,10 @@ void with_team(bool whole, int cols, F &&fn) {
         else if (cols <= 1024) D8_TEAM(64, 16);
         else if (cols <= 2048) D8_TEAM(256, 8);
         else if (cols <= 4096) D8_TEAM(256, 16);
-        else if constexpr (most_held(sizeof(T), GRAD) == 8192) D8_TEAM(1024, 8);
-        else if (cols <= 8192) D8_TEAM(512, 16);
+        else if (cols <= 8192) {
+            if constexpr (GRAD && sizeof(T) == 4) D8_TEAM(1024, 8);
+            else D8_TEAM(512, 16);
+        }
         else D8_TEAM(1024, 16);
 #undef D8_TEAM
     };

@@ -9,9 +9,8 @@ from test_kernel_registers import _code_objects, _kernels
 
 NAMES = ("layer_norm_kernel", "layer_norm_grad_kernel", "layer_norm_long_kernel", "layer_norm_grad_long_kernel", "layer_norm_sums_kernel", "quantize_rows_kernel",
          "quantize_long_rows_kernel", "cache_append_kernel", "cache_read_kernel", "attention_cache_kernel", "attention_cache_join_kernel")
-# gradients of rows in half of more than 8192 elements that start anywhere: 16 elements a thread of 1024, with what moves a row's last piece down
-SHORT = {("layer_norm_grad_kernel", "DF16_Li8ELi1024ELi16ELb1E"): 20}
-
+# gradients of rows of more than 8192 elements, 16 a thread of 1024: half, with what moves a row's last piece down; single either way
+SHORT = {("layer_norm_grad_kernel", "DF16_Li8ELi1024ELi16ELb1E"): 20, ("layer_norm_grad_kernel", "fLi4ELi1024ELi16ELb0E"): 10, ("layer_norm_grad_kernel", "fLi4ELi1024ELi16ELb1E"): 14}
 
 def _found():
     with open(capi.LIB_PATH, "rb") as f:
