@@ -10,6 +10,8 @@
 // second time out of cache), values are transposed through LDS, and a page that holds tokens already is read and written whole.  Bound
 // by memory where pages are filled (8192 tokens of 8 heads of 128 halves: 13 us written, 11.5 read back, 3.9 and 4.4 TB/s), by the chain of its loads
 // (sequence, page, scale, codes) where they get a token each: 5 us.
+#include <type_traits>
+
 #include "cache.h"
 #include "lanes.h"
 
@@ -57,7 +59,7 @@ __device__ __forceinline__ int rescaled(int word, float by) {
 
 template <class T, int V>
 struct Piece {
-    typedef T type __attribute__((ext_vector_type(V)));
+    typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));  // (rows may start anywhere)
 };
 template <class T>
 struct Piece<T, 1> {
@@ -67,8 +69,8 @@ __device__ __forceinline__ unsigned code_of(float x, float back) { return (unsig
 
 enum { WORDS = 17 };  // words of LDS between two elements' 16 of tokens: four elements of one token in different banks
 
-// Rows r .. r + rows - 1 of the call are places slot .. of `page`, which holds `slot` tokens already (or none that count).  V: elements of a 16-byte
-// piece, or 1 where rows cannot be moved in such.  An item is a piece of four tokens, of keys and of values: a word of codes of each of its elements.
+// Rows r .. r + rows - 1 of the call are places slot .. of `page`, which holds `slot` tokens already (or none that count).  V: elements of a piece of a
+// row (in_pieces).  An item is a piece of four tokens, of keys and of values: a word of codes of each of its elements.
 template <class T, int V>
 __device__ __forceinline__ void append(const Args &a, int r, int rows, int slot, int page, int head, unsigned *sizes, unsigned *words) {
     const Pages &c = a.c;
@@ -308,22 +310,24 @@ int check_rows(const Args &a, const char *name) {
     return 0;
 }
 
-template <class T>
-bool in_pieces(const Args &a) {
+// fn(V) for the largest pieces of 16 or 8 bytes that heads are made of, or single elements
+template <class T, class F>
+void in_pieces(int dim, F &&fn) {
     constexpr int V = 16 / (int)sizeof(T);
-    return a.c.dim % V == 0 && a.ldk % V == 0 && a.ldv % V == 0 && (((size_t)a.k | (size_t)a.v) & 15) == 0;
+    if (dim % V == 0) return fn(std::integral_constant<int, V>());
+    if constexpr (V == 8)
+        if (dim % 4 == 0) return fn(std::integral_constant<int, 4>());
+    fn(std::integral_constant<int, 1>());
 }
 
 template <class T>
 void launch_append(const Args &a, dim3 grid, hipStream_t stream) {
-    if (in_pieces<T>(a)) hipLaunchKernelGGL((cache_append_kernel<T, 16 / sizeof(T)>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((cache_append_kernel<T, 1>), grid, dim3(256), 0, stream, a);
+    in_pieces<T>(a.c.dim, [&](auto v) { hipLaunchKernelGGL((cache_append_kernel<T, decltype(v)::value>), grid, dim3(256), 0, stream, a); });
 }
 
 template <class T>
 void launch_read(const Args &a, dim3 grid, hipStream_t stream) {
-    if (in_pieces<T>(a)) hipLaunchKernelGGL((cache_read_kernel<T, 16 / sizeof(T)>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((cache_read_kernel<T, 1>), grid, dim3(256), 0, stream, a);
+    in_pieces<T>(a.c.dim, [&](auto v) { hipLaunchKernelGGL((cache_read_kernel<T, decltype(v)::value>), grid, dim3(256), 0, stream, a); });
 }
 
 }  // namespace

@@ -48,7 +48,8 @@ def _same(cache, want, table, lengths):
 
 # tokens of each sequence that come in each call; heads, dim, pad
 FILLS = [([[5]], 1, 8, 0), ([[1, 1]] * 5, 2, 64, 0), ([[64, 0, 130], [1, 1, 1], [3, 70, 62]], 2, 80, 8), ([[200, 63], [1, 1], [1, 1]], 3, 128, 0), ([[17, 0, 1], [47, 64, 0], [1, 65, 129]], 1, 33, 1),
-         ([[2] * 70, [1] * 70], 2, 16, 0), ([[100, 3]], 2, 256, 0), ([[90, 31], [5, 40]], 1, 7, 3), ([[300, 700]], 4, 96, 0)]
+         ([[2] * 70, [1] * 70], 2, 16, 0), ([[100, 3]], 2, 256, 0), ([[90, 31], [5, 40]], 1, 7, 3), ([[300, 700]], 4, 96, 0),
+         ([[70, 3], [1, 62]], 2, 100, 0), ([[70, 3], [30, 1]], 2, 64, 3), ([[5, 90], [64, 1]], 3, 44, 1)]
 
 
 @pytest.mark.gpu
