@@ -243,26 +243,26 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(NormArgs a) 
     }
 }
 
-// 64 of the columns of dw (blockIdx.y 0) or db: each of 16 waves adds every 16th workgroup's sums, then the waves' are added in order
-template <class T>
+// C of the columns of dw (blockIdx.y 0) or db: C threads side by side add every 1024 / C-th workgroup's sums, then 1024 / C threads a column's, in a fixed order.
+// 32 columns where 64 would leave compute units without any (back at 32768 x 256: 16 us for 17), 64 where there are enough (2048 x 11111: 74 for 75.5).
+template <class T, int C>
 __global__ __launch_bounds__(1024) void layer_norm_sums_kernel(NormArgs a) {
-    __shared__ float sums[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, k = blockIdx.y;
+    constexpr int G = 1024 / C;
+    __shared__ float sums[G][C + 1];
+    const int c = blockIdx.x * C + threadIdx.x % C, k = blockIdx.y;
     T *to = (T *)(k ? a.dbias : a.dweight);
     if (!to) return;
     float s = 0.f;
     if (c < a.cols) {
         const float *from = a.partial + (long)k * a.cols + c;
 #pragma unroll 8
-        for (int g = wave; g < a.groups; g += 16) s += from[(long)g * 2 * a.cols];
+        for (int g = threadIdx.x / C; g < a.groups; g += G) s += from[(long)g * 2 * a.cols];
     }
-    sums[wave][lane] = s;
+    sums[threadIdx.x / C][threadIdx.x % C] = s;
     __syncthreads();
-    if (wave || c >= a.cols) return;
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s += sums[i][lane];
-    to[c] = (T)(a.overwrite & 2 ? s : s + (float)to[c]);
+    s = over_lanes<G>(sums[threadIdx.x % G][threadIdx.x / G], [](float x, float y) { return x + y; });
+    const int own = blockIdx.x * C + threadIdx.x / G;
+    if (threadIdx.x % G == 0 && own < a.cols) to[own] = (T)(a.overwrite & 2 ? s : s + (float)to[own]);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -313,6 +313,12 @@ void launch_grad(NormArgs &a, bool whole, hipStream_t stream) {
     });
 }
 
+template <class T>
+void launch_sums(const NormArgs &a, hipStream_t stream) {
+    if (a.cols < 16 * cu_count()) hipLaunchKernelGGL((layer_norm_sums_kernel<T, 32>), dim3(ceil_div(a.cols, 32), 2), dim3(1024), 0, stream, a);
+    else hipLaunchKernelGGL((layer_norm_sums_kernel<T, 64>), dim3(ceil_div(a.cols, 64), 2), dim3(1024), 0, stream, a);
+}
+
 }  // namespace
 }  // namespace d8
 
@@ -356,9 +362,8 @@ extern "C" int d8_layer_norm_grad(int dtype, const void *x, long ldx, const void
         D8_LAUNCH_CHECK();
     }
     if (sums) {  // (without a row the sums are zero)
-        const dim3 grid(ceil_div(cols, 64), 2);
-        if (dtype == D8_FLOAT16) hipLaunchKernelGGL(layer_norm_sums_kernel<f16>, grid, dim3(1024), 0, as_stream(stream), a);
-        else hipLaunchKernelGGL(layer_norm_sums_kernel<float>, grid, dim3(1024), 0, as_stream(stream), a);
+        if (dtype == D8_FLOAT16) launch_sums<f16>(a, as_stream(stream));
+        else launch_sums<float>(a, as_stream(stream));
         D8_LAUNCH_CHECK();
     }
     return 0;
