@@ -16,27 +16,33 @@ namespace {
 
 __device__ __forceinline__ void mma(i32x4 &acc, const i32x4 &a, const i32x4 &b) { acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc, 0, 0, 0); }
 
-// four sums of row m, columns n .. n + 3: scaled into z, or as they are into part number `part`
+// four sums of row m, columns n .. n + 3: scaled by that row's scale and those columns' into z, or as they are into part number `part`
 template <class T>
-__device__ __forceinline__ void put(const Args &a, int part, int m, int n, const i32x4 &sum) {
+__device__ __forceinline__ void put(const Args &a, int part, int m, int n, const i32x4 &sum, float row, const float (&cols)[4]) {
     if (m >= a.rows || n >= a.cols) return;
     if (a.parts > 1) {  // (rows of parts are whole pieces)
         *(i32x4 *)(a.part + ((long)part * a.rows + m) * a.part_ld + n) = sum;
         return;
     }
     T *z = (T *)a.z + (long)m * a.ldz + n;
-    const float s = a.x_scales[m];
     if (a.vec && n + 4 <= a.cols) {
         typedef T quad __attribute__((ext_vector_type(4)));
         quad out;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = scaled<T>(sum[e], s, a.w_scales[n + e]);
+        for (int e = 0; e < 4; ++e) out[e] = scaled<T>(sum[e], row, cols[e]);
         *(quad *)z = out;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (n + e < a.cols) z[e] = scaled<T>(sum[e], s, a.w_scales[n + e]);
+            if (n + e < a.cols) z[e] = scaled<T>(sum[e], row, cols[e]);
     }
+}
+template <class T>
+__device__ __forceinline__ void put(const Args &a, int part, int m, int n, const i32x4 &sum) {
+    float cols[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) cols[e] = a.w_scales[min(n + e, a.cols - 1)];
+    put<T>(a, part, m, n, sum, a.x_scales[min(m, a.rows - 1)], cols);
 }
 
 // the parts' sums of four columns of a row
@@ -58,8 +64,7 @@ enum { ROWS_WAVES = 8, ROWS_COLS = 32 };
 template <class T, int RT>
 __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
     __shared__ i32x4 sums[ROWS_WAVES][2 * RT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int blocks = (a.cols + ROWS_COLS - 1) / ROWS_COLS, part = blockIdx.x / blocks, n0 = (blockIdx.x - part * blocks) * ROWS_COLS;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = blockIdx.y, n0 = blockIdx.x * ROWS_COLS;
     const int first = (int)((long)a.steps * part / a.parts), end = (int)((long)a.steps * (part + 1) / a.parts);
     // a lane's 16 bytes of a step of 128: columns (rows) lane % 16 of each tile, bytes 16 (lane / 16) .. of both halves.  Beyond the last
     // column or row the last one is read again; what comes of it is not stored.
@@ -70,6 +75,15 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < RT; ++j) x[j] = a.x + (long)min(16 * j + r, a.rows - 1) * a.pitch + at;
     i32x4 acc[2][RT] = {};
+    // scales of what the wave stores, if any, on their way meanwhile
+    static_assert(2 * RT <= ROWS_WAVES);
+    const int m = 16 * (wave % RT) + r, n = n0 + 16 * (wave / RT) + (lane >> 4) * 4;
+    float row = 0.f, four[4] = {};
+    if (wave < 2 * RT) {
+        row = a.x_scales[min(m, a.rows - 1)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] = a.w_scales[min(n + e, a.cols - 1)];
+    }
     // the loads of several steps at once (those beyond the last: it again, not multiplied)
     constexpr int U = RT == 1 ? 4 : 2;
     for (int s = first + wave; s < end; s += ROWS_WAVES * U) {
@@ -102,12 +116,11 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < RT; ++j) sums[wave][i * RT + j][lane] = acc[i][j];
     __syncthreads();
-    for (int q = wave; q < 2 * RT; q += ROWS_WAVES) {
-        i32x4 sum = sums[0][q][lane];
+    if (wave >= 2 * RT) return;
+    i32x4 sum = sums[0][wave][lane];
 #pragma unroll
-        for (int k = 1; k < ROWS_WAVES; ++k) sum += sums[k][q][lane];
-        put<T>(a, part, 16 * (q % RT) + r, n0 + 16 * (q / RT) + (lane >> 4) * 4, sum);
-    }
+    for (int k = 1; k < ROWS_WAVES; ++k) sum += sums[k][wave][lane];
+    put<T>(a, part, m, n, sum, row, four);
 }
 
 // ---- tiles ----------------------------------------------------------------------------------------------------------
@@ -117,19 +130,18 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
 // there are many tiles: two fragments read for each two products, 1000 TOP/s (1024 x 4096 x 4096 in 33 us; tiles of 128 x 128, of which fewer fit a compute
 // unit: 35, and 14 for 8.5 at 777 x 1024 x 1352).
 // QUADS: w is the left operand, a lane has four columns of a row; else x is, and 16 lanes have a row's columns side by side, which is what rows of z that cannot
-// be stored four elements at a time want (777 x 1000 x 1351 in single: 64 separate words a store before, 11 us for 9.2).
-enum { TILE = 64 };
+// be stored four elements at a time want (777 x 1000 x 1351 in single: 64 separate words a store before, 11 us for 9.2, and 8.1 with the scales loaded ahead and the tile's place in the launch's
+// three axes).
+enum { TILE = 64, MOST_Y = 32768 };
 
 template <class T, bool QUADS>
 __global__ __launch_bounds__(256) void int8_tile_kernel(Args a) {
     constexpr int B = TILE, F = B / 32, PIECES = B * STEP / 16 / 256;
     __shared__ __attribute__((aligned(16))) signed char lds[2][2][B * STEP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-    const int tilesM = (a.rows + B - 1) / B, tilesN = (a.cols + B - 1) / B;
-    int id = blockIdx.x;
-    const int part = id / (tilesM * tilesN);
-    id -= part * tilesM * tilesN;
-    const int m0 = id % tilesM * B, n0 = id / tilesM * B;
+    // tiles of rows, of columns, parts: (x, y, z); or, where there is one part, y and z both the columns' (a launch has less than 2^16 along either)
+    const int part = a.parts > 1 ? blockIdx.z : 0, m0 = blockIdx.x * B, n0 = (a.parts > 1 ? blockIdx.y : blockIdx.z * MOST_Y + blockIdx.y) * B;
+    if (n0 >= a.cols) return;
     const int first = (int)((long)a.steps * part / a.parts), end = (int)((long)a.steps * (part + 1) / a.parts);
     const signed char *from[2][PIECES];
     int to[PIECES];
@@ -142,6 +154,17 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(Args a) {
     }
     constexpr int D = 3;
     i32x4 ahead[D][2][PIECES], acc[F][F] = {};
+    // scales of what the lane stores, on their way meanwhile (QUADS: of its row and four columns; else of its column and four rows)
+    float own[F], four[F][4];
+    {
+        const int n = n0 + wn * (B / 2), m = m0 + wm * (B / 2), l15 = lane & 15, l4 = (lane >> 4) * 4;
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+            own[i] = QUADS ? a.x_scales[min(m + 16 * i + l15, a.rows - 1)] : a.w_scales[min(n + 16 * i + l15, a.cols - 1)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) four[i][e] = QUADS ? a.w_scales[min(n + 16 * i + l4 + e, a.cols - 1)] : a.x_scales[min(m + 16 * i + l4 + e, a.rows - 1)];
+        }
+    }
     auto fetch = [&](i32x4 (&to)[2][PIECES], int s) {
 #pragma unroll
         for (int o = 0; o < 2; ++o)
@@ -195,12 +218,12 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(Args a) {
         for (int k = 0; k < F; ++k) {
             const int m = m0 + wm * (B / 2) + 16 * k, n = n0 + wn * (B / 2) + 16 * i;
             if constexpr (QUADS) {
-                put<T>(a, part, m + r, n + j * 4, acc[i][k]);
+                put<T>(a, part, m + r, n + j * 4, acc[i][k], own[k], four[i]);
             } else {
+                T *z = (T *)a.z + (long)(m + j * 4) * a.ldz + n + r;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (m + j * 4 + e < a.rows && n + r < a.cols)
-                        ((T *)a.z)[(long)(m + j * 4 + e) * a.ldz + n + r] = scaled<T>(acc[i][k][e], a.x_scales[m + j * 4 + e], a.w_scales[n + r]);
+                    if (m + j * 4 + e < a.rows && n + r < a.cols) z[e * a.ldz] = scaled<T>(acc[i][k][e], four[k][e], own[i]);
             }
         }
 }
@@ -237,15 +260,17 @@ int launch(Args a, const Plan &p, hipStream_t stream) {
     if (p.few) {
         const long groups = ceil_div(a.cols, ROWS_COLS) * (long)p.parts;
         D8_REQUIRE(groups < (1L << 23), "matmul_int8: a result of %d x %d is too large", a.rows, a.cols);
-        const dim3 grid((unsigned)groups), threads(ROWS_WAVES * 64);
+        const dim3 grid(ceil_div(a.cols, ROWS_COLS), p.parts), threads(ROWS_WAVES * 64);
         if (a.rows <= 16) hipLaunchKernelGGL((int8_rows_kernel<T, 1>), grid, threads, 0, stream, a);
         else if (a.rows <= 32) hipLaunchKernelGGL((int8_rows_kernel<T, 2>), grid, threads, 0, stream, a);
         else hipLaunchKernelGGL((int8_rows_kernel<T, 4>), grid, threads, 0, stream, a);
     } else {
         const long groups = (long)ceil_div(a.rows, TILE) * ceil_div(a.cols, TILE) * p.parts;
+        const unsigned tiles = ceil_div(a.cols, TILE);
+        const dim3 grid(ceil_div(a.rows, TILE), tiles < MOST_Y ? tiles : MOST_Y, p.parts > 1 ? p.parts : ceil_div(tiles, MOST_Y));
         D8_REQUIRE(groups < (1L << 24), "matmul_int8: a result of %d x %d is too large", a.rows, a.cols);
-        if (a.vec || a.parts > 1) hipLaunchKernelGGL((int8_tile_kernel<T, true>), dim3((unsigned)groups), dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((int8_tile_kernel<T, false>), dim3((unsigned)groups), dim3(256), 0, stream, a);
+        if (a.vec || a.parts > 1) hipLaunchKernelGGL((int8_tile_kernel<T, true>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((int8_tile_kernel<T, false>), grid, dim3(256), 0, stream, a);
     }
     D8_LAUNCH_CHECK();
     if (p.parts > 1) {

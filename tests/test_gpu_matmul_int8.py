@@ -197,6 +197,24 @@ def test_nothing_to_do():
     assert ops.matmul_int8(codes, scales, *one, 24).shape == (0, 3) and ops.matmul_int8(*one, codes, scales, 24).shape == (3, 0)
 
 
+@pytest.mark.gpu
+def test_more_tiles_of_columns_than_a_launch_has_along_an_axis():
+    """32768 tiles of 64 columns and two more, some rows too many for the kernel of few; results at both sides of the turn and at random places"""
+    from deep8_amd import capi
+    lib, r, rows, cols = capi.init(), rng(41), 65, 32768 * 64 + 70
+    w, x = np.zeros((cols, 128), np.int8), np.zeros((rows, 128), np.int8)
+    w[:, 0], x[:, 0] = r.integers(-127, 128, cols), r.integers(-127, 128, rows)
+    xs, ws = np.exp2(r.integers(-4, 3, rows)).astype(np.float32), np.exp2(r.integers(-4, 3, cols)).astype(np.float32)
+    d = [capi.DeviceArray.from_numpy(a) for a in (x, xs, w, ws)]
+    z = capi.DeviceArray((rows, cols), np.float16)
+    capi.check(lib.d8_matmul_int8(capi.FLOAT16, d[0].ptr, d[1].ptr, rows, 1, d[2].ptr, d[3].ptr, cols, z.ptr, cols, None, 0, None))
+    capi.sync()
+    at = np.r_[0:70, 32768 * 64 - 70:cols, r.integers(0, cols, 500)]
+    want = (x[:, :1].astype(np.float64) * xs[:, None]) * (w[at, 0].astype(np.float64) * ws[at])
+    with np.errstate(over="ignore"):  # (some are more than half holds)
+        assert np.array_equal(z.numpy()[:, at], want.astype(np.float16))
+
+
 def test_refusals():
     """(refused before anything is launched: the tensors need not be there, nor a device)"""
     from deep8_amd import capi
