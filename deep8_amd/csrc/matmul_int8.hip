@@ -3,11 +3,13 @@
 //
 // Three ways, by size:
 //   few rows (64 at most)      bound by memory, the weight: no LDS on its way, a wave reads 16 codes a lane straight into the operand
-//                              of v_mfma_i32_16x16x64_i8 (32 columns of w as left operand, all rows of x as right one); eight waves
+//                              of v_mfma_i32_16x16x64_i8 (16 or 32 columns of w as left operand, all rows of x as right one); eight waves
 //                              share out the steps of the reduction and join through LDS: 4 x 4096 x 8192 in 8.9 us, 3.8 TB/s
 //   many rows and columns      matmul_int8_wide.hip
 //   between                    tiles of 64 x 64 through LDS, cut along the reduction where they leave compute units idle and it is long
 // Where w is the left operand, a lane ends up with four columns of a row side by side.
+#include <type_traits>
+
 #include "int8.h"
 
 namespace d8 {
@@ -58,28 +60,28 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Args a) {
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-enum { ROWS_WAVES = 8, ROWS_COLS = 32 };
+enum { ROWS_WAVES = 8 };
 
-// RT tiles of 16 rows
-template <class T, int RT>
+// RT tiles of 16 rows, CT of 16 columns
+template <class T, int RT, int CT>
 __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
-    __shared__ i32x4 sums[ROWS_WAVES][2 * RT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = blockIdx.y, n0 = blockIdx.x * ROWS_COLS;
+    __shared__ i32x4 sums[ROWS_WAVES][CT * RT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = blockIdx.y, n0 = blockIdx.x * 16 * CT;
     const int first = (int)((long)a.steps * part / a.parts), end = (int)((long)a.steps * (part + 1) / a.parts);
     // a lane's 16 bytes of a step of 128: columns (rows) lane % 16 of each tile, bytes 16 (lane / 16) .. of both halves.  Beyond the last
     // column or row the last one is read again; what comes of it is not stored.
     const int r = lane & 15, at = (lane >> 4) * 16;
-    const signed char *w[2], *x[RT];
+    const signed char *w[CT], *x[RT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w[i] = a.w + (long)min(n0 + 16 * i + r, a.cols - 1) * a.pitch + at;
+    for (int i = 0; i < CT; ++i) w[i] = a.w + (long)min(n0 + 16 * i + r, a.cols - 1) * a.pitch + at;
 #pragma unroll
     for (int j = 0; j < RT; ++j) x[j] = a.x + (long)min(16 * j + r, a.rows - 1) * a.pitch + at;
-    i32x4 acc[2][RT] = {};
+    i32x4 acc[CT][RT] = {};
     // scales of what the wave stores, if any, on their way meanwhile
-    static_assert(2 * RT <= ROWS_WAVES);
+    static_assert(CT * RT <= ROWS_WAVES);
     const int m = 16 * (wave % RT) + r, n = n0 + 16 * (wave / RT) + (lane >> 4) * 4;
     float row = 0.f, four[4] = {};
-    if (wave < 2 * RT) {
+    if (wave < CT * RT) {
         row = a.x_scales[min(m, a.rows - 1)];
 #pragma unroll
         for (int e = 0; e < 4; ++e) four[e] = a.w_scales[min(n + e, a.cols - 1)];
@@ -87,14 +89,14 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
     // the loads of several steps at once (those beyond the last: it again, not multiplied)
     constexpr int U = RT == 1 ? 4 : 2;
     for (int s = first + wave; s < end; s += ROWS_WAVES * U) {
-        i32x4 fw[U][2][2], fx[U][RT][2];
+        i32x4 fw[U][CT][2], fx[U][RT][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long k = (long)min(s + ROWS_WAVES * u, end - 1) * STEP;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) fw[u][i][h] = *(const i32x4 *)(w[i] + k + 64 * h);
+                for (int i = 0; i < CT; ++i) fw[u][i][h] = *(const i32x4 *)(w[i] + k + 64 * h);
 #pragma unroll
                 for (int j = 0; j < RT; ++j) fx[u][j][h] = *(const i32x4 *)(x[j] + k + 64 * h);
             }
@@ -106,17 +108,17 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < CT; ++i)
 #pragma unroll
                     for (int j = 0; j < RT; ++j) mma(acc[i][j], fw[u][i][h], fx[u][j][h]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < CT; ++i)
 #pragma unroll
         for (int j = 0; j < RT; ++j) sums[wave][i * RT + j][lane] = acc[i][j];
     __syncthreads();
-    if (wave >= 2 * RT) return;
+    if (wave >= CT * RT) return;
     i32x4 sum = sums[0][wave][lane];
 #pragma unroll
     for (int k = 1; k < ROWS_WAVES; ++k) sum += sums[k][wave][lane];
@@ -234,21 +236,27 @@ enum { FEW_ROWS = 64 };
 // How a call runs.
 struct Plan {
     bool few;
-    int parts;
+    int parts, few_cols;
     long part_ld;
     size_t bytes(int rows) const { return parts > 1 ? sizeof(int) * (size_t)parts * rows * part_ld : 0; }
 };
 
 // Parts where workgroups are fewer than compute units, of 16 steps at least: a join costs 3 us and more, as much as some ten steps take (64 x 64 tiles, one part
-// and two: 512 x 1024 x 1024 6.5 and 9.3 us, 256 x 2048 x 2048 8.6 and 10.2, 65 x 4096 x 4096 13.2 and 12.2).
+// and two: 512 x 1024 x 1024 6.5 and 9.3 us, 256 x 2048 x 2048 8.6 and 10.2, 65 x 4096 x 4096 13.2 and 12.2).  Few rows, whose steps eight waves share: of 64, 32
+// or 16 steps for 1, 2 or 4 tiles of rows (4 x 4096 x 2048 4.8 us, 7.6 in two parts; 40 x 8192 x 1024 16 in one, 9.7 in four).
 Plan plan_of(int rows, int inner, int cols) {
     Plan p;
     const long steps = pitch_of(inner) / STEP, cus = cu_count();
     p.part_ld = (cols + 3L) / 4 * 4;
     p.few = rows <= FEW_ROWS;
-    const long groups = p.few ? ceil_div(cols, ROWS_COLS) : (long)ceil_div(rows, TILE) * ceil_div(cols, TILE);
+    const int tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;  // of 16 rows
+    // 32 columns a workgroup read x half as often; 16 where those would leave half the compute units idle (16 x 4096 x 4096 6.1 us, 10.8 with 32 and two parts,
+    // but 8 x 2048 x 6144 7.9 and 7.0), unless x is large (64 x 11008 x 4096 28 and 27).
+    p.few_cols = tiles < 4 && 2 * ceil_div(cols, 32) <= cus ? 16 : 32;
+    const long groups = p.few ? ceil_div(cols, p.few_cols) : (long)ceil_div(rows, TILE) * ceil_div(cols, TILE);
     long parts = groups >= cus ? 1 : (2 * cus) / groups;
-    parts = parts > steps / 16 ? steps / 16 : parts;
+    const long most = steps / (p.few ? 64 / tiles : 16);
+    parts = parts > most ? most : parts;
     p.parts = (int)(parts < 1 ? 1 : parts);
     return p;
 }
@@ -258,12 +266,22 @@ int launch(Args a, const Plan &p, hipStream_t stream) {
     a.parts = p.parts, a.part_ld = p.part_ld;
     a.vec = a.ldz % 4 == 0 && ((size_t)a.z & (4 * sizeof(T) - 1)) == 0;
     if (p.few) {
-        const long groups = ceil_div(a.cols, ROWS_COLS) * (long)p.parts;
+        const long groups = ceil_div(a.cols, p.few_cols) * (long)p.parts;
         D8_REQUIRE(groups < (1L << 23), "matmul_int8: a result of %d x %d is too large", a.rows, a.cols);
-        const dim3 grid(ceil_div(a.cols, ROWS_COLS), p.parts), threads(ROWS_WAVES * 64);
-        if (a.rows <= 16) hipLaunchKernelGGL((int8_rows_kernel<T, 1>), grid, threads, 0, stream, a);
-        else if (a.rows <= 32) hipLaunchKernelGGL((int8_rows_kernel<T, 2>), grid, threads, 0, stream, a);
-        else hipLaunchKernelGGL((int8_rows_kernel<T, 4>), grid, threads, 0, stream, a);
+        const dim3 grid(ceil_div(a.cols, p.few_cols), p.parts), threads(ROWS_WAVES * 64);
+        auto few = [&](auto rt) {
+            constexpr int RT = decltype(rt)::value;
+            if constexpr (RT < 4) {
+                if (p.few_cols == 16) {
+                    hipLaunchKernelGGL((int8_rows_kernel<T, RT, 1>), grid, threads, 0, stream, a);
+                    return;
+                }
+            }
+            hipLaunchKernelGGL((int8_rows_kernel<T, RT, 2>), grid, threads, 0, stream, a);
+        };
+        if (a.rows <= 16) few(std::integral_constant<int, 1>());
+        else if (a.rows <= 32) few(std::integral_constant<int, 2>());
+        else few(std::integral_constant<int, 4>());
     } else {
         const long groups = (long)ceil_div(a.rows, TILE) * ceil_div(a.cols, TILE) * p.parts;
         const unsigned tiles = ceil_div(a.cols, TILE);

@@ -80,7 +80,8 @@ def test_rows_of_zeros_of_the_smallest_and_of_no_numbers(cols, dtype):
 
 
 PRODUCTS = [(1, 1, 1), (1, 64, 31), (3, 200, 33), (4, 4096, 512), (16, 1000, 100), (17, 300, 64), (32, 2048, 70), (33, 130, 5), (64, 8192, 48), (5, 16, 9000), (2, 131071, 3),
-            (65, 128, 65), (128, 4096, 128), (130, 1000, 257), (777, 1000, 1351), (200, 100, 4100), (2000, 700, 2050), (100, 20000, 70)]
+            (65, 128, 65), (128, 4096, 128), (130, 1000, 257), (777, 1000, 1351), (200, 100, 4100), (2000, 700, 2050), (100, 20000, 70),
+            (4, 16384, 130), (20, 8192, 100), (40, 8192, 1000), (32, 200, 9000), (50, 100, 9000)]
 
 
 def _product(rows, inner, cols, seed):
@@ -154,7 +155,7 @@ def test_a_product_with_its_quantised_operands_is_near_the_product():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,inner,cols", [(4, 4096, 512), (300, 1000, 130), (4096, 256, 4096)])
+@pytest.mark.parametrize("rows,inner,cols", [(4, 4096, 512), (4, 16384, 512), (300, 1000, 130), (4096, 256, 4096)])
 def test_captured_and_replayed(rows, inner, cols):
     from deep8_amd import capi, ops
     lib = capi.init()
@@ -232,8 +233,8 @@ def test_refusals():
         refused(fn, rows, [(0, capi.FLOAT64), (0, 0)], 10002)
     refused(lib.d8_quantize_rows, rows, [(4, 0), (4, 131072)])
     refused(lib.d8_quantize_columns, rows, [(3, 0), (3, 131072)])
-    product = (capi.FLOAT16, p, p, 4, 4096, p, p, 8, p, 8, p, 1 << 40, None)
-    assert lib.d8_matmul_int8_scratch_bytes(4, 4096, 8) > 0
+    product = (capi.FLOAT16, p, p, 4, 16384, p, p, 8, p, 8, p, 1 << 40, None)
+    assert lib.d8_matmul_int8_scratch_bytes(4, 16384, 8) > 0
     refused(lib.d8_matmul_int8, product, [(1, None), (1, 72), (2, None), (3, -1), (4, 0), (4, 131072), (5, None), (5, 65), (6, None), (7, -1), (8, None), (9, 7), (10, None), (10, 72),
                                           (11, 0)])
     refused(lib.d8_matmul_int8, product, [(0, capi.FLOAT64)], 10002)
