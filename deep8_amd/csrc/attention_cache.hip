@@ -28,7 +28,9 @@
 // the others, no gain; accumulators in units of the pages' scales: 139 for 126.)  Short calls are bound by latency: a wave's
 // way from the first length to its last store is 10 us, and the join 4.
 //
-// Maxima, sums and accumulators are fp32.  Half: probabilities (at most 1) are halves in the second product.
+// Maxima, sums and accumulators are fp32.  Probabilities are halves in the second product (single: two), 2^LIFT times what they are: one of 2^-28 of the row's
+// largest so far still has all of a half's bits, and below that they are off by 2^-39 of it, which a million keys make 2^-19.  (As they are, those below 2^-25 would
+// be lost from the result and kept in the sum: a first key that takes nearly all the weight, and 131072 others that have 2^-25 each, 0.4 % of the values' size.)
 #include "cache.h"
 #include "lanes.h"
 
@@ -37,6 +39,7 @@ namespace cache {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LIFT = 14.f, LOWER = 1.f / 16384.f;  // (log2 of what probabilities are multiplied by: the largest, 1, stays in half's range; and back)
 enum { KEYS_WAVES = 4, KEYS_ROWS = 16, ROWS_WAVES = 8, MANY_ROWS = 128 };
 
 struct Join;
@@ -208,13 +211,11 @@ struct Precision;
 template <>
 struct Precision<f16> {
     static constexpr int QUERY = 1, WEIGHT = 1;
-    static constexpr float LIFT = 0.f;
 };
-// So that what is left stays in half's range too, a row of queries is brought to 2^13 .. 2^14 by a power of two, and probabilities by LIFT.
+// So that what is left stays in half's range too, a row of queries is brought to 2^13 .. 2^14 by a power of two, as probabilities are by LIFT.
 template <>
 struct Precision<float> {
     static constexpr int QUERY = 3, WEIGHT = 2;
-    static constexpr float LIFT = 14.f;
 };
 
 template <int PARTS>
@@ -272,7 +273,7 @@ struct Wave {
     f16x8 q[NC][P::QUERY][2];
     float q_scale;  // of the lane's row (single precision)
     f32x4 o[NC * 4];
-    float m, sum;  // of scores times log2 e; the lane's part of the sum
+    float m, sum;  // of scores times log2 e; the lane's part of the sum, 2^LIFT times it
     int limit;     // keys that the lane's row sees
 
     const T *from;  // the lane's row of queries, or another's where it has none
@@ -378,25 +379,21 @@ struct Wave {
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by, P::LIFT - base));
+            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by, LIFT - base));
             add += x[i];
         }
         split<P::WEIGHT>(x, p);
-        if (P::LIFT != 0.f) {
-            constexpr float LOWER = 1.f / 16384.f;
-            add *= LOWER, into *= LOWER;
-        }
         sum += add;
     }
 
-    // 64 pages of a sequence: lane i has page, and scales, of number i
+    // 64 pages of a sequence: lane i has page, and scales, of number i (that of values for probabilities 2^LIFT times what they are)
     struct List {
         int ids, there;
         float ks, vs;
         __device__ __forceinline__ void load(const Pages &c, int s, int head, int first, int count, int step) {
             const int i = threadIdx.x & 63, p = i < count ? c.page_of(s, first + i * step) : -1;
             there = p >= 0, ids = max(p, 0), ks = vs = 0.f;
-            if (p >= 0) ks = c.k_scales[(long)p * c.kv_heads + head], vs = c.v_scales[(long)p * c.kv_heads + head];
+            if (p >= 0) ks = c.k_scales[(long)p * c.kv_heads + head], vs = c.v_scales[(long)p * c.kv_heads + head] * LOWER;
         }
         __device__ __forceinline__ int id(int n) const { return __builtin_amdgcn_readlane(ids, n); }
         __device__ __forceinline__ bool is(int n) const { return __builtin_amdgcn_readlane(there, n) != 0; }
@@ -614,7 +611,7 @@ __global__ __launch_bounds__((ROWS ? ROWS_WAVES : KEYS_WAVES) * 64, NC == 4 ? 1 
             }
             const int lane = fresh_lane(), r = lane & 15, g = lane >> 4;
             at += end - first;
-            w.sum = row_sum(w.sum);
+            w.sum = row_sum(w.sum) * LOWER;
             if constexpr (!ROWS) {
 #pragma unroll
                 for (int i = 0; i < NC * 4; ++i) others[wave][i][lane] = w.o[i];
