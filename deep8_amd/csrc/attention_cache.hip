@@ -371,15 +371,15 @@ struct Wave {
             for (int i = 0; i < NC * 4; ++i) o[i] *= less;
             m = top;
         }
-        float add = 0.f;
-        if (__ballot(fabsf(base) >= LARGE)) {
+        float add = 0.f, shift = LIFT - base;
+        if (__ballot(fabsf(base) >= LARGE)) {  // (nor is LIFT added to a maximum that large: from 2^25 on it would be rounded to 16, which is past half's range)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] *= by;
-            by = 1.f;
+            for (int i = 0; i < 16; ++i) x[i] = x[i] * by - base;
+            by = 1.f, shift = LIFT;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by, LIFT - base));
+            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by, shift));
             add += x[i];
         }
         split<P::WEIGHT>(x, p);
