@@ -26,17 +26,15 @@ __device__ __forceinline__ void put(const Args &a, int part, int m, int n, const
         *(i32x4 *)(a.part + ((long)part * a.rows + m) * a.part_ld + n) = sum;
         return;
     }
-    T *z = (T *)a.z + (long)m * a.ldz + n;
+    T *z = (T *)a.z + (long)m * a.ldz + n, out[4];
+    scale_row<T, 4>(sum, row, cols, out);
     if (a.vec && n + 4 <= a.cols) {
         typedef T quad __attribute__((ext_vector_type(4)));
-        quad out;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = scaled<T>(sum[e], row, cols[e]);
-        *(quad *)z = out;
+        *(quad *)z = *(const quad *)out;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (n + e < a.cols) z[e] = scaled<T>(sum[e], row, cols[e]);
+            if (n + e < a.cols) z[e] = out[e];
     }
 }
 template <class T>

@@ -98,8 +98,7 @@ __device__ __forceinline__ void store_scaled(const Args &a, const wide::Where &w
 #pragma unroll
                 for (int h = 0; h < 2; ++h) part[h] = *(const i32x4 *)(patch + row * 128 + (column<T>(l15, 4 * h) ^ (t * 16)));
                 T out[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) out[e] = scaled<T>(part[e >> 2][e & 3], by.x[i * 4 + t], by.w[e]);
+                scale_row<T, 8>(__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7), by.x[i * 4 + t], by.w, out);
                 typedef T piece __attribute__((ext_vector_type(16 / sizeof(T))));
                 T *z = (T *)a.z + (long)m * a.ldz + n;
 #pragma unroll
@@ -112,10 +111,11 @@ __device__ __forceinline__ void store_scaled(const Args &a, const wide::Where &w
                 int sums[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) sums[k] = __float_as_int(patch[row * 128 + ((k * 16 + l15) ^ (t * 16))]);
-                T *z = (T *)a.z + (long)m * a.ldz + n + l15;
+                T *z = (T *)a.z + (long)m * a.ldz + n + l15, out[8];
+                scale_row<T, 8>(sums, by.x[i * 4 + t], along, out);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    if (m >= w.m_own && n + l15 + k * 16 >= w.n_own) z[k * 16] = scaled<T>(sums[k], by.x[i * 4 + t], along[k]);
+                    if (m >= w.m_own && n + l15 + k * 16 >= w.n_own) z[k * 16] = out[k];
             }
         }
     }

@@ -531,7 +531,7 @@ int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner
  *                        whole number, halves to the even one, from the exact quotient.  A row with NaN or an infinity: scale NaN, codes 0.
  * d8_quantize_columns    the same for each column of w [rows][cols] (rows ldw apart), whose codes become a row: for weights, laid out once.
  * d8_matmul_int8         z[i][j] = x_scales[i] w_scales[j] sum over k of x[i][k] w[j][k], rows of z ldz apart: x (rows) and w (cols) as above, sums exact,
- *                        scaled in fp32, rounded once to the element type.
+ *                        multiplied by one scale and then the other in fp32, rounded once to the element type.
  *     scratch: d8_matmul_int8_scratch_bytes, 16-byte aligned.
  *
  * A cache of keys and values in 8-bit integers, in pages of D8_CACHE_PAGE tokens with a scale for each page and key head.  With pitch = dim rounded up to 16:
