@@ -552,12 +552,12 @@ __device__ __forceinline__ void put(const AttArgs &a, T *to, int d, const f32x4 
         typedef T quad __attribute__((ext_vector_type(4)));
         quad v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(x[e] * by);
+        for (int e = 0; e < 4; ++e) v[e] = (T)within<T>(x[e] * by);
         *(quad *)(to + d) = v;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (d + e < a.c.dim) to[d + e] = (T)(x[e] * by);
+            if (d + e < a.c.dim) to[d + e] = (T)within<T>(x[e] * by);
     }
 }
 

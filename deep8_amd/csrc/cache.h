@@ -35,6 +35,13 @@ struct Pages {
     }
 };
 
+// a value or a mean of such; where the largest elements' codes round up past what the type holds, its largest number
+template <class T>
+__device__ __forceinline__ float within(float x) {
+    constexpr float MOST = sizeof(T) == 2 ? 65504.f : 3.4028234663852886e38f;
+    return fabsf(x) > MOST ? copysignf(MOST, x) : x;
+}
+
 int check(const Pages &p, int dtype, const char *name);
 
 }  // namespace cache

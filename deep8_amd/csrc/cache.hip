@@ -241,14 +241,6 @@ __device__ __forceinline__ void store(T *p, const float (&x)[V]) {
     *(typename Piece<T, V>::type *)p = v;
 }
 
-// a code's value; where the largest elements' codes round up past what the type holds, its largest number
-template <class T>
-__device__ __forceinline__ float value_of(signed char code, float scale) {
-    constexpr float MOST = sizeof(T) == 2 ? 65504.f : 3.4028234663852886e38f;
-    const float x = (float)code * scale;
-    return fabsf(x) > MOST ? copysignf(MOST, x) : x;
-}
-
 // Rows r .. of the call: the values of places slot .. of `page`, zeros if there is none.
 template <class T, int V>
 __device__ __forceinline__ void read(const Args &a, int r, int rows, int slot, int page, int head, unsigned *words) {
@@ -281,8 +273,8 @@ __device__ __forceinline__ void read(const Args &a, int r, int rows, int slot, i
             else code[0] = *from;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                x[e] = value_of<T>(code[e], ks);
-                y[e] = value_of<T>((signed char)(words[(d + e) * WORDS + (t >> 2)] >> (8 * (t & 3))), vs);
+                x[e] = within<T>((float)code[e] * ks);
+                y[e] = within<T>((float)(signed char)(words[(d + e) * WORDS + (t >> 2)] >> (8 * (t & 3))) * vs);
             }
         }
         store<T, V>(k + row * a.ldk + d, x), store<T, V>(v + row * a.ldv + d, y);

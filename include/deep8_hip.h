@@ -545,7 +545,8 @@ int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner
  *                        its page and head's scale NaN, and so everything that is read from it, until its first token is written anew.  A token whose
  *                        place is before the first or has no page is left out.  Two sequences must not bring tokens to one page in one
  *                        call, nor one sequence to a page that stands twice in its table; full pages may be in any number of tables.
- * d8_cache_read          the values of those places into rows of k and v, zeros for a token whose place is before the first or has no page.
+ * d8_cache_read          the values of those places into rows of k and v, zeros for a token whose place is before the first or has no page.  Where codes stand
+ *                        for more than the type holds (65504 as half is 64 steps of 1024), its largest number, here and in attention's results.
  * d8_attention_cache     o = softmax(scale q k^T) v over the values that such a cache holds, head i with the keys and values of head i / (heads / kv_heads);
  *                        scales may be any numbers.  causal != 0: query t of a sequence's n sees the keys of its places up to t + length - n, so the
  *                        last one sees them all; 0: every key.  Keys without a page are not seen.  lse[heads][q_tokens] (may be NULL) as

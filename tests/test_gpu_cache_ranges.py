@@ -37,3 +37,25 @@ def test_scores_of_any_size(order, n, dtype):
         assert np.array_equal(f(got)[:, 0], np.broadcast_to((v[0, -1] * 2.0 ** -6).astype(np.float32), (len(e), 16)))
         score = 2.0 ** e * 63 * scale
         assert (np.abs(lse[0] - score) <= 8 * 2.0 ** -24 * score).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("keys", [1, 64, 700])
+@pytest.mark.parametrize("top", [65504, 65472, 61000, 40000])
+def test_values_next_to_the_largest_half(top, keys, n):
+    """codes of the largest halves may stand for more than a half holds (65504 is 64 steps of 1024); the cache is read as 65504 there, and so is a mean of such
+    values, which is off by half a step of 1024, of the sums' fp32 and of its own rounding, 2^-11 (weights: all alike)"""
+    from deep8_amd import ops
+    pages = -(-keys // PAGE)
+    cache, table = ops.PagedCache(pages, 1, 32), np.arange(pages, dtype=np.int32)[None]
+    v = np.zeros((keys, 1, 32), np.float16)
+    v[:] = np.array([top, -top, top / 2, 1] * 8)
+    cache.append(np.ones_like(v), v, [0, keys], [keys], table)
+    back = cache.read(keys, [0, keys], [keys], table, np.float16)[1]
+    got, lse = cache.attention(np.ones((n, 1, 32), np.float16), [0, n], [keys], table, 0.125, False)
+    got = f(got)[:, 0].astype(np.float64)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - f(back)[0, 0]) <= 2.0 ** -10 * np.abs(f(back)[0, 0])).all()
+    assert (np.abs(got - f(v)[0, 0]) <= 512 + 2.0 ** -10 * np.abs(f(v)[0, 0])).all()
+    assert (np.abs(lse - (4 + np.log(keys))) <= 1e-5 * 12).all()
