@@ -280,6 +280,7 @@ int check(const NormArgs &a, int dtype, bool grad) {
     if (!a.rows) return 0;
     D8_REQUIRE(a.x && (grad ? a.dy != nullptr : a.out != nullptr), "%s: null tensor", name);
     D8_REQUIRE(a.ldx >= a.cols && (!a.out || a.ldout >= a.cols) && (!grad || a.lddy >= a.cols), "%s: rows of %d elements do not fit their leading dimension", name, a.cols);
+    D8_REQUIRE(a.rows == 1 || ((a.out != a.x || a.ldout == a.ldx) && (!grad || a.out != a.dy || a.ldout == a.lddy)), "%s: rows over an input lie where its rows do", name);
     return 0;
 }
 
