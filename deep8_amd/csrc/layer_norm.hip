@@ -314,6 +314,8 @@ void launch_grad(NormArgs &a, bool whole, hipStream_t stream) {
     });
 }
 
+enum { MOST_SUMS = 1 << 27 };  // columns whose sums a launch has threads for
+
 template <class T>
 void launch_sums(const NormArgs &a, hipStream_t stream) {
     if (a.cols < 16 * cu_count()) hipLaunchKernelGGL((layer_norm_sums_kernel<T, 32>), dim3(ceil_div(a.cols, 32), 2), dim3(1024), 0, stream, a);
@@ -339,7 +341,7 @@ extern "C" int d8_layer_norm(int dtype, const void *x, long ldx, const void *wei
 }
 
 extern "C" size_t d8_layer_norm_grad_scratch_bytes(int dtype, int rows, int cols) {
-    if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || rows < 0 || cols < 1 || cols >= (1 << 30)) return 0;
+    if ((dtype != D8_FLOAT16 && dtype != D8_FLOAT32) || rows < 0 || cols < 1 || cols > MOST_SUMS) return 0;
     const int groups = rows < 2 * cu_count() ? rows : 2 * cu_count();
     return sizeof(float) * 2 * (size_t)(groups ? groups : 1) * cols;
 }
@@ -353,6 +355,7 @@ extern "C" int d8_layer_norm_grad(int dtype, const void *x, long ldx, const void
     if (int rc = check(a, dtype, true)) return rc;
     const bool sums = dweight || dbias;
     if (sums) {
+        D8_REQUIRE(cols <= MOST_SUMS, "layer_norm_grad: weights' gradients have at most %d columns, not %d", (int)MOST_SUMS, cols);
         const size_t need = d8_layer_norm_grad_scratch_bytes(dtype, rows, cols);
         D8_REQUIRE(scratch && scratch_bytes >= need && ((size_t)scratch & 15) == 0, "layer_norm_grad: 16-byte aligned scratch of %zu bytes is needed, not %zu", need, scratch_bytes);
         a.partial = (float *)scratch;

@@ -226,6 +226,7 @@ extern "C" int d8_quantize_columns(int dtype, const void *w, long ldw, int rows,
     QuantizeArgs a = {w, codes, scales, ldw, int8::pitch_of(rows), rows, cols};
     if (int rc = check(a, dtype, rows, "quantize_columns")) return rc;
     if (!cols) return 0;
+    D8_REQUIRE(cols <= 1 << 29, "quantize_columns: %d columns are too many for a launch", cols);
     const dim3 grid(ceil_div(cols, 64));
     if (dtype == D8_FLOAT16) hipLaunchKernelGGL(quantize_columns_kernel<f16>, grid, dim3(256), 0, as_stream(stream), a);
     else hipLaunchKernelGGL(quantize_columns_kernel<float>, grid, dim3(256), 0, as_stream(stream), a);
