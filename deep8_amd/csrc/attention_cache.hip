@@ -14,16 +14,16 @@
 // KEYS, for few rows: a workgroup has 16 rows, its four waves share out the pages, each by itself and a page ahead, and join through LDS.
 // ROWS, for more, and heads of 128 elements at most: eight waves have 16 rows each and go through the pages together; a page's codes
 // are converted once and go through LDS as operands, in two buffers.  (512 queries of 4 sequences and 32 heads over 32768 keys of 8: 320 us with every wave converting
-// for itself, 122 so.)
+// for itself, 123 so.)
 //
 // All tiles' pages, one after the other, are cut into as many equal runs as workgroups run at once, whatever sequences have how many: a workgroup
 // goes through its run and leaves, for a tile that it has not all of, sums in scratch, which a second launch joins.  Cuts are found from the
 // lengths on the device, so a call can be captured and replayed as sequences grow.
 //
-// KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 62 us, 4.3 TB/s, where
+// KEYS is bound by memory (a page and head is 16 KB at 128 elements): 16 queries over 131072 keys of 8 heads of 128, 269 MB, take 60.6 us, 4.4 TB/s, where
 // a large copy moves 5.2; single precision 65 us.  ROWS by no unit alone: 1 x 2048 queries of 32 heads over
-// 8192 keys take 345 us, 700 TFLOP/s, where a large product of the library makes 1200; counters have the vector units, matrix
-// instructions' issue among it, busy for 68 % of the time, the matrix units for 30 %, LDS for 39 %.  What takes vector instructions away helps, as long as no
+// 8192 keys take 347 us, 700 TFLOP/s, where a large product of the library makes 1200; counters of the 512 queries above have the vector units, matrix
+// instructions' issue among it, busy for 63 % of the time, the matrix units for 30 %, LDS for 38 %.  What takes vector instructions away helps, as long as no
 // register more is needed.  (Two sets of rows a wave, which halve what LDS reads and leave two waves a SIMD: 155 us in place of 133; half the waves a phase behind
 // the others, no gain; accumulators in units of the pages' scales: 139 for 126.)  Short calls are bound by latency: a wave's
 // way from the first length to its last store is 10 us, and the join 4.

@@ -4,7 +4,7 @@
 // Three ways, by size:
 //   few rows (64 at most)      bound by memory, the weight: no LDS on its way, a wave reads 16 codes a lane straight into the operand
 //                              of v_mfma_i32_16x16x64_i8 (16 or 32 columns of w as left operand, all rows of x as right one); eight waves
-//                              share out the steps of the reduction and join through LDS: 4 x 4096 x 8192 in 8.9 us, 3.8 TB/s
+//                              share out the steps of the reduction and join through LDS: 4 x 4096 x 8192 in 8.5 us, 4.0 TB/s
 //   many rows and columns      matmul_int8_wide.hip
 //   between                    tiles of 64 x 64 through LDS, cut along the reduction where they leave compute units idle and it is long
 // Where w is the left operand, a lane ends up with four columns of a row side by side.
@@ -127,8 +127,8 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void int8_rows_kernel(Args a) {
 // 64 x 64 of z a workgroup, four waves of 32 x 32.  Two stages of LDS; the three steps of the reduction after the next are on their way into registers: a
 // workgroup alone on its compute unit would else take as long as memory answers for each (65 x 4096 x 4096: 13.2 us, 16.3 with one ahead).
 // Rows of 128 bytes, 16-byte piece c of row r at position c ^ (r / 2 % 8): the 16 rows of a fragment then take all banks in turn.  Bound by LDS where
-// there are many tiles: two fragments read for each two products, 1000 TOP/s (1024 x 4096 x 4096 in 33 us; tiles of 128 x 128, of which fewer fit a compute
-// unit: 35, and 14 for 8.5 at 777 x 1024 x 1352).
+// there are many tiles: two fragments read for each two products, 880 TOP/s (1024 x 4096 x 4096 in 39 us).  Tiles of 128 x 128 on the same way through registers, of which fewer fit a compute
+// unit, took 6 % longer there, and 14 us for 8.5 at 777 x 1024 x 1352.
 // QUADS: w is the left operand, a lane has four columns of a row; else x is, and 16 lanes have a row's columns side by side, which is what rows of z that cannot
 // be stored four elements at a time want (777 x 1000 x 1351 in single: 64 separate words a store before, 11 us for 9.2, and 8.1 with the scales loaded ahead and the tile's place in the launch's
 // three axes).
@@ -248,7 +248,7 @@ Plan plan_of(int rows, int inner, int cols) {
     p.part_ld = (cols + 3L) / 4 * 4;
     p.few = rows <= FEW_ROWS;
     const int tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;  // of 16 rows
-    // 32 columns a workgroup read x half as often; 16 where those would leave half the compute units idle (16 x 4096 x 4096 6.1 us, 10.8 with 32 and two parts,
+    // 32 columns a workgroup read x half as often; 16 where those would leave half the compute units idle (16 x 4096 x 4096 6.2 us, 10.8 with 32 and two parts,
     // but 8 x 2048 x 6144 7.9 and 7.0), unless x is large (64 x 11008 x 4096 28 and 27).
     p.few_cols = tiles < 4 && 2 * ceil_div(cols, 32) <= cus ? 16 : 32;
     const long groups = p.few ? ceil_div(cols, p.few_cols) : (long)ceil_div(rows, TILE) * ceil_div(cols, TILE);

@@ -1,7 +1,7 @@
 // The product in 8-bit integers of many rows and columns: the 256 x 256 tile loop of gemm_wide_kernel.h on the same bytes.  Two codes take the place
 // of one half, so a step of 64 halves is one of 128 codes, a fragment of 16 x 32 halves one of 16 x 64 codes, and only the matrix
 // instruction is another (v_mfma_i32_16x16x64_i8, twice the products in the same cycles, sums in int32).  The epilogue scales.  Bound by the matrix units and what power lets
-// them do: 8192 x 4096 x 8192 in 205 to 230 us, 2.7 to 2.4 POP/s (one call alone, and many in a row), where the library's product of the same bytes takes 246.
+// them do: 8192 x 4096 x 8192 in 210 to 234 us, 2.6 to 2.35 POP/s (as the clock is: the first of a row of calls, and many of them), where the library's product of the same bytes takes 246.
 #include "gemm_wide_kernel.h"
 #include "int8.h"
 
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256) void int8_wide_kernel(WideArgs wa) {
 }
 
 // Where these tiles are estimated to be through before those of 64 x 64: a step of 128 codes takes 1.05 us, a call 8 us beside them; the others go at 1000 TOP/s
-// after 5 us.  (us here / there: 1024 x 4096 x 4096 40 / 34, 2048 x 4096 x 4096 39 / 66, 4096 x 1024 x 4096 19 / 36, 3000 x 256 x 1024 11 / 7.)
+// after 5 us.  (us here / there: 1024 x 4096 x 4096 41 / 39, 2048 x 4096 x 4096 43 / 67, 4096 x 1024 x 4096 21 / 43, 2048 x 2048 x 2048 25 / 20, 3000 x 256 x 1024 14.5 / 6.4.)
 bool wide_eligible(const Args &a) {
     if (a.rows < 256 || a.cols < 256) return false;
     if (a.rows * a.pitch >= (1L << 31) || a.cols * a.pitch >= (1L << 31)) return false;

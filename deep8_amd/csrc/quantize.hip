@@ -8,8 +8,9 @@
 // three times.  A row that holds NaN or an infinity gets the scale NaN and codes 0, so its results are NaN.
 //
 // Rows: bound by memory, x read once (a team of threads holds a row: row_team.h) and a byte written for each element: 8192 x 4096
-// halves in 22 us, 4.6 TB/s, where a large copy moves 5.2.  Columns are laid out once
-// when a model is loaded: a workgroup goes down 64 columns twice (the second time mostly out of cache) and transposes through LDS.
+// halves in 18.5 us alone and 22 before a product that reads them, 5.4 and 4.6 TB/s, where a large copy moves 5.2.  Columns are laid out once
+// when a model is loaded: a workgroup goes down 64 columns twice (the second time mostly out of cache) and transposes through LDS: 4096 x 8192 halves in 367 us, bound
+// by the chain of its steps on half the compute units (at a copy's rate it would be 20).
 #include "int8.h"
 #include "row_team.h"
 

@@ -8,7 +8,7 @@
 // visits nodes breadth first (a node whose output is read at two depths would pass its gradient on before it is whole).
 // Serving: the trained block's keys and values go into a cache with room for `CAPACITY` tokens a sequence; half of each
 // sequence is read at once, the rest token by token, and the outputs must be those of the whole pass.  Then the same in 8-bit integers: products of
-// quantised rows with weights laid out once, and a cache of 8-bit pages.
+// quantised rows with weights laid out once, and a cache of 8-bit pages (the gated product, which has no 8-bit form, stays as it is).
 //
 //   deep8_transformer_block [steps]     exit code 0 if the loss fell below half and serving agrees, in 8 bits within what codes are off by
 #include <algorithm>

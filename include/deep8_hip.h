@@ -520,6 +520,7 @@ int d8_matmul_gated_grad(int dtype, const void *x, void *dx, int rows, int inner
  *
  * d8_layer_norm          each row x of `cols` elements becomes (x - m) / sqrt(mean((x - m)^2) + epsilon) * weight + bias, m = mean(x) (weight, bias:
  *                        cols elements, or NULL for ones and zeros).  Rows lie ldx and ldy elements apart; y may be x (ldy = ldx then).
+ *                        (The sum of a row's squares has to be one that fp32 holds: elements of less than 10^17 or so.)
  * d8_layer_norm_grad     from x and the gradient of y (dy) those of x (bit 0 of overwrite; NULL: not wanted) and of weight and bias (bit 1; NULL: not
  *                        wanted); gradients are added to what their destination holds unless their bit of `overwrite` is set.  dx may be dy or x (its rows then lie
  *                        where theirs do).  The same bits every time.  scratch: d8_layer_norm_grad_scratch_bytes, 16-byte aligned; none if neither weight's nor bias'
